@@ -443,6 +443,83 @@ TSHIP_EXPORT int TSHip_TransformerModelDecode(void* hidden, int hidden_size, int
                                               int num_kv_heads, int max_seq_len, int position, float eps, float rope_base,
                                               float rope_freq_scale, int intermediate_size, int rope_mode);
 
+/* ---- many sequences: rotary positions, a paged cache, attention over its pages, sampling ------------
+ * No bridge exports: the reference serves one sequence at a time.  Device pointers only, asynchronous on the calling thread's stream;
+ * descriptors are host memory, read before the call returns.  Lengths, page tables and sampling settings are device arrays, so
+ * that a captured step serves other lengths when it is replayed. */
+
+/* How positions turn a head.  Pair i of the first `dims` dimensions (a multiple of 4) is turned by
+ *   theta_i = position * base^(-2 i / dims) / freq_factors[i] * (freq_scale * (1 - kept_i) + kept_i)
+ * kept_i = ext_factor * (1 - clamp((i - low) / max(high - low, 0.001), 0, 1)) (0 where ext_factor is 0: plain linear scaling), low and
+ * high = the pairs that turn beta_fast and beta_slow times over original_context positions (floor / ceil, inside 0 .. dims - 1).
+ * Cosine and sine are multiplied by attn_factor, and where ext_factor is not 0 by 1 + 0.1 ln(1 / freq_scale) too.
+ * mode 0: adjacent dimensions are a pair; 2: dimensions dims / 2 apart. */
+typedef struct TSHipRope {
+    int dims;
+    int mode;
+    double base;
+    double freq_scale;
+    double ext_factor;
+    double attn_factor;
+    double beta_fast;
+    double beta_slow;
+    int64_t original_context;
+    const float* freq_factors;   /* device, dims / 2 of them; NULL: 1 */
+} TSHipRope;
+
+/* A cache of pages.  Position p of sequence s has its key of head h at k + page * k_page_stride + (p % page_size) * k_token_stride +
+ * h * k_head_stride elements, page = page_table[s * table_stride + p / page_size], and its value likewise.  Rows of head_dim
+ * elements (a multiple of 16 up to 256) are contiguous and 16-byte aligned.  A page id outside [0, num_pages) holds nothing: it is
+ * neither written nor read. */
+typedef struct TSHipPagedCache {
+    void* k;
+    void* v;
+    int element_type;            /* TSHIP_TYPE_F32, _F16 or _BF16 */
+    int num_kv_heads;
+    int head_dim;
+    int page_size;
+    int64_t num_pages;
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    const int32_t* page_table;   /* device */
+    int64_t table_stride;
+    int num_seqs;
+    int max_pages;               /* entries of a sequence in the table */
+} TSHipPagedCache;
+
+/* Rotary positions: result[t][h] = input[t][h] turned by positions[t] (device).  Views [tokens x heads x head_dim] with head_dim a multiple of
+ * 4 up to 256 and 16-byte aligned heads; result may be input (in place) but may not overlap it otherwise. */
+TSHIP_EXPORT int TSHip_RoPEF32Device(TSHipTensorView3D result, TSHipTensorView3D input, const int32_t* positions, const TSHipRope* rope);
+
+/* What lies between a fused QKV projection and the attention over a paged cache.  Rows row_starts[s] .. row_starts[s + 1] - 1 of qkv
+ * [rows x (num_heads + 2 num_kv_heads) head_dim] are the new tokens of sequence s, the last of context_lens[s] (both device; these
+ * tokens counted).  Per head of q and k: RMSNorm * q_norm / k_norm (skipped when NULL), rotation by the token's position in its
+ * sequence (or positions[row], device, when given).  q goes to query [rows x num_heads head_dim] (may be the q columns of qkv), k and
+ * v are rounded to the cache's type and stored at the token's position.  A token whose position is negative, beyond the table or on no page is not
+ * stored; rows that belong to no sequence are left as they were. */
+TSHIP_EXPORT int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv, int num_heads, const TSHipPagedCache* cache,
+                                               const int32_t* row_starts, const int32_t* context_lens, const int32_t* positions,
+                                               const float* q_norm, const float* k_norm, float eps, const TSHipRope* rope);
+
+/* Attention of new tokens over a paged cache that holds their own keys and values already: row i of sequence s (rows as above) is at
+ * position p = context_lens[s] - new tokens + i and sees positions max(0, p - window + 1) .. p (window 0: all from 0),
+ *   result[row][h] = sum_j e^(scale q.k_j - m) v_j / (sum_j e^(scale q.k_j - m) + e^(sinks[h] - m)),
+ * grouped heads sharing KV head h / (num_heads / num_kv_heads); sinks (device, num_heads logits) may be NULL (no such term).  A row that sees
+ * nothing is zero, rows that belong to no sequence are left as they were.  query and result [rows x num_heads head_dim]; result may be
+ * query.  Sums are fp32; 16-bit caches are multiplied on the matrix cores with queries and weights in as many 16-bit parts as fp32 needs. */
+TSHIP_EXPORT int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
+                                               const int32_t* row_starts, const int32_t* context_lens, float scale, int window,
+                                               const float* sinks);
+
+/* One token for each row of logits [rows x vocab] (vocab up to 2^20); every other pointer is a device array with one entry per row.
+ * Weights e^((l - l_max) / temperature) in 64 bits; candidates ranked by logit, the lowest index first among equals.  Of these stay, in
+ * this order: the first top_k (all where top_k <= 0); the fewest whose weights reach top_p of what is left (all where top_p >= 1, at
+ * least one); those of weight >= min_p, the first always.  The token is the first in index order whose cumulated weight exceeds
+ * uniforms[row] (in [0, 1)) of the total.  temperature not above 0: the first candidate.  NaN logits count as -infinity, a row without anything else gives
+ * -1.  probabilities (may be NULL): what the chosen token had.  top_k, top_p and min_p may be NULL (all stay). */
+TSHIP_EXPORT int TSHip_SampleTokensF32Device(TSHipTensorView2D logits, const float* uniforms, const float* temperature, const int32_t* top_k,
+                                             const float* top_p, const float* min_p, int32_t* tokens, float* probabilities);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@
 #include "tship_internal.h"
 
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -2956,6 +2957,294 @@ int TSHip_TransformerModelDecode(void* hidden, int hidden_size, int num_layers, 
             }
             return true;
         });
+    });
+}
+
+}  // extern "C"
+
+// ---- many sequences: rotary positions, paged cache, attention over its pages, sampling ---------------------------
+namespace {
+
+bool validate_rope(const TSHipRope* r, int head_dim, RopeSpec* out)
+{
+    if (r == nullptr) {
+        set_last_error("rope: null descriptor.");
+        return false;
+    }
+    if (r->mode != 0 && r->mode != 2) {
+        set_last_error("rope: mode must be 0 (adjacent pairs) or 2 (halves).");
+        return false;
+    }
+    if (r->dims <= 0 || r->dims % 4 != 0 || r->dims > head_dim) {
+        set_last_error("rope: dims must be a multiple of 4 and at most head_dim.");
+        return false;
+    }
+    if (!(r->base > 0.0) || !(r->freq_scale > 0.0) || !std::isfinite(r->base) || !std::isfinite(r->freq_scale) || !std::isfinite(r->ext_factor) ||
+        !std::isfinite(r->attn_factor)) {
+        set_last_error("rope: base and freq_scale must be positive, the factors finite.");
+        return false;
+    }
+    *out = {};
+    out->dims = r->dims;
+    out->mode = r->mode;
+    out->step = -2.0 * std::log2(r->base) / r->dims;
+    out->freq_scale = r->freq_scale;
+    out->range = 1.0;
+    out->factors = r->freq_factors;
+    double size = r->attn_factor;
+    if (r->ext_factor != 0.0) {
+        if (r->original_context <= 0 || !(r->beta_fast > 0.0) || !(r->beta_slow > 0.0) || !std::isfinite(r->beta_fast) || !std::isfinite(r->beta_slow) ||
+            !(r->base > 1.0)) {
+            set_last_error("rope: ext_factor needs original_context, beta_fast and beta_slow above 0 and a base above 1.");
+            return false;
+        }
+        // the pair that turns `beta` times over the original context
+        const double pi = 3.14159265358979323846;
+        auto pair = [&](double beta) { return r->dims * std::log((double)r->original_context / (beta * 2.0 * pi)) / (2.0 * std::log(r->base)); };
+        out->ext = r->ext_factor;
+        out->low = std::max(0.0, std::floor(pair(r->beta_fast)));
+        out->range = std::max(0.001, std::min(r->dims - 1.0, std::ceil(pair(r->beta_slow))) - out->low);
+        size *= 1.0 + 0.1 * std::log(1.0 / r->freq_scale);
+    }
+    out->size = (float)size;
+    return true;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// rows of `columns` floats that the kernels read and write 16 bytes at a time
+bool validate_rows(const TSHipTensorView2D& d, int64_t columns, bool written, const char* name)
+{
+    if (!validate_desc(d, name)) return false;
+    if (d.dim1 != columns) {
+        set_last_error(std::string("Size mismatch: ") + name + " does not have heads * head_dim columns.");
+        return false;
+    }
+    if (d.stride1 != 1 || (written && !is_standard_view(d))) {
+        set_last_error(std::string("Rows of ") + name + " must be contiguous and may not overlap.");
+        return false;
+    }
+    if (!aligned16(d.data) || (d.dim0 > 1 && (d.stride0 & 3) != 0)) {
+        set_last_error(std::string("Rows of ") + name + " must be 16-byte aligned on the device.");
+        return false;
+    }
+    return true;
+}
+
+bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_starts, const int32_t* context_lens, PagedKv* out)
+{
+    if (c == nullptr || c->k == nullptr || c->v == nullptr || c->page_table == nullptr || row_starts == nullptr || context_lens == nullptr) {
+        set_last_error("paged cache: null pointer.");
+        return false;
+    }
+    if (c->element_type != kTypeF32 && c->element_type != kTypeF16 && c->element_type != kTypeBF16) {
+        set_last_error("paged cache: the element type must be F32, F16 or BF16.");
+        return false;
+    }
+    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16 != 0) {
+        set_last_error("paged cache: head_dim must be a multiple of 16 up to 256.");
+        return false;
+    }
+    if (c->num_kv_heads <= 0 || num_heads <= 0 || num_heads % c->num_kv_heads != 0) {
+        set_last_error("paged cache: the heads are not a multiple of the KV heads.");
+        return false;
+    }
+    if (c->page_size <= 0 || c->num_pages <= 0 || c->num_pages > INT32_MAX || c->num_seqs <= 0 || c->max_pages <= 0 ||
+        (int64_t)c->max_pages * c->page_size > INT32_MAX || (c->num_seqs > 1 && c->table_stride < c->max_pages)) {
+        set_last_error("paged cache: invalid page size, page table or number of pages or sequences.");
+        return false;
+    }
+    const int64_t per = 16 / block_bytes(c->element_type);           // elements of 16 bytes
+    const int64_t strides[6] = {c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride, c->v_token_stride, c->v_head_stride};
+    const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
+    int64_t s[6];
+    for (int i = 0; i < 6; ++i) {
+        s[i] = counts[i % 3] > 1 ? strides[i] : 0;
+        if (counts[i % 3] > 1 && (s[i] < c->head_dim || s[i] % per != 0)) {
+            set_last_error("paged cache: strides must be multiples of 16 bytes and at least head_dim.");
+            return false;
+        }
+    }
+    if (!aligned16(c->k) || !aligned16(c->v)) {
+        set_last_error("paged cache: keys and values must be 16-byte aligned.");
+        return false;
+    }
+    *out = {};
+    out->k = static_cast<char*>(c->k);
+    out->v = static_cast<char*>(c->v);
+    out->k_page = s[0], out->k_token = s[1], out->k_head = s[2], out->v_page = s[3], out->v_token = s[4], out->v_head = s[5];
+    out->table = c->page_table;
+    out->table_stride = c->table_stride;
+    out->row_starts = row_starts;
+    out->context_lens = context_lens;
+    out->element_type = c->element_type;
+    out->kv_heads = c->num_kv_heads;
+    out->head_dim = c->head_dim;
+    out->num_pages = (int)c->num_pages;
+    out->max_pages = c->max_pages;
+    out->seqs = c->num_seqs;
+    out->page = FastDiv((uint32_t)c->page_size);
+    return true;
+}
+
+// Whether a and b, views of one shape, share memory in another way than element by element: not where their spans are apart, nor where
+// they have the same strides and their rows lie beside each other.
+bool overlaps_otherwise(const TSHipTensorView3D& a, const TSHipTensorView3D& b)
+{
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a.data), pb = reinterpret_cast<uintptr_t>(b.data);
+    auto span = [](const TSHipTensorView3D& d) {
+        return (uintptr_t)(((int64_t)(d.dim0 - 1) * d.stride0 + (int64_t)(d.dim1 - 1) * d.stride1 + d.dim2) * 4);
+    };
+    if (pa + span(a) <= pb || pb + span(b) <= pa) return false;
+    const bool same = (a.dim0 == 1 || a.stride0 == b.stride0) && (a.dim1 == 1 || a.stride1 == b.stride1);
+    if (!same) return true;
+    if (pa == pb) return false;
+    if (a.dim0 == 1 || a.stride0 <= 0) return true;
+    const int64_t row = (int64_t)a.stride0 * 4, wide = ((int64_t)(a.dim1 - 1) * a.stride1 + a.dim2) * 4;
+    const int64_t beside = (int64_t)((pa > pb ? pa - pb : pb - pa) % (uintptr_t)row);
+    return beside < wide || row - beside < wide;
+}
+
+}  // namespace
+
+extern "C" {
+
+int TSHip_RoPEF32Device(TSHipTensorView3D result, TSHipTensorView3D input, const int32_t* positions, const TSHipRope* rope)
+{
+    return guarded(0, "rope", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        if (!validate_desc3(result, "result") || !validate_desc3(input, "input")) return 0;
+        if (positions == nullptr) {
+            set_last_error("rope: null positions.");
+            return 0;
+        }
+        if (result.dim0 != input.dim0 || result.dim1 != input.dim1 || result.dim2 != input.dim2) {
+            set_last_error("Size mismatch: result and input differ in rope.");
+            return 0;
+        }
+        const int T = input.dim0, heads = input.dim1, dim = input.dim2;
+        if (dim % 4 != 0 || dim > 256) {
+            set_last_error("rope: head_dim must be a multiple of 4 up to 256.");
+            return 0;
+        }
+        RopeSpec spec;
+        if (!validate_rope(rope, dim, &spec)) return 0;
+        for (const TSHipTensorView3D* d : {&result, &input})
+            if (d->stride2 != 1 || !aligned16(d->data) || (T > 1 && (d->stride0 & 3) != 0) || (heads > 1 && (d->stride1 & 3) != 0)) {
+                set_last_error("rope: heads must be contiguous and 16-byte aligned on the device.");
+                return 0;
+            }
+        // (tokens before heads in memory, or heads before tokens)
+        const TSHipTensorView3D swapped{result.data, heads, T, dim, result.stride1, result.stride0, 1, result.raw_bytes};
+        if (!is_standard_view3(result) && !is_standard_view3(swapped)) {
+            set_last_error("rope: heads of result may not overlap.");
+            return 0;
+        }
+        if (overlaps_otherwise(result, input)) {
+            set_last_error("rope: result overlaps input without being the same view.");
+            return 0;
+        }
+        if (!launch_rope(static_cast<const float*>(input.data), T > 1 ? input.stride0 : 0, heads > 1 ? input.stride1 : 0,
+                         static_cast<float*>(result.data), T > 1 ? result.stride0 : 0, heads > 1 ? result.stride1 : 0, T, heads, dim, positions,
+                         spec, t_stream))
+            return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv, int num_heads, const TSHipPagedCache* cache,
+                                  const int32_t* row_starts, const int32_t* context_lens, const int32_t* positions, const float* q_norm,
+                                  const float* k_norm, float eps, const TSHipRope* rope)
+{
+    return guarded(0, "rope_store_paged", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        PagedKv kv;
+        RopeSpec spec;
+        if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv) || !validate_rope(rope, kv.head_dim, &spec)) return 0;
+        if (!validate_rows(query, (int64_t)num_heads * kv.head_dim, true, "query") ||
+            !validate_rows(qkv, ((int64_t)num_heads + 2 * (int64_t)kv.kv_heads) * kv.head_dim, false, "qkv"))
+            return 0;
+        if (query.dim0 != qkv.dim0) {
+            set_last_error("Size mismatch: query and qkv differ in rows.");
+            return 0;
+        }
+        if ((q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm))) {
+            set_last_error("rope_store_paged: norm weights must be 16-byte aligned.");
+            return 0;
+        }
+        const int T = qkv.dim0;
+        const uintptr_t q0 = reinterpret_cast<uintptr_t>(query.data), x0 = reinterpret_cast<uintptr_t>(qkv.data);
+        const uintptr_t q1 = q0 + ((int64_t)(T - 1) * query.stride0 + query.dim1) * 4, x1 = x0 + ((int64_t)(T - 1) * qkv.stride0 + qkv.dim1) * 4;
+        const bool apart = q1 <= x0 || x1 <= q0, in_place = q0 == x0 && (T == 1 || query.stride0 == qkv.stride0);
+        if (!apart && !in_place) {
+            set_last_error("rope_store_paged: query overlaps qkv without being its first columns.");
+            return 0;
+        }
+        if (!launch_rope_store(static_cast<const float*>(qkv.data), qkv.stride0, static_cast<float*>(query.data), query.stride0, T, num_heads, kv,
+                               positions, q_norm, k_norm, eps, spec, t_stream))
+            return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
+                                  const int32_t* row_starts, const int32_t* context_lens, float scale, int window, const float* sinks)
+{
+    return guarded(0, "paged_attention", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        PagedKv kv;
+        if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv)) return 0;
+        const int64_t columns = (int64_t)num_heads * kv.head_dim;
+        if (!validate_rows(result, columns, true, "result") || !validate_rows(query, columns, false, "query")) return 0;
+        if (query.dim0 != result.dim0) {
+            set_last_error("Size mismatch: query and result differ in rows.");
+            return 0;
+        }
+        if (window < 0 || !std::isfinite(scale)) {
+            set_last_error("paged_attention: the window must not be negative and the scale finite.");
+            return 0;
+        }
+        const int T = query.dim0;
+        const TSHipTensorView3D r3{result.data, T, 1, result.dim1, result.stride0, 0, 1, result.raw_bytes};
+        const TSHipTensorView3D q3{query.data, T, 1, query.dim1, query.stride0, 0, 1, query.raw_bytes};
+        if (overlaps_otherwise(r3, q3)) {
+            set_last_error("paged_attention: result overlaps query without being the same view.");
+            return 0;
+        }
+        const PagedAttnPlan plan = plan_paged_attention(T, num_heads, kv, window);
+        WsLease lease(t_stream, plan.ws_bytes);
+        if (!lease.ok()) return 0;
+        if (!launch_paged_attention(plan, static_cast<const float*>(query.data), query.stride0, static_cast<float*>(result.data), result.stride0, T,
+                                    num_heads, kv, scale, window, sinks, lease.ptr(), t_stream))
+            return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+int TSHip_SampleTokensF32Device(TSHipTensorView2D logits, const float* uniforms, const float* temperature, const int32_t* top_k,
+                                const float* top_p, const float* min_p, int32_t* tokens, float* probabilities)
+{
+    return guarded(0, "sample_tokens", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        if (!validate_desc(logits, "logits")) return 0;
+        if (uniforms == nullptr || temperature == nullptr || tokens == nullptr || logits.stride1 != 1) {
+            set_last_error("Invalid arguments for sample_tokens.");
+            return 0;
+        }
+        if (logits.dim1 > kMaxSampleVocab) {
+            set_last_error("sample_tokens: at most 2^20 logits per row.");
+            return 0;
+        }
+        WsLease lease(t_stream, sample_ws_bytes(logits.dim0, logits.dim1));
+        if (!lease.ok()) return 0;
+        if (!launch_sample(static_cast<const float*>(logits.data), logits.dim0 > 1 ? logits.stride0 : 0, logits.dim0, logits.dim1, uniforms, temperature,
+                           top_k, top_p, min_p, tokens, probabilities, lease.ptr(), t_stream))
+            return 0;
+        clear_last_error();
+        return 1;
     });
 }
 

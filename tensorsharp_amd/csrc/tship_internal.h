@@ -294,4 +294,66 @@ bool launch_moe_group(const int* ids, int A, int k, int E, int bm, int max_tiles
 bool launch_moe_combine(const float* dn, const float* bias, const int* ids, const float* weights, const int* pos_of, int T,
                         int k, int E, int H, bool slot_order, float* out, int64_t ldo, hipStream_t stream);
 
+// ---- many sequences: rotary positions, paged cache, attention over its pages, sampling -----------------
+// n / d for 0 <= n < 2^31 as one multiplication: with 2^(s-1) < d <= 2^s, m = ceil(2^(31+s) / d) fits 32 bits and n (m d - 2^(31+s))
+// stays below 2^(31+s), so that the product's excess never reaches the next quotient.
+struct FastDiv {
+    uint32_t d = 1, m = 1u << 31, shift = 31;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div)
+    {
+        uint32_t s = 0;
+        while (((uint64_t)1 << s) < div) ++s;
+        shift = 31 + s;
+        m = (uint32_t)((((uint64_t)1 << shift) + div - 1) / div);
+    }
+    __host__ __device__ uint32_t quot(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> shift); }
+};
+
+// How the angles of a position come about: pair i turns by position * 2^(step i) [/ factors[i]] * (freq_scale (1 - kept_i) + kept_i)
+// radians, kept_i = ext (1 - clamp((i - low) / range, 0, 1)); cosine and sine are multiplied by size.
+struct RopeSpec {
+    int dims;                  // leading dimensions of a head that are turned, a multiple of 4
+    int mode;                  // 0: adjacent pairs, 2: pairs half of dims apart
+    double step, freq_scale, ext, low, range;
+    float size;
+    const float* factors;      // device, dims / 2 of them, optional
+};
+
+// The cache as the kernels see it; strides in elements, 0 where there is one page (token, head).
+struct PagedKv {
+    char* k;
+    char* v;
+    int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* row_starts;
+    const int32_t* context_lens;
+    int element_type, kv_heads, head_dim;
+    int num_pages, max_pages, seqs;
+    FastDiv page;
+};
+
+// x [tokens x heads x head_dim] (strides in elements) -> out, which may be x
+bool launch_rope(const float* x, int64_t x_token, int64_t x_head, float* out, int64_t o_token, int64_t o_head, int tokens, int heads,
+                 int head_dim, const int32_t* positions, const RopeSpec& rope, hipStream_t stream);
+// rows [q heads | k heads | v heads] -> query rows and the cache; norm weights, positions optional
+bool launch_rope_store(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int rows, int heads, const PagedKv& cache,
+                       const int32_t* positions, const float* q_norm, const float* k_norm, float eps, const RopeSpec& rope, hipStream_t stream);
+
+// How the attention of a call is cut; depends on the shapes alone.
+struct PagedAttnPlan {
+    int tile_rows;             // (token, head of the group) rows of a workgroup
+    int tiles, splits;
+    size_t ws_bytes;
+};
+PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window);
+bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64_t ld_query, float* out, int64_t ld_out, int rows, int heads,
+                            const PagedKv& cache, float scale, int window, const float* sinks, void* ws, hipStream_t stream);
+
+constexpr int kMaxSampleVocab = 1 << 20;
+size_t sample_ws_bytes(int rows, int vocab);
+bool launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* uniforms, const float* temperature, const int32_t* top_k,
+                   const float* top_p, const float* min_p, int32_t* tokens, float* probabilities, void* ws, hipStream_t stream);
+
 }  // namespace tship

@@ -275,6 +275,78 @@ def _device_view(t):
     return N.TensorView2D(t.data_ptr(), rows, cols, s0, 1, ((rows - 1) * s0 + cols) * 4)
 
 
+def _vector(t, dtype, count, name, like):
+    """address of a contiguous device vector of `count` values (None stays None)"""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {str(dtype).split('.')[-1]} tensor of {count} values.")
+    if t.device != like.device:
+        raise ValueError(f"{name} is not on the device of the other tensors.")
+    return t.data_ptr()
+
+
+def _use_stream_of(t):
+    """Launches go to the current stream, which is one of the current device: a tensor of another one has no stream here."""
+    torch = _torch()
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError("the tensors must be on the current device.")
+    HipBasicOps.UseCurrentStream()
+
+
+class RotaryPositions:
+    """How positions turn a head (the descriptor of RoPE and RoPEStorePaged): the first `dims` dimensions in adjacent pairs (mode 0) or
+    in halves (mode 2), pair i by position * base^(-2 i / dims) radians.  freq_factors (float32 device tensor [dims / 2]) divide the
+    frequencies, freq_scale multiplies them (a context n times as long: 1 / n); with ext_factor above 0 only those of pairs that turn
+    less than beta_slow times over original_context, those between beta_slow and beta_fast in part, and the result is
+    multiplied by 1 + 0.1 ln(1 / freq_scale).  attn_factor multiplies it too."""
+
+    def __init__(self, dims, mode=2, base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0,
+                 original_context=0, freq_factors=None):
+        address = None
+        if freq_factors is not None:
+            torch = _torch()
+            if not freq_factors.is_cuda:
+                raise ValueError("freq_factors must be in GPU memory.")
+            address = _vector(freq_factors, torch.float32, int(dims) // 2, "freq_factors", freq_factors)
+        self._keepalive = freq_factors
+        self.native = N.Rope(int(dims), int(mode), float(base), float(freq_scale), float(ext_factor), float(attn_factor), float(beta_fast),
+                             float(beta_slow), int(original_context), address)
+        self.ref = C.byref(self.native)
+
+
+class PagedKVCache:
+    """Keys and values of many sequences in pages: k and v [pages, tokens of a page, kv heads, head_dim] device tensors of float32, float16 or
+    bfloat16 (any strides with contiguous rows of head_dim, so that heads may lie before tokens in memory), page_table [sequences,
+    pages of a sequence] int32 on the device.  Position p of sequence s is token p % page_size of page page_table[s, p // page_size]; an
+    entry outside the pages stands for none.  The contiguous cache [kv heads, max_seq, head_dim] of the whole-layer
+    decode is one page: PagedKVCache(k.transpose(0, 1)[None], v.transpose(0, 1)[None], table of one 0)."""
+
+    def __init__(self, k, v, page_table):
+        torch = _torch()
+        types = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16}
+        if k.dim() != 4 or k.shape != v.shape:
+            raise ValueError("PagedKVCache requires 4D tensors of one shape for k and v.")
+        if k.dtype not in types or v.dtype != k.dtype:
+            raise ValueError("PagedKVCache requires Float32, Float16 or BFloat16 keys and values of one type.")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32:
+            raise ValueError("PagedKVCache requires a 2D Int32 page table.")
+        if not k.is_cuda or v.device != k.device or page_table.device != k.device:
+            raise ValueError("PagedKVCache requires tensors in GPU memory of one device.")
+        if k.stride(3) != 1 or v.stride(3) != 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise NotImplementedError("PagedKVCache requires contiguous rows of head_dim and of the page table.")
+        self.k, self.v, self.page_table = k, v, page_table
+        self.num_kv_heads, self.head_dim, self.num_seqs = k.shape[2], k.shape[3], page_table.shape[0]
+        self.native = N.PagedCache(k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[2], k.shape[3], k.shape[1], k.shape[0], *k.stride()[:3],
+                                   *v.stride()[:3], page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1])
+        self.ref = C.byref(self.native)
+
+    def _sequences(self, row_starts, context_lens):
+        torch = _torch()
+        return (_vector(row_starts, torch.int32, self.num_seqs + 1, "row_starts", self.k),
+                _vector(context_lens, torch.int32, self.num_seqs, "context_lens", self.k))
+
+
 class HipBasicOps:
     """Static quantized-matmul entry points of the HIP backend."""
 
@@ -681,6 +753,72 @@ class HipBasicOps:
             int(head_dim), int(num_heads), int(num_kv_heads), int(l0["k_cache"].shape[1]), int(position), float(eps),
             float(rope_base), float(rope_freq_scale), int(gu.ne1 // 2), int(rope_mode))
         N.check_result(ok, "transformer_model_decode")
+
+    # -- many sequences: rotary positions, a paged cache, attention over its pages, sampling (device tensors) ------------
+    @staticmethod
+    def RoPE(result, input, positions, rope):
+        """result[t, h] = input[t, h] turned by positions[t]: [tokens, heads, head_dim] float32 device tensors (result may be input), positions
+        int32 [tokens], rope a RotaryPositions."""
+        torch = _torch()
+        if result.dim() != 3 or input.dim() != 3 or result.dtype != torch.float32 or input.dtype != torch.float32:
+            raise ValueError("RoPE requires 3D Float32 tensors.")
+        if not input.is_cuda or result.device != input.device:
+            raise ValueError("RoPE requires tensors in GPU memory of one device.")
+        pos = _vector(positions, torch.int32, input.shape[0], "positions", input)
+        _use_stream_of(input)
+        ok = N.lib().TSHip_RoPEF32Device(HipBasicOps._view3(result), HipBasicOps._view3(input), pos, rope.ref)
+        N.check_result(ok, "rope")
+
+    @staticmethod
+    def RoPEStorePaged(query, qkv, cache, row_starts, context_lens, rope, q_norm=None, k_norm=None, eps=1e-6, positions=None):
+        """From a fused QKV projection to the attention over a PagedKVCache: rows row_starts[s] .. row_starts[s + 1] - 1 of qkv [rows, (heads +
+        2 kv heads) head_dim] are the last tokens of the context_lens[s] of sequence s.  q and k heads are normed (q_norm / k_norm
+        [head_dim], None: not) and turned by their position in the sequence (or positions[row]); q goes to query [rows, heads
+        head_dim], k and v into the cache."""
+        torch = _torch()
+        qv, xv = _device_view(query), _device_view(qkv)
+        dim = cache.head_dim
+        starts, lens = cache._sequences(row_starts, context_lens)
+        pos = _vector(positions, torch.int32, qkv.shape[0], "positions", cache.k)
+        qn, kn = _vector(q_norm, torch.float32, dim, "q_norm", cache.k), _vector(k_norm, torch.float32, dim, "k_norm", cache.k)
+        if query.device != cache.k.device or qkv.device != cache.k.device:
+            raise ValueError("query and qkv must be on the device of the cache.")
+        _use_stream_of(qkv)
+        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, query.shape[1] // dim, cache.ref, starts, lens, pos, qn, kn, eps, rope.ref)
+        N.check_result(ok, "rope_store_paged")
+
+    @staticmethod
+    def PagedAttention(result, query, cache, row_starts, context_lens, scale, window=0, sinks=None):
+        """Attention of the sequences' new tokens (rows as in RoPEStorePaged) over a PagedKVCache that holds their keys and values already:
+        each sees the positions up to its own, the last `window` of them (0: all).  query and result [rows, heads head_dim]
+        float32 (may be one tensor); sinks [heads] float32: logits that take part in the softmax and carry no value."""
+        rv, qv = _device_view(result), _device_view(query)
+        heads = query.shape[1] // cache.head_dim
+        starts, lens = cache._sequences(row_starts, context_lens)
+        extra = _vector(sinks, _torch().float32, heads, "sinks", cache.k)
+        if query.device != cache.k.device or result.device != cache.k.device:
+            raise ValueError("query and result must be on the device of the cache.")
+        _use_stream_of(query)
+        ok = N.lib().TSHip_PagedAttentionF32Device(rv, qv, heads, cache.ref, starts, lens, scale, window, extra)
+        N.check_result(ok, "paged_attention")
+
+    @staticmethod
+    def SampleTokens(tokens, logits, uniforms, temperature, top_k=None, top_p=None, min_p=None, probabilities=None):
+        """tokens[r] (int32) drawn from logits [rows, vocab] (float32): e^(l / temperature[r]) of the top_k[r] (int32) likeliest, of these the
+        fewest that reach top_p[r], of these those with min_p[r] of the likeliest's weight; the first in index order whose
+        cumulated weight exceeds uniforms[r] of the total.  temperature 0: the likeliest.  None: no such limit.  probabilities
+        [rows] float32: of the tokens drawn."""
+        torch = _torch()
+        lv = _device_view(logits)
+        rows = logits.shape[0]
+        f32, i32 = torch.float32, torch.int32
+        if tokens is None or uniforms is None or temperature is None:
+            raise ValueError("SampleTokens requires tokens, uniforms and temperature.")
+        args = [_vector(uniforms, f32, rows, "uniforms", logits), _vector(temperature, f32, rows, "temperature", logits),
+                _vector(top_k, i32, rows, "top_k", logits), _vector(top_p, f32, rows, "top_p", logits), _vector(min_p, f32, rows, "min_p", logits),
+                _vector(tokens, i32, rows, "tokens", logits), _vector(probabilities, f32, rows, "probabilities", logits)]
+        _use_stream_of(logits)
+        N.check_result(N.lib().TSHip_SampleTokensF32Device(lv, *args), "sample_tokens")
 
     # -- LinearForward twin (ModelBase.cs:875-905): allocate result, route by residency -----
     @staticmethod

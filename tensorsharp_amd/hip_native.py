@@ -35,6 +35,21 @@ class ContiguousTensor(C.Structure):
     _fields_ = [("data", C.c_void_p), ("element_count", C.c_int64), ("element_type", C.c_int)]
 
 
+class Rope(C.Structure):
+    """TSHipRope: how positions turn a head."""
+    _fields_ = [("dims", C.c_int), ("mode", C.c_int), ("base", C.c_double), ("freq_scale", C.c_double), ("ext_factor", C.c_double),
+                ("attn_factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("original_context", C.c_int64),
+                ("freq_factors", C.c_void_p)]
+
+
+class PagedCache(C.Structure):
+    """TSHipPagedCache: pages of keys and values and the table that names them; strides in elements."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("element_type", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("num_pages", C.c_int64), ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("num_seqs", C.c_int), ("max_pages", C.c_int)]
+
+
 class NativeLibraryMissing(RuntimeError):
     """Twin of DllNotFoundException: the HIP library has not been built."""
 
@@ -133,6 +148,14 @@ SIGNATURES = {
         C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_int64,
         C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, C.c_float, C.c_int, C.c_int]),
 }
+SIGNATURES.update({
+    "TSHip_RoPEF32Device": (C.c_int, [TensorView3D, TensorView3D, C.c_void_p, C.POINTER(Rope)]),
+    "TSHip_RoPEStorePagedF32Device": (C.c_int, [TensorView2D, TensorView2D, C.c_int, C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_void_p,
+                                                C.c_void_p, C.c_void_p, C.c_float, C.POINTER(Rope)]),
+    "TSHip_PagedAttentionF32Device": (C.c_int, [TensorView2D, TensorView2D, C.c_int, C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_float,
+                                                C.c_int, C.c_void_p]),
+    "TSHip_SampleTokensF32Device": (C.c_int, [TensorView2D, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+})
 # the host-pointer forms take the same argument lists
 for _name in ("TSHip_FusedOutProjFFNQuantF32", "TSHip_FusedOutProjNormRouterQuantF32", "TSHip_MoEExpertsForwardF32",
               "TSHip_MoEExpertsSwiGLUForwardF32", "TSHip_MoEExpertsSwiGLUResidualF32"):
