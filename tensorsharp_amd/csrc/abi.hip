@@ -3050,7 +3050,7 @@ bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_
         return false;
     }
     if (c->page_size <= 0 || c->num_pages <= 0 || c->num_pages > INT32_MAX || c->num_seqs <= 0 || c->max_pages <= 0 ||
-        (int64_t)c->max_pages * c->page_size > INT32_MAX || (c->num_seqs > 1 && c->table_stride < c->max_pages)) {
+        (int64_t)c->max_pages * c->page_size > (1 << 30) || (c->num_seqs > 1 && c->table_stride < c->max_pages)) {
         set_last_error("paged cache: invalid page size, page table or number of pages or sequences.");
         return false;
     }

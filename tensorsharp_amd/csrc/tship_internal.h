@@ -343,8 +343,8 @@ bool launch_rope_store(const float* qkv, int64_t ld_qkv, float* query, int64_t l
 
 // How the attention of a call is cut; depends on the shapes alone.
 struct PagedAttnPlan {
-    int tile_rows;             // (token, head of the group) rows of a workgroup
-    int tiles, splits;
+    int tiles;                 // at most, over all sequences
+    int splits, min_keys;      // workgroups that share a tile's keys at most, and how many keys each has at least
     size_t ws_bytes;
 };
 PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window);
