@@ -505,10 +505,14 @@ struct Attn {
         uint64_t at = (uint64_t)__shfl((unsigned long long)rows, row);
         if (piece * 16 >= A.cache.head_dim * kElem) at = (uint64_t)(uintptr_t)g_zero_row;
         at += piece * 16;
-        // (in assembly, because the compiler would wait for every copy under way in front of each transposed read; it writes no register)
+        // (In assembly, because the compiler would wait for every copy under way in front of each transposed read.  It writes no register
+        // but m0, which nothing else here uses.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(block + n * 1024))),
                      "v"(at)
                      : "memory", "m0");
+#pragma clang diagnostic pop
     }
 
     // ---- one product step ----

@@ -4,6 +4,14 @@
 // many of its equals stay.  Weights e^((l - l_max) / T) are formed in 64-bit floating point and held as whole multiples of 2^-43:
 // sums of them are exact and the same in every order, so that neither a tile nor an atomic can move the border of a prefix or the
 // place of a draw.  (What is rounded away is below 2^-44 of the likeliest candidate's weight.)
+//
+// A row is cut into chunks, a workgroup each, and those into 16 segments, a wavefront each.
+//   sample_top_kernel    the largest logit of each chunk
+//   sample_sums_kernel   nothing but min-p to cut: weights per segment; else a histogram of the chunk over the distance to the largest logit
+//                        (counts for top-k, weights for top-p)
+//   sample_list_kernel   the bin in which the cut falls, from the histograms; the indices up to it, in order, per segment
+//   sample_draw_kernel   one workgroup per row: the exact cut among the listed, the draw
+// Each row's settings are device data, so every launch finds out for itself what its row needs.
 #include "tship_internal.h"
 
 #include <algorithm>
@@ -12,6 +20,10 @@ namespace tship {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kBins = 1024;
+constexpr int kMinChunk = 4096, kMaxChunks = 32;
+constexpr int kListed = 4096;                                        // candidates that the last kernel keeps in LDS
+constexpr int kRanked = 256;                                         // up to so many are ranked by comparing each with each
 constexpr double kOne = 8796093022208.0;                             // 2^43: 2^20 of them stay below 2^63
 constexpr uint32_t kLowestKey = 0x007fffffu;                         // of -infinity; NaN has 0
 
@@ -23,210 +35,516 @@ __device__ __forceinline__ uint32_t key_of(float l)
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
 
-struct Settings {
-    double temperature;
-    float top;                   // largest logit
-    uint32_t top_key;
+struct SampleArgs {
+    const float* logits;
+    int64_t ld;
+    int vocab, chunks, seg_len;                                      // a chunk has 16 segments of seg_len logits
+    const float* uniforms;
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int32_t* tokens;
+    float* probabilities;
+    uint64_t* tops;                                                  // [row][chunk]: key of the largest logit, complement of its index
+    uint64_t* hist;                                                  // [row][chunk][bin]
+    uint64_t* totals;                                                // [row]: all weights (top-p)
+    uint64_t* sums;                                                  // [row][segment]: weights
+    uint32_t* counts;                                                // [row][segment]: listed
+    uint32_t* list;                                                  // [row][segment][seg_len]: indices
 };
-__device__ __forceinline__ double weight_of(uint32_t key, const Settings& S)
-{
-    if (key <= kLowestKey) return 0.0;
-    if (key == S.top_key) return 1.0;                                // (an infinite maximum too)
-    return exp(((double)logit_of(key) - (double)S.top) / S.temperature);
-}
-__device__ __forceinline__ uint64_t whole(double w) { return (uint64_t)(w * kOne + 0.5); }
 
+enum { kDone, kWhole, kTopK, kTopP };                                // nothing to draw; no cut but min-p; cut by count; by weight only
+
+struct Row {
+    double temperature, p, least;
+    float top;
+    uint32_t top_key;
+    int top_index, k, kind;
+};
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__shfl_xor((unsigned long long)v, o); }
 __device__ __forceinline__ uint64_t wave_max(uint64_t v)
 {
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint64_t)__shfl_xor((unsigned long long)v, o));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, shfl_xor64(v, o));
     return v;
 }
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v)
 {
-    for (int o = 32; o > 0; o >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, o);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += shfl_xor64(v, o);
+    return v;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v)             // inclusive
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t below = (uint64_t)__shfl_up((unsigned long long)v, o);
+        if (lane >= o) v += below;
+    }
     return v;
 }
 
+// every wavefront works it out for itself
+__device__ __forceinline__ Row row_of(const SampleArgs& A, int row)
+{
+    const int lane = threadIdx.x & 63;
+    Row r;
+    const uint64_t best = wave_max(lane < A.chunks ? A.tops[row * A.chunks + lane] : 0);
+    const float t = A.temperature[row];
+    r.top_key = (uint32_t)(best >> 32);
+    r.top_index = (int)~(uint32_t)best;
+    r.top = logit_of(r.top_key);
+    r.temperature = t;
+    r.k = A.top_k ? A.top_k[row] : 0;
+    r.p = A.top_p ? (double)A.top_p[row] : 1.0;
+    r.least = A.min_p ? (double)A.min_p[row] : 0.0;
+    r.kind = r.top_key <= kLowestKey || !(t > 0.f) ? kDone : r.k > 0 && r.k < A.vocab ? kTopK : r.p < 1.0 ? kTopP : kWhole;
+    return r;
+}
+__device__ __forceinline__ double weight_of(uint32_t key, const Row& r)
+{
+    if (key <= kLowestKey) return 0.0;
+    if (key == r.top_key) return 1.0;                                // (an infinite maximum too)
+    return exp(((double)logit_of(key) - (double)r.top) / r.temperature);
+}
+// w 2^43 to the nearest whole number: what an addition of 2^52 leaves in the fraction
+__device__ __forceinline__ uint64_t whole(double w) { return (uint64_t)__double_as_longlong(__builtin_fma(w, kOne, 4503599627370496.0)) & 0xfffffffffffffull; }
+
+// Bins of the distance to the largest logit, 64 to an octave from 1/16 to 4096; a larger logit never has the higher bin.
+__device__ __forceinline__ int bin_of(uint32_t key, const Row& r)
+{
+    const float d = r.top_key == key ? 0.f : r.top - logit_of(key);
+    return min(kBins - 1, max(0, (int)(__float_as_uint(d) >> 17) - (123 << 6) + 1));
+}
+
+// inclusive sum over the threads of the workgroup; *total: over all
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* red, uint64_t* total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) red[wave] = v;
+    __syncthreads();
+    uint64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const uint64_t s = red[w];
+        before += w < wave ? s : 0;
+        all += s;
+    }
+    *total = all;
+    return v + before;
+}
+// what a share of a total is, as the least sum that has it: 1 at least
+__device__ __forceinline__ uint64_t share_of(double p, uint64_t total)
+{
+    return min((uint64_t)fmin((double)total, fmax(1.0, ceil(p * (double)total))), total);
+}
+// the first sum in index order that exceeds u of the total is the first that reaches this
+__device__ __forceinline__ uint64_t drawn(const SampleArgs& A, int row, uint64_t total)
+{
+    const double u = fmin(fmax((double)A.uniforms[row], 0.0), 1.0);
+    return min((uint64_t)(u * (double)total) + 1, total);
+}
+__device__ __forceinline__ void chosen(const SampleArgs& A, int row, int index, uint32_t key, uint64_t total, const Row& r)
+{
+    A.tokens[row] = index;
+    if (A.probabilities) A.probabilities[row] = (float)(weight_of(key, r) * kOne / (double)total);
+}
+
+// grid (chunks, rows)
+__global__ void __launch_bounds__(kThreads) sample_top_kernel(const SampleArgs A)
+{
+    __shared__ uint64_t red[kWaves];
+    const int row = blockIdx.y, begin = blockIdx.x * kWaves * A.seg_len, end = min(A.vocab, begin + kWaves * A.seg_len);
+    const float* x = A.logits + row * A.ld;
+    uint64_t best = 0;
+#pragma unroll 4
+    for (int i = begin + threadIdx.x; i < end; i += kThreads) best = max(best, (uint64_t)key_of(x[i]) << 32 | (uint32_t)~i);
+    best = wave_max(best);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < kWaves; ++w) best = max(best, red[w]);
+        A.tops[row * A.chunks + blockIdx.x] = best;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs A)
+{
+    __shared__ uint64_t hist[kBins];
+    const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Row r = row_of(A, row);
+    if (r.kind == kDone) return;
+    const float* x = A.logits + row * A.ld;
+    const int seg = chunk * kWaves + wave, begin = seg * A.seg_len, end = min(A.vocab, begin + A.seg_len);
+    if (r.kind == kWhole) {
+        uint64_t sum = 0;
+#pragma unroll 4
+        for (int i = begin + lane; i < end; i += 64) {
+            const double w = weight_of(key_of(x[i]), r);
+            sum += w >= r.least || i == r.top_index ? whole(w) : 0;
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) A.sums[(int64_t)row * A.chunks * kWaves + seg] = sum;
+        return;
+    }
+    hist[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = begin + lane; i < end; i += 64) {
+        const uint32_t key = key_of(x[i]);
+        const uint64_t v = key <= kLowestKey ? 0 : r.kind == kTopK ? 1 : whole(weight_of(key, r));
+        if (v) atomicAdd((unsigned long long*)&hist[bin_of(key, r)], (unsigned long long)v);
+    }
+    __syncthreads();
+    A.hist[((int64_t)row * A.chunks + chunk) * kBins + threadIdx.x] = hist[threadIdx.x];
+}
+
+__global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleArgs A)
+{
+    __shared__ uint64_t red[kWaves];
+    __shared__ int cut;
+    const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Row r = row_of(A, row);
+    if (r.kind == kDone || r.kind == kWhole) return;
+    uint64_t mine = 0, total;
+    for (int c = 0; c < A.chunks; ++c) mine += A.hist[((int64_t)row * A.chunks + c) * kBins + threadIdx.x];
+    const uint64_t cum = block_scan(mine, red, &total), need = r.kind == kTopK ? (uint64_t)r.k : share_of(r.p, total);
+    if (threadIdx.x == 0) {
+        cut = kBins - 1;                                             // (fewer candidates than k)
+        if (chunk == 0) A.totals[row] = total;
+    }
+    __syncthreads();
+    if (cum >= need && cum - mine < need) cut = threadIdx.x;
+    __syncthreads();
+    const int last = cut, seg = chunk * kWaves + wave, begin = seg * A.seg_len, end = min(A.vocab, begin + A.seg_len);
+    const float* x = A.logits + row * A.ld;
+    uint32_t* list = A.list + ((int64_t)row * A.chunks * kWaves + seg) * A.seg_len;
+    uint32_t n = 0;
+    for (int i0 = begin; i0 < end; i0 += 256) {
+        uint32_t key[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) key[j] = i0 + 64 * j + lane < end ? key_of(x[i0 + 64 * j + lane]) : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = key[j] > kLowestKey && bin_of(key[j], r) <= last;
+            const uint64_t lanes = __ballot(in);
+            if (in) list[n + __popcll(lanes & ((1ull << lane) - 1))] = i0 + 64 * j + lane;
+            n += __popcll(lanes);
+        }
+    }
+    if (lane == 0) A.counts[(int64_t)row * A.chunks * kWaves + seg] = n;
+}
+
 struct Prefix {
-    uint32_t key;                // logits above stay, and `ties` of the equal ones (UINT32_MAX: all of them)
+    uint32_t key;                // logits above stay, and `ties` of the equal ones
     uint32_t ties;
 };
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(const float* logits, int64_t ld, int vocab, const float* uniforms, const float* temperature,
-                                                          const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
-                                                          float* probabilities)
+__global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs A)
 {
-    __shared__ uint64_t hist[256], red[kWaves], found[2];
-    __shared__ uint32_t count[256];
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float* x = logits + row * ld;
-
-    // the largest logit, and its lowest index
-    uint64_t best = 0;
-    for (int i = tid; i < vocab; i += kThreads) best = max(best, (uint64_t)key_of(x[i]) << 32 | (uint32_t)~i);
-    best = wave_max(best);
-    if (lane == 0) red[wave] = best;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) best = max(best, red[w]);
-    const int top_index = (int)~(uint32_t)best;
-    Settings S;
-    S.top_key = (uint32_t)(best >> 32);
-    S.top = logit_of(S.top_key);
-    const float T = temperature[row];
-    S.temperature = T;
-    if (S.top_key <= kLowestKey || !(T > 0.f)) {
+    __shared__ uint64_t red[kWaves], hist[256], rest;
+    __shared__ int place;
+    __shared__ uint32_t offset[kMaxChunks * kWaves + 1], keys[kListed], indices[kListed];
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, segs = A.chunks * kWaves;
+    const float* x = A.logits + row * A.ld;
+    const Row r = row_of(A, row);
+    if (r.kind == kDone) {
         if (tid == 0) {
-            tokens[row] = S.top_key <= kLowestKey ? -1 : top_index;
-            if (probabilities) probabilities[row] = S.top_key <= kLowestKey ? 0.f : 1.f;
+            A.tokens[row] = r.top_key <= kLowestKey ? -1 : r.top_index;
+            if (A.probabilities) A.probabilities[row] = r.top_key <= kLowestKey ? 0.f : 1.f;
+        }
+        return;
+    }
+    if (r.kind == kWhole) {
+        // the segment that the draw falls in, then the place in it
+        uint64_t total;
+        const uint64_t mine = tid < segs ? A.sums[(int64_t)row * segs + tid] : 0, cum = block_scan(mine, red, &total), want = drawn(A, row, total);
+        if (cum >= want && cum - mine < want) {
+            rest = want - (cum - mine);
+            place = tid;
+        }
+        __syncthreads();
+        uint64_t left = rest;
+        const int begin = place * A.seg_len, end = min(A.vocab, begin + A.seg_len);
+        for (int i0 = begin; i0 < end; i0 += kThreads) {
+            const int i = i0 + tid;
+            const uint32_t key = i < end ? key_of(x[i]) : 0;
+            const double w = weight_of(key, r);
+            const uint64_t v = w >= r.least || i == r.top_index ? whole(w) : 0;
+            uint64_t all;
+            const uint64_t c = block_scan(v, red, &all);
+            if (c >= left && c - v < left) chosen(A, row, i, key, total, r);
+            if (all >= left) return;                                 // uniform
+            left -= all;
         }
         return;
     }
 
-    Prefix P{kLowestKey, 0};
-    auto each = [&](auto&& f) {
-        for (int i = tid; i < vocab; i += kThreads) f(i, key_of(x[i]));
-    };
-    // top-k: the key of the k-th candidate, eight bits at a time
-    const int k = top_k ? top_k[row] : 0;
-    if (k > 0 && k < vocab) {
-        uint32_t prefix = 0, left = k;
-        bool cut = true;
-        for (int shift = 24; shift >= 0 && cut; shift -= 8) {
-            if (tid < 256) count[tid] = 0;
-            __syncthreads();
-            const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            each([&](int, uint32_t key) {
-                if (key > kLowestKey && (key & mask) == prefix) atomicAdd(&count[(key >> shift) & 255], 1u);
-            });
-            __syncthreads();
-            int d = 255;
-            while (d > 0 && count[d] < left) left -= count[d--];
-            if (d == 0 && count[0] < left) cut = false;              // fewer candidates than k
-            prefix |= (uint32_t)d << shift;
-            __syncthreads();
-        }
-        if (cut) P = {prefix, left};
+    // the listed candidates by their position in index order
+    uint64_t listed;
+    {
+        const uint64_t mine = tid < segs ? A.counts[(int64_t)row * segs + tid] : 0, cum = block_scan(mine, red, &listed);
+        if (tid < segs) offset[tid + 1] = (uint32_t)cum;
+        if (tid == 0) offset[0] = 0;
+        __syncthreads();
     }
-    auto block_sum = [&](uint64_t v) {
-        v = wave_sum(v);
-        __syncthreads();
-        if (lane == 0) red[wave] = v;
-        __syncthreads();
-        uint64_t s = 0;
-        for (int w = 0; w < kWaves; ++w) s += red[w];
-        return s;
+    const int n = (int)listed;
+    const uint32_t* list = A.list + (int64_t)row * segs * A.seg_len;
+    const bool near = n <= kListed;
+    // segment of position i: the last one that begins at or before it
+    auto index_at = [&](int i) {
+        int lo = 0, hi = segs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((int)offset[mid] <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        return (int)list[(int64_t)lo * A.seg_len + (i - (int)offset[lo])];
     };
-    // top-p: the same over the weights
-    const double p = top_p ? (double)top_p[row] : 1.0;
-    const uint64_t tied = P.ties ? whole(weight_of(P.key, S)) * P.ties : 0;
-    if (p < 1.0) {
-        uint64_t total = 0;
-        each([&](int, uint32_t key) { total += key > P.key ? whole(weight_of(key, S)) : 0; });
-        total = block_sum(total) + tied;
-        uint64_t left = (uint64_t)fmin((double)total, fmax(1.0, ceil(p * (double)total)));
-        left = min(left, total);
-        uint32_t prefix = 0;
+    if (near) {
+        for (int i = tid; i < n; i += kThreads) {
+            const int at = index_at(i);
+            indices[i] = at;
+            keys[i] = key_of(x[at]);
+        }
+        __syncthreads();
+    }
+    auto at = [&](int i, uint32_t* key) {
+        if (near) {
+            *key = keys[i];
+            return (int)indices[i];
+        }
+        const int index = index_at(i);
+        *key = key_of(x[index]);
+        return index;
+    };
+
+    if (n <= kRanked) {
+        // everyone counts who is ahead and what they weigh
+        __shared__ uint64_t weights[kRanked];
+        const bool in = tid < n;
+        const uint32_t key = in ? keys[tid] : 0;
+        const double w = in ? weight_of(key, r) : 0.0;
+        const uint64_t mine = in ? whole(w) : 0;
+        if (in) weights[tid] = mine;
+        __syncthreads();
+        int rank = 0;
+        uint64_t ahead = 0;
+        if (wave * 64 < n) {
+            for (int j = 0; j < n; ++j) {
+                const bool before = keys[j] > key || (keys[j] == key && j < tid);
+                rank += before;
+                ahead += before ? weights[j] : 0;
+            }
+        }
+        bool stays = in && (r.kind == kTopP || rank < r.k);
+        if (r.p < 1.0) {
+            uint64_t total = r.kind == kTopP ? A.totals[row] : 0, all;
+            if (r.kind == kTopK) {
+                block_scan(stays ? mine : 0, red, &all);
+                total = all;
+            }
+            stays = stays && (rank == 0 || ahead < share_of(r.p, total));
+        }
+        stays = stays && (w >= r.least || rank == 0);
+        uint64_t total;
+        const uint64_t v = stays ? mine : 0, cum = block_scan(v, red, &total), want = drawn(A, row, total);
+        if (cum >= want && cum - v < want) chosen(A, row, (int)indices[tid], key, total, r);
+        return;
+    }
+
+    // A key eight bits at a time: the digit in whose bin `left` falls, counted from the top; left becomes what is needed of that bin.
+    // False where all bins together hold less.
+    auto each = [&](auto&& f) {
+        for (int i = tid; i < n; i += kThreads) {
+            uint32_t key;
+            at(i, &key);
+            f(key);
+        }
+    };
+    auto select = [&](uint64_t& left, uint32_t& prefix, auto&& values) {
+        prefix = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) hist[tid] = 0;
+            if (tid == 0) place = -1;
             __syncthreads();
             const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            each([&](int, uint32_t key) {
-                if (key > P.key && (key & mask) == prefix) atomicAdd((unsigned long long*)&hist[(key >> shift) & 255], (unsigned long long)whole(weight_of(key, S)));
+            values([&](uint32_t key, uint64_t v) {
+                if ((key & mask) == prefix) atomicAdd((unsigned long long*)&hist[(key >> shift) & 255], (unsigned long long)v);
             });
-            if (tid == 0 && tied && (P.key & mask) == prefix) atomicAdd((unsigned long long*)&hist[(P.key >> shift) & 255], (unsigned long long)tied);
             __syncthreads();
-            int d = 255;
-            while (d > 0 && hist[d] < left) left -= hist[d--];
-            prefix |= (uint32_t)d << shift;
+            if (wave == 0) {
+                uint64_t b[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    b[i] = hist[255 - 4 * lane - i];
+                    sum += b[i];
+                }
+                const uint64_t cum = wave_scan(sum), lanes = __ballot(cum >= left);
+                if (lanes != 0 && lane == __ffsll((unsigned long long)lanes) - 1) {
+                    uint64_t needed = left - (cum - sum);
+                    int i = 0;
+                    while (i < 3 && b[i] < needed) needed -= b[i++];
+                    place = 255 - 4 * lane - i;
+                    rest = needed;
+                }
+            }
+            __syncthreads();
+            if (place < 0) return false;                             // uniform
+            prefix |= (uint32_t)place << shift;
+            left = rest;
             __syncthreads();
         }
-        const uint64_t w = whole(weight_of(prefix, S));
-        const uint32_t ties = (uint32_t)((left + w - 1) / max(w, (uint64_t)1));
-        if (prefix > P.key) P = {prefix, ties};
+        return true;
+    };
+    Prefix P{kLowestKey, 0};
+    if (r.kind == kTopK) {
+        uint64_t left = (uint64_t)r.k;
+        uint32_t key;
+        if (select(left, key, [&](auto&& add) { each([&](uint32_t k) { add(k, 1); }); })) P = {key, (uint32_t)left};
+    }
+    if (r.p < 1.0) {
+        const uint64_t tied = P.ties ? whole(weight_of(P.key, r)) * P.ties : 0;
+        uint64_t total = r.kind == kTopP ? A.totals[row] : 0;
+        if (r.kind == kTopK) {
+            uint64_t sum = 0;
+            each([&](uint32_t key) { sum += key > P.key ? whole(weight_of(key, r)) : 0; });
+            block_scan(sum, red, &total);
+            total += tied;
+        }
+        uint64_t left = share_of(r.p, total);
+        uint32_t key;
+        select(left, key, [&](auto&& add) {
+            each([&](uint32_t k) {
+                if (k > P.key) add(k, whole(weight_of(k, r)));
+            });
+            if (tid == 0 && tied) add(P.key, tied);
+        });
+        const uint64_t w = max(whole(weight_of(key, r)), (uint64_t)1);
+        const uint32_t ties = (uint32_t)min((left + w - 1) / w, (uint64_t)0xffffffffu);
+        if (key > P.key) P = {key, ties};
         else P.ties = min(P.ties, ties);
     }
-    // the index behind the last of the equal ones that stay
-    int tie_end = vocab;
+    // Every thread has a run of positions.  First the one that holds the last of the equal ones that stay.
+    const int per = (n + kThreads - 1) / kThreads, first = min(n, tid * per), end = min(n, first + per);
+    int tie_end = 0;
     if (P.ties) {
-        uint32_t seen = 0;
-        for (int i0 = 0; i0 < vocab; i0 += kThreads) {
-            const bool is = i0 + tid < vocab && key_of(x[i0 + tid]) == P.key;
-            const uint64_t lanes = __ballot(is);
-            __syncthreads();
-            if (lane == 0) count[wave] = __popcll(lanes);
-            __syncthreads();
-            uint32_t before = seen, all = 0;
-            for (int w = 0; w < kWaves; ++w) {
-                if (w < wave) before += count[w];
-                all += count[w];
+        uint64_t seen = 0, all;
+        uint32_t key;
+        for (int i = first; i < end; ++i) {
+            at(i, &key);
+            seen += key == P.key;
+        }
+        const uint64_t before = block_scan(seen, red, &all) - seen;
+        if (tid == 0) place = n;
+        __syncthreads();
+        if (before < P.ties && before + seen >= P.ties) {
+            uint64_t c = before;
+            int i = first;
+            for (; c < P.ties; ++i) {
+                at(i, &key);
+                c += key == P.key;
             }
-            if (is && before + __popcll(lanes & ((1ull << lane) - 1)) + 1 == P.ties) found[0] = i0 + tid + 1;
-            seen += all;
-            if (seen >= P.ties) break;                               // uniform
+            place = i;
         }
         __syncthreads();
-        tie_end = (int)found[0];
+        tie_end = place;
     }
-    const double least = min_p ? (double)min_p[row] : 0.0;
-    auto kept = [&](int i) -> uint64_t {
-        const uint32_t key = key_of(x[i]);
-        if (key < P.key || (key == P.key && (P.ties == 0 || i >= tie_end))) return 0;
-        const double w = weight_of(key, S);
-        return w >= least || i == top_index ? whole(w) : 0;
+    auto kept = [&](int i, uint32_t* key, int* index) -> uint64_t {
+        *index = at(i, key);
+        if (*key < P.key || (*key == P.key && i >= tie_end)) return 0;
+        const double w = weight_of(*key, r);
+        return w >= r.least || *index == r.top_index ? whole(w) : 0;
     };
-    // the draw: ranges of indices, cut in sixteen until one is left
-    int begin = 0, end = vocab;
-    uint64_t left = 0, total = 0;
-    while (end - begin > 64) {
-        const int part = ((end - begin + kWaves - 1) / kWaves + 63) / 64 * 64;
-        uint64_t sum = 0;
-        const int b = begin + wave * part, e = min(end, b + part);
-        for (int i = b + lane; i < e; i += 64) sum += kept(i);
-        sum = wave_sum(sum);
-        __syncthreads();
-        if (lane == 0) red[wave] = sum;
-        __syncthreads();
-        if (total == 0) {
-            for (int w = 0; w < kWaves; ++w) total += red[w];
-            const double u = fmin(fmax((double)uniforms[row], 0.0), 1.0);
-            left = min((uint64_t)(u * (double)total) + 1, total);    // the first index that brings the sum to this
-        }
-        int w = 0;
-        while (w < kWaves - 1 && red[w] < left) left -= red[w++];
-        begin += w * part;
-        end = min(end, begin + part);
-        __syncthreads();
-    }
-    if (wave == 0) {
-        const bool in = begin + lane < end;
-        uint64_t v = in ? kept(begin + lane) : 0, cum = v;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t below = (uint64_t)__shfl_up((unsigned long long)cum, o);
-            if (lane >= o) cum += below;
-        }
-        if (total == 0) {                                            // (a vocabulary of 64 or less)
-            total = (uint64_t)__shfl((unsigned long long)cum, 63);
-            const double u = fmin(fmax((double)uniforms[row], 0.0), 1.0);
-            left = min((uint64_t)(u * (double)total) + 1, total);
-        }
-        const int at = __ffsll((unsigned long long)__ballot(in && cum >= left)) - 1;
-        if (lane == at) {
-            tokens[row] = begin + at;
-            if (probabilities) probabilities[row] = (float)(weight_of(key_of(x[begin + at]), S) * kOne / (double)total);
-        }
+    uint64_t sum = 0, total;
+    uint32_t key = 0;
+    int index = 0;
+    for (int i = first; i < end; ++i) sum += kept(i, &key, &index);
+    const uint64_t cum = block_scan(sum, red, &total), want = drawn(A, row, total);
+    if (cum >= want && cum - sum < want) {
+        uint64_t c = cum - sum;
+        for (int i = first; c < want; ++i) c += kept(i, &key, &index);
+        chosen(A, row, index, key, total, r);
     }
 }
 
+struct SampleLayout {
+    int chunks, seg_len;
+    size_t tops, hist, totals, sums, counts, list, total;            // byte offsets; for `rows` rows
+};
+SampleLayout layout_of(int rows, int vocab)
+{
+    SampleLayout L{};
+    // about a workgroup per CU, and chunks that are worth one
+    L.chunks = std::max(1, std::min({kMaxChunks, device_info().num_cus / rows, (vocab + kMinChunk - 1) / kMinChunk}));
+    L.seg_len = ((vocab + L.chunks * kWaves - 1) / (L.chunks * kWaves) + 63) / 64 * 64;
+    size_t off = 0;
+    auto take = [&](size_t b) {
+        const size_t o = off;
+        off += (b + 255) & ~(size_t)255;
+        return o;
+    };
+    const size_t n = rows, segs = (size_t)L.chunks * kWaves;
+    L.tops = take(n * L.chunks * 8);
+    L.hist = take(n * L.chunks * kBins * 8);
+    L.totals = take(n * 8);
+    L.sums = take(n * segs * 8);
+    L.counts = take(n * segs * 4);
+    L.list = take(n * segs * L.seg_len * 4);
+    L.total = off;
+    return L;
+}
+// rows of a launch: their lists take as much memory as their logits
+int rows_at_once(int rows, int vocab) { return (int)std::max<int64_t>(1, std::min<int64_t>({rows, 65535, ((int64_t)1 << 26) / vocab})); }
+
 }  // namespace
 
-size_t sample_ws_bytes(int, int) { return 0; }
+size_t sample_ws_bytes(int rows, int vocab) { return layout_of(rows_at_once(rows, vocab), vocab).total; }
 
 bool launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* uniforms, const float* temperature, const int32_t* top_k,
-                   const float* top_p, const float* min_p, int32_t* tokens, float* probabilities, void*, hipStream_t stream)
+                   const float* top_p, const float* min_p, int32_t* tokens, float* probabilities, void* ws, hipStream_t stream)
 {
-    hipLaunchKernelGGL(sample_kernel, dim3(rows), dim3(kThreads), 0, stream, logits, ld, vocab, uniforms, temperature, top_k, top_p, min_p, tokens,
-                       probabilities);
-    return hip_ok(hipGetLastError(), "sample launch");
+    const int most = rows_at_once(rows, vocab);
+    const SampleLayout L = layout_of(most, vocab);
+    char* base = static_cast<char*>(ws);
+    for (int r0 = 0; r0 < rows; r0 += most) {
+        const int n = std::min(most, rows - r0);
+        SampleArgs a{};
+        a.logits = logits + r0 * ld;
+        a.ld = ld;
+        a.vocab = vocab;
+        a.chunks = L.chunks;
+        a.seg_len = L.seg_len;
+        a.uniforms = uniforms + r0;
+        a.temperature = temperature + r0;
+        a.top_k = top_k ? top_k + r0 : nullptr;
+        a.top_p = top_p ? top_p + r0 : nullptr;
+        a.min_p = min_p ? min_p + r0 : nullptr;
+        a.tokens = tokens + r0;
+        a.probabilities = probabilities ? probabilities + r0 : nullptr;
+        a.tops = reinterpret_cast<uint64_t*>(base + L.tops);
+        a.hist = reinterpret_cast<uint64_t*>(base + L.hist);
+        a.totals = reinterpret_cast<uint64_t*>(base + L.totals);
+        a.sums = reinterpret_cast<uint64_t*>(base + L.sums);
+        a.counts = reinterpret_cast<uint32_t*>(base + L.counts);
+        a.list = reinterpret_cast<uint32_t*>(base + L.list);
+        const dim3 grid(L.chunks, n), block(kThreads);
+        hipLaunchKernelGGL(sample_top_kernel, grid, block, 0, stream, a);
+        if (!hip_ok(hipGetLastError(), "sample launch")) return false;
+        hipLaunchKernelGGL(sample_sums_kernel, grid, block, 0, stream, a);
+        if (!hip_ok(hipGetLastError(), "sample launch")) return false;
+        if (top_k || top_p) {
+            hipLaunchKernelGGL(sample_list_kernel, grid, block, 0, stream, a);
+            if (!hip_ok(hipGetLastError(), "sample launch")) return false;
+        }
+        hipLaunchKernelGGL(sample_draw_kernel, dim3(n), block, 0, stream, a);
+        if (!hip_ok(hipGetLastError(), "sample launch")) return false;
+    }
+    return true;
 }
 
 }  // namespace tship
