@@ -6,11 +6,14 @@
 // place of a draw.  (What is rounded away is below 2^-44 of the likeliest candidate's weight.)
 //
 // A row is cut into chunks, a workgroup each, and those into 16 segments, a wavefront each.
-//   sample_top_kernel    the largest logit of each chunk
-//   sample_sums_kernel   nothing but min-p to cut: weights per segment; else a histogram of the chunk over the distance to the largest logit
-//                        (counts for top-k, weights for top-p)
-//   sample_list_kernel   the bin in which the cut falls, from the histograms; the indices up to it, in order, per segment
-//   sample_draw_kernel   one workgroup per row: the exact cut among the listed, the draw
+//   sample_top_kernel    the largest logit of each chunk, and of each of 64 groups of it
+//   sample_sums_kernel   by what the row asks for:
+//                        top-k with k at most the number of groups: as many groups reach the k-th largest of their maxima, so the k
+//                        candidates are among those that do - these are listed, in order, per segment
+//                        another cut: a histogram of the chunk over the distance to the largest logit, of counts (a larger k) or weights (top-p)
+//                        nothing but min-p: the weights of each segment
+//   sample_draw_kernel   one workgroup per row: from a histogram the bin in which the cut falls and the list up to it; the exact cut
+//                        among the listed; the draw
 // Each row's settings are device data, so every launch finds out for itself what its row needs.
 #include "tship_internal.h"
 
@@ -21,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 1024;
+constexpr int kGroups = 64;                                          // of a chunk: what 16 lanes of a segment's wavefront read
 constexpr int kMinChunk = 4096, kMaxChunks = 32;
 constexpr int kListed = 4096;                                        // candidates that the last kernel keeps in LDS
 constexpr int kRanked = 256;                                         // up to so many are ranked by comparing each with each
@@ -47,17 +51,17 @@ struct SampleArgs {
     int32_t* tokens;
     float* probabilities;
     uint64_t* tops;                                                  // [row][chunk]: key of the largest logit, complement of its index
+    uint32_t* groups;                                                // [row][chunk][group]: key of the largest logit
     uint64_t* hist;                                                  // [row][chunk][bin]
-    uint64_t* totals;                                                // [row]: all weights (top-p)
     uint64_t* sums;                                                  // [row][segment]: weights
     uint32_t* counts;                                                // [row][segment]: listed
-    uint32_t* list;                                                  // [row][segment][seg_len]: indices
+    uint64_t* list;                                                  // [row][segment][seg_len]: key and index
 };
 
-enum { kDone, kWhole, kTopK, kTopP };                                // nothing to draw; no cut but min-p; cut by count; by weight only
+enum { kDone, kWhole, kTopK, kManyK, kTopP };                        // nothing to draw; no cut but min-p; cut by count (of few, of many); by weight only
 
 struct Row {
-    double temperature, p, least;
+    double by, p, least;         // by: log2 e / temperature
     float top;
     uint32_t top_key;
     int top_index, k, kind;
@@ -96,18 +100,39 @@ __device__ __forceinline__ Row row_of(const SampleArgs& A, int row)
     r.top_key = (uint32_t)(best >> 32);
     r.top_index = (int)~(uint32_t)best;
     r.top = logit_of(r.top_key);
-    r.temperature = t;
+    r.by = 1.44269504088896340736 / (double)t;
     r.k = A.top_k ? A.top_k[row] : 0;
     r.p = A.top_p ? (double)A.top_p[row] : 1.0;
     r.least = A.min_p ? (double)A.min_p[row] : 0.0;
-    r.kind = r.top_key <= kLowestKey || !(t > 0.f) ? kDone : r.k > 0 && r.k < A.vocab ? kTopK : r.p < 1.0 ? kTopP : kWhole;
+    r.kind = r.top_key <= kLowestKey || !(t > 0.f) ? kDone : r.k > 0 && r.k < A.vocab ? (r.k <= A.chunks * kGroups ? kTopK : kManyK) : r.p < 1.0 ? kTopP : kWhole;
     return r;
+}
+// 2^y, -60 <= y <= 0 (what is below counts as 2^-60, which no sum holds): the whole part of y goes to the exponent; the rest, at most a
+// half, through the Taylor series of e^(y ln 2) up to the 11th power (what is left out: (ln 2 / 2)^12 / 12! = 6e-15).
+__device__ __forceinline__ double power_of_two(double y)
+{
+    constexpr double L = 0.693147180559945309417, kRound = 6755399441055744.0;       // 1.5 x 2^52: an addition rounds to whole numbers
+    const double t = fmax(y, -60.0) + kRound, z = fmax(y, -60.0) - (t - kRound);
+    constexpr double L2 = L * L, L3 = L2 * L, L4 = L3 * L, L5 = L4 * L, L6 = L5 * L, L7 = L6 * L, L8 = L7 * L, L9 = L8 * L, L10 = L9 * L, L11 = L10 * L;
+    double s = L11 / 39916800.0;
+    s = __builtin_fma(s, z, L10 / 3628800.0);
+    s = __builtin_fma(s, z, L9 / 362880.0);
+    s = __builtin_fma(s, z, L8 / 40320.0);
+    s = __builtin_fma(s, z, L7 / 5040.0);
+    s = __builtin_fma(s, z, L6 / 720.0);
+    s = __builtin_fma(s, z, L5 / 120.0);
+    s = __builtin_fma(s, z, L4 / 24.0);
+    s = __builtin_fma(s, z, L3 / 6.0);
+    s = __builtin_fma(s, z, L2 / 2.0);
+    s = __builtin_fma(s, z, L);
+    s = __builtin_fma(s, z, 1.0);
+    return __hiloint2double(__double2hiint(s) + (__double2loint(t) << 20), __double2loint(s));
 }
 __device__ __forceinline__ double weight_of(uint32_t key, const Row& r)
 {
-    if (key <= kLowestKey) return 0.0;
-    if (key == r.top_key) return 1.0;                                // (an infinite maximum too)
-    return exp(((double)logit_of(key) - (double)r.top) / r.temperature);
+    // (the largest is 1 where it is infinite too, and its distance to the others no number)
+    const double w = power_of_two(((double)logit_of(key) - (double)r.top) * r.by);
+    return key <= kLowestKey ? 0.0 : key == r.top_key ? 1.0 : w;
 }
 // w 2^43 to the nearest whole number: what an addition of 2^52 leaves in the fraction
 __device__ __forceinline__ uint64_t whole(double w) { return (uint64_t)__double_as_longlong(__builtin_fma(w, kOne, 4503599627370496.0)) & 0xfffffffffffffull; }
@@ -158,13 +183,18 @@ __device__ __forceinline__ void chosen(const SampleArgs& A, int row, int index, 
 __global__ void __launch_bounds__(kThreads) sample_top_kernel(const SampleArgs A)
 {
     __shared__ uint64_t red[kWaves];
-    const int row = blockIdx.y, begin = blockIdx.x * kWaves * A.seg_len, end = min(A.vocab, begin + kWaves * A.seg_len);
+    const int row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int begin = (blockIdx.x * kWaves + wave) * A.seg_len, end = min(A.vocab, begin + A.seg_len);
     const float* x = A.logits + row * A.ld;
     uint64_t best = 0;
 #pragma unroll 4
-    for (int i = begin + threadIdx.x; i < end; i += kThreads) best = max(best, (uint64_t)key_of(x[i]) << 32 | (uint32_t)~i);
-    best = wave_max(best);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
+    for (int i = begin + lane; i < end; i += 64) best = max(best, (uint64_t)key_of(x[i]) << 32 | (uint32_t)~i);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) best = max(best, shfl_xor64(best, o));
+    if ((lane & 15) == 0) A.groups[(row * A.chunks + blockIdx.x) * kGroups + threadIdx.x / 16] = (uint32_t)(best >> 32);
+    best = max(best, shfl_xor64(best, 16));
+    best = max(best, shfl_xor64(best, 32));
+    if (lane == 0) red[wave] = best;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 0; w < kWaves; ++w) best = max(best, red[w]);
@@ -172,10 +202,54 @@ __global__ void __launch_bounds__(kThreads) sample_top_kernel(const SampleArgs A
     }
 }
 
+// Candidates in bins up to `last` among the segments seg0 .. seg0 + segs - 1 (at most 64), in order, from list on; returns how many.
+// Of the candidates most segments have none, which their groups tell.
+__device__ __forceinline__ uint32_t list_segments(const SampleArgs& A, const Row& r, int row, int seg0, int segs, int last, uint64_t* list)
+{
+    const int lane = threadIdx.x & 63, begin = seg0 * A.seg_len, end = min(A.vocab, begin + segs * A.seg_len);
+    const float* x = A.logits + row * A.ld;
+    uint32_t top = 0;
+    if (lane < segs) {
+        const uint4 g = *reinterpret_cast<const uint4*>(A.groups + (row * A.chunks * kWaves + seg0 + lane) * 4);
+        top = max(max(g.x, g.y), max(g.z, g.w));
+    }
+    const uint64_t some = __ballot(top > kLowestKey && bin_of(top, r) <= last);
+    // bin_of(l) <= last in one subtraction, where no infinity is in the way
+    const bool plain = last < kBins - 1 && r.top < INFINITY;
+    const float border = __uint_as_float((uint32_t)(last + (123 << 6)) << 17);
+    uint32_t n = 0;
+    constexpr int W = 16;
+    for (int i0 = begin; i0 < end; i0 += 64 * W) {
+        const int s0 = (i0 - begin) / A.seg_len, s1 = min(63, (i0 - begin + 64 * W - 1) / A.seg_len);
+        if (((some >> s0) & (~0ull >> (63 - (s1 - s0)))) == 0) continue;
+        float l[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) l[j] = i0 + 64 * j + lane < end ? x[i0 + 64 * j + lane] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const bool in = plain ? r.top - l[j] < border : key_of(l[j]) > kLowestKey && bin_of(key_of(l[j]), r) <= last;
+            const uint64_t lanes = __ballot(in);
+            if (lanes == 0) continue;
+            if (in) list[n + __popcll(lanes & ((1ull << lane) - 1))] = (uint64_t)key_of(l[j]) << 32 | (uint32_t)(i0 + 64 * j + lane);
+            n += __popcll(lanes);
+        }
+    }
+    return n;
+}
+
 __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs A)
 {
-    __shared__ uint64_t hist[kBins];
+    __shared__ uint64_t hist[kBins], red[kWaves];
+    __shared__ int cut;
     const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // (asked for beside what the row's settings come from)
+    const int groups = A.chunks * kGroups;
+    uint32_t tops[kMaxChunks * kGroups / kThreads];
+#pragma unroll
+    for (int i = 0; i < kMaxChunks * kGroups / kThreads; ++i) {
+        const int g = threadIdx.x + i * kThreads;
+        tops[i] = g < groups ? A.groups[row * groups + g] : 0;
+    }
     const Row r = row_of(A, row);
     if (r.kind == kDone) return;
     const float* x = A.logits + row * A.ld;
@@ -193,50 +267,28 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
     }
     hist[threadIdx.x] = 0;
     __syncthreads();
+    if (r.kind == kTopK) {
+#pragma unroll
+        for (int i = 0; i < kMaxChunks * kGroups / kThreads; ++i)
+            if (tops[i] > kLowestKey) atomicAdd((unsigned long long*)&hist[bin_of(tops[i], r)], 1ull);
+        if (threadIdx.x == 0) cut = kBins - 1;                       // (fewer groups with a candidate than k)
+        __syncthreads();
+        uint64_t all;
+        const uint64_t mine = hist[threadIdx.x], cum = block_scan(mine, red, &all);
+        if (cum >= (uint64_t)r.k && cum - mine < (uint64_t)r.k) cut = threadIdx.x;
+        __syncthreads();
+        const uint32_t n = list_segments(A, r, row, seg, 1, cut, A.list + ((int64_t)row * A.chunks * kWaves + seg) * A.seg_len);
+        if (lane == 0) A.counts[(int64_t)row * A.chunks * kWaves + seg] = n;
+        return;
+    }
 #pragma unroll 4
     for (int i = begin + lane; i < end; i += 64) {
         const uint32_t key = key_of(x[i]);
-        const uint64_t v = key <= kLowestKey ? 0 : r.kind == kTopK ? 1 : whole(weight_of(key, r));
+        const uint64_t v = key <= kLowestKey ? 0 : r.kind == kManyK ? 1 : whole(weight_of(key, r));
         if (v) atomicAdd((unsigned long long*)&hist[bin_of(key, r)], (unsigned long long)v);
     }
     __syncthreads();
     A.hist[((int64_t)row * A.chunks + chunk) * kBins + threadIdx.x] = hist[threadIdx.x];
-}
-
-__global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleArgs A)
-{
-    __shared__ uint64_t red[kWaves];
-    __shared__ int cut;
-    const int row = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Row r = row_of(A, row);
-    if (r.kind == kDone || r.kind == kWhole) return;
-    uint64_t mine = 0, total;
-    for (int c = 0; c < A.chunks; ++c) mine += A.hist[((int64_t)row * A.chunks + c) * kBins + threadIdx.x];
-    const uint64_t cum = block_scan(mine, red, &total), need = r.kind == kTopK ? (uint64_t)r.k : share_of(r.p, total);
-    if (threadIdx.x == 0) {
-        cut = kBins - 1;                                             // (fewer candidates than k)
-        if (chunk == 0) A.totals[row] = total;
-    }
-    __syncthreads();
-    if (cum >= need && cum - mine < need) cut = threadIdx.x;
-    __syncthreads();
-    const int last = cut, seg = chunk * kWaves + wave, begin = seg * A.seg_len, end = min(A.vocab, begin + A.seg_len);
-    const float* x = A.logits + row * A.ld;
-    uint32_t* list = A.list + ((int64_t)row * A.chunks * kWaves + seg) * A.seg_len;
-    uint32_t n = 0;
-    for (int i0 = begin; i0 < end; i0 += 256) {
-        uint32_t key[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) key[j] = i0 + 64 * j + lane < end ? key_of(x[i0 + 64 * j + lane]) : 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool in = key[j] > kLowestKey && bin_of(key[j], r) <= last;
-            const uint64_t lanes = __ballot(in);
-            if (in) list[n + __popcll(lanes & ((1ull << lane) - 1))] = i0 + 64 * j + lane;
-            n += __popcll(lanes);
-        }
-    }
-    if (lane == 0) A.counts[(int64_t)row * A.chunks * kWaves + seg] = n;
 }
 
 struct Prefix {
@@ -251,6 +303,9 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs 
     __shared__ uint32_t offset[kMaxChunks * kWaves + 1], keys[kListed], indices[kListed];
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, segs = A.chunks * kWaves;
     const float* x = A.logits + row * A.ld;
+    // (both asked for beside what the row's settings come from; which of them was written depends on these)
+    const uint32_t count = tid < segs ? A.counts[(int64_t)row * segs + tid] : 0;
+    const uint64_t sum_here = tid < segs ? A.sums[(int64_t)row * segs + tid] : 0;
     const Row r = row_of(A, row);
     if (r.kind == kDone) {
         if (tid == 0) {
@@ -262,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs 
     if (r.kind == kWhole) {
         // the segment that the draw falls in, then the place in it
         uint64_t total;
-        const uint64_t mine = tid < segs ? A.sums[(int64_t)row * segs + tid] : 0, cum = block_scan(mine, red, &total), want = drawn(A, row, total);
+        const uint64_t mine = sum_here, cum = block_scan(mine, red, &total), want = drawn(A, row, total);
         if (cum >= want && cum - mine < want) {
             rest = want - (cum - mine);
             place = tid;
@@ -284,32 +339,54 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs 
         return;
     }
 
+    // all weights, where a share of them is wanted; the lists are of segments, or of the run of segments of each wavefront here
+    uint64_t weights_of_all = 0;
+    int lists = segs, list_len = A.seg_len;
+    uint32_t listed_here;
+    if (r.kind != kTopK) {
+        uint64_t mine = 0, total;
+#pragma unroll 8
+        for (int c = 0; c < A.chunks; ++c) mine += A.hist[((int64_t)row * A.chunks + c) * kBins + tid];
+        const uint64_t cum = block_scan(mine, red, &total), need = r.kind == kManyK ? (uint64_t)r.k : share_of(r.p, total);
+        if (tid == 0) place = kBins - 1;                             // (fewer candidates than k)
+        __syncthreads();
+        if (cum >= need && cum - mine < need) place = tid;
+        __syncthreads();
+        const int last = place;
+        lists = kWaves;
+        list_len = A.chunks * A.seg_len;
+        listed_here = list_segments(A, r, row, wave * A.chunks, A.chunks, last, A.list + (int64_t)row * segs * A.seg_len + (int64_t)wave * list_len);
+        weights_of_all = total;
+        if (lane == 0) offset[wave + 1] = listed_here;
+        __syncthreads();
+    }
+
     // the listed candidates by their position in index order
     uint64_t listed;
     {
-        const uint64_t mine = tid < segs ? A.counts[(int64_t)row * segs + tid] : 0, cum = block_scan(mine, red, &listed);
-        if (tid < segs) offset[tid + 1] = (uint32_t)cum;
+        const uint64_t mine = tid >= lists ? 0 : r.kind == kTopK ? count : offset[tid + 1], cum = block_scan(mine, red, &listed);
+        if (tid < lists) offset[tid + 1] = (uint32_t)cum;
         if (tid == 0) offset[0] = 0;
         __syncthreads();
     }
     const int n = (int)listed;
-    const uint32_t* list = A.list + (int64_t)row * segs * A.seg_len;
+    const uint64_t* list = A.list + (int64_t)row * segs * A.seg_len;
     const bool near = n <= kListed;
-    // segment of position i: the last one that begins at or before it
-    auto index_at = [&](int i) {
-        int lo = 0, hi = segs - 1;
+    // list of position i: the last one that begins at or before it
+    auto entry_at = [&](int i) {
+        int lo = 0, hi = lists - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if ((int)offset[mid] <= i) lo = mid;
             else hi = mid - 1;
         }
-        return (int)list[(int64_t)lo * A.seg_len + (i - (int)offset[lo])];
+        return list[(int64_t)lo * list_len + (i - (int)offset[lo])];
     };
     if (near) {
         for (int i = tid; i < n; i += kThreads) {
-            const int at = index_at(i);
-            indices[i] = at;
-            keys[i] = key_of(x[at]);
+            const uint64_t e = entry_at(i);
+            indices[i] = (uint32_t)e;
+            keys[i] = (uint32_t)(e >> 32);
         }
         __syncthreads();
     }
@@ -318,36 +395,52 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs 
             *key = keys[i];
             return (int)indices[i];
         }
-        const int index = index_at(i);
-        *key = key_of(x[index]);
-        return index;
+        const uint64_t e = entry_at(i);
+        *key = (uint32_t)(e >> 32);
+        return (int)(uint32_t)e;
     };
 
     if (n <= kRanked) {
-        // everyone counts who is ahead and what they weigh
-        __shared__ uint64_t weights[kRanked];
+        // Everyone counts who is ahead and what they weigh; the others are shared by as many threads as there are for each.
+        struct Entry { uint64_t order, weight; };
+        __shared__ Entry entries[kRanked];
+        __shared__ uint64_t aheads[kRanked];
+        __shared__ int ranks[kRanked];
         const bool in = tid < n;
         const uint32_t key = in ? keys[tid] : 0;
         const double w = in ? weight_of(key, r) : 0.0;
         const uint64_t mine = in ? whole(w) : 0;
-        if (in) weights[tid] = mine;
+        if (tid < kRanked) {
+            entries[tid] = {(uint64_t)key << 32 | (uint32_t)~tid, mine};
+            aheads[tid] = 0;
+            ranks[tid] = 0;
+        }
         __syncthreads();
-        int rank = 0;
-        uint64_t ahead = 0;
-        if (wave * 64 < n) {
-            for (int j = 0; j < n; ++j) {
-                const bool before = keys[j] > key || (keys[j] == key && j < tid);
+        {
+            const int wide = n <= 64 ? 64 : n <= 128 ? 128 : 256, e = tid & (wide - 1), share = (n + kThreads / wide - 1) / (kThreads / wide);
+            const int j0 = min(n, tid / wide * share), j1 = min(n, j0 + share);
+            const uint64_t order = entries[e].order;
+            int rank = 0;
+            uint64_t ahead = 0;
+#pragma unroll 4
+            for (int j = j0; j < j1; ++j) {
+                const Entry o = entries[j];
+                const bool before = o.order > order;
                 rank += before;
-                ahead += before ? weights[j] : 0;
+                ahead += before ? o.weight : 0;
+            }
+            if (rank > 0) {
+                atomicAdd(&ranks[e], rank);
+                atomicAdd((unsigned long long*)&aheads[e], (unsigned long long)ahead);
             }
         }
+        __syncthreads();
+        const int rank = in ? ranks[tid] : 0;
+        const uint64_t ahead = in ? aheads[tid] : 0;
         bool stays = in && (r.kind == kTopP || rank < r.k);
         if (r.p < 1.0) {
-            uint64_t total = r.kind == kTopP ? A.totals[row] : 0, all;
-            if (r.kind == kTopK) {
-                block_scan(stays ? mine : 0, red, &all);
-                total = all;
-            }
+            uint64_t total = weights_of_all;
+            if (r.kind != kTopP) block_scan(stays ? mine : 0, red, &total);
             stays = stays && (rank == 0 || ahead < share_of(r.p, total));
         }
         stays = stays && (w >= r.least || rank == 0);
@@ -402,15 +495,15 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs 
         return true;
     };
     Prefix P{kLowestKey, 0};
-    if (r.kind == kTopK) {
+    if (r.kind != kTopP) {
         uint64_t left = (uint64_t)r.k;
         uint32_t key;
         if (select(left, key, [&](auto&& add) { each([&](uint32_t k) { add(k, 1); }); })) P = {key, (uint32_t)left};
     }
     if (r.p < 1.0) {
         const uint64_t tied = P.ties ? whole(weight_of(P.key, r)) * P.ties : 0;
-        uint64_t total = r.kind == kTopP ? A.totals[row] : 0;
-        if (r.kind == kTopK) {
+        uint64_t total = weights_of_all;
+        if (r.kind != kTopP) {
             uint64_t sum = 0;
             each([&](uint32_t key) { sum += key > P.key ? whole(weight_of(key, r)) : 0; });
             block_scan(sum, red, &total);
@@ -474,13 +567,13 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs 
 
 struct SampleLayout {
     int chunks, seg_len;
-    size_t tops, hist, totals, sums, counts, list, total;            // byte offsets; for `rows` rows
+    size_t tops, groups, hist, sums, counts, list, total;            // byte offsets; for `rows` rows
 };
 SampleLayout layout_of(int rows, int vocab)
 {
     SampleLayout L{};
-    // about a workgroup per CU, and chunks that are worth one
-    L.chunks = std::max(1, std::min({kMaxChunks, device_info().num_cus / rows, (vocab + kMinChunk - 1) / kMinChunk}));
+    // chunks that are worth a workgroup, two workgroups per CU at most
+    L.chunks = std::max(1, std::min({kMaxChunks, 2 * device_info().num_cus / rows, (vocab + kMinChunk - 1) / kMinChunk}));
     L.seg_len = ((vocab + L.chunks * kWaves - 1) / (L.chunks * kWaves) + 63) / 64 * 64;
     size_t off = 0;
     auto take = [&](size_t b) {
@@ -490,16 +583,16 @@ SampleLayout layout_of(int rows, int vocab)
     };
     const size_t n = rows, segs = (size_t)L.chunks * kWaves;
     L.tops = take(n * L.chunks * 8);
+    L.groups = take(n * L.chunks * kGroups * 4);
     L.hist = take(n * L.chunks * kBins * 8);
-    L.totals = take(n * 8);
     L.sums = take(n * segs * 8);
     L.counts = take(n * segs * 4);
-    L.list = take(n * segs * L.seg_len * 4);
+    L.list = take(n * segs * L.seg_len * 8);
     L.total = off;
     return L;
 }
-// rows of a launch: their lists take as much memory as their logits
-int rows_at_once(int rows, int vocab) { return (int)std::max<int64_t>(1, std::min<int64_t>({rows, 65535, ((int64_t)1 << 26) / vocab})); }
+// rows of a launch: their lists take twice the memory of their logits
+int rows_at_once(int rows, int vocab) { return (int)std::max<int64_t>(1, std::min<int64_t>({rows, 65535, ((int64_t)1 << 25) / vocab})); }
 
 }  // namespace
 
@@ -528,19 +621,15 @@ bool launch_sample(const float* logits, int64_t ld, int rows, int vocab, const f
         a.probabilities = probabilities ? probabilities + r0 : nullptr;
         a.tops = reinterpret_cast<uint64_t*>(base + L.tops);
         a.hist = reinterpret_cast<uint64_t*>(base + L.hist);
-        a.totals = reinterpret_cast<uint64_t*>(base + L.totals);
+        a.groups = reinterpret_cast<uint32_t*>(base + L.groups);
         a.sums = reinterpret_cast<uint64_t*>(base + L.sums);
         a.counts = reinterpret_cast<uint32_t*>(base + L.counts);
-        a.list = reinterpret_cast<uint32_t*>(base + L.list);
+        a.list = reinterpret_cast<uint64_t*>(base + L.list);
         const dim3 grid(L.chunks, n), block(kThreads);
         hipLaunchKernelGGL(sample_top_kernel, grid, block, 0, stream, a);
         if (!hip_ok(hipGetLastError(), "sample launch")) return false;
         hipLaunchKernelGGL(sample_sums_kernel, grid, block, 0, stream, a);
         if (!hip_ok(hipGetLastError(), "sample launch")) return false;
-        if (top_k || top_p) {
-            hipLaunchKernelGGL(sample_list_kernel, grid, block, 0, stream, a);
-            if (!hip_ok(hipGetLastError(), "sample launch")) return false;
-        }
         hipLaunchKernelGGL(sample_draw_kernel, dim3(n), block, 0, stream, a);
         if (!hip_ok(hipGetLastError(), "sample launch")) return false;
     }
