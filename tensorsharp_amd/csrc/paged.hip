@@ -219,7 +219,7 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 //
 // Sequences with at most 32 rows (answers): all wavefronts have the same rows and walk over different keys, each through LDS of its
 // own, and meet at the end.  Others (prompts): tiles of 128 rows, each wavefront has 32 of them and all share the keys in LDS.
-// With few tiles the keys are cut further over workgroups (splits), whose states paged_combine_kernel joins.
+// With few tiles the keys are cut further over workgroups, whose states paged_combine_kernel joins.
 
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
@@ -245,86 +245,185 @@ struct AttnArgs {
     const float* query;
     float* out;
     const float* sinks;
-    float* partial;              // [row][head][split][head_dim] weighted values, then [row][head][split] (maximum, sum)
+    float* partial;              // [piece][KV head][row of the tile][head_dim] weighted values, then [piece][KV head][row] (maximum, sum)
     int64_t ld_query, ld_out;
     float c;                     // |scale| log2 e
     float sign;                  // of scale, 0 where it is 0
-    int rows, heads, group, window, splits, min_keys;
+    int rows, heads, group, window;
+    int pieces;                  // per KV head that the chip takes at once; 0: keys are not cut
+    int slots, slot_rows;        // of partial
     FastDiv by_group;
     PagedKv cache;
 };
 
 // A tile: rows row0 .. row0 + count - 1 of the rows of a sequence, whose new tokens are rows first .. of the batch and begin at
-// position p0; and its keys.
+// position p0; and the keys that it has, or the piece of them that a workgroup takes.
 struct AttnTile {
     int first, tokens, p0, row0, count;
     int seq;
     int lo, hi;
+    int cuts, slot;              // pieces of its keys; where the first one's (this one's) state goes
 };
 __device__ __forceinline__ int tiles_of(int rows) { return rows <= kKeyRows ? (rows > 0 ? 1 : 0) : (rows + kTileRows - 1) / kTileRows; }
-__device__ __forceinline__ void keys_of(const AttnArgs& A, AttnTile& t)
+__device__ __forceinline__ int clamped(int v, int hi) { return max(0, min(v, hi)); }
+// inclusive sum over the lanes of a wavefront, in registers
+__device__ __forceinline__ int lane_scan(int v)
 {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);          // from the lane 1, 2, 4, 8 below, within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);         // the last lane of 16 to the next 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);         // of 32 to the upper 32
+    return v;
+}
+__device__ __forceinline__ int lane_sum(int v) { return __builtin_amdgcn_readlane(lane_scan(v), 63); }
+
+// 64 sequences, one per lane
+struct Lanes {
+    int start, n, context;
+    int tiles, steps;            // steps of 128 keys that a tile has at most
+    __device__ __forceinline__ void load(const AttnArgs& A, int s0)
+    {
+        const int s = s0 + (threadIdx.x & 63);
+        start = n = context = 0;
+        if (s < A.cache.seqs) {
+            start = clamped(A.cache.row_starts[s], A.rows);
+            n = max(0, clamped(A.cache.row_starts[s + 1], A.rows) - start);
+            context = A.cache.context_lens[s];
+        }
+        tiles = tiles_of(n * A.group);
+        const int in_tile = min(n, tiles == 1 ? n : kTileRows / A.group + 2);
+        int span = (int)min((int64_t)max(0, context), (int64_t)A.cache.max_pages * A.cache.page.d);
+        if (A.window > 0) span = (int)min((int64_t)span, (int64_t)A.window + in_tile);
+        steps = (span + 127) >> 7;
+    }
+    __device__ __forceinline__ int cuts(int len) const { return max(1, (steps + len - 1) / len); }
+};
+
+// How many steps of 128 keys a piece has, so that the pieces of all tiles are about as many as the chip takes at once and as long as one
+// another (more would wait for a second round, fewer or unequal ones leave compute units without work).  At least their mean, in
+// a few tries up to what is certain to be enough.  32 sequences of 4096 keys and 8 KV heads: 104 us in 512 pieces, 107 in 1024, 136 in 4096.
+__device__ __forceinline__ int piece_steps(const AttnArgs& A, Lanes& L)
+{
+    constexpr int kUncut = 1 << 24;
+    L.load(A, 0);
+    if (A.pieces == 0) return kUncut;
+    int tiles = 0;
+    float steps = 0.f;
+    for (int s0 = 0;;) {
+        tiles += lane_sum(L.tiles);
+        steps += (float)lane_sum(min(L.tiles * min(L.steps, 1 << 16), 1 << 24));
+        s0 += 64;
+        if (s0 >= A.cache.seqs) break;
+        L.load(A, s0);
+    }
+    if (tiles >= A.pieces) {
+        if (A.cache.seqs > 64) L.load(A, 0);
+        return kUncut;
+    }
+    const float mean = steps / (float)A.pieces, enough = fmaxf(steps / (float)(A.pieces - tiles), mean);
+    int len = 0;
+    bool worth = false;
+    float f = 1.f;
+    for (int i = 0;; ++i, f *= 1.15f) {
+        // (a length that no tile exceeds ends it in any case)
+        len = i < 5 ? max(1, (int)ceilf(fminf(mean * f, enough))) : i == 5 ? max(1, (int)ceilf(enough)) : len + len / 8 + 1;
+        int all = 0;
+        worth = false;
+        for (int s0 = 0; s0 < A.cache.seqs; s0 += 64) {
+            if (A.cache.seqs > 64) L.load(A, s0);
+            all += lane_sum(L.tiles * L.cuts(len));
+            worth |= __any(L.steps - len >= (L.n * A.group > kKeyRows ? 2 : tiles * A.cache.kv_heads >= 64 ? 7 : 4));
+        }
+        if (all <= A.pieces) break;
+    }
+    // Joining the pieces takes 5 us, a step of a short tile 1.5 us (more where many are under way) and one of a long tile 4 us.
+    if (!worth) len = kUncut;
+    if (A.cache.seqs > 64) L.load(A, 0);
+    return len;
+}
+
+// rows and keys of tile number `tile` of the sequence of lane `at`
+__device__ __forceinline__ void set_tile(const AttnArgs& A, const Lanes& L, int s0, int at, int tile, int len, AttnTile& t)
+{
+    t.seq = s0 + at;
+    t.first = __builtin_amdgcn_readlane(L.start, at);
+    t.tokens = __builtin_amdgcn_readlane(L.n, at);
+    t.p0 = __builtin_amdgcn_readlane(L.context, at) - t.tokens;
+    t.cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
+    const int rows = t.tokens * A.group;
+    t.row0 = tile * kTileRows;
+    t.count = min(rows - t.row0, rows <= kKeyRows ? kKeyRows : kTileRows);
     const int p_first = t.p0 + (int)A.by_group.quot(t.row0), p_last = t.p0 + (int)A.by_group.quot(t.row0 + t.count - 1);
     t.lo = A.window > 0 ? max(0, p_first - A.window + 1) : 0;
     t.hi = (int)min((int64_t)p_last + 1, (int64_t)A.cache.max_pages * A.cache.page.d);
 }
-// keys of a split, a multiple of 128 (a step of four wavefronts), and from it how many splits there are
-__device__ __forceinline__ int split_keys(const AttnArgs& A, const AttnTile& t)
+// keys of each piece of a tile, whole steps of 128
+__device__ __forceinline__ int piece_keys(const AttnTile& t) { return ((max(0, t.hi - t.lo) + 127) / 128 + t.cuts - 1) / t.cuts * 128; }
+
+__device__ __forceinline__ int64_t slot_row(const AttnArgs& A, int slot, int kvh, int row) { return ((int64_t)slot * A.cache.kv_heads + kvh) * A.slot_rows + row; }
+__device__ __forceinline__ f2_t* states_of(const AttnArgs& A)
 {
-    const int span = t.hi - t.lo;
-    const int wanted = max(1, min(A.splits, (span + A.min_keys - 1) / A.min_keys));
-    return ((span + wanted - 1) / wanted + 127) / 128 * 128;
+    return reinterpret_cast<f2_t*>(A.partial + (int64_t)A.slots * A.cache.kv_heads * A.slot_rows * A.cache.head_dim);
 }
-__device__ __forceinline__ int clamped(int v, int hi) { return max(0, min(v, hi)); }
-// The idx-th tile from the end (the last tiles of a prompt have the most keys and go first); every wavefront looks for itself.
-__device__ __forceinline__ bool find_tile(const AttnArgs& A, int idx, AttnTile& t)
+// behind the states: piece_steps, from the attention for the kernel that joins
+__device__ __forceinline__ int* steps_of(const AttnArgs& A) { return reinterpret_cast<int*>(states_of(A) + (int64_t)A.slots * A.cache.kv_heads * A.slot_rows); }
+
+// The idx-th piece from the end (the last tiles of a prompt have the most keys and go first); every wavefront looks for itself.
+__device__ __forceinline__ bool find_piece(const AttnArgs& A, int idx, AttnTile& t)
 {
-    const int lane = threadIdx.x & 63;
-    int total = 0;
-    for (int s0 = 0; s0 < A.cache.seqs; s0 += 64) {
-        const int s = s0 + lane;
-        int n = 0;
-        if (s < A.cache.seqs) n = max(0, clamped(A.cache.row_starts[s + 1], A.rows) - clamped(A.cache.row_starts[s], A.rows));
-        int sum = tiles_of(n * A.group);
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        total += sum;
+    Lanes L;
+    const int len = piece_steps(A, L);
+    if (A.pieces > 0 && blockIdx.x == 0 && threadIdx.x == 0) *steps_of(A) = len;
+    int cum = lane_scan(L.tiles * L.cuts(len)), total = __builtin_amdgcn_readlane(cum, 63);
+    for (int s0 = 64; s0 < A.cache.seqs; s0 += 64) {
+        L.load(A, s0);
+        total += lane_sum(L.tiles * L.cuts(len));
     }
-    int want = total - 1 - idx;
+    int want = total - 1 - idx, s0 = 0;
     if (want < 0) return false;
-    for (int s0 = 0;; s0 += 64) {
-        const int s = s0 + lane;
-        int start = 0, n = 0;
-        if (s < A.cache.seqs) {
-            start = clamped(A.cache.row_starts[s], A.rows);
-            n = max(0, clamped(A.cache.row_starts[s + 1], A.rows) - start);
-        }
-        const int mine = tiles_of(n * A.group);
-        int cum = mine;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int below = __shfl_up(cum, o);
-            if (lane >= o) cum += below;
-        }
-        const uint64_t here = __ballot(want < cum);
-        if (here == 0) {
-            want -= __shfl(cum, 63);
-            continue;
-        }
-        const int at = __ffsll((unsigned long long)here) - 1;
-        t.seq = s0 + at;
-        t.first = __builtin_amdgcn_readlane(start, at);
-        t.tokens = __builtin_amdgcn_readlane(n, at);
-        want -= __builtin_amdgcn_readlane(cum - mine, at);
-        break;
+    t.slot = want;
+    if (A.cache.seqs > 64) L.load(A, 0);
+    while (want >= __builtin_amdgcn_readlane(cum, 63)) {             // (fewer than the total)
+        want -= __builtin_amdgcn_readlane(cum, 63);
+        s0 += 64;
+        L.load(A, s0);
+        cum = lane_scan(L.tiles * L.cuts(len));
     }
-    want = __builtin_amdgcn_readfirstlane(want);
-    const int rows = t.tokens * A.group;
-    t.row0 = want * kTileRows;
-    t.count = min(rows - t.row0, rows <= kKeyRows ? kKeyRows : kTileRows);
-    t.p0 = __builtin_amdgcn_readfirstlane(A.cache.context_lens[t.seq]) - t.tokens;
-    keys_of(A, t);
+    const int at = __ffsll((unsigned long long)__ballot(want < cum)) - 1;
+    const int cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
+    want -= __builtin_amdgcn_readlane(cum, at) - __builtin_amdgcn_readlane(L.tiles, at) * cuts;
+    set_tile(A, L, s0, at, want / cuts, len, t);
+    const int keys = piece_keys(t), begin = t.lo + want % cuts * keys;
+    t.hi = min(begin + keys, t.hi);
+    t.lo = begin;
     return true;
 }
-
+// the tile of a row and head and its first piece; false: of no sequence
+__device__ __forceinline__ bool find_row(const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)
+{
+    const int len = *steps_of(A);
+    Lanes L;
+    int before = 0;
+    for (int s0 = 0; s0 < A.cache.seqs; s0 += 64) {
+        L.load(A, s0);
+        const int cum = lane_scan(L.tiles * L.cuts(len));
+        const uint64_t has = __ballot(row >= L.start && row < L.start + L.n);
+        if (has) {
+            const int at = __ffsll((unsigned long long)has) - 1;
+            const int cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
+            const int r = (row - __builtin_amdgcn_readlane(L.start, at)) * A.group + head % A.group;
+            const int tile = __builtin_amdgcn_readlane(L.n, at) * A.group <= kKeyRows ? 0 : r / kTileRows;
+            set_tile(A, L, s0, at, tile, len, t);
+            t.slot = before + __builtin_amdgcn_readlane(cum, at) + (tile - __builtin_amdgcn_readlane(L.tiles, at)) * cuts;
+            *in_tile = r - t.row0;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(cum, 63);
+    }
+    return false;
+}
 __device__ __forceinline__ uint32_t high_halves(float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); }
 __device__ __forceinline__ float below_bf16(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 // eight floats as three times eight bf16 that sum up to them
@@ -366,7 +465,9 @@ struct Attn {
     static constexpr int kCacheParts = TYPE == 0 ? 3 : 1;
     static constexpr int kSteps = HD / 16, kDims = HD / 32;
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
-    static constexpr int kKeyWaves = TYPE == 0 ? 2 : 4;              // wavefronts that have keys of their own
+    static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU
+    static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD == 128);
+    static constexpr int kKeyWaves = TYPE != 0 || HD == 64 ? 4 : HD == 96 || HD == 192 ? 3 : 2;    // wavefronts that have keys of their own
     static constexpr int kBlock = 32 * kRow;                         // bytes of 32 keys
     static constexpr int kCopies = kPieces / 2;                      // wavefront-wide copies of 32 keys
     static constexpr int kLds = kBlock * 2 * (2 * NT > kKeyWaves ? 2 * NT : kKeyWaves);
@@ -459,14 +560,25 @@ struct Attn {
                 cut3(x, part);
             }
 #pragma unroll
-            for (int i = 0; i < kParts; ++i) q[i][s] = part[i];
+            for (int i = 0; i < kParts; ++i) {
+                q[i][s] = part[i];
+                // (large heads: what the accumulators leave of the accumulation registers holds rows, which the matrix instruction reads there
+                // as well; left to itself the compiler spills to memory, whose loads would wait for the copies under way)
+                if (kOneWave && kDims * 16 + (i + 1) * kSteps * 4 <= 256) asm volatile("" : "+a"(q[i][s]));
+            }
         }
+        no_rows();
+    }
+    // nothing seen yet
+    __device__ __forceinline__ void no_rows()
+    {
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
         m = -INFINITY;
         l = 0.f;
+        stay();
     }
 
     // ---- keys and values into LDS ----
@@ -497,11 +609,18 @@ struct Attn {
         const int64_t v = (int64_t)(uintptr_t)A.cache.v + (id * A.cache.v_page + within * A.cache.v_token + kvh * A.cache.v_head) * kElem;
         return {(uint64_t)(ok ? k : zero), (uint64_t)(ok ? v : zero), __ballot(ok)};
     }
+    // the lane's number, for the copies of one step: where registers are short, their places are worked out at every step
+    __device__ __forceinline__ int lane_here() const
+    {
+        int ln = lane;
+        if constexpr (kTight) asm volatile("" : "+v"(ln));
+        return ln;
+    }
     // copy n of a block: 64 pieces that follow one another in LDS
     template <bool V>
-    __device__ __forceinline__ void copy(uint64_t rows, int n, lds_t block) const
+    __device__ __forceinline__ void copy(uint64_t rows, int n, lds_t block, int ln) const
     {
-        const int slot = n * 64 + lane, row = slot / kPieces, piece = (slot - row * kPieces) ^ (V ? v_swizzle(row) : k_swizzle(row));
+        const int slot = n * 64 + ln, row = slot / kPieces, piece = (slot - row * kPieces) ^ (V ? v_swizzle(row) : k_swizzle(row));
         uint64_t at = (uint64_t)__shfl((unsigned long long)rows, row);
         if (piece * 16 >= A.cache.head_dim * kElem) at = (uint64_t)(uintptr_t)g_zero_row;
         at += piece * 16;
@@ -588,6 +707,15 @@ struct Attn {
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
             m = mn;
         }
+        stay();
+    }
+    // large heads: the accumulators stay in accumulation registers from one step to the next
+    __device__ __forceinline__ void stay()
+    {
+        if constexpr (kOneWave) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) asm volatile("" : "+a"(o[d]));
+        }
     }
     // weights of a block's scores, their sum, and O^T += V^T P^T
     __device__ __forceinline__ void weigh(const f16_t& s, lds_t block)
@@ -639,15 +767,8 @@ struct Attn {
     }
 
     // ---- where a row's state goes ----
-    __device__ __forceinline__ float* values_of(int token, int head, int split) const
-    {
-        return A.partial + (((int64_t)(t.first + token) * A.heads + head) * A.splits + split) * A.cache.head_dim;
-    }
-    __device__ __forceinline__ f2_t* state_of(int token, int head, int split) const
-    {
-        return reinterpret_cast<f2_t*>(A.partial + (int64_t)A.rows * A.heads * A.splits * A.cache.head_dim) +
-               (((int64_t)(t.first + token) * A.heads + head) * A.splits + split);
-    }
+    __device__ __forceinline__ float* values_of(int row) const { return A.partial + slot_row(A, t.slot, kvh, row) * A.cache.head_dim; }
+    __device__ __forceinline__ f2_t* state_of(int row) const { return states_of(A) + slot_row(A, t.slot, kvh, row); }
     // what a row's sum is divided by: with the sink, 1 / 0 never
     __device__ __forceinline__ float over_sum(float sum, float top, int head) const
     {
@@ -657,21 +778,22 @@ struct Attn {
     }
 
     // all wavefronts over the same keys, 32 rows each
-    __device__ __forceinline__ void shared_keys(int begin, int end, int split)
+    __device__ __forceinline__ void shared_keys()
     {
+        const int begin = t.lo, end = t.hi;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        load_rows(32 * wave + col);
         const int p_first = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave, t.count - 1));
         const int p_last = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave + 31, t.count - 1));
         const int lo_last = A.window > 0 ? p_last - A.window + 1 : 0;
         constexpr int kKeys = 32 * NT;
         const int mine = lane & (kKeys - 1);
         auto stage = [&](const Rows& r, lds_t buffer) {
+            const int ln = lane_here();
 #pragma unroll
             for (int n = 0; n < (NT * kCopies + kAttnWaves - 1) / kAttnWaves; ++n)
                 if (NT * kCopies % kAttnWaves == 0 || wave + kAttnWaves * n < NT * kCopies) {
-                    copy<false>(r.k, wave + kAttnWaves * n, buffer);
-                    copy<true>(r.v, wave + kAttnWaves * n, buffer + NT * kBlock);
+                    copy<false>(r.k, wave + kAttnWaves * n, buffer, ln);
+                    copy<true>(r.v, wave + kAttnWaves * n, buffer + NT * kBlock, ln);
                 }
         };
         int buffer = 0;
@@ -679,6 +801,7 @@ struct Attn {
             // copies go a step ahead; those behind the last key bring zeros that nothing reads
             Rows rows = rows_of(begin + mine, page_id<kKeys>(begin, begin + mine, end));
             stage(rows, lds);
+            load_rows(32 * wave + col);                              // (while the first keys are on their way)
             for (int key0 = begin; key0 < end; key0 += kKeys) {
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 const lds_t here = lds + buffer * (2 * NT * kBlock);
@@ -701,6 +824,8 @@ struct Attn {
                 }
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the last copies, before this LDS may be another workgroup's
+        } else {
+            no_rows();
         }
         const int row = 32 * wave + col;
         l = both_halves(l, added);
@@ -709,12 +834,12 @@ struct Attn {
         place(row, &token, &head);
         float* dst;
         float by = 1.f;
-        if (A.splits == 1) {
+        if (t.cuts == 1) {
             dst = A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim;
             by = over_sum(l, m, head);
         } else {
-            dst = values_of(token, head, split);
-            if (half == 0) *state_of(token, head, split) = f2_t{m, l};
+            dst = values_of(row);
+            if (half == 0) *state_of(row) = f2_t{m, l};
         }
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
@@ -727,11 +852,11 @@ struct Attn {
     }
 
     // every wavefront over keys of its own, the same (up to 32) rows
-    __device__ __forceinline__ void own_keys(int begin, int end, int split)
+    __device__ __forceinline__ void own_keys()
     {
+        const int begin = t.lo, end = t.hi;
         __shared__ f2_t states[kAttnWaves][32];
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        load_rows(col);
         const int p_last = t.p0 + t.tokens - 1;
         const int lo_last = A.window > 0 ? p_last - A.window + 1 : 0;
         const lds_t kb = lds + wave * 2 * kBlock, vb = kb + kBlock;
@@ -739,12 +864,14 @@ struct Attn {
         constexpr int kStride = 32 * kKeyWaves;
         if (wave < kKeyWaves && key0 < end) {
             auto stage = [&](auto is_v, uint64_t rows, lds_t block) {
+                const int ln = lane_here();
 #pragma unroll
-                for (int n = 0; n < kCopies; ++n) copy<decltype(is_v)::value>(rows, n, block);
+                for (int n = 0; n < kCopies; ++n) copy<decltype(is_v)::value>(rows, n, block, ln);
             };
             Rows rows = rows_of(key0 + col, page_id<32>(key0, key0 + col, end));
             stage(std::false_type(), rows.k, kb);
             stage(std::true_type(), rows.v, vb);
+            load_rows(col);                                          // (while the first keys are on their way)
             for (; key0 < end; key0 += kStride) {
                 // loads answer in order: with kCopies of them left, the values behind the keys, the keys have arrived
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");
@@ -760,6 +887,9 @@ struct Attn {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::true_type(), rows.v, vb);
             }
+        }
+        else {
+            no_rows();
         }
         l = both_halves(l, added);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -791,71 +921,93 @@ struct Attn {
             }
             int token, head;
             place(row, &token, &head);
-            if (A.splits == 1) {
+            if (t.cuts == 1) {
                 *reinterpret_cast<f4_t*>(A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim + 4 * piece) =
                     v * over_sum(sum, top, head);
             } else {
-                *reinterpret_cast<f4_t*>(values_of(token, head, split) + 4 * piece) = v;
-                if (piece == 0) *state_of(token, head, split) = f2_t{top, sum};
+                *reinterpret_cast<f4_t*>(values_of(row) + 4 * piece) = v;
+                if (piece == 0) *state_of(row) = f2_t{top, sum};
             }
         }
     }
 };
 
-// grid (KV heads x tiles, splits)
+// grid: KV heads x pieces
 template <int TYPE, int HD>
-__global__ void __launch_bounds__(kAttnThreads, HD <= 128 ? 2 : 1) paged_attention_kernel(const AttnArgs A)
+__global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 2)) paged_attention_kernel(const AttnArgs A)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    const int kvh = blockIdx.x % A.cache.kv_heads, idx = blockIdx.x / A.cache.kv_heads, split = blockIdx.y;
+    const int kvh = blockIdx.x % A.cache.kv_heads, idx = blockIdx.x / A.cache.kv_heads;
     AttnTile t;
-    if (!find_tile(A, idx, t)) return;
-    const int len = split_keys(A, t), begin = t.lo + split * len, end = min(begin + len, t.hi);
-    if (begin >= end && (split > 0 || A.splits > 1)) return;         // (rows that see nothing are set to zero by the first split, or when splits are joined)
+    if (!find_piece(A, idx, t)) return;
     Attn<TYPE, HD> a(A, t, kvh, (lds_t)smem);
-    if (t.tokens * A.group <= kKeyRows) a.own_keys(begin, end, split);
-    else a.shared_keys(begin, end, split);
+    if (t.tokens * A.group <= kKeyRows) a.own_keys();
+    else a.shared_keys();
 }
 
-// one wavefront per (row, head): the splits of its tile
+// The pieces of a row's tile, for one head: WAVES wavefronts (one where there are many rows; four share the pieces of few).
+template <int WAVES>
 __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(const AttnArgs A)
 {
-    const int lane = threadIdx.x & 63, row = blockIdx.x, head = blockIdx.y * kAttnWaves + (threadIdx.x >> 6), dim = A.cache.head_dim;
-    const Place at = place_of_row(A.cache, row);
-    if (at.seq < 0 || head >= A.heads) return;
+    __shared__ f2_t sums[kAttnWaves];
+    __shared__ f4_t values_in[kAttnWaves][kMaxDim / 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x, dim = A.cache.head_dim;
+    const int head = WAVES == 1 ? blockIdx.y * kAttnWaves + wave : blockIdx.y;
     AttnTile t;
-    const int start = clamped(at.first, A.rows);
-    t.first = start;
-    t.tokens = clamped(at.first + at.count, A.rows) - start;
-    t.seq = at.seq;
-    t.p0 = A.cache.context_lens[at.seq] - t.tokens;
-    const int r = (row - start) * A.group + head % A.group, rows = t.tokens * A.group;
-    t.row0 = rows <= kKeyRows ? 0 : r / kTileRows * kTileRows;
-    t.count = min(rows - t.row0, rows <= kKeyRows ? kKeyRows : kTileRows);
-    keys_of(A, t);
-    const int span = t.hi - t.lo, len = split_keys(A, t), splits = span > 0 ? (span + len - 1) / len : 0;
-    const int64_t first = ((int64_t)row * A.heads + head) * A.splits;
+    int in_tile;
+    if (head >= A.heads || !find_row(A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all wavefronts of a head)
+    const int cuts = t.cuts;
+    const int64_t first = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
     const float* values = A.partial + first * dim;
-    const f2_t* states = reinterpret_cast<const f2_t*>(A.partial + (int64_t)A.rows * A.heads * A.splits * dim) + first;
-    float top = -INFINITY;
-    for (int s = lane; s < splits; s += 64) top = fmaxf(top, states[s].x);
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    const f2_t* states = states_of(A) + first;
+    // a head takes 16, 32 or 64 lanes; as many pieces as that leaves room for are read at a time
+    const int wide = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, d = 4 * (lane & (wide - 1)), parts = 64 / wide;
+    const int part = lane / wide + (WAVES == 1 ? 0 : wave * parts);
+    const bool mine = d < dim;
+    constexpr int U = 4;
     f4_t acc = {0.f, 0.f, 0.f, 0.f};
-    const bool mine = 4 * lane < dim;
-    for (int s = 0; s < splits; ++s) {
-        const f2_t st = states[s];
-        const float f = __builtin_amdgcn_exp2f(st.x - base);
-        sum += st.y * f;
-        if (mine) acc += *reinterpret_cast<const f4_t*>(values + (int64_t)s * dim + 4 * lane) * f;
+    float top = -INFINITY, sum = 0.f;
+    auto join = [&](float t, float w, const f4_t& v) {
+        const float m = fmaxf(top, t), base = m == -INFINITY ? 0.f : m;
+        const float f = __builtin_amdgcn_exp2f(top - base), g = __builtin_amdgcn_exp2f(t - base);
+        sum = sum * f + w * g;
+        acc = acc * f + v * g;
+        top = m;
+    };
+    for (int s0 = part; s0 < cuts; s0 += U * WAVES * parts) {
+        f2_t st[U];
+        f4_t v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = min(s0 + u * WAVES * parts, cuts - 1);
+            st[u] = states[s * next];
+            v[u] = mine ? *reinterpret_cast<const f4_t*>(values + s * next * dim + d) : f4_t{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u * WAVES * parts < cuts) join(st[u].x, st[u].y, v[u]);
+    }
+    for (int o = wide; o < 64; o <<= 1) {
+        const float t = __shfl_xor(top, o), w = __shfl_xor(sum, o);
+        f4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __shfl_xor(acc[i], o);
+        join(t, w, v);
+    }
+    if constexpr (WAVES > 1) {
+        if (lane == 0) sums[wave] = f2_t{top, sum};
+        if (lane < wide) values_in[wave][lane] = acc;
+        __syncthreads();
+        if (wave > 0 || lane >= wide) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) join(sums[w].x, sums[w].y, values_in[w][lane]);
     }
     float by = 0.f;
     if (sum > 0.f) {
-        if (A.sinks) sum += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2e - base + kBias);
+        if (A.sinks) sum += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2e - top + kBias);
         by = 1.0f / sum;
     }
-    if (mine) *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + 4 * lane) = acc * by;
+    if (mine && lane < wide) *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * by;
 }
 
 }  // namespace
@@ -906,18 +1058,21 @@ bool launch_rope_store(const float* qkv, int64_t ld_qkv, float* query, int64_t l
 
 PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window)
 {
-    const int group = heads / cache.kv_heads;
+    const int group = heads / cache.kv_heads, dim = cache.head_dim;
     const int64_t all = (int64_t)rows * group;
     PagedAttnPlan plan{};
     // (a sequence of at most 32 rows has one tile, others a tile per 128 rows begun: no more than this, whatever the lengths)
-    plan.tiles = (int)(all / kTileRows + std::min<int64_t>(cache.seqs, rows));
-    const int64_t items = (int64_t)plan.tiles * cache.kv_heads, keys = (int64_t)cache.max_pages * cache.page.d;
-    const bool few = all <= (int64_t)kKeyRows * cache.seqs;          // mostly answers
-    plan.min_keys = few ? 256 : 512;
-    const int64_t span = window > 0 ? std::min<int64_t>(keys, (int64_t)window + (few ? kKeyRows : kTileRows)) : keys;
-    const int64_t wanted = few ? 2048 / items : items >= 384 ? 1 : 768 / items;
-    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (span + plan.min_keys - 1) / plan.min_keys, 1024}));
-    if (plan.splits > 1) plan.ws_bytes = (size_t)rows * heads * plan.splits * (cache.head_dim + 2) * sizeof(float);
+    const int64_t tiles = all / kTileRows + std::min<int64_t>(cache.seqs, rows);
+    // workgroups that are resident at once
+    const int at_once = device_info().num_cus * (dim <= 64 && cache.element_type != kTypeF32 ? 3 : dim <= 128 ? 2 : 1);
+    const int64_t pieces = std::max(1, at_once / cache.kv_heads), keys = (int64_t)cache.max_pages * cache.page.d;
+    const int64_t most = std::min<int64_t>(keys, window > 0 ? window : keys);
+    const bool cut = (all + kTileRows - 1) / kTileRows < pieces && most > (all <= (int64_t)kKeyRows * cache.seqs ? 512 : 256);
+    plan.pieces = cut ? (int)pieces : 0;
+    plan.slots = (int)std::min<int64_t>(INT32_MAX, cut ? std::max(tiles, pieces) : tiles);
+    plan.slot_rows = all <= kKeyRows ? kKeyRows : kTileRows;
+    // (a tile that is cut is one of at most `pieces` pieces)
+    if (cut) plan.ws_bytes = (size_t)pieces * cache.kv_heads * plan.slot_rows * (dim + 2) * sizeof(float) + sizeof(int);
     return plan;
 }
 
@@ -957,23 +1112,27 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     args.heads = heads;
     args.group = heads / cache.kv_heads;
     args.window = window;
-    args.splits = plan.splits;
-    args.min_keys = plan.min_keys;
+    args.pieces = plan.pieces;
+    args.slots = plan.pieces;
+    args.slot_rows = plan.slot_rows;
     args.by_group = FastDiv((uint32_t)args.group);
     args.cache = cache;
-    if ((int64_t)plan.tiles * cache.kv_heads > INT32_MAX || (int64_t)rows * args.group > INT32_MAX) {
+    if ((int64_t)plan.slots * cache.kv_heads > INT32_MAX || (int64_t)rows * args.group > INT32_MAX) {
         set_last_error("paged_attention: too many rows for one call.");
         return false;
     }
-    const dim3 grid((unsigned)(plan.tiles * cache.kv_heads), plan.splits);
+    const dim3 grid((unsigned)(plan.slots * cache.kv_heads));
     bool ok;
     switch (cache.element_type) {
     case kTypeF32: ok = launch_attention<0>(args, grid, stream); break;
     case kTypeF16: ok = launch_attention<1>(args, grid, stream); break;
     default: ok = launch_attention<2>(args, grid, stream); break;
     }
-    if (!ok || plan.splits == 1) return ok;
-    hipLaunchKernelGGL(paged_combine_kernel, dim3(rows, (heads + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, args);
+    if (!ok || plan.pieces == 0) return ok;
+    if ((int64_t)rows * heads <= 8 * device_info().num_cus)
+        hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, args);
+    else
+        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(rows, (heads + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, args);
     return hip_ok(hipGetLastError(), "paged attention combine launch");
 }
 

@@ -341,10 +341,10 @@ bool launch_rope(const float* x, int64_t x_token, int64_t x_head, float* out, in
 bool launch_rope_store(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int rows, int heads, const PagedKv& cache,
                        const int32_t* positions, const float* q_norm, const float* k_norm, float eps, const RopeSpec& rope, hipStream_t stream);
 
-// How the attention of a call is cut; depends on the shapes alone.
+// How the attention of a call is cut; depends on the shapes alone (where the cuts are, the kernels find out from the lengths).
 struct PagedAttnPlan {
-    int tiles;                 // at most, over all sequences
-    int splits, min_keys;      // workgroups that share a tile's keys at most, and how many keys each has at least
+    int pieces;                // per KV head that the keys are cut into, 0: not cut
+    int slots, slot_rows;      // pieces there can be, rows of each
     size_t ws_bytes;
 };
 PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window);

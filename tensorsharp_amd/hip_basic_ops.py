@@ -275,23 +275,40 @@ def _device_view(t):
     return N.TensorView2D(t.data_ptr(), rows, cols, s0, 1, ((rows - 1) * s0 + cols) * 4)
 
 
-def _vector(t, dtype, count, name, like):
-    """address of a contiguous device vector of `count` values (None stays None)"""
+def _vector(t, dtype, count, name, device):
+    """address of a contiguous vector of `count` values on that device (its index); None stays None"""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() != count or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {str(dtype).split('.')[-1]} tensor of {count} values.")
-    if t.device != like.device:
+    if t.get_device() != device:
         raise ValueError(f"{name} is not on the device of the other tensors.")
     return t.data_ptr()
 
 
-def _use_stream_of(t):
-    """Launches go to the current stream, which is one of the current device: a tensor of another one has no stream here."""
+def _use_stream_of(device):
+    """Launches go to the current stream, which is one of the current device: tensors of another one have no stream here."""
     torch = _torch()
-    if t.get_device() != torch.cuda.current_device():
+    try:                                        # (see UseCurrentStream)
+        current = torch._C._cuda_getDevice()
+        handle = torch._C._cuda_getCurrentRawStream(current)
+    except AttributeError:
+        current = torch.cuda.current_device()
+        handle = torch.cuda.current_stream().cuda_stream
+    if device != current:
         raise ValueError("the tensors must be on the current device.")
-    HipBasicOps.UseCurrentStream()
+    N.lib().TSHip_SetStream(handle)
+
+
+def _device_view3(t, name):
+    torch = _torch()
+    if t.dim() != 3 or t.dtype is not torch.float32:
+        raise ValueError(f"{name} requires 3D Float32 tensors.")
+    if not t.is_cuda:
+        raise ValueError(f"{name} requires tensors in GPU memory of one device.")
+    d0, d1, d2 = t.shape
+    s0, s1, s2 = t.stride()
+    return N.TensorView3D(t.data_ptr(), d0, d1, d2, s0, s1, s2, ((d0 - 1) * s0 + (d1 - 1) * s1 + (d2 - 1) * s2 + 1) * 4)
 
 
 class RotaryPositions:
@@ -308,7 +325,7 @@ class RotaryPositions:
             torch = _torch()
             if not freq_factors.is_cuda:
                 raise ValueError("freq_factors must be in GPU memory.")
-            address = _vector(freq_factors, torch.float32, int(dims) // 2, "freq_factors", freq_factors)
+            address = _vector(freq_factors, torch.float32, int(dims) // 2, "freq_factors", freq_factors.get_device())
         self._keepalive = freq_factors
         self.native = N.Rope(int(dims), int(mode), float(base), float(freq_scale), float(ext_factor), float(attn_factor), float(beta_fast),
                              float(beta_slow), int(original_context), address)
@@ -340,11 +357,11 @@ class PagedKVCache:
         self.native = N.PagedCache(k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[2], k.shape[3], k.shape[1], k.shape[0], *k.stride()[:3],
                                    *v.stride()[:3], page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1])
         self.ref = C.byref(self.native)
+        self.device = k.get_device()
 
-    def _sequences(self, row_starts, context_lens):
-        torch = _torch()
-        return (_vector(row_starts, torch.int32, self.num_seqs + 1, "row_starts", self.k),
-                _vector(context_lens, torch.int32, self.num_seqs, "context_lens", self.k))
+    def _sequences(self, row_starts, context_lens, i32):
+        return (_vector(row_starts, i32, self.num_seqs + 1, "row_starts", self.device),
+                _vector(context_lens, i32, self.num_seqs, "context_lens", self.device))
 
 
 class HipBasicOps:
@@ -759,14 +776,13 @@ class HipBasicOps:
     def RoPE(result, input, positions, rope):
         """result[t, h] = input[t, h] turned by positions[t]: [tokens, heads, head_dim] float32 device tensors (result may be input), positions
         int32 [tokens], rope a RotaryPositions."""
-        torch = _torch()
-        if result.dim() != 3 or input.dim() != 3 or result.dtype != torch.float32 or input.dtype != torch.float32:
-            raise ValueError("RoPE requires 3D Float32 tensors.")
-        if not input.is_cuda or result.device != input.device:
+        rv, iv = _device_view3(result, "RoPE"), _device_view3(input, "RoPE")
+        device = input.get_device()
+        if result.get_device() != device:
             raise ValueError("RoPE requires tensors in GPU memory of one device.")
-        pos = _vector(positions, torch.int32, input.shape[0], "positions", input)
-        _use_stream_of(input)
-        ok = N.lib().TSHip_RoPEF32Device(HipBasicOps._view3(result), HipBasicOps._view3(input), pos, rope.ref)
+        pos = _vector(positions, _torch().int32, iv.dim0, "positions", device)
+        _use_stream_of(device)
+        ok = N.lib().TSHip_RoPEF32Device(rv, iv, pos, rope.ref)
         N.check_result(ok, "rope")
 
     @staticmethod
@@ -776,15 +792,16 @@ class HipBasicOps:
         [head_dim], None: not) and turned by their position in the sequence (or positions[row]); q goes to query [rows, heads
         head_dim], k and v into the cache."""
         torch = _torch()
+        f32, i32 = torch.float32, torch.int32
         qv, xv = _device_view(query), _device_view(qkv)
-        dim = cache.head_dim
-        starts, lens = cache._sequences(row_starts, context_lens)
-        pos = _vector(positions, torch.int32, qkv.shape[0], "positions", cache.k)
-        qn, kn = _vector(q_norm, torch.float32, dim, "q_norm", cache.k), _vector(k_norm, torch.float32, dim, "k_norm", cache.k)
-        if query.device != cache.k.device or qkv.device != cache.k.device:
+        dim, device = cache.head_dim, cache.device
+        starts, lens = cache._sequences(row_starts, context_lens, i32)
+        pos = _vector(positions, i32, xv.dim0, "positions", device)
+        qn, kn = _vector(q_norm, f32, dim, "q_norm", device), _vector(k_norm, f32, dim, "k_norm", device)
+        if query.get_device() != device or qkv.get_device() != device:
             raise ValueError("query and qkv must be on the device of the cache.")
-        _use_stream_of(qkv)
-        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, query.shape[1] // dim, cache.ref, starts, lens, pos, qn, kn, eps, rope.ref)
+        _use_stream_of(device)
+        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, qv.dim1 // dim, cache.ref, starts, lens, pos, qn, kn, eps, rope.ref)
         N.check_result(ok, "rope_store_paged")
 
     @staticmethod
@@ -792,13 +809,14 @@ class HipBasicOps:
         """Attention of the sequences' new tokens (rows as in RoPEStorePaged) over a PagedKVCache that holds their keys and values already:
         each sees the positions up to its own, the last `window` of them (0: all).  query and result [rows, heads head_dim]
         float32 (may be one tensor); sinks [heads] float32: logits that take part in the softmax and carry no value."""
+        torch = _torch()
         rv, qv = _device_view(result), _device_view(query)
-        heads = query.shape[1] // cache.head_dim
-        starts, lens = cache._sequences(row_starts, context_lens)
-        extra = _vector(sinks, _torch().float32, heads, "sinks", cache.k)
-        if query.device != cache.k.device or result.device != cache.k.device:
+        heads, device = qv.dim1 // cache.head_dim, cache.device
+        starts, lens = cache._sequences(row_starts, context_lens, torch.int32)
+        extra = _vector(sinks, torch.float32, heads, "sinks", device)
+        if query.get_device() != device or result.get_device() != device:
             raise ValueError("query and result must be on the device of the cache.")
-        _use_stream_of(query)
+        _use_stream_of(device)
         ok = N.lib().TSHip_PagedAttentionF32Device(rv, qv, heads, cache.ref, starts, lens, scale, window, extra)
         N.check_result(ok, "paged_attention")
 
@@ -810,15 +828,15 @@ class HipBasicOps:
         [rows] float32: of the tokens drawn."""
         torch = _torch()
         lv = _device_view(logits)
-        rows = logits.shape[0]
+        rows, device = lv.dim0, logits.get_device()
         f32, i32 = torch.float32, torch.int32
         if tokens is None or uniforms is None or temperature is None:
             raise ValueError("SampleTokens requires tokens, uniforms and temperature.")
-        args = [_vector(uniforms, f32, rows, "uniforms", logits), _vector(temperature, f32, rows, "temperature", logits),
-                _vector(top_k, i32, rows, "top_k", logits), _vector(top_p, f32, rows, "top_p", logits), _vector(min_p, f32, rows, "min_p", logits),
-                _vector(tokens, i32, rows, "tokens", logits), _vector(probabilities, f32, rows, "probabilities", logits)]
-        _use_stream_of(logits)
-        N.check_result(N.lib().TSHip_SampleTokensF32Device(lv, *args), "sample_tokens")
+        u, t = _vector(uniforms, f32, rows, "uniforms", device), _vector(temperature, f32, rows, "temperature", device)
+        k, p, m = _vector(top_k, i32, rows, "top_k", device), _vector(top_p, f32, rows, "top_p", device), _vector(min_p, f32, rows, "min_p", device)
+        out, probs = _vector(tokens, i32, rows, "tokens", device), _vector(probabilities, f32, rows, "probabilities", device)
+        _use_stream_of(device)
+        N.check_result(N.lib().TSHip_SampleTokensF32Device(lv, u, t, k, p, m, out, probs), "sample_tokens")
 
     # -- LinearForward twin (ModelBase.cs:875-905): allocate result, route by residency -----
     @staticmethod
