@@ -249,8 +249,7 @@ struct AttnArgs {
     int64_t ld_query, ld_out;
     float c;                     // |scale| log2 e
     float sign;                  // of scale, 0 where it is 0
-    int rows, heads, group, window;
-    int pieces;                  // per KV head that the chip takes at once; 0: keys are not cut
+    int rows, heads, group, window, capacity;
     int slots, slot_rows;        // of partial
     FastDiv by_group;
     PagedKv cache;
@@ -279,23 +278,36 @@ __device__ __forceinline__ int lane_scan(int v)
 }
 __device__ __forceinline__ int lane_sum(int v) { return __builtin_amdgcn_readlane(lane_scan(v), 63); }
 
+// What the kernels need to find their piece.  It stands in front of the other arguments: the hardware delivers the first 14 dwords in
+// registers at wave launch (a structure is read from the argument block instead), so that the lengths are asked for at once.
+struct Lens {
+    const int32_t* row_starts;
+    const int32_t* context_lens;
+    int seqs, rows, group, window;
+    int pieces;                  // per KV head that the chip takes at once; 0: keys are not cut
+    int capacity;                // positions that the page table has room for
+};
+#define TSHIP_LENS_ARGS const int32_t *row_starts, const int32_t *context_lens, int seqs, int rows, int group, int window, int pieces, int capacity
+#define TSHIP_LENS Lens{row_starts, context_lens, seqs, rows, group, window, pieces, capacity}
+
 // 64 sequences, one per lane
 struct Lanes {
     int start, n, context;
     int tiles, steps;            // steps of 128 keys that a tile has at most
-    __device__ __forceinline__ void load(const AttnArgs& A, int s0)
+    __device__ __forceinline__ void load(const Lens& H, int s0)
     {
         const int s = s0 + (threadIdx.x & 63);
         start = n = context = 0;
-        if (s < A.cache.seqs) {
-            start = clamped(A.cache.row_starts[s], A.rows);
-            n = max(0, clamped(A.cache.row_starts[s + 1], A.rows) - start);
-            context = A.cache.context_lens[s];
+        if (s < H.seqs) {
+            const int a = H.row_starts[s], b = H.row_starts[s + 1];
+            context = H.context_lens[s];
+            start = clamped(a, H.rows);
+            n = max(0, clamped(b, H.rows) - start);
         }
-        tiles = tiles_of(n * A.group);
-        const int in_tile = min(n, tiles == 1 ? n : kTileRows / A.group + 2);
-        int span = (int)min((int64_t)max(0, context), (int64_t)A.cache.max_pages * A.cache.page.d);
-        if (A.window > 0) span = (int)min((int64_t)span, (int64_t)A.window + in_tile);
+        tiles = tiles_of(n * H.group);
+        // (a tile's rows are of at most 128 tokens)
+        int span = min(max(0, context), H.capacity);
+        if (H.window > 0) span = (int)min((int64_t)span, (int64_t)H.window + min(n, kTileRows));
         steps = (span + 127) >> 7;
     }
     __device__ __forceinline__ int cuts(int len) const { return max(1, (steps + len - 1) / len); }
@@ -304,25 +316,25 @@ struct Lanes {
 // How many steps of 128 keys a piece has, so that the pieces of all tiles are about as many as the chip takes at once and as long as one
 // another (more would wait for a second round, fewer or unequal ones leave compute units without work).  At least their mean, in
 // a few tries up to what is certain to be enough.  32 sequences of 4096 keys and 8 KV heads: 104 us in 512 pieces, 107 in 1024, 136 in 4096.
-__device__ __forceinline__ int piece_steps(const AttnArgs& A, Lanes& L)
+__device__ __forceinline__ int piece_steps(const Lens& H, int kv_heads, Lanes& L)
 {
     constexpr int kUncut = 1 << 24;
-    L.load(A, 0);
-    if (A.pieces == 0) return kUncut;
+    L.load(H, 0);
+    if (H.pieces == 0) return kUncut;
     int tiles = 0;
     float steps = 0.f;
     for (int s0 = 0;;) {
         tiles += lane_sum(L.tiles);
         steps += (float)lane_sum(min(L.tiles * min(L.steps, 1 << 16), 1 << 24));
         s0 += 64;
-        if (s0 >= A.cache.seqs) break;
-        L.load(A, s0);
+        if (s0 >= H.seqs) break;
+        L.load(H, s0);
     }
-    if (tiles >= A.pieces) {
-        if (A.cache.seqs > 64) L.load(A, 0);
+    if (tiles >= H.pieces) {
+        if (H.seqs > 64) L.load(H, 0);
         return kUncut;
     }
-    const float mean = steps / (float)A.pieces, enough = fmaxf(steps / (float)(A.pieces - tiles), mean);
+    const float mean = steps / (float)H.pieces, enough = fmaxf(steps / (float)(H.pieces - tiles), mean);
     int len = 0;
     bool worth = false;
     float f = 1.f;
@@ -331,16 +343,16 @@ __device__ __forceinline__ int piece_steps(const AttnArgs& A, Lanes& L)
         len = i < 5 ? max(1, (int)ceilf(fminf(mean * f, enough))) : i == 5 ? max(1, (int)ceilf(enough)) : len + len / 8 + 1;
         int all = 0;
         worth = false;
-        for (int s0 = 0; s0 < A.cache.seqs; s0 += 64) {
-            if (A.cache.seqs > 64) L.load(A, s0);
+        for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+            if (H.seqs > 64) L.load(H, s0);
             all += lane_sum(L.tiles * L.cuts(len));
-            worth |= __any(L.steps - len >= (L.n * A.group > kKeyRows ? 2 : tiles * A.cache.kv_heads >= 64 ? 7 : 4));
+            worth |= __any(L.steps - len >= (L.n * H.group > kKeyRows ? 2 : tiles * kv_heads >= 64 ? 7 : 4));
         }
-        if (all <= A.pieces) break;
+        if (all <= H.pieces) break;
     }
     // Joining the pieces takes 5 us, a step of a short tile 1.5 us (more where many are under way) and one of a long tile 4 us.
     if (!worth) len = kUncut;
-    if (A.cache.seqs > 64) L.load(A, 0);
+    if (H.seqs > 64) L.load(H, 0);
     return len;
 }
 
@@ -357,7 +369,7 @@ __device__ __forceinline__ void set_tile(const AttnArgs& A, const Lanes& L, int 
     t.count = min(rows - t.row0, rows <= kKeyRows ? kKeyRows : kTileRows);
     const int p_first = t.p0 + (int)A.by_group.quot(t.row0), p_last = t.p0 + (int)A.by_group.quot(t.row0 + t.count - 1);
     t.lo = A.window > 0 ? max(0, p_first - A.window + 1) : 0;
-    t.hi = (int)min((int64_t)p_last + 1, (int64_t)A.cache.max_pages * A.cache.page.d);
+    t.hi = min(p_last + 1, A.capacity);
 }
 // keys of each piece of a tile, whole steps of 128
 __device__ __forceinline__ int piece_keys(const AttnTile& t) { return ((max(0, t.hi - t.lo) + 127) / 128 + t.cuts - 1) / t.cuts * 128; }
@@ -371,24 +383,24 @@ __device__ __forceinline__ f2_t* states_of(const AttnArgs& A)
 __device__ __forceinline__ int* steps_of(const AttnArgs& A) { return reinterpret_cast<int*>(states_of(A) + (int64_t)A.slots * A.cache.kv_heads * A.slot_rows); }
 
 // The idx-th piece from the end (the last tiles of a prompt have the most keys and go first); every wavefront looks for itself.
-__device__ __forceinline__ bool find_piece(const AttnArgs& A, int idx, AttnTile& t)
+__device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int kv_heads, int idx, AttnTile& t)
 {
     Lanes L;
-    const int len = piece_steps(A, L);
-    if (A.pieces > 0 && blockIdx.x == 0 && threadIdx.x == 0) *steps_of(A) = len;
+    const int len = piece_steps(H, kv_heads, L);
+    if (H.pieces > 0 && blockIdx.x == 0 && idx == 0 && threadIdx.x == 0) *steps_of(A) = len;
     int cum = lane_scan(L.tiles * L.cuts(len)), total = __builtin_amdgcn_readlane(cum, 63);
-    for (int s0 = 64; s0 < A.cache.seqs; s0 += 64) {
-        L.load(A, s0);
+    for (int s0 = 64; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
         total += lane_sum(L.tiles * L.cuts(len));
     }
     int want = total - 1 - idx, s0 = 0;
     if (want < 0) return false;
     t.slot = want;
-    if (A.cache.seqs > 64) L.load(A, 0);
+    if (H.seqs > 64) L.load(H, 0);
     while (want >= __builtin_amdgcn_readlane(cum, 63)) {             // (fewer than the total)
         want -= __builtin_amdgcn_readlane(cum, 63);
         s0 += 64;
-        L.load(A, s0);
+        L.load(H, s0);
         cum = lane_scan(L.tiles * L.cuts(len));
     }
     const int at = __ffsll((unsigned long long)__ballot(want < cum)) - 1;
@@ -401,20 +413,20 @@ __device__ __forceinline__ bool find_piece(const AttnArgs& A, int idx, AttnTile&
     return true;
 }
 // the tile of a row and head and its first piece; false: of no sequence
-__device__ __forceinline__ bool find_row(const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)
+__device__ __forceinline__ bool find_row(const Lens& H, const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)
 {
     const int len = *steps_of(A);
     Lanes L;
     int before = 0;
-    for (int s0 = 0; s0 < A.cache.seqs; s0 += 64) {
-        L.load(A, s0);
+    for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
         const int cum = lane_scan(L.tiles * L.cuts(len));
         const uint64_t has = __ballot(row >= L.start && row < L.start + L.n);
         if (has) {
             const int at = __ffsll((unsigned long long)has) - 1;
             const int cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
-            const int r = (row - __builtin_amdgcn_readlane(L.start, at)) * A.group + head % A.group;
-            const int tile = __builtin_amdgcn_readlane(L.n, at) * A.group <= kKeyRows ? 0 : r / kTileRows;
+            const int r = (row - __builtin_amdgcn_readlane(L.start, at)) * H.group + head % H.group;
+            const int tile = __builtin_amdgcn_readlane(L.n, at) * H.group <= kKeyRows ? 0 : r / kTileRows;
             set_tile(A, L, s0, at, tile, len, t);
             t.slot = before + __builtin_amdgcn_readlane(cum, at) + (tile - __builtin_amdgcn_readlane(L.tiles, at)) * cuts;
             *in_tile = r - t.row0;
@@ -932,14 +944,14 @@ struct Attn {
     }
 };
 
-// grid: KV heads x pieces
+// grid (KV heads, pieces)
 template <int TYPE, int HD>
-__global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 2)) paged_attention_kernel(const AttnArgs A)
+__global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 2)) paged_attention_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    const int kvh = blockIdx.x % A.cache.kv_heads, idx = blockIdx.x / A.cache.kv_heads;
+    const int kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
     AttnTile t;
-    if (!find_piece(A, idx, t)) return;
+    if (!find_piece(TSHIP_LENS, A, gridDim.x, idx, t)) return;
     Attn<TYPE, HD> a(A, t, kvh, (lds_t)smem);
     if (t.tokens * A.group <= kKeyRows) a.own_keys();
     else a.shared_keys();
@@ -947,7 +959,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 
 
 // The pieces of a row's tile, for one head: WAVES wavefronts (one where there are many rows; four share the pieces of few).
 template <int WAVES>
-__global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(const AttnArgs A)
+__global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
 {
     __shared__ f2_t sums[kAttnWaves];
     __shared__ f4_t values_in[kAttnWaves][kMaxDim / 4];
@@ -955,7 +967,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(const AttnA
     const int head = WAVES == 1 ? blockIdx.y * kAttnWaves + wave : blockIdx.y;
     AttnTile t;
     int in_tile;
-    if (head >= A.heads || !find_row(A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all wavefronts of a head)
+    if (head >= A.heads || !find_row(TSHIP_LENS, A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all wavefronts of a head)
     const int cuts = t.cuts;
     const int64_t first = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
     const float* values = A.partial + first * dim;
@@ -1077,23 +1089,23 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
 }
 
 template <int TYPE, int HD>
-static bool launch_attention(const AttnArgs& args, const dim3& grid, hipStream_t stream)
+static bool launch_attention(const Lens& H, const AttnArgs& args, const dim3& grid, hipStream_t stream)
 {
     const auto kern = paged_attention_kernel<TYPE, HD>;
     constexpr size_t lds = Attn<TYPE, HD>::kLds;
     if (!raise_lds_limit(reinterpret_cast<const void*>(kern), lds)) return false;
-    hipLaunchKernelGGL(kern, grid, dim3(kAttnThreads), lds, stream, args);
+    hipLaunchKernelGGL(kern, grid, dim3(kAttnThreads), lds, stream, H.row_starts, H.context_lens, H.seqs, H.rows, H.group, H.window, H.pieces, H.capacity, args);
     return hip_ok(hipGetLastError(), "paged attention launch");
 }
 template <int TYPE>
-static bool launch_attention(const AttnArgs& args, const dim3& grid, hipStream_t stream)
+static bool launch_attention(const Lens& H, const AttnArgs& args, const dim3& grid, hipStream_t stream)
 {
     const int dim = args.cache.head_dim;
-    if (dim <= 64) return launch_attention<TYPE, 64>(args, grid, stream);
-    if (dim <= 96) return launch_attention<TYPE, 96>(args, grid, stream);
-    if (dim <= 128) return launch_attention<TYPE, 128>(args, grid, stream);
-    if (dim <= 192) return launch_attention<TYPE, 192>(args, grid, stream);
-    return launch_attention<TYPE, 256>(args, grid, stream);
+    if (dim <= 64) return launch_attention<TYPE, 64>(H, args, grid, stream);
+    if (dim <= 96) return launch_attention<TYPE, 96>(H, args, grid, stream);
+    if (dim <= 128) return launch_attention<TYPE, 128>(H, args, grid, stream);
+    if (dim <= 192) return launch_attention<TYPE, 192>(H, args, grid, stream);
+    return launch_attention<TYPE, 256>(H, args, grid, stream);
 }
 
 bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64_t ld_query, float* out, int64_t ld_out, int rows, int heads,
@@ -1112,7 +1124,7 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     args.heads = heads;
     args.group = heads / cache.kv_heads;
     args.window = window;
-    args.pieces = plan.pieces;
+    args.capacity = cache.max_pages * (int)cache.page.d;
     args.slots = plan.pieces;
     args.slot_rows = plan.slot_rows;
     args.by_group = FastDiv((uint32_t)args.group);
@@ -1121,18 +1133,22 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
         set_last_error("paged_attention: too many rows for one call.");
         return false;
     }
-    const dim3 grid((unsigned)(plan.slots * cache.kv_heads));
+    const Lens H{cache.row_starts, cache.context_lens, cache.seqs, rows, args.group, window, plan.pieces, args.capacity};
+    const unsigned layers = (plan.slots + 65534u) / 65535u;
+    const dim3 grid(cache.kv_heads, (plan.slots + layers - 1) / layers, layers);
     bool ok;
     switch (cache.element_type) {
-    case kTypeF32: ok = launch_attention<0>(args, grid, stream); break;
-    case kTypeF16: ok = launch_attention<1>(args, grid, stream); break;
-    default: ok = launch_attention<2>(args, grid, stream); break;
+    case kTypeF32: ok = launch_attention<0>(H, args, grid, stream); break;
+    case kTypeF16: ok = launch_attention<1>(H, args, grid, stream); break;
+    default: ok = launch_attention<2>(H, args, grid, stream); break;
     }
     if (!ok || plan.pieces == 0) return ok;
     if ((int64_t)rows * heads <= 8 * device_info().num_cus)
-        hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, args);
+        hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs, H.rows, H.group, H.window,
+                           H.pieces, H.capacity, args);
     else
-        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(rows, (heads + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, args);
+        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(rows, (heads + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs,
+                           H.rows, H.group, H.window, H.pieces, H.capacity, args);
     return hip_ok(hipGetLastError(), "paged attention combine launch");
 }
 
