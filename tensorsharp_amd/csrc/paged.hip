@@ -529,13 +529,10 @@ struct Attn {
         const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * A.cache.head_dim;
         p = t.p0 + token;
         lo = A.window > 0 ? p - A.window + 1 : 0;
+        if (!live) src = reinterpret_cast<const float*>(g_zero_row);
         auto eight = [&](int s, float (&x)[8]) {
-            const int d = 16 * s + 8 * half;
-            f4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;
-            if (live && d < A.cache.head_dim) {
-                a = *reinterpret_cast<const f4_t*>(src + d);
-                b = *reinterpret_cast<const f4_t*>(src + d + 4);
-            }
+            const float* at = (16 * s < A.cache.head_dim ? src : reinterpret_cast<const float*>(g_zero_row)) + 16 * s + 8 * half;
+            const f4_t a = *reinterpret_cast<const f4_t*>(at), b = *reinterpret_cast<const f4_t*>(at + 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = a[i] * A.sign;
@@ -544,32 +541,32 @@ struct Attn {
         };
         c = A.c;
         int e = 0;
+        // fp16: the row's largest is brought to 2^13 .. 2^14, so it is needed first; where the row does not fit beside its parts, it is read twice
+        constexpr bool kTwice = TYPE == 1 && HD > 128;
+        float all[kSteps][8];
         if constexpr (TYPE == 1) {
-            // the row's largest at 2^13 .. 2^14 (its own pass: kept in between, the row would not fit beside its parts)
             float top = 0.f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                float x[8];
-                eight(s, x);
+                eight(s, all[s]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(all[s][i]));
             }
             top = both_halves(top, larger);
             if (top > 0.f && top < INFINITY) e = 14 - __builtin_amdgcn_frexp_expf(top);
             c = ldexpf(A.c, -e);
-            asm volatile("" ::: "memory");
+            if constexpr (kTwice) asm volatile("" ::: "memory");
         }
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            float x[8];
-            eight(s, x);
             u4_t part[kParts];
+            if constexpr (TYPE != 1 || kTwice) eight(s, all[s]);
             if constexpr (TYPE == 1) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = ldexpf(x[i], e);
-                cut2(x, part);
+                for (int i = 0; i < 8; ++i) all[s][i] = ldexpf(all[s][i], e);
+                cut2(all[s], part);
             } else {
-                cut3(x, part);
+                cut3(all[s], part);
             }
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {
