@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 namespace tship {
 namespace {
@@ -468,6 +469,17 @@ __device__ __forceinline__ float both_halves(float x, float (*op)(float, float))
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float added(float a, float b) { return a + b; }
 
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f)
+{
+    (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each_of(F&& f)
+{
+    each_of(std::make_integer_sequence<int, N>(), f);
+}
+
 // TYPE: 0 fp32, 1 fp16, 2 bf16 cache; HD: head_dim rounded up to what the tiles are made for
 template <int TYPE, int HD>
 struct Attn {
@@ -594,29 +606,53 @@ struct Attn {
     // Lane i has the id of page id_base + i; read again when a step passes the last of them.  (Held like this they cost a load
     // every 64 pages and no load beside the copies, whose waits count loads.)
     int ids, id_base = -64;
-    template <int KEYS>
-    __device__ __forceinline__ int page_id(int key0, int mine, int end)
+    __device__ __forceinline__ int page_id(int key, int end) const
     {
+        const int id = __shfl(ids, (int)A.cache.page.quot((uint32_t)key) - id_base);
+        return key < end && (uint32_t)id < (uint32_t)A.cache.num_pages ? id : -1;
+    }
+    // Where a row takes 8, 16 or 32 lanes of a copy, its address reaches them from a lane of the same 16 in a register permutation: a lane
+    // finds the address of the row that its 16 lanes copy by number lane % 16 of the copies that its wavefront makes (copies wave,
+    // wave + 4, .. where wavefronts share the keys).  In other cases lane i finds that of row i, and it goes through a shuffle.
+    static constexpr bool kNear = kPieces == 8 || kPieces == 16 || kPieces == 32;
+    template <bool SHARED>
+    __device__ __forceinline__ int held_row(int wave) const
+    {
+        if constexpr (!kNear) return lane & (SHARED ? 32 * NT - 1 : 31);
+        constexpr int kMine = SHARED ? NT * kCopies / kAttnWaves : kCopies;
+        static_assert(!kNear || kMine <= (kPieces == 8 ? 8 : 16));
+        const int j = lane & (kPieces == 8 ? 7 : 15) & (kMine - 1), n = SHARED ? wave + kAttnWaves * j : j, group = lane >> 4;
+        return kPieces == 8 ? 8 * n + 2 * group + ((lane >> 3) & 1) : kPieces == 16 ? 4 * n + group : 2 * n + (group >> 1);
+    }
+    struct Rows {
+        uint64_t k, v;               // addresses of a key and its value
+        uint64_t there;              // which keys of the step are in the cache
+    };
+    // of the step from key0 on; keys from `end` on are not there
+    template <bool SHARED>
+    __device__ __forceinline__ Rows rows_of(int key0, int end, int wave)
+    {
+        constexpr int kKeys = SHARED ? 32 * NT : 32;
         const int first = (int)A.cache.page.quot((uint32_t)key0);   // uniform
-        if ((int)A.cache.page.quot((uint32_t)(key0 + KEYS - 1)) - id_base >= 64) {
+        if ((int)A.cache.page.quot((uint32_t)(key0 + kKeys - 1)) - id_base >= 64) {
             id_base = first;
             ids = A.cache.table[t.seq * A.cache.table_stride + min(first + lane, A.cache.max_pages - 1)];
         }
-        const int id = __shfl(ids, (int)A.cache.page.quot((uint32_t)mine) - id_base);
-        return mine < end ? id : -1;
-    }
-    struct Rows {
-        uint64_t k, v;               // addresses of this lane's key and value
-        uint64_t there;              // which lanes' are in the cache
-    };
-    __device__ __forceinline__ Rows rows_of(int key, int id) const
-    {
-        const bool ok = (uint32_t)id < (uint32_t)A.cache.num_pages;
+        const int key = key0 + held_row<SHARED>(wave), id = page_id(key, end);
+        const uint64_t there = __ballot((kNear ? page_id(key0 + (lane & (kKeys - 1)), end) : id) >= 0);
         const int within = key - (int)A.cache.page.quot((uint32_t)key) * (int)A.cache.page.d;
         const int64_t zero = (int64_t)(uintptr_t)g_zero_row;
         const int64_t k = (int64_t)(uintptr_t)A.cache.k + (id * A.cache.k_page + within * A.cache.k_token + kvh * A.cache.k_head) * kElem;
         const int64_t v = (int64_t)(uintptr_t)A.cache.v + (id * A.cache.v_page + within * A.cache.v_token + kvh * A.cache.v_head) * kElem;
-        return {(uint64_t)(ok ? k : zero), (uint64_t)(ok ? v : zero), __ballot(ok)};
+        return {(uint64_t)(id >= 0 ? k : zero), (uint64_t)(id >= 0 ? v : zero), there};
+    }
+    // x of lane J of the 16 (rows of 8 lanes: of lane J for the lower eight, 8 + J for the upper)
+    template <int J>
+    __device__ __forceinline__ static uint32_t from_near(uint32_t x)
+    {
+        int r = __builtin_amdgcn_update_dpp(0, (int)x, 0x150 + J, 0xf, 0xf, true);
+        if constexpr (kPieces == 8) r = __builtin_amdgcn_update_dpp(r, (int)x, 0x150 + 8 + J, 0xf, 0xc, false);
+        return (uint32_t)r;
     }
     // the lane's number, for the copies of one step: where registers are short, their places are worked out at every step
     __device__ __forceinline__ int lane_here() const
@@ -625,12 +661,14 @@ struct Attn {
         if constexpr (kTight) asm volatile("" : "+v"(ln));
         return ln;
     }
-    // copy n of a block: 64 pieces that follow one another in LDS
-    template <bool V>
+    // copy n of a block, the wavefront's J-th: 64 pieces that follow one another in LDS
+    template <bool V, int J>
     __device__ __forceinline__ void copy(uint64_t rows, int n, lds_t block, int ln) const
     {
         const int slot = n * 64 + ln, row = slot / kPieces, piece = (slot - row * kPieces) ^ (V ? v_swizzle(row) : k_swizzle(row));
-        uint64_t at = (uint64_t)__shfl((unsigned long long)rows, row);
+        uint64_t at;
+        if constexpr (kNear) at = (uint64_t)from_near<J>((uint32_t)(rows >> 32)) << 32 | from_near<J>((uint32_t)rows);
+        else at = (uint64_t)__shfl((unsigned long long)rows, row);
         if (piece * 16 >= A.cache.head_dim * kElem) at = (uint64_t)(uintptr_t)g_zero_row;
         at += piece * 16;
         // (In assembly, because the compiler would wait for every copy under way in front of each transposed read.  It writes no register
@@ -794,21 +832,22 @@ struct Attn {
         const int p_first = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave, t.count - 1));
         const int p_last = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave + 31, t.count - 1));
         const int lo_last = A.window > 0 ? p_last - A.window + 1 : 0;
-        constexpr int kKeys = 32 * NT;
-        const int mine = lane & (kKeys - 1);
+        constexpr int kKeys = 32 * NT, kMine = (NT * kCopies + kAttnWaves - 1) / kAttnWaves;
         auto stage = [&](const Rows& r, lds_t buffer) {
             const int ln = lane_here();
-#pragma unroll
-            for (int n = 0; n < (NT * kCopies + kAttnWaves - 1) / kAttnWaves; ++n)
-                if (NT * kCopies % kAttnWaves == 0 || wave + kAttnWaves * n < NT * kCopies) {
-                    copy<false>(r.k, wave + kAttnWaves * n, buffer, ln);
-                    copy<true>(r.v, wave + kAttnWaves * n, buffer + NT * kBlock, ln);
+            each_of<kMine>([&](auto j) {
+                constexpr int J = decltype(j)::value;
+                const int n = wave + kAttnWaves * J;
+                if (NT * kCopies % kAttnWaves == 0 || n < NT * kCopies) {
+                    copy<false, J>(r.k, n, buffer, ln);
+                    copy<true, J>(r.v, n, buffer + NT * kBlock, ln);
                 }
+            });
         };
         int buffer = 0;
         if (begin < end) {
             // copies go a step ahead; those behind the last key bring zeros that nothing reads
-            Rows rows = rows_of(begin + mine, page_id<kKeys>(begin, begin + mine, end));
+            Rows rows = rows_of<true>(begin, end, wave);
             stage(rows, lds);
             load_rows(32 * wave + col);                              // (while the first keys are on their way)
             for (int key0 = begin; key0 < end; key0 += kKeys) {
@@ -816,7 +855,7 @@ struct Attn {
                 const lds_t here = lds + buffer * (2 * NT * kBlock);
                 const uint64_t there = rows.there;
                 buffer ^= 1;
-                rows = rows_of(key0 + kKeys + mine, page_id<kKeys>(key0 + kKeys, key0 + kKeys + mine, end));
+                rows = rows_of<true>(key0 + kKeys, end, wave);
                 stage(rows, lds + buffer * (2 * NT * kBlock));
                 // (a wavefront without rows copies only, as does one whose rows see none of the keys)
                 if (32 * wave < t.count && key0 <= p_last) {
@@ -874,10 +913,9 @@ struct Attn {
         if (wave < kKeyWaves && key0 < end) {
             auto stage = [&](auto is_v, uint64_t rows, lds_t block) {
                 const int ln = lane_here();
-#pragma unroll
-                for (int n = 0; n < kCopies; ++n) copy<decltype(is_v)::value>(rows, n, block, ln);
+                each_of<kCopies>([&](auto n) { copy<decltype(is_v)::value, decltype(n)::value>(rows, decltype(n)::value, block, ln); });
             };
-            Rows rows = rows_of(key0 + col, page_id<32>(key0, key0 + col, end));
+            Rows rows = rows_of<false>(key0, end, wave);
             stage(std::false_type(), rows.k, kb);
             stage(std::true_type(), rows.v, vb);
             load_rows(col);                                          // (while the first keys are on their way)
@@ -886,7 +924,7 @@ struct Attn {
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");
                 f16_t s[1] = {scores(kb)};
                 const uint64_t there = rows.there;
-                rows = rows_of(key0 + kStride + col, page_id<32>(key0 + kStride, key0 + kStride + col, end));
+                rows = rows_of<false>(key0 + kStride, end, wave);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::false_type(), rows.k, kb);
                 if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
