@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_kernel(const float* q
     if (at.seq < 0) return;                                          // uniform
     const int u = threadIdx.x % LANES, dim = C.head_dim, all = heads + 2 * C.kv_heads;
     const bool live = 4 * u < dim;
-    const int where = C.context_lens[at.seq] - at.count + (t - at.first);
+    const int where = max(C.context_lens[at.seq], -(1 << 30)) - at.count + (t - at.first);
     const int position = positions ? positions[t] : where;
     int within = 0;
     const int page = where >= 0 ? page_of(C, at.seq, where, &within) : -1;
@@ -301,7 +301,7 @@ struct Lanes {
         start = n = context = 0;
         if (s < H.seqs) {
             const int a = H.row_starts[s], b = H.row_starts[s + 1];
-            context = H.context_lens[s];
+            context = max(H.context_lens[s], -(1 << 30));
             start = clamped(a, H.rows);
             n = max(0, clamped(b, H.rows) - start);
         }
@@ -764,6 +764,26 @@ struct Attn {
             for (int d = 0; d < kDims; ++d) asm volatile("" : "+a"(o[d]));
         }
     }
+    // Whether a block's 32 values hold an infinity or NaN.  The matrix instruction would bring those to rows that do not see them (0 x NaN),
+    // so they are looked for where the rows of a tile see different keys; such a tile is done again by plainly().
+    __device__ __forceinline__ bool odd_values(lds_t block) const
+    {
+        typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
+        const lds_t row = block + col * kRow;
+        us2_t top2 = {0, 0};
+        uint32_t top = 0;
+#pragma unroll 2
+        for (int piece = half; piece < kPieces; piece += 2) {
+            const u4_t v = read16(row + (piece << 4));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (TYPE == 0) top = max(top, v[i] & 0x7fffffffu);
+                else top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(us2_t, v[i] & 0x7fff7fffu));
+            }
+        }
+        constexpr uint32_t kInf = TYPE == 0 ? 0x7f800000u : TYPE == 1 ? 0x7c00u : 0x7f80u;
+        return __any(TYPE == 0 ? top >= kInf : top2.x >= kInf || top2.y >= kInf);
+    }
     // weights of a block's scores, their sum, and O^T += V^T P^T
     __device__ __forceinline__ void weigh(const f16_t& s, lds_t block)
     {
@@ -824,10 +844,80 @@ struct Attn {
         return 1.0f / sum;
     }
 
-    // all wavefronts over the same keys, 32 rows each
-    __device__ __forceinline__ void shared_keys()
+    __device__ __forceinline__ bool odd_anywhere(bool odd, int wave) const
+    {
+        __shared__ int found[kAttnWaves];
+        if (lane == 0) found[wave] = odd;
+        __syncthreads();
+        return (found[0] | found[1] | found[2] | found[3]) != 0;
+    }
+
+    // A tile (piece) again, each row over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
+    // 64) for the values.  Slow, for tiles with infinities or NaN among their values.
+    __device__ __forceinline__ void plainly()
+    {
+        const int dim = A.cache.head_dim;
+        for (int row = threadIdx.x >> 6; row < t.count; row += kAttnWaves) {
+            int token, head;
+            place(row, &token, &head);
+            const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
+            const int last = t.p0 + token, first = A.window > 0 ? last - A.window + 1 : 0;
+            float top = -INFINITY, sum = 0.f, acc[HD / 64 + 1] = {};
+            for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
+                const int j = j0 + lane;
+                int id = -1;
+                if (j < t.hi && j >= first && j <= last) id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)j)];
+                const bool seen = (uint32_t)id < (uint32_t)A.cache.num_pages;
+                const uint64_t lanes = __ballot(seen);
+                if (lanes == 0) continue;
+                const int within = j - (int)A.cache.page.quot((uint32_t)j) * (int)A.cache.page.d;
+                const int64_t v_at = seen ? id * A.cache.v_page + within * A.cache.v_token + kvh * A.cache.v_head : 0;
+                float score = -INFINITY;
+                if (seen) {
+                    const int64_t k_at = id * A.cache.k_page + within * A.cache.k_token + kvh * A.cache.k_head;
+                    float dot = 0.f;
+                    for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(A.cache.k, k_at + d);
+                    score = dot * A.c;
+                }
+                float most = score;
+                for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+                const float mn = fmaxf(top, most), base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
+                const float w = seen ? __builtin_amdgcn_exp2f(score - base + kBias) : 0.f;
+                float all = w;
+                for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
+                sum = sum * f + all;
+                top = mn;
+#pragma unroll
+                for (int i = 0; i <= HD / 64; ++i) acc[i] *= f;
+                for (uint64_t rest = lanes; rest != 0; rest &= rest - 1) {
+                    const int at = __ffsll((unsigned long long)rest) - 1;
+                    const float wk = __shfl(w, at);
+                    const int64_t vk = (int64_t)__shfl((long long)v_at, at);
+#pragma unroll
+                    for (int i = 0; i <= HD / 64; ++i)
+                        if (64 * i + lane < dim) acc[i] += wk * element(A.cache.v, vk + 64 * i + lane);
+                }
+            }
+            float* dst = t.cuts == 1 ? A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * dim : values_of(row);
+            const float by = t.cuts == 1 ? over_sum(sum, top, head) : 1.f;
+#pragma unroll
+            for (int i = 0; i <= HD / 64; ++i)
+                if (64 * i + lane < dim) dst[64 * i + lane] = acc[i] * by;
+            if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top, sum};
+        }
+    }
+    __device__ __forceinline__ float element(const char* base, int64_t at) const
+    {
+        if constexpr (TYPE == 0) return reinterpret_cast<const float*>(base)[at];
+        else if constexpr (TYPE == 1) return __half2float(reinterpret_cast<const __half*>(base)[at]);
+        else return __bfloat162float(reinterpret_cast<const __hip_bfloat16*>(base)[at]);
+    }
+
+    // all wavefronts over the same keys, 32 rows each (the return of both: whether the tile has to be done by plainly())
+    __device__ __forceinline__ bool shared_keys()
     {
         const int begin = t.lo, end = t.hi;
+        bool odd = false;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_first = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave, t.count - 1));
         const int p_last = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave + 31, t.count - 1));
@@ -862,9 +952,14 @@ struct Attn {
                     f16_t s[NT];
 #pragma unroll
                     for (int b = 0; b < NT; ++b) s[b] = scores(here + b * kBlock);
-                    if (~there != 0 || key0 + kKeys - 1 > p_first || key0 < lo_last) {
+                    const bool differ = key0 + kKeys - 1 > p_first || key0 < lo_last;
+                    if (~there != 0 || differ) {
 #pragma unroll
                         for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b));
+                    }
+                    if (differ) {
+#pragma unroll
+                        for (int b = 0; b < NT; ++b) odd |= odd_values(here + (NT + b) * kBlock);
                     }
                     follow_maximum(s, NT);
 #pragma unroll
@@ -875,9 +970,10 @@ struct Attn {
         } else {
             no_rows();
         }
+        if (odd_anywhere(odd, wave)) return true;
         const int row = 32 * wave + col;
         l = both_halves(l, added);
-        if (row >= t.count) return;
+        if (row >= t.count) return false;
         int token, head;
         place(row, &token, &head);
         float* dst;
@@ -897,12 +993,14 @@ struct Attn {
                 if (at < A.cache.head_dim)
                     *reinterpret_cast<f4_t*>(dst + at) = f4_t{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * by;
             }
+        return false;
     }
 
     // every wavefront over keys of its own, the same (up to 32) rows
-    __device__ __forceinline__ void own_keys()
+    __device__ __forceinline__ bool own_keys()
     {
         const int begin = t.lo, end = t.hi;
+        bool odd = false;
         __shared__ f2_t states[kAttnWaves][32];
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_last = t.p0 + t.tokens - 1;
@@ -927,9 +1025,11 @@ struct Attn {
                 rows = rows_of<false>(key0 + kStride, end, wave);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::false_type(), rows.k, kb);
-                if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
+                const bool differ = key0 + 31 > t.p0 || key0 < lo_last;
+                if (~there != 0 || differ) mask(s[0], key0, there);
                 follow_maximum(s, 1);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");                 // the values too: the next keys are left
+                if (differ && t.tokens > 1) odd |= odd_values(vb);
                 weigh(s[0], vb);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::true_type(), rows.v, vb);
@@ -940,6 +1040,7 @@ struct Attn {
         }
         l = both_halves(l, added);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t.tokens > 1 && odd_anywhere(odd, wave)) return true;    // (one token's rows see the same keys)
         if (wave < kKeyWaves) {
             if (half == 0) states[wave][col] = f2_t{m, l};
             const lds_t row = lds + (wave * 32 + col) * HD * 4;
@@ -976,6 +1077,7 @@ struct Attn {
                 if (piece == 0) *state_of(row) = f2_t{top, sum};
             }
         }
+        return false;
     }
 };
 
@@ -988,8 +1090,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 
     AttnTile t;
     if (!find_piece(TSHIP_LENS, A, gridDim.x, idx, t)) return;
     Attn<TYPE, HD> a(A, t, kvh, (lds_t)smem);
-    if (t.tokens * A.group <= kKeyRows) a.own_keys();
-    else a.shared_keys();
+    if (t.tokens * A.group <= kKeyRows ? a.own_keys() : a.shared_keys()) a.plainly();
 }
 
 // The pieces of a row's tile, for one head: WAVES wavefronts (one where there are many rows; four share the pieces of few).

@@ -222,3 +222,32 @@ def test_offsets_beyond_32_bits(hip):
     out = torch.zeros_like(q)
     hip.PagedAttention(out, q, PagedKVCache(k, v, table), starts_of([20], torch), torch.tensor([ctx], dtype=torch.int32, device="cuda"), 0.1)
     check(out, c, q, [20], [ctx], heads, dim, 0.1, 0, None)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("n,window,dim", [(100, 0, 64), (100, 40, 64), (3, 0, 128), (3, 60, 96), (70, 0, 256)])
+def test_what_is_no_number_reaches_the_rows_that_see_it_only(hip, dtype, n, window, dim):
+    """infinities and NaN among the keys and values of tokens that some rows see and earlier (or, behind a window, later) ones do not"""
+    import torch
+    rng = np.random.default_rng(n)
+    heads, kv, ctx = 8, 2, 300
+    c = po.Cache(torch, rng, [ctx], 16, kv, dim, getattr(torch, dtype))
+
+    def poison(host, token, head, d, value):
+        host[c.table[0, token // 16], token % 16, head, d] = value
+    poison(c.host[1], ctx - 2, 0, 3, np.inf)
+    poison(c.host[1], ctx - 2, 0, dim - 1, -np.inf)
+    poison(c.host[1], ctx - n // 2 - 1, 1, 0, np.nan)
+    poison(c.host[0], ctx - 1, 1, slice(None), np.nan)
+    if window:
+        poison(c.host[1], ctx - window - 1, 1, 5, np.inf)
+    c.k, c.v = (torch.from_numpy(t).cuda().to(c.dtype) for t in c.host)
+    q = torch.from_numpy(rng.standard_normal((n, heads * dim)).astype(np.float32)).cuda()
+    out = run(hip, torch, c, q, [n], [ctx], dim ** -0.5, window).cpu().numpy().reshape(n, heads, dim)
+    k, v = c.rows(0)
+    with np.errstate(invalid="ignore"):
+        ref, _ = po.attend(q.cpu().numpy().reshape(n, heads, dim), k, v, np.arange(ctx - n, ctx), dim ** -0.5, window)
+    fine = np.isfinite(ref)
+    assert 0 < fine.sum() < fine.size
+    assert np.array_equal(np.isnan(ref), np.isnan(out)) and np.array_equal(ref[np.isinf(ref)], out[np.isinf(ref)])
+    assert np.linalg.norm(out[fine] - ref[fine]) <= 4e-6 * np.linalg.norm(ref[fine])
