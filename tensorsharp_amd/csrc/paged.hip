@@ -314,10 +314,27 @@ struct Lanes {
     __device__ __forceinline__ int cuts(int len) const { return max(1, (steps + len - 1) / len); }
 };
 
+// Steps of 128 keys that pieces have to save a tile to be worth it.  Joining them takes 5 us where they are few, 8.5 for many short tiles, 7.5
+// for long ones (3 of it the second launch, which comes wherever the page table has room for as many positions).  A step takes a short tile of
+// 64, 128, 256 dimensions 1.0, 1.4, 2.9 us in fp16 (bf16 0.9, 1.6, 3.5; fp32, by fewer wavefronts, 2.1, 8.4, 19.3) and a long one 2.6, 4.4,
+// 8.7 (bf16 4.1, 5.6, 12.2; fp32 7.4, 12.5, 29.5): by the dimensions, near enough.  One sequence of 512 keys, 256 dimensions and 8 KV heads: cut
+// 37 us, uncut 90 in fp32, 18 and 22 in fp16; 16 of 128 dimensions in fp16: 17 and 13.
+struct Worth {
+    int few, many, tall;
+};
+__host__ __device__ constexpr Worth worth_of(int type, int hd, int key_waves)
+{
+    const int step = hd * (type == kTypeF32 ? 14 : 5) / (10 * key_waves);                  // 0.1 us
+    const int tall = hd * (type == kTypeF32 ? 110 : type == kTypeF16 ? 40 : 55) / 100;
+    return {(50 + step - 1) / step, (85 + step - 1) / step, (75 + tall - 1) / tall};
+}
+__host__ __device__ constexpr int key_waves_of(int type, int hd) { return type != kTypeF32 || hd == 64 ? 4 : hd == 96 || hd == 192 ? 3 : 2; }
+__host__ __device__ constexpr int dims_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+
 // How many steps of 128 keys a piece has, so that the pieces of all tiles are about as many as the chip takes at once and as long as one
 // another (more would wait for a second round, fewer or unequal ones leave compute units without work).  At least their mean, in
 // a few tries up to what is certain to be enough.  32 sequences of 4096 keys and 8 KV heads: 104 us in 512 pieces, 107 in 1024, 136 in 4096.
-__device__ __forceinline__ int piece_steps(const Lens& H, int kv_heads, Lanes& L)
+__device__ __forceinline__ int piece_steps(const Lens& H, int kv_heads, Worth least, Lanes& L)
 {
     constexpr int kUncut = 1 << 24;
     L.load(H, 0);
@@ -347,11 +364,10 @@ __device__ __forceinline__ int piece_steps(const Lens& H, int kv_heads, Lanes& L
         for (int s0 = 0; s0 < H.seqs; s0 += 64) {
             if (H.seqs > 64) L.load(H, s0);
             all += lane_sum(L.tiles * L.cuts(len));
-            worth |= __any(L.steps - len >= (L.n * H.group > kKeyRows ? 2 : tiles * kv_heads >= 64 ? 7 : 4));
+            worth |= __any(L.steps - len >= (L.n * H.group > kKeyRows ? least.tall : tiles * kv_heads >= 64 ? least.many : least.few));
         }
         if (all <= H.pieces) break;
     }
-    // Joining the pieces takes 5 us, a step of a short tile 1.5 us (more where many are under way) and one of a long tile 4 us.
     if (!worth) len = kUncut;
     if (H.seqs > 64) L.load(H, 0);
     return len;
@@ -384,10 +400,10 @@ __device__ __forceinline__ f2_t* states_of(const AttnArgs& A)
 __device__ __forceinline__ int* steps_of(const AttnArgs& A) { return reinterpret_cast<int*>(states_of(A) + (int64_t)A.slots * A.cache.kv_heads * A.slot_rows); }
 
 // The idx-th piece from the end (the last tiles of a prompt have the most keys and go first); every wavefront looks for itself.
-__device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int kv_heads, int idx, AttnTile& t)
+__device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int kv_heads, Worth least, int idx, AttnTile& t)
 {
     Lanes L;
-    const int len = piece_steps(H, kv_heads, L);
+    const int len = piece_steps(H, kv_heads, least, L);
     if (H.pieces > 0 && blockIdx.x == 0 && idx == 0 && threadIdx.x == 0) *steps_of(A) = len;
     int cum = lane_scan(L.tiles * L.cuts(len)), total = __builtin_amdgcn_readlane(cum, 63);
     for (int s0 = 64; s0 < H.seqs; s0 += 64) {
@@ -491,7 +507,7 @@ struct Attn {
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
     static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU
     static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD == 128);
-    static constexpr int kKeyWaves = TYPE != 0 || HD == 64 ? 4 : HD == 96 || HD == 192 ? 3 : 2;    // wavefronts that have keys of their own
+    static constexpr int kKeyWaves = key_waves_of(TYPE, HD);   // wavefronts that have keys of their own
     static constexpr int kBlock = 32 * kRow;                         // bytes of 32 keys
     static constexpr int kCopies = kPieces / 2;                      // wavefront-wide copies of 32 keys
     static constexpr int kLds = kBlock * 2 * (2 * NT > kKeyWaves ? 2 * NT : kKeyWaves);
@@ -1088,7 +1104,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
     AttnTile t;
-    if (!find_piece(TSHIP_LENS, A, gridDim.x, idx, t)) return;
+    if (!find_piece(TSHIP_LENS, A, gridDim.x, worth_of(TYPE, HD, key_waves_of(TYPE, HD)), idx, t)) return;
     Attn<TYPE, HD> a(A, t, kvh, (lds_t)smem);
     if (t.tokens * A.group <= kKeyRows ? a.own_keys() : a.shared_keys()) a.plainly();
 }
@@ -1215,7 +1231,12 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
     const int at_once = device_info().num_cus * (dim <= 64 && cache.element_type != kTypeF32 ? 3 : dim <= 128 ? 2 : 1);
     const int64_t pieces = std::max(1, at_once / cache.kv_heads), keys = (int64_t)cache.max_pages * cache.page.d;
     const int64_t most = std::min<int64_t>(keys, window > 0 ? window : keys);
-    const bool cut = (all + kTileRows - 1) / kTileRows < pieces && most > (all <= (int64_t)kKeyRows * cache.seqs ? 512 : 256);
+    const int hd = dims_of(dim);
+    const Worth least = worth_of(cache.element_type, hd, key_waves_of(cache.element_type, hd));
+    const bool cut = (all + kTileRows - 1) / kTileRows < pieces &&
+        most > 128 * (all > (int64_t)kKeyRows * cache.seqs                                 ? std::min(least.few, least.tall)
+                      : std::min<int64_t>(cache.seqs, rows) * cache.kv_heads >= 64 ? least.many
+                                                                                   : least.few);
     plan.pieces = cut ? (int)pieces : 0;
     plan.slots = (int)std::min<int64_t>(INT32_MAX, cut ? std::max(tiles, pieces) : tiles);
     plan.slot_rows = all <= kKeyRows ? kKeyRows : kTileRows;
@@ -1236,12 +1257,13 @@ static bool launch_attention(const Lens& H, const AttnArgs& args, const dim3& gr
 template <int TYPE>
 static bool launch_attention(const Lens& H, const AttnArgs& args, const dim3& grid, hipStream_t stream)
 {
-    const int dim = args.cache.head_dim;
-    if (dim <= 64) return launch_attention<TYPE, 64>(H, args, grid, stream);
-    if (dim <= 96) return launch_attention<TYPE, 96>(H, args, grid, stream);
-    if (dim <= 128) return launch_attention<TYPE, 128>(H, args, grid, stream);
-    if (dim <= 192) return launch_attention<TYPE, 192>(H, args, grid, stream);
-    return launch_attention<TYPE, 256>(H, args, grid, stream);
+    switch (dims_of(args.cache.head_dim)) {
+    case 64: return launch_attention<TYPE, 64>(H, args, grid, stream);
+    case 96: return launch_attention<TYPE, 96>(H, args, grid, stream);
+    case 128: return launch_attention<TYPE, 128>(H, args, grid, stream);
+    case 192: return launch_attention<TYPE, 192>(H, args, grid, stream);
+    default: return launch_attention<TYPE, 256>(H, args, grid, stream);
+    }
 }
 
 bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64_t ld_query, float* out, int64_t ld_out, int rows, int heads,
