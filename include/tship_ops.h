@@ -493,7 +493,7 @@ TSHIP_EXPORT int TSHip_RoPEF32Device(TSHipTensorView3D result, TSHipTensorView3D
 
 /* What lies between a fused QKV projection and the attention over a paged cache.  Rows row_starts[s] .. row_starts[s + 1] - 1 of qkv
  * [rows x (num_heads + 2 num_kv_heads) head_dim] are the new tokens of sequence s, the last of context_lens[s] (both device; these
- * tokens counted).  Per head of q and k: RMSNorm * q_norm / k_norm (skipped when NULL), rotation by the token's position in its
+ * tokens counted; row_starts must not fall, and what is outside the rows is cut off).  Rows of keys and values may not overlap.  Per head of q and k: RMSNorm * q_norm / k_norm (skipped when NULL), rotation by the token's position in its
  * sequence (or positions[row], device, when given).  q goes to query [rows x num_heads head_dim] (may be the q columns of qkv), k and
  * v are rounded to the cache's type and stored at the token's position.  A token whose position is negative, beyond the table or on no page is not
  * stored; rows that belong to no sequence are left as they were. */

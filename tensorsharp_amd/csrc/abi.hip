@@ -5,12 +5,14 @@
 #include "../../include/tship_ops.h"
 #include "tship_internal.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 namespace tship {
@@ -3087,6 +3089,23 @@ bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_
     return true;
 }
 
+// rows of a cache that share memory, which may not be written
+bool rows_overlap(const TSHipPagedCache* c)
+{
+    const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
+    for (const int64_t* s : {&c->k_page_stride, &c->v_page_stride}) {
+        std::pair<int64_t, int64_t> d[3] = {{s[0], counts[0]}, {s[1], counts[1]}, {s[2], counts[2]}};
+        std::sort(d, d + 3);
+        int64_t span = c->head_dim;
+        for (const auto& [stride, count] : d) {
+            if (count == 1) continue;
+            if (stride < span) return true;
+            span += stride * (count - 1);
+        }
+    }
+    return false;
+}
+
 // Whether a and b, views of one shape, share memory in another way than element by element: not where their spans are apart, nor where
 // they have the same strides and their rows lie beside each other.
 bool overlaps_otherwise(const TSHipTensorView3D& a, const TSHipTensorView3D& b)
@@ -3173,6 +3192,10 @@ int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv
             set_last_error("rope_store_paged: norm weights must be 16-byte aligned.");
             return 0;
         }
+        if (rows_overlap(cache)) {
+            set_last_error("rope_store_paged: rows of keys or values overlap.");
+            return 0;
+        }
         const int T = qkv.dim0;
         const uintptr_t q0 = reinterpret_cast<uintptr_t>(query.data), x0 = reinterpret_cast<uintptr_t>(qkv.data);
         const uintptr_t q1 = q0 + ((int64_t)(T - 1) * query.stride0 + query.dim1) * 4, x1 = x0 + ((int64_t)(T - 1) * qkv.stride0 + qkv.dim1) * 4;
@@ -3202,7 +3225,7 @@ int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D qu
             set_last_error("Size mismatch: query and result differ in rows.");
             return 0;
         }
-        if (window < 0 || !std::isfinite(scale)) {
+        if (window < 0 || !std::isfinite(scale * 2.0f)) {              // (the kernels take scale log2 e)
             set_last_error("paged_attention: the window must not be negative and the scale finite.");
             return 0;
         }

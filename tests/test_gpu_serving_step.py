@@ -214,6 +214,24 @@ def test_streams_and_threads_beside_one_another(hip):
             assert torch.equal(a, b)
 
 
+def test_row_starts_outside_the_rows_are_cut_off(hip):
+    """a batch of fewer rows than its row starts speak of (and one whose first begins in front of it): as if these ended with the rows"""
+    import torch
+    got = []
+    for starts in ([0, 1, 3, 6], [-4, 1, 3, 50]):
+        s = build_step(torch, 3, 20)
+        s["qkv"] = s["qkv"].repeat(2, 1)
+        s["qkv"].add_(torch.arange(6, device="cuda")[:, None] / 7)
+        s["query"], s["out"] = (torch.zeros((6, HEADS * DIM), device="cuda") for _ in range(2))
+        s["starts"], s["lens"] = i32(torch, starts), i32(torch, [40, 17, 200])
+        hip.RoPEStorePaged(s["query"], s["qkv"], s["cache"], s["starts"], s["lens"], s["rope"])
+        hip.PagedAttention(s["out"], s["query"], s["cache"], s["starts"], s["lens"], DIM ** -0.5)
+        got.append([s[n].clone() for n in ("query", "out", "k", "v")])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert bool(got[0][1].abs().sum(1).min() > 0)
+
+
 def test_the_likeliest_token_of_a_quantized_head(hip):
     """hidden states through a quantized head into the sampler: greedy rows take the largest logit, top-k 1 as well"""
     import torch

@@ -38,7 +38,7 @@ for call in calls:
 """
 GOOD = ["do_rope()", "do_rope(v3(), v3())", "do_rope(v3(0, s=(D, T * D, 1)), v3(HALF))", "do_rope(v3(0, s=(1024, D, 1)), v3(2048, s=(1024, D, 1)))",
         "do_rope(r=rope(ext_factor=1.0, original_context=4096, freq_scale=0.25))", "do_rope(v3(HALF, (T, H, 36), (H * 36, 36, 1)), v3(0, (T, H, 36), (H * 36, 36, 1)), r=rope(dims=8))",
-        "do_store()", "do_store(v2(0, stride=(H + 2 * KV) * D))", "do_store(c=cache(element_type=0))", "do_store(c=cache(element_type=30, page_size=1, num_pages=1, k_page_stride=0))",
+        "do_store()", "do_store(v2(0, stride=(H + 2 * KV) * D))", "do_store(c=cache(element_type=0))", "do_store(c=cache(k_token_stride=D, k_head_stride=PAGE * D))", "do_attend(c=cache(k_token_stride=D))", "do_store(c=cache(element_type=30, page_size=1, num_pages=1, k_page_stride=0))",
         "do_attend()", "do_attend(v2(), v2())", "do_attend(window=5)", "do_attend(c=cache(element_type=30))", "do_attend(c=cache(element_type=0))",
         "do_attend(c=cache(num_kv_heads=1, k_head_stride=3, v_head_stride=0))", "do_attend(heads=2, query=v2(cols=2 * D), result=v2(HALF, cols=2 * D))",
         "do_sample()", "do_sample(v2(4, rows=3, cols=7, stride=9))", "do_sample(v2(0, rows=1, cols=1))"]
@@ -63,7 +63,8 @@ BAD = [
     ("do_attend(c=cache(max_pages=1 << 28, table_stride=1 << 28))", "page size"), ("do_attend(c=cache(table_stride=3))", "page size"),
     ("do_attend(c=cache(k_token_stride=D - 8))", "strides"), ("do_attend(c=cache(v_page_stride=PAGE * KV * D + 4))", "strides"), ("do_attend(c=cache(v_head_stride=-D))", "strides"),
     ("do_attend(c=cache(v=at(8)))", "16-byte aligned"), ("do_attend(heads=4)", "columns"), ("do_attend(v2(HALF, rows=5))", "differ in rows"), ("do_attend(window=-1)", "window"),
-    ("do_attend(scale=float('nan'))", "scale"), ("do_attend(scale=float('inf'))", "scale"), ("do_attend(v2(16), v2())", "overlaps query"), ("do_attend(v2(None))", "Null pointer"),
+    ("do_attend(scale=float('nan'))", "scale"), ("do_attend(scale=float('inf'))", "scale"), ("do_attend(scale=-2e38)", "scale"),
+    ("do_store(c=cache(k_token_stride=D))", "overlap"), ("do_store(c=cache(v_page_stride=PAGE * KV * D - 64))", "overlap"), ("do_store(c=cache(v_head_stride=PAGE * KV * D))", "overlap"), ("do_attend(v2(16), v2())", "overlaps query"), ("do_attend(v2(None))", "Null pointer"),
     ("do_attend(query=v2(0, inner=2))", "contiguous"),
     ("do_sample(u=None)", "Invalid arguments"), ("do_sample(t=None)", "Invalid arguments"), ("do_sample(tokens=None)", "Invalid arguments"), ("do_sample(v2(0, inner=2))", "Invalid arguments"),
     ("do_sample(v2(0, rows=1, cols=(1 << 20) + 1))", "2^20"), ("do_sample(v2(None))", "Null pointer"),
