@@ -95,7 +95,7 @@ constexpr int kRopeThreads = 256;
 
 // grid (tokens, head chunks): LANES lanes hold a head, a workgroup takes 256 / LANES heads at a time.  The angles of a token are worked
 // out once per workgroup, one pair per thread.
-// Bound: memory (1024 tokens of 32 heads of 128: 11.9 us, 67 MB in and out at 5.7 TB/s, a large copy 5.2), and for few tokens the latency of
+// Bound: memory (2048 tokens of 32 heads of 128: 11.9 us, 67 MB in and out at 5.7 TB/s, a large copy 5.2), and for few tokens the latency of
 // the angles and one trip to memory (24 tokens: 3.1 us).
 template <int LANES>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const float* x, float* out, const int32_t* positions, int heads, int head_dim,
@@ -145,8 +145,8 @@ __device__ __forceinline__ int page_of(const PagedKv& C, int seq, int position, 
 }
 
 // grid (rows, head chunks), lanes and angles as above; the lanes of a head add the squares of its norm.  One pass: a row is read once, and what
-// a query, key and value head become is written where the attention reads it.  Bound: memory (2048 rows of 32 + 2 x 8 heads of 128 into fp16 pages: 32 us
-// on the device, 158 MB at 4.9 TB/s), and for few rows the way from lengths to page to address (32 rows: 4.1 us).
+// a query, key and value head become is written where the attention reads it.  Bound: memory (3515 rows of 32 + 2 x 8 heads of 128 into bf16 pages: 32 us
+// on the device, 158 MB at 4.9 TB/s), and for few rows the way from lengths to page to address (24 rows: 4 us).
 template <int LANES, typename T>
 __global__ void __launch_bounds__(kRopeThreads) rope_store_kernel(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int heads,
                                                                   const int32_t* positions, const float* q_norm, const float* k_norm,
@@ -1113,26 +1113,28 @@ __global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 
     if (t.tokens * A.group <= kKeyRows ? a.own_keys() : a.shared_keys()) a.plainly();
 }
 
-// The pieces of a row's tile, for one head: WAVES wavefronts (one where there are many rows; four share the pieces of few).
+__host__ __device__ constexpr int wide_of(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
+
+// The pieces of a row's tile, for one head.  A head takes 16, 32 or 64 lanes; with WAVES 1, where there are many rows, the lanes beside
+// them have other heads and go through all pieces of theirs, with WAVES 4 the lanes beside them and the other wavefronts have other pieces.
+// Bound: the way from the lengths to the states, then memory (512 rows of 32 heads of 128 in 4 pieces, 34 MB: 11 us).
 template <int WAVES>
 __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
 {
     __shared__ f2_t sums[kAttnWaves];
     __shared__ f4_t values_in[kAttnWaves][kMaxDim / 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x, dim = A.cache.head_dim;
-    const int head = WAVES == 1 ? blockIdx.y * kAttnWaves + wave : blockIdx.y;
+    const int wide = wide_of(dim), d = 4 * (lane & (wide - 1)), parts = 64 / wide, part = lane / wide;
+    const int head = WAVES == 1 ? (blockIdx.y * kAttnWaves + wave) * parts + part : blockIdx.y;
     AttnTile t;
     int in_tile;
-    if (head >= A.heads || !find_row(TSHIP_LENS, A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all wavefronts of a head)
-    const int cuts = t.cuts;
-    const int64_t first = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
+    if (!find_row(TSHIP_LENS, A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all heads of a row)
+    const bool mine = d < dim && head < A.heads;
+    const int cuts = t.cuts, step = WAVES == 1 ? 1 : WAVES * parts;
+    const int64_t first = slot_row(A, t.slot, min(head, A.heads - 1) / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
     const float* values = A.partial + first * dim;
     const f2_t* states = states_of(A) + first;
-    // a head takes 16, 32 or 64 lanes; as many pieces as that leaves room for are read at a time
-    const int wide = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, d = 4 * (lane & (wide - 1)), parts = 64 / wide;
-    const int part = lane / wide + (WAVES == 1 ? 0 : wave * parts);
-    const bool mine = d < dim;
-    constexpr int U = 4;
+    constexpr int U = WAVES == 1 ? 8 : 4;
     f4_t acc = {0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.f;
     auto join = [&](float t, float w, const f4_t& v) {
@@ -1142,27 +1144,27 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
         acc = acc * f + v * g;
         top = m;
     };
-    for (int s0 = part; s0 < cuts; s0 += U * WAVES * parts) {
+    for (int s0 = WAVES == 1 ? 0 : wave * parts + part; s0 < cuts; s0 += U * step) {
         f2_t st[U];
         f4_t v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = min(s0 + u * WAVES * parts, cuts - 1);
+            const int s = min(s0 + u * step, cuts - 1);
             st[u] = states[s * next];
             v[u] = mine ? *reinterpret_cast<const f4_t*>(values + s * next * dim + d) : f4_t{0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (s0 + u * WAVES * parts < cuts) join(st[u].x, st[u].y, v[u]);
-    }
-    for (int o = wide; o < 64; o <<= 1) {
-        const float t = __shfl_xor(top, o), w = __shfl_xor(sum, o);
-        f4_t v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __shfl_xor(acc[i], o);
-        join(t, w, v);
+            if (s0 + u * step < cuts) join(st[u].x, st[u].y, v[u]);
     }
     if constexpr (WAVES > 1) {
+        for (int o = wide; o < 64; o <<= 1) {
+            const float t = __shfl_xor(top, o), w = __shfl_xor(sum, o);
+            f4_t v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __shfl_xor(acc[i], o);
+            join(t, w, v);
+        }
         if (lane == 0) sums[wave] = f2_t{top, sum};
         if (lane < wide) values_in[wave][lane] = acc;
         __syncthreads();
@@ -1170,12 +1172,13 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) join(sums[w].x, sums[w].y, values_in[w][lane]);
     }
+    if (!mine) return;
     float by = 0.f;
     if (sum > 0.f) {
         if (A.sinks) sum += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2e - top + kBias);
         by = 1.0f / sum;
     }
-    if (mine && lane < wide) *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * by;
+    *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * by;
 }
 
 }  // namespace
@@ -1305,11 +1308,12 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     default: ok = launch_attention<2>(H, args, grid, stream); break;
     }
     if (!ok || plan.pieces == 0) return ok;
+    const int per = kAttnWaves * 64 / wide_of(cache.head_dim);
     if ((int64_t)rows * heads <= 8 * device_info().num_cus)
         hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs, H.rows, H.group, H.window,
                            H.pieces, H.capacity, args);
     else
-        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(rows, (heads + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs,
+        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(rows, (heads + per - 1) / per), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs,
                            H.rows, H.group, H.window, H.pieces, H.capacity, args);
     return hip_ok(hipGetLastError(), "paged attention combine launch");
 }
