@@ -1115,23 +1115,36 @@ __global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 
 
 __host__ __device__ constexpr int wide_of(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
 
-// The pieces of a row's tile, for one head.  A head takes 16, 32 or 64 lanes; with WAVES 1, where there are many rows, the lanes beside
-// them have other heads and go through all pieces of theirs, with WAVES 4 the lanes beside them and the other wavefronts have other pieces.
-// Bound: the way from the lengths to the states, then memory (512 rows of 32 heads of 128 in 4 pieces, 34 MB: 11 us).
+// The pieces of a row's tile, for one head.  A head takes 16, 32 or 64 lanes.  WAVES 1, where there are many rows: grid (KV heads, wavefronts / 4),
+// a wavefront has a row's heads of one KV head, the lanes side by side different ones, and goes through all pieces.  (KV heads lead in both kernels'
+// grids: with 8 of them a piece is read on the die whose cache it was written through.)  WAVES 4: grid (rows, heads), the lanes side by side and the
+// wavefronts have different pieces.  Bound: the way from the lengths to the states, then memory (512 rows of 32 heads of 128 in 4 pieces, 34 MB: 9.7
+// us; 11.0 with rows leading).
 template <int WAVES>
 __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
 {
     __shared__ f2_t sums[kAttnWaves];
     __shared__ f4_t values_in[kAttnWaves][kMaxDim / 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x, dim = A.cache.head_dim;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), dim = A.cache.head_dim;
     const int wide = wide_of(dim), d = 4 * (lane & (wide - 1)), parts = 64 / wide, part = lane / wide;
-    const int head = WAVES == 1 ? (blockIdx.y * kAttnWaves + wave) * parts + part : blockIdx.y;
+    int row, head;
+    bool mine = d < dim;
+    if constexpr (WAVES == 1) {
+        const int chunks = (A.group + parts - 1) / parts, at = blockIdx.y * kAttnWaves + wave;
+        row = at / chunks;
+        const int in_group = at % chunks * parts + part;
+        if (row >= A.rows) return;
+        mine = mine && in_group < A.group;
+        head = blockIdx.x * A.group + min(in_group, A.group - 1);
+    } else {
+        row = blockIdx.x;
+        head = blockIdx.y;
+    }
     AttnTile t;
     int in_tile;
     if (!find_row(TSHIP_LENS, A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all heads of a row)
-    const bool mine = d < dim && head < A.heads;
     const int cuts = t.cuts, step = WAVES == 1 ? 1 : WAVES * parts;
-    const int64_t first = slot_row(A, t.slot, min(head, A.heads - 1) / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
+    const int64_t first = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
     const float* values = A.partial + first * dim;
     const f2_t* states = states_of(A) + first;
     constexpr int U = WAVES == 1 ? 8 : 4;
@@ -1308,13 +1321,14 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     default: ok = launch_attention<2>(H, args, grid, stream); break;
     }
     if (!ok || plan.pieces == 0) return ok;
-    const int per = kAttnWaves * 64 / wide_of(cache.head_dim);
-    if ((int64_t)rows * heads <= 8 * device_info().num_cus)
+    if ((int64_t)rows * heads <= 8 * device_info().num_cus) {
         hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs, H.rows, H.group, H.window,
                            H.pieces, H.capacity, args);
-    else
-        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(rows, (heads + per - 1) / per), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs,
-                           H.rows, H.group, H.window, H.pieces, H.capacity, args);
+    } else {
+        const int parts = 64 / wide_of(cache.head_dim), waves = rows * ((args.group + parts - 1) / parts);
+        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(cache.kv_heads, (waves + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens,
+                           H.seqs, H.rows, H.group, H.window, H.pieces, H.capacity, args);
+    }
     return hip_ok(hipGetLastError(), "paged attention combine launch");
 }
 
