@@ -784,25 +784,16 @@ struct Attn {
             for (int d = 0; d < kDims; ++d) asm volatile("" : "+a"(o[d]));
         }
     }
-    // Whether a block's 32 values hold an infinity or NaN.  The matrix instruction would bring those to rows that do not see them (0 x NaN),
-    // so they are looked for where the rows of a tile see different keys; such a tile is done again by plainly().
-    __device__ __forceinline__ bool odd_values(lds_t block) const
+    // Whether one of the wavefront's rows has an infinity or NaN in its result.  The matrix instruction brings those of values to rows that do not see them (0 x
+    // NaN) and they stay, so they are looked for at the end, where rows may see different keys; such rows are done again by plainly().
+    __device__ __forceinline__ bool odd_result(int row) const
     {
-        typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
-        const lds_t row = block + col * kRow;
-        us2_t top2 = {0, 0};
-        uint32_t top = 0;
-#pragma unroll 2
-        for (int piece = half; piece < kPieces; piece += 2) {
-            const u4_t v = read16(row + (piece << 4));
+        float z = 0.f;                                               // (a chain: a tree of comparisons takes registers from the loop)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (TYPE == 0) top = max(top, v[i] & 0x7fffffffu);
-                else top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(us2_t, v[i] & 0x7fff7fffu));
-            }
-        }
-        constexpr uint32_t kInf = TYPE == 0 ? 0x7f800000u : TYPE == 1 ? 0x7c00u : 0x7f80u;
-        return __any(TYPE == 0 ? top >= kInf : top2.x >= kInf || top2.y >= kInf);
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z = __builtin_fmaf(o[d][i], 0.f, z);
+        return __any(row < t.count && z != z);
     }
     // weights of a block's scores, their sum, and O^T += V^T P^T
     __device__ __forceinline__ void weigh(const f16_t& s, lds_t block)
@@ -872,12 +863,12 @@ struct Attn {
         return (found[0] | found[1] | found[2] | found[3]) != 0;
     }
 
-    // A tile (piece) again, each row over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
-    // 64) for the values.  Slow, for tiles with infinities or NaN among their values.
-    __device__ __forceinline__ void plainly()
+    // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
+    // 64) for the values.  Slow, for rows with infinities or NaN in their results.
+    __device__ __forceinline__ void plainly(int row, int step)
     {
         const int dim = A.cache.head_dim;
-        for (int row = threadIdx.x >> 6; row < t.count; row += kAttnWaves) {
+        for (int n = 0; n < 32 && row < t.count; ++n, row += step) {
             int token, head;
             place(row, &token, &head);
             const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
@@ -933,11 +924,10 @@ struct Attn {
         else return __bfloat162float(reinterpret_cast<const __hip_bfloat16*>(base)[at]);
     }
 
-    // all wavefronts over the same keys, 32 rows each (the return of both: whether the tile has to be done by plainly())
+    // all wavefronts over the same keys, 32 rows each (the return of both: whether these, of own_keys() all, have to be done by plainly())
     __device__ __forceinline__ bool shared_keys()
     {
         const int begin = t.lo, end = t.hi;
-        bool odd = false;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_first = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave, t.count - 1));
         const int p_last = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave + 31, t.count - 1));
@@ -972,14 +962,9 @@ struct Attn {
                     f16_t s[NT];
 #pragma unroll
                     for (int b = 0; b < NT; ++b) s[b] = scores(here + b * kBlock);
-                    const bool differ = key0 + kKeys - 1 > p_first || key0 < lo_last;
-                    if (~there != 0 || differ) {
+                    if (~there != 0 || key0 + kKeys - 1 > p_first || key0 < lo_last) {
 #pragma unroll
                         for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b));
-                    }
-                    if (differ) {
-#pragma unroll
-                        for (int b = 0; b < NT; ++b) odd |= odd_values(here + (NT + b) * kBlock);
                     }
                     follow_maximum(s, NT);
 #pragma unroll
@@ -990,8 +975,8 @@ struct Attn {
         } else {
             no_rows();
         }
-        if (odd_anywhere(odd, wave)) return true;
         const int row = 32 * wave + col;
+        if (odd_result(row)) return true;
         l = both_halves(l, added);
         if (row >= t.count) return false;
         int token, head;
@@ -1020,7 +1005,6 @@ struct Attn {
     __device__ __forceinline__ bool own_keys()
     {
         const int begin = t.lo, end = t.hi;
-        bool odd = false;
         __shared__ f2_t states[kAttnWaves][32];
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_last = t.p0 + t.tokens - 1;
@@ -1045,11 +1029,9 @@ struct Attn {
                 rows = rows_of<false>(key0 + kStride, end, wave);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::false_type(), rows.k, kb);
-                const bool differ = key0 + 31 > t.p0 || key0 < lo_last;
-                if (~there != 0 || differ) mask(s[0], key0, there);
+                if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
                 follow_maximum(s, 1);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");                 // the values too: the next keys are left
-                if (differ && t.tokens > 1) odd |= odd_values(vb);
                 weigh(s[0], vb);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::true_type(), rows.v, vb);
@@ -1060,7 +1042,7 @@ struct Attn {
         }
         l = both_halves(l, added);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t.tokens > 1 && odd_anywhere(odd, wave)) return true;    // (one token's rows see the same keys)
+        if (t.tokens > 1 && odd_anywhere(odd_result(col), wave)) return true;    // (one token's rows see the same keys)
         if (wave < kKeyWaves) {
             if (half == 0) states[wave][col] = f2_t{m, l};
             const lds_t row = lds + (wave * 32 + col) * HD * 4;
@@ -1110,7 +1092,9 @@ __global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 
     AttnTile t;
     if (!find_piece(TSHIP_LENS, A, gridDim.x, worth_of(TYPE, HD, key_waves_of(TYPE, HD)), idx, t)) return;
     Attn<TYPE, HD> a(A, t, kvh, (lds_t)smem);
-    if (t.tokens * A.group <= kKeyRows ? a.own_keys() : a.shared_keys()) a.plainly();
+    const bool own = t.tokens * A.group <= kKeyRows;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (own ? a.own_keys() : a.shared_keys()) a.plainly(own ? wave : 32 * wave, own ? kAttnWaves : 1);
 }
 
 __host__ __device__ constexpr int wide_of(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }

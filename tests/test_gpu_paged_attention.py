@@ -73,6 +73,8 @@ CASES = [
     (2, 1, 16, "float16", 3, "token", [50, 10], [17, 10], 0, False),
     (12, 12, 48, "bfloat16", 256, "head", [300, 1], [129, 1], 0, False),
     (36, 4, 160, "float16", 16, "token", [100], [20], 0, False),
+    (6, 2, 192, "float32", 16, "head", [140, 90], [50, 1], 0, False),
+    (8, 1, 176, "bfloat16", 64, "token", [200, 60], [30, 3], 70, True),
 ]
 
 
@@ -225,12 +227,13 @@ def test_offsets_beyond_32_bits(hip):
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
-@pytest.mark.parametrize("n,window,dim", [(100, 0, 64), (100, 40, 64), (3, 0, 128), (3, 60, 96), (70, 0, 256)])
-def test_what_is_no_number_reaches_the_rows_that_see_it_only(hip, dtype, n, window, dim):
+@pytest.mark.parametrize("n,window,dim,ctx", [(100, 0, 64, 300), (100, 40, 64, 300), (3, 0, 128, 300), (3, 60, 96, 300), (70, 0, 256, 300), (3, 0, 192, 3001),
+                                              (90, 0, 128, 2500)])
+def test_what_is_no_number_reaches_the_rows_that_see_it_only(hip, dtype, n, window, dim, ctx):
     """infinities and NaN among the keys and values of tokens that some rows see and earlier (or, behind a window, later) ones do not"""
     import torch
     rng = np.random.default_rng(n)
-    heads, kv, ctx = 8, 2, 300
+    heads, kv = 8, 2
     c = po.Cache(torch, rng, [ctx], 16, kv, dim, getattr(torch, dtype))
 
     def poison(host, token, head, d, value):

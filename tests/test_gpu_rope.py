@@ -82,7 +82,9 @@ def layout(contexts, news, torch):
     (32, 8, 128, 128, 2, "none", True, "float16", 16, "token"), (8, 8, 64, 32, 0, "yarn", False, "bfloat16", 5, "head"),
     (6, 2, 80, 80, 2, "factors", True, "float32", 1, "token"), (5, 1, 256, 64, 0, "linear", True, "float16", 64, "head"),
     (7, 7, 16, 16, 2, "none", False, "float32", 100, "head"), (12, 4, 112, 56, 2, "yarn_part", True, "bfloat16", 24, "token"),
-    (40, 8, 192, 192, 0, "none", False, "float16", 32, "token")])
+    (40, 8, 192, 192, 0, "none", False, "float16", 32, "token"), (9, 3, 176, 88, 0, "yarn", True, "bfloat16", 16, "token"),
+    (4, 4, 256, 256, 2, "linear", True, "float32", 7, "head"), (8, 2, 32, 32, 0, "none", True, "float16", 16, "token"),
+    (6, 1, 16, 8, 2, "factors", False, "bfloat16", 3, "head")])
 def test_store(hip, heads, kv, dim, dims, mode, scaling, normed, dtype, page, order):
     import torch
     from tensorsharp_amd import PagedKVCache
