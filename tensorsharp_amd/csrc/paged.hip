@@ -784,8 +784,9 @@ struct Attn {
             for (int d = 0; d < kDims; ++d) asm volatile("" : "+a"(o[d]));
         }
     }
-    // Whether one of the wavefront's rows has an infinity or NaN in its result.  The matrix instruction brings those of values to rows that do not see them (0 x
-    // NaN) and they stay, so they are looked for at the end, where rows may see different keys; such rows are done again by plainly().
+    // Whether one of the wavefront's rows has an infinity or NaN in its result.  The matrix instruction brings those of values to rows that do
+    // not see them, and an infinity meets the zero parts of what is cut; either leaves NaN (0 x infinity) that stays, so it is looked for at
+    // the end, and such rows are done again by plainly().
     __device__ __forceinline__ bool odd_result(int row) const
     {
         float z = 0.f;                                               // (a chain: a tree of comparisons takes registers from the loop)
@@ -853,14 +854,6 @@ struct Attn {
         if (!(sum > 0.f)) return 0.f;
         if (A.sinks) sum += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2e - top + kBias);
         return 1.0f / sum;
-    }
-
-    __device__ __forceinline__ bool odd_anywhere(bool odd, int wave) const
-    {
-        __shared__ int found[kAttnWaves];
-        if (lane == 0) found[wave] = odd;
-        __syncthreads();
-        return (found[0] | found[1] | found[2] | found[3]) != 0;
     }
 
     // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
@@ -1006,6 +999,7 @@ struct Attn {
     {
         const int begin = t.lo, end = t.hi;
         __shared__ f2_t states[kAttnWaves][32];
+        __shared__ int odd[kAttnWaves];
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_last = t.p0 + t.tokens - 1;
         const int lo_last = A.window > 0 ? p_last - A.window + 1 : 0;
@@ -1042,8 +1036,8 @@ struct Attn {
         }
         l = both_halves(l, added);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t.tokens > 1 && odd_anywhere(odd_result(col), wave)) return true;    // (one token's rows see the same keys)
         if (wave < kKeyWaves) {
+            if (const bool found = odd_result(col); lane == 0) odd[wave] = found;
             if (half == 0) states[wave][col] = f2_t{m, l};
             const lds_t row = lds + (wave * 32 + col) * HD * 4;
 #pragma unroll
@@ -1054,6 +1048,10 @@ struct Attn {
                         f4_t{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
         }
         __syncthreads();
+        int any = 0;
+#pragma unroll
+        for (int w = 0; w < kKeyWaves; ++w) any |= odd[w];
+        if (__builtin_amdgcn_readfirstlane(any)) return true;
         const int pieces = A.cache.head_dim / 4;
         for (int i = threadIdx.x; i < t.count * pieces; i += kAttnThreads) {
             const int row = i / pieces, piece = i - row * pieces;

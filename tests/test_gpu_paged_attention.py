@@ -228,9 +228,10 @@ def test_offsets_beyond_32_bits(hip):
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("n,window,dim,ctx", [(100, 0, 64, 300), (100, 40, 64, 300), (3, 0, 128, 300), (3, 60, 96, 300), (70, 0, 256, 300), (3, 0, 192, 3001),
-                                              (90, 0, 128, 2500)])
+                                              (90, 0, 128, 2500), (1, 0, 128, 300), (1, 0, 64, 5000), (1, 7, 80, 300)])
 def test_what_is_no_number_reaches_the_rows_that_see_it_only(hip, dtype, n, window, dim, ctx):
-    """infinities and NaN among the keys and values of tokens that some rows see and earlier (or, behind a window, later) ones do not"""
+    """infinities and NaN among the keys and values of tokens that some rows see and earlier (or, behind a window, later) ones do not; one
+    token sees them all (an infinite key gives a weight of zero or no number, by the sign of the query)"""
     import torch
     rng = np.random.default_rng(n)
     heads, kv = 8, 2
@@ -241,7 +242,7 @@ def test_what_is_no_number_reaches_the_rows_that_see_it_only(hip, dtype, n, wind
     poison(c.host[1], ctx - 2, 0, 3, np.inf)
     poison(c.host[1], ctx - 2, 0, dim - 1, -np.inf)
     poison(c.host[1], ctx - n // 2 - 1, 1, 0, np.nan)
-    poison(c.host[0], ctx - 1, 1, slice(None), np.nan)
+    poison(c.host[0], ctx - 1, 1, slice(None) if n > 1 else 2, np.nan if n > 1 else np.inf)
     if window:
         poison(c.host[1], ctx - window - 1, 1, 5, np.inf)
     c.k, c.v = (torch.from_numpy(t).cuda().to(c.dtype) for t in c.host)
