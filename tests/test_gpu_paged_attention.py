@@ -98,6 +98,21 @@ def test_attention(hip, heads, kv, dim, dtype, page, order, contexts, news, wind
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("dim", [192, 256])
+@pytest.mark.parametrize("news,contexts", [([1, 7, 1], [300, 129, 31]), ([130, 5], [700, 64]), ([20], [1200])])
+def test_large_heads(hip, dtype, dim, news, contexts):
+    """the sizes whose rows and accumulators fill the registers, with short and long tiles, cut and whole"""
+    import torch
+    rng = np.random.default_rng(dim + len(news))
+    heads, kv = 6, 2
+    c = po.Cache(torch, rng, contexts, 16, kv, dim, getattr(torch, dtype))
+    q = torch.from_numpy((2.0 * rng.standard_normal((sum(news), heads * dim))).astype(np.float32)).cuda()
+    for window in (0, 150):
+        out = run(hip, torch, c, q, news, contexts, dim ** -0.5, window)
+        check(out, c, q, news, contexts, heads, dim, dim ** -0.5, window, None)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("news,contexts", [([1, 1], [9000, 4100]), ([40], [5000]), ([2, 0, 70], [3001, 50, 2999])])
 def test_long_contexts(hip, dtype, news, contexts):
     """few rows and many keys: the keys are shared out and the parts joined"""
