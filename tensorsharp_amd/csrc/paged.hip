@@ -389,8 +389,8 @@ __device__ __forceinline__ void set_tile(const AttnArgs& A, const Lanes& L, int 
     t.row0 = tile * kTileRows;
     t.count = min(rows - t.row0, rows <= kKeyRows ? kKeyRows : kTileRows);
     const int p_first = t.p0 + (int)A.by_group.quot(t.row0), p_last = t.p0 + (int)A.by_group.quot(t.row0 + t.count - 1);
-    t.lo = A.window > 0 ? max(0, p_first - A.window + 1) : 0;
     t.hi = min(p_last + 1, A.capacity);
+    t.lo = min(first_key(p_first, A.window), max(0, t.hi));          // (a window may lie behind what the table has room for)
 }
 // keys of each piece of a tile, whole steps of 128
 __device__ __forceinline__ int piece_keys(const AttnTile& t) { return ((max(0, t.hi - t.lo) + 127) / 128 + t.cuts - 1) / t.cuts * 128; }
@@ -560,7 +560,7 @@ struct Attn {
         place(live ? row : 0, &token, &head);
         const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * A.cache.head_dim;
         p = t.p0 + token;
-        lo = A.window > 0 ? p - A.window + 1 : 0;
+        lo = first_key(p, A.window);
         if (!live) src = reinterpret_cast<const float*>(g_zero_row);
         auto eight = [&](int s, float (&x)[8]) {
             const float* at = (16 * s < A.cache.head_dim ? src : reinterpret_cast<const float*>(g_zero_row)) + 16 * s + 8 * half;
@@ -864,7 +864,7 @@ struct Attn {
             int token, head;
             place(row, &token, &head);
             const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
-            const int last = t.p0 + token, first = A.window > 0 ? last - A.window + 1 : 0;
+            const int last = t.p0 + token, first = first_key(last, A.window);
             float top = -INFINITY, sum = 0.f, acc[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
                 const int j = j0 + lane;
@@ -923,7 +923,7 @@ struct Attn {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_first = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave, t.count - 1));
         const int p_last = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave + 31, t.count - 1));
-        const int lo_last = A.window > 0 ? p_last - A.window + 1 : 0;
+        const int lo_last = first_key(p_last, A.window);
         constexpr int kKeys = 32 * NT, kMine = (NT * kCopies + kAttnWaves - 1) / kAttnWaves;
         auto stage = [&](const Rows& r, lds_t buffer) {
             const int ln = lane_here();
@@ -1001,7 +1001,7 @@ struct Attn {
         __shared__ int odd[kAttnWaves];
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int p_last = t.p0 + t.tokens - 1;
-        const int lo_last = A.window > 0 ? p_last - A.window + 1 : 0;
+        const int lo_last = first_key(p_last, A.window);
         const lds_t kb = lds + wave * 2 * kBlock, vb = kb + kBlock;
         int key0 = begin + 32 * wave;
         constexpr int kStride = 32 * kKeyWaves;

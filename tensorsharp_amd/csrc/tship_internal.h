@@ -310,6 +310,10 @@ struct FastDiv {
     __host__ __device__ uint32_t quot(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> shift); }
 };
 
+// First key that position p sees (window 0: all).  In 32 bits p - window + 1 wraps where a batch has more new tokens than the context holds
+// (p < 0) and the window is next to 2^31: such a position sees nothing in any case.
+__host__ __device__ constexpr int first_key(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
+
 // How the angles of a position come about: pair i turns by position * 2^(step i) [/ factors[i]] * (freq_scale (1 - kept_i) + kept_i)
 // radians, kept_i = ext (1 - clamp((i - low) / range, 0, 1)); cosine and sine are multiplied by size.
 struct RopeSpec {

@@ -1,0 +1,57 @@
+"""GPU: attention over pages at the ends of what its arguments may be."""
+import numpy as np
+import pytest
+
+import paged_oracle as po
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(torch, v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def attend(hip, torch, c, q, news, contexts, scale, window):
+    from tensorsharp_amd import PagedKVCache
+    out = torch.full_like(q, 7.5)
+    hip.PagedAttention(out, q, PagedKVCache(c.k, c.v, c.table_dev), i32(torch, np.concatenate([[0], np.cumsum(news)])), i32(torch, contexts), scale, window=window)
+    return out
+
+
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("heads,news,contexts", [(4, [5], [2]), (4, [8, 3, 2], [3, 3, 9]), (4, [60], [20]), (8, [200, 7], [130, 3]), (4, [3], [6000]), (4, [90], [5000])])
+def test_a_window_beyond_every_position_is_none(hip, heads, news, contexts, page):
+    """with more new tokens than the context holds as well: those in front of the sequence see nothing, the others what they see without a window"""
+    import torch
+    rng = np.random.default_rng(sum(news))
+    c = po.Cache(torch, rng, contexts, page, 2, 64, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((sum(news), heads * 64)).astype(np.float32)).cuda()
+    want = attend(hip, torch, c, q, news, contexts, 0.125, 0)
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, max(contexts)):
+        assert torch.equal(attend(hip, torch, c, q, news, contexts, 0.125, window), want), window
+    at = 0
+    for n, ctx in zip(news, contexts):
+        hidden = max(0, n - ctx)
+        assert torch.all(want[at:at + hidden] == 0) and torch.all(want[at + hidden:at + n].abs().sum(1) > 0)
+        at += n
+
+
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("n", [1, 100])
+def test_windows_behind_the_page_table(hip, n, page):
+    """a context far beyond what the table has room for: a window that ends in front of nothing that is there sees nothing"""
+    import torch
+    rng = np.random.default_rng(n)
+    c = po.Cache(torch, rng, [160], page, 2, 64, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((n, 256)).astype(np.float32)).cuda()
+    for context in (2 ** 31 - 1, 2 ** 31 - 50, 2 ** 30 + 5, 400):
+        for window in (1, 64):
+            assert torch.all(attend(hip, torch, c, q, [n], [context], 0.125, window) == 0), (context, window)
+    # all of them, and the last ones that are there
+    everything = attend(hip, torch, c, q, [n], [2 ** 31 - 1], 0.125, 0)
+    k, v = c.rows(0)
+    ref, _ = po.attend(q.cpu().numpy().astype(np.float64).reshape(n, 4, 64), k, v, np.full(n, 10 ** 6), 0.125)
+    assert np.abs(everything.cpu().numpy().reshape(n, 4, 64) - ref).max() < 1e-5
+    some = attend(hip, torch, c, q, [n], [200], 0.125, 120)
+    ref, _ = po.attend(q.cpu().numpy().astype(np.float64).reshape(n, 4, 64), k, v, np.arange(200 - n, 200), 0.125, 120)
+    assert np.abs(some.cpu().numpy().reshape(n, 4, 64) - ref).max() < 1e-5

@@ -1,0 +1,45 @@
+"""CPU: the whole-number arithmetic of the attention over pages, compiled for the host from the library's own header."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = """
+#include "tship_internal.h"
+#include <cstdio>
+#include <cstring>
+using namespace tship;
+int main(int argc, char** argv)
+{
+    long long a, b;
+    while (std::scanf("%lld %lld", &a, &b) == 2)
+        if (!std::strcmp(argv[1], "first_key")) std::printf("%d\\n", first_key((int)a, (int)b));
+        else return 1;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def compiled(tmp_path_factory):
+    where = tmp_path_factory.mktemp("arithmetic")
+    (where / "a.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-ftrapv", "-w", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(ROOT, "tensorsharp_amd", "csrc"),
+                    str(where / "a.cpp"), "-o", str(where / "a")], check=True)
+
+    def run(name, pairs):
+        text = "\n".join(f"{int(a)} {int(b)}" for a, b in pairs)
+        out = subprocess.run([str(where / "a"), name], input=text, capture_output=True, text=True, check=True).stdout
+        return [int(v) for v in out.split()]
+    return run
+
+
+def test_first_key_of_a_window(compiled):
+    """max(0, p - window + 1) as whole numbers without a width, for positions in front of the sequence and windows up to the largest too"""
+    edge = [0, 1, 2, 5, 127, 128, 129, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 2, 2 ** 31 - 1]
+    positions = edge + [-v for v in edge if v] + [-2 ** 31] + [int(v) for v in np.random.default_rng(0).integers(-2 ** 31, 2 ** 31, 50)]
+    pairs = [(p, w) for p in positions for w in edge]
+    for (p, w), got in zip(pairs, compiled("first_key", pairs)):
+        assert got == (max(0, p - w + 1) if w else 0), (p, w, got)
