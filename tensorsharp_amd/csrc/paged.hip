@@ -510,7 +510,7 @@ struct Attn {
     static constexpr int kSteps = HD / 16, kDims = HD / 32;
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
     static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU
-    static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD == 128);
+    static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD >= 128);
     static constexpr int kKeyWaves = key_waves_of(TYPE, HD);   // wavefronts that have keys of their own
     static constexpr int kBlock = 32 * kRow;                         // bytes of 32 keys
     static constexpr int kCopies = kPieces / 2;                      // wavefront-wide copies of 32 keys
@@ -603,9 +603,9 @@ struct Attn {
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {
                 q[i][s] = part[i];
-                // (large heads: what the accumulators leave of the accumulation registers holds rows, which the matrix instruction reads there
-                // as well; left to itself the compiler spills to memory, whose loads would wait for the copies under way)
-                if (kOneWave && kDims * 16 + (i + 1) * kSteps * 4 <= 256) asm volatile("" : "+a"(q[i][s]));
+                // (large heads: what the accumulators of the result and of the scores leave of the accumulation registers holds rows, which the matrix
+                // instruction reads there as well; left to itself the compiler spills to memory)
+                if (kOneWave && kDims * 16 + 16 + (i + 1) * kSteps * 4 <= 256) asm volatile("" : "+a"(q[i][s]));
             }
         }
         no_rows();
@@ -674,7 +674,7 @@ struct Attn {
         if constexpr (kPieces == 8) r = __builtin_amdgcn_update_dpp(r, (int)x, 0x150 + 8 + J, 0xf, 0xc, false);
         return (uint32_t)r;
     }
-    // the lane's number, for the copies of one step: where registers are short, their places are worked out at every step
+    // the lane's number: where registers are short, what follows from it is worked out at every step
     __device__ __forceinline__ int lane_here() const
     {
         int ln = lane;
@@ -705,11 +705,13 @@ struct Attn {
     __device__ __forceinline__ u4_t read16(lds_t at) const { return *reinterpret_cast<const __attribute__((address_space(3))) u4_t*>(at); }
     __device__ __forceinline__ float read4(lds_t at) const { return *reinterpret_cast<const __attribute__((address_space(3))) float*>(at); }
 
-    // S^T of 32 keys.  The products of an fp32 cache's parts below the first have an accumulator of their own, which leaves a sixth of the roundings
-    // at the size of the score: 2 rows at 7345 positions of 192 dimensions 5.1e-7 off, 1.0e-6 with one accumulator.  (Prompts take 1 to 5 % longer
-    // for it, answers of 192 and 256 dimensions 10 and 20 %, by registers.)
+    // S^T of 32 keys.  The products of an fp32 cache's parts below the first are summed apart from the large ones, which leaves a sixth of the roundings
+    // at the size of the score: 2 rows at 7345 positions of 192 dimensions 5.1e-7 off, 1.0e-6 in one sum.  Up to 192 dimensions they have an accumulator
+    // of their own; there are no registers for one beyond, and they go first, the keys being read a second time for the large ones (32 x 4096 positions of
+    // 256 dimensions 675 us, a prompt of 1024 1005; with an accumulator of their own 60 to 90 registers are spilled, 777 and 950).
     __device__ __forceinline__ f16_t scores(lds_t block) const
     {
+        constexpr bool kTwoSums = TYPE == 0 && HD <= 192, kTwoPasses = TYPE == 0 && HD > 192;
         f16_t s, below;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = below[i] = 0.f;
@@ -717,39 +719,63 @@ struct Attn {
         const int x = k_swizzle(col);
         // (the swizzle changes the lower bits of a piece's number only, so that one address serves every kAgain-th step)
         constexpr int kAgain = (kPieces % 8 == 0 ? 8 : 4) / (TYPE == 0 ? 4 : 2);
+        auto eight = [&](int i, float (&v)[8]) {
+            const int j = i % kAgain, further = (i - j) * 64;
+            const u4_t a0 = read16(row + (((4 * j + 2 * half) ^ x) << 4) + further), a1 = read16(row + (((4 * j + 2 * half + 1) ^ x) << 4) + further);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                v[n] = __uint_as_float(a0[n]);
+                v[4 + n] = __uint_as_float(a1[n]);
+            }
+        };
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const int j = i % kAgain, further = (i - j) * (TYPE == 0 ? 64 : 32);
             if constexpr (TYPE != 0) {
+                const int j = i % kAgain, further = (i - j) * 32;
                 const u4_t a = read16(row + (((2 * j + half) ^ x) << 4) + further);
 #pragma unroll
                 for (int n = 0; n < kParts; ++n) s = mfma(a, q[n][i], s);
             } else {
-                const u4_t a0 = read16(row + (((4 * j + 2 * half) ^ x) << 4) + further), a1 = read16(row + (((4 * j + 2 * half + 1) ^ x) << 4) + further);
+                step_here();
                 float v[8];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    v[n] = __uint_as_float(a0[n]);
-                    v[4 + n] = __uint_as_float(a1[n]);
-                }
+                eight(i, v);
                 u4_t a[3];
                 cut3(v, a);
-                below = mfma(a[2], q[0][i], below);
-                below = mfma(a[1], q[1][i], below);
-                below = mfma(a[0], q[2][i], below);
-                below = mfma(a[1], q[0][i], below);
-                below = mfma(a[0], q[1][i], below);
-                s = mfma(a[0], q[0][i], s);
+                f16_t& small = kTwoSums ? below : s;
+                small = mfma(a[2], q[0][i], small);
+                small = mfma(a[1], q[1][i], small);
+                small = mfma(a[0], q[2][i], small);
+                small = mfma(a[1], q[0][i], small);
+                small = mfma(a[0], q[1][i], small);
+                if constexpr (kTwoSums) s = mfma(a[0], q[0][i], s);
             }
         }
-        if constexpr (TYPE == 0) s += below;
+        if constexpr (kTwoSums) s += below;
+        if constexpr (kTwoPasses) {
+            asm volatile("" ::: "memory");                           // (the parts of all steps do not fit)
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                step_here();
+                float v[8];
+                eight(i, v);
+                const u4_t a = {high_halves(v[0], v[1]), high_halves(v[2], v[3]), high_halves(v[4], v[5]), high_halves(v[6], v[7])};
+                s = mfma(a, q[0][i], s);
+            }
+        }
         return s;
+    }
+    // Where registers are short, a step's reads stay behind the step before.  No instantiation may spill vector registers: of a spilled operand the
+    // compiler has brought back three of the four registers (of a second part of q, results 2e-3 off).
+    __device__ __forceinline__ static void step_here()
+    {
+        if constexpr (TYPE == 0 && HD == 128) __builtin_amdgcn_sched_barrier(0);
     }
     // Of the 16 scores of a lane number i belongs to key 8 (i / 4) + 4 half + i % 4 of the block.
     __device__ __forceinline__ void mask(f16_t& s, int key0, uint64_t there) const
     {
-        const uint32_t bits = (uint32_t)(there >> (4 * half));
-        const int last = p - key0 - 4 * half, first = lo - key0 - 4 * half;
+        const int below = 4 * (lane_here() >> 5);
+        const uint32_t bits = (uint32_t)(there >> below);
+        const int last = p - key0 - below, first = lo - key0 - below;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int k = 8 * (i / 4) + i % 4;
@@ -813,6 +839,7 @@ struct Attn {
             else cut3(w, part);
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
+                step_here();
                 if constexpr (TYPE != 0) {
                     // a lane gives the place of four dimensions of one key and gets one dimension of four keys, within 16 lanes
                     const int piece = (4 * (d & 1) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ x;
@@ -967,7 +994,7 @@ struct Attn {
         } else {
             no_rows();
         }
-        const int row = 32 * wave + col;
+        const int row = 32 * wave + (lane_here() & 31);
         if (odd_result(row)) return true;
         l = both_halves(l, added);
         if (row >= t.count) return false;
