@@ -537,7 +537,7 @@ struct Attn {
     lds_t lds;
     u4_t q[kParts][kSteps];
     f16_t o[kDims];
-    float c, m, l;                   // score to exponent, running maximum (as an exponent), this lane's part of the sum
+    float c, m, l, l_rest;           // score to exponent, running maximum (as an exponent), this lane's part of the sum and what its roundings left
     int p, lo;                       // position of this lane's row, first key it sees
 
     __device__ __forceinline__ Attn(const AttnArgs& args, const AttnTile& tile, int kv_head, lds_t smem)
@@ -618,7 +618,7 @@ struct Attn {
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
         m = -INFINITY;
-        l = 0.f;
+        l = l_rest = 0.f;
         stay();
     }
 
@@ -793,6 +793,7 @@ struct Attn {
         if (__any(top > m + kSlack)) {                               // (m starts at -infinity)
             const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             l *= f;
+            l_rest *= f;
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -821,9 +822,18 @@ struct Attn {
             for (int i = 0; i < 16; ++i) z = __builtin_fmaf(o[d][i], 0.f, z);
         return __any(row < t.count && z != z);
     }
-    // weights of a block's scores, their sum, and O^T += V^T P^T
-    __device__ __forceinline__ void weigh(const f16_t& s, lds_t block)
+    // The sum of the weights goes over all keys of a row, one step after the other.  Small weights beside a large sum lose the same bits at every step
+    // (4096 keys 16 e-folds below the first one: 4e-4 of the sum), so what each addition rounds away is kept and added at the end.
+    __device__ __forceinline__ void add_weights(float sum)
     {
+        const float large = fmaxf(l, sum), small = fminf(l, sum);
+        l = large + small;
+        l_rest += small - (l - large);
+    }
+    // weights of a block's scores, and O^T += V^T P^T; returns their sum
+    __device__ __forceinline__ float weigh(const f16_t& s, lds_t block)
+    {
+        float sum = 0.f;
         const float bias = kBias - (m == -INFINITY ? 0.f : m);
         const int x = v_swizzle((lane & 15) >> 2);
 #pragma unroll
@@ -832,7 +842,7 @@ struct Attn {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * h + i], c, bias));
-                l += w[i];
+                sum += w[i];
             }
             u4_t part[kParts];
             if constexpr (TYPE == 1) cut2(w, part);
@@ -869,6 +879,7 @@ struct Attn {
                 }
             }
         }
+        return sum;
     }
 
     // ---- where a row's state goes ----
@@ -986,8 +997,10 @@ struct Attn {
                         for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b));
                     }
                     follow_maximum(s, NT);
+                    float sum = 0.f;
 #pragma unroll
-                    for (int b = 0; b < NT; ++b) weigh(s[b], here + (NT + b) * kBlock);
+                    for (int b = 0; b < NT; ++b) sum += weigh(s[b], here + (NT + b) * kBlock);
+                    add_weights(sum);
                 }
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the last copies, before this LDS may be another workgroup's
@@ -996,7 +1009,7 @@ struct Attn {
         }
         const int row = 32 * wave + (lane_here() & 31);
         if (odd_result(row)) return true;
-        l = both_halves(l, added);
+        l = both_halves(l + l_rest, added);
         if (row >= t.count) return false;
         int token, head;
         place(row, &token, &head);
@@ -1052,7 +1065,7 @@ struct Attn {
                 if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
                 follow_maximum(s, 1);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");                 // the values too: the next keys are left
-                weigh(s[0], vb);
+                add_weights(weigh(s[0], vb));
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::true_type(), rows.v, vb);
             }
@@ -1060,7 +1073,7 @@ struct Attn {
         else {
             no_rows();
         }
-        l = both_halves(l, added);
+        l = both_halves(l + l_rest, added);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (wave < kKeyWaves) {
             if (const bool found = odd_result(col); lane == 0) odd[wave] = found;

@@ -1,0 +1,90 @@
+"""GPU: what the softmax weights of the attention over pages keep of their bits.
+
+Bounds.  Where one product makes a score it is exact; the exponent's argument rounds twice relative to the score (the scale in powers of two, the
+fused product) and once to its own size, the exponential once: 2^-24 (2 |s| + 4) of each weight, twice that of a result (its sum has the same).  Weights
+and their sum add the 2^-20 of sum p |v| of test_gpu_paged_attention.py: all of a row's weights keep that, however small they are against its largest.
+The weighted values of a long run of keys are summed in 32 bits, 16 keys and one part of the weights (six products of parts in fp32) at a time: each of these
+additions rounds by at most 2^-24 of what is summed by then, which is no more than the whole (`additions`)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(torch, v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def one_sequence(torch, k, v, page):
+    """k, v [positions, kv heads, dim] into pages in reverse order"""
+    from tensorsharp_amd import PagedKVCache
+    n, kv, dim = k.shape
+    pages = -(-n // page)
+    put = [torch.zeros((pages, page, kv, dim), dtype=k.dtype, device="cuda") for _ in range(2)]
+    for to, t in zip(put, (k, v)):
+        padded = torch.zeros((pages * page, kv, dim), dtype=k.dtype, device="cuda")
+        padded[:n] = t
+        to.copy_(padded.view(pages, page, kv, dim).flip(0))
+    return PagedKVCache(*put, torch.arange(pages - 1, -1, -1, dtype=torch.int32, device="cuda")[None])
+
+
+def attend(hip, torch, q, cache, contexts, scale):
+    """a sequence over the same pages for every context"""
+    from tensorsharp_amd import PagedKVCache
+    out = torch.full_like(q, 7.5)
+    seqs = len(contexts)
+    starts = np.arange(seqs + 1) * (len(q) // seqs)
+    if seqs > 1:
+        cache = PagedKVCache(cache.k, cache.v, cache.page_table.expand(seqs, -1).contiguous())
+    hip.PagedAttention(out, q, cache, i32(torch, starts), i32(torch, contexts), scale)
+    return out
+
+
+def additions(dtype, keys, together):
+    """roundings of a run of keys: one that all wavefronts take together, or that at least two share out between them"""
+    return 2.0 ** -24 * (keys if together else keys / 2) / 16 * {"float16": 2, "bfloat16": 3, "float32": 6}[dtype]
+
+
+def definition(q, k, v, position, sink=None):
+    """one head; q [rows], k [keys]: the one dimension that is not zero; v [keys, dim]"""
+    ref, size = (np.zeros((len(q),) + v.shape[1:]) for _ in range(2))
+    for r in range(len(q)):
+        s = q[r] * k[:position[r] + 1]
+        m = s.max() if sink is None else max(s.max(), sink)
+        w = np.exp(s - m)
+        total = w.sum() + (0.0 if sink is None else np.exp(sink - m))
+        ref[r], size[r] = w @ v[:position[r] + 1] / total, w @ np.abs(v[:position[r] + 1]) / total
+    return ref, size
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("gap", [4.0, 8.0, 12.0, 16.0, 20.0, 23.0, 30.0, 40.0])
+@pytest.mark.parametrize("rows,seqs,ctx", [(300, 1, 16384), (4, 4, 16384), (1, 1, 40000), (160, 1, 3000)])
+def test_a_key_that_takes_nearly_all(hip, dtype, gap, rows, seqs, ctx):
+    """the first key (or one in the middle) stands `gap` above the others, which are alike or nearly so, and has the value 0 or 0.05: what is left
+    of the result is the others', to the last bits of each (256 KV heads leave the keys of 300 rows, or 4 sequences, in one piece)"""
+    import torch
+    rng = np.random.default_rng(int(gap) + rows)
+    kv, dim = (256, 16) if ctx == 16384 else (2, 64)
+    heads = [0, kv // 2, kv - 1]
+    at = [0, 0, ctx // 2 + 7] if rows < ctx // 2 - 8 else [0, 0, 0]
+    k = torch.zeros((ctx, kv, dim), device="cuda")
+    v = torch.randn((ctx, kv, dim), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 0.5 + 1.0
+    k[:, heads[1]:, 3] = torch.from_numpy(rng.uniform(-0.5, 0.5, ctx).astype(np.float32)).cuda()[:, None]
+    for h, a in zip(heads, at):
+        k[a, h, 3] = gap
+        v[a, h] = 0.0 if h != heads[1] else 0.05
+    k, v = (t.to(getattr(torch, dtype)) for t in (k, v))
+    q = torch.zeros((rows, kv, dim), device="cuda")
+    q[:, :, 3] = torch.from_numpy(rng.choice([1.0, 0.75, 0.5], rows).astype(np.float32)).cuda()[:, None] if rows > 1 else 1.0
+    contexts = [ctx - 5 * i for i in range(seqs)]
+    cache = one_sequence(torch, k, v, 16)
+    out = attend(hip, torch, q.view(rows, -1), cache, contexts, 1.0).view(rows, kv, dim).double().cpu().numpy()
+    some = np.unique(np.linspace(0, rows - 1, 12).astype(int))
+    position = np.concatenate([np.arange(c - rows // seqs, c) for c in contexts])
+    for h in heads:
+        kh, vh, qh = k[:, h, 3].double().cpu().numpy(), v[:, h].double().cpu().numpy(), q[some, h, 3].double().cpu().numpy()
+        ref, size = definition(qh, kh, vh, position[some])
+        most = (np.abs(qh) * np.abs(kh).max())[:, None]
+        d = np.abs(out[some, h] - ref)
+        assert np.all(d <= (2.0 ** -23 * (2 * most + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size), (h, float((d / size).max()))
