@@ -222,12 +222,20 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 // own), or three of bf16 (24 bits), and an fp32 cache likewise when it is read from LDS.  Products per element of a score: 2 for an fp16 cache,
 // 3 for bf16, 6 for fp32 (those above 2^-24).
 //
+// m need not be the maximum: weights are 2^kUnit times what they are against m, a whole number that follows when a step's largest score is more
+// than kRise above it, so that the accumulators are rescaled (exactly) a few times a row and not at every step.  In two parts of fp16 a weight's last
+// bit is 2^-24, so below 2^-2 it has not all of its own.  For an fp16 cache m therefore lies kAhead above the largest score that it was set by,
+// whose weight is 2^8 then, grows up to 2^15 and falls down to 2^1 (kFall below m) before m follows - down too: the keys behind one that takes nearly
+// all have the same bits as before it, however little they count.
+//
 // Sequences with at most 32 rows (answers): all wavefronts have the same rows and walk over different keys, each through LDS of its
 // own, and meet at the end.  Others (prompts): tiles of 128 rows, each wavefront has 32 of them and all share the keys in LDS.
 // With few tiles the keys are cut further over workgroups, whose states paged_combine_kernel joins.
 
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef float f16_t __attribute__((ext_vector_type(16)));
@@ -238,11 +246,6 @@ constexpr int kAttnWaves = 4, kAttnThreads = 64 * kAttnWaves;
 constexpr int kKeyRows = 32;         // rows of a sequence up to which its wavefronts share rows and not keys
 constexpr int kTileRows = 32 * kAttnWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
-// Weights are kept as 2^7 times what they are against the running maximum, which follows the true one only when that is 2^8 larger:
-// they stay below 2^15, which fp16 holds, the accumulators are rescaled a few times a row instead of at every step, and weights down to
-// 2^-21 of the largest have all their 22 bits.
-constexpr float kBias = 7.f, kSlack = 8.f;
-
 // rows that a lane's page has not (past the end, or no page at all) are read from here
 __device__ __attribute__((aligned(16))) uint8_t g_zero_row[kMaxDim * 4];
 
@@ -250,7 +253,7 @@ struct AttnArgs {
     const float* query;
     float* out;
     const float* sinks;
-    float* partial;              // [piece][KV head][row of the tile][head_dim] weighted values, then [piece][KV head][row] (maximum, sum)
+    float* partial;              // [piece][KV head][row of the tile][head_dim] weighted values, then [piece][KV head][row] (unit, sum)
     int64_t ld_query, ld_out;
     float c;                     // |scale| log2 e
     float sign;                  // of scale, 0 where it is 0
@@ -433,6 +436,15 @@ __device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int
     t.lo = begin;
     return true;
 }
+// What a row's weighted values are multiplied by: 1 / (sum + the sink's weight), sum being counted in units of 2^unit; 1 / 0 never.  (The sink may be far
+// above the units that m came down to.)
+__device__ __forceinline__ float over_sum(const AttnArgs& A, float sum, float unit, int head)
+{
+    if (!(sum > 0.f)) return 0.f;
+    if (!A.sinks) return 1.0f / sum;
+    const float e = A.sinks[head] * kLog2e - unit, h = fmaxf(e, 0.f), by = __builtin_amdgcn_exp2f(-h);
+    return by / (sum * by + __builtin_amdgcn_exp2f(e - h));
+}
 // the tile of a row and head and its first piece; false: of no sequence
 __device__ __forceinline__ bool find_row(const Lens& H, const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)
 {
@@ -470,13 +482,13 @@ __device__ __forceinline__ void cut3(const float (&x)[8], u4_t (&part)[3])
         part[2][i] = high_halves(below_bf16(y0), below_bf16(y1));
     }
 }
-// eight floats in fp16's range as twice eight fp16: what two roundings towards zero leave is below 2^-20 of each
+// eight floats in fp16's range as twice eight fp16, both to nearest: what is left is below 2^-24 of each, or 2^-25 where that is more
 __device__ __forceinline__ void cut2(const float (&x)[8], u4_t (&part)[2])
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const auto hi = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-        const auto lo = __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)hi[0], x[2 * i + 1] - (float)hi[1]);
+        const h2_t hi = __builtin_convertvector((f2_t{x[2 * i], x[2 * i + 1]}), h2_t);
+        const h2_t lo = __builtin_convertvector((f2_t{x[2 * i] - (float)hi[0], x[2 * i + 1] - (float)hi[1]}), h2_t);
         part[0][i] = __builtin_bit_cast(uint32_t, hi);
         part[1][i] = __builtin_bit_cast(uint32_t, lo);
     }
@@ -508,6 +520,8 @@ struct Attn {
     static constexpr int kParts = TYPE == 1 ? 2 : 3;                 // of q and of the weights
     static constexpr int kCacheParts = TYPE == 0 ? 3 : 1;
     static constexpr int kSteps = HD / 16, kDims = HD / 32;
+    // of the weights, as exponents (see above)
+    static constexpr float kUnit = TYPE == 1 ? 15.f : 7.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 14.f, kMost = 64.f, kApart = 20.f;
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
     static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU
     static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD >= 128);
@@ -537,7 +551,8 @@ struct Attn {
     lds_t lds;
     u4_t q[kParts][kSteps];
     f16_t o[kDims];
-    float c, m, l, l_rest;           // score to exponent, running maximum (as an exponent), this lane's part of the sum and what its roundings left
+    float c, m, l, l_rest;           // score to exponent, what weights are counted against, this lane's part of their sum and what its roundings left
+    float low;                       // fp16: a step's largest score below this takes m with it
     int p, lo;                       // position of this lane's row, first key it sees
 
     __device__ __forceinline__ Attn(const AttnArgs& args, const AttnTile& tile, int kv_head, lds_t smem)
@@ -617,7 +632,7 @@ struct Attn {
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-        m = -INFINITY;
+        m = low = -INFINITY;
         l = l_rest = 0.f;
         stay();
     }
@@ -782,16 +797,33 @@ struct Attn {
             if (k > last || k < first || !((bits >> k) & 1)) s[i] = -INFINITY;
         }
     }
-    __device__ __forceinline__ void follow_maximum(const f16_t* s, int blocks)
+    // Returns whether (fp16) a step's largest score, which m rose for, stands kApart above the row's others.
+    __device__ __forceinline__ bool follow_maximum(const f16_t* s, int blocks)
     {
+        bool apart = false;
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < blocks; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
         top = both_halves(top, larger) * c;
-        if (__any(top > m + kSlack)) {                               // (m starts at -infinity)
-            const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        const bool above = top > m + kRise, below = TYPE == 1 && top < low && top > -INFINITY;
+        if (__any(above || below)) {                                 // (m starts at -infinity)
+            float mn = m;
+            if (above) mn = __builtin_ceilf(top) + kAhead;
+            if constexpr (TYPE == 1) {
+                if (above) low = mn - kFall;
+                const float others = others_of(s[0]) * c;
+                apart = __any(above && others > -INFINITY && top - others > kApart);
+                // (not so far down that the sum passes 2^kMost: with values up to 2^16 the accumulators stay finite)
+                const float least = m - fmaxf(0.f, kMost - (float)__builtin_amdgcn_frexp_expf(both_halves(l, larger)));
+                if (below) {
+                    mn = __builtin_ceilf(top) + kAhead;
+                    low = mn - kFall;
+                    if (mn < least) mn = least, low = -INFINITY;
+                }
+            }
+            const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             l *= f;
             l_rest *= f;
 #pragma unroll
@@ -801,6 +833,57 @@ struct Attn {
             m = mn;
         }
         stay();
+        return apart;
+    }
+    // a score that all but one or two of a row's in a step are certain to be below if it is far below the largest: the lower of the maxima of eight keys
+    // and eight others
+    __device__ __forceinline__ float others_of(const f16_t& s) const
+    {
+        const float a = fmaxf(fmaxf(s[1], s[6]), fmaxf(s[11], s[12])), b = fmaxf(fmaxf(s[3], s[4]), fmaxf(s[9], s[14]));
+        return fminf(both_halves(a, larger), both_halves(b, larger));
+    }
+    // Where one or two keys of a step stand kApart above its others, these would have few bits of their own in fp16 (and where the large ones' values are 0,
+    // as those of a first token that takes what no other key asks for nearly are, the others are the result).  The large ones, at most two, are weighed in 32
+    // bits by themselves, and m follows what is left.  Looked for where m rises, so that it costs nothing at other steps (32 x 4096 positions of 128
+    // dimensions 103.5 -> 103.4 us, a prompt's chunk of 512 at 4096 79.8 -> 80.7).
+    __device__ __forceinline__ void take_apart(f16_t* s, int blocks, lds_t values)
+    {
+        const float others = others_of(s[0]) * c;
+        for (int n = 0; n < 2; ++n) {
+            float big = -INFINITY;
+            int at = 0;
+#pragma unroll
+            for (int b = 0; b < blocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (s[b][i] > big) {
+                        big = s[b][i];
+                        at = 32 * b + 8 * (i / 4) + i % 4;
+                    }
+            const u2_t bigs = __builtin_amdgcn_permlane32_swap(__float_as_uint(big), __float_as_uint(big), false, false);
+            at += 4 * half;
+            const u2_t ats = __builtin_amdgcn_permlane32_swap(at, at, false, false);
+            const int from = __uint_as_float(bigs.x) >= __uint_as_float(bigs.y) ? 0 : 1, key = from ? (int)ats.y : (int)ats.x;
+            big = __uint_as_float(from ? bigs.y : bigs.x) * c;
+            if (!(others > -INFINITY && big - others > kApart)) continue;                   // (a lane whose row is not like this)
+            const float w = __builtin_amdgcn_exp2f(big - (m - kUnit));
+            if (half == 0) add_weights(w);
+#pragma unroll
+            for (int b = 0; b < blocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (half == from && 32 * b + 8 * (i / 4) + i % 4 + 4 * half == key) s[b][i] = -INFINITY;
+            const lds_t row = values + key * kRow + half * 8;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const h4_t v = *reinterpret_cast<const __attribute__((address_space(3))) h4_t*>(row + (((4 * d + i) ^ v_swizzle(key)) << 4));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[d][4 * i + j] = __builtin_fmaf(w, (float)v[j], o[d][4 * i + j]);
+                }
+        }
+        follow_maximum(s, blocks);
     }
     // large heads: the accumulators stay in accumulation registers from one step to the next
     __device__ __forceinline__ void stay()
@@ -834,7 +917,7 @@ struct Attn {
     __device__ __forceinline__ float weigh(const f16_t& s, lds_t block)
     {
         float sum = 0.f;
-        const float bias = kBias - (m == -INFINITY ? 0.f : m);
+        const float bias = kUnit - (m == -INFINITY ? 0.f : m);
         const int x = v_swizzle((lane & 15) >> 2);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                                // 16 keys
@@ -885,14 +968,6 @@ struct Attn {
     // ---- where a row's state goes ----
     __device__ __forceinline__ float* values_of(int row) const { return A.partial + slot_row(A, t.slot, kvh, row) * A.cache.head_dim; }
     __device__ __forceinline__ f2_t* state_of(int row) const { return states_of(A) + slot_row(A, t.slot, kvh, row); }
-    // what a row's sum is divided by: with the sink, 1 / 0 never
-    __device__ __forceinline__ float over_sum(float sum, float top, int head) const
-    {
-        if (!(sum > 0.f)) return 0.f;
-        if (A.sinks) sum += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2e - top + kBias);
-        return 1.0f / sum;
-    }
-
     // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
     // 64) for the values.  Slow, for rows with infinities or NaN in their results.
     __device__ __forceinline__ void plainly(int row, int step)
@@ -923,7 +998,7 @@ struct Attn {
                 float most = score;
                 for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
                 const float mn = fmaxf(top, most), base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
-                const float w = seen ? __builtin_amdgcn_exp2f(score - base + kBias) : 0.f;
+                const float w = seen ? __builtin_amdgcn_exp2f(score - base + kUnit) : 0.f;
                 float all = w;
                 for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
                 sum = sum * f + all;
@@ -940,11 +1015,11 @@ struct Attn {
                 }
             }
             float* dst = t.cuts == 1 ? A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * dim : values_of(row);
-            const float by = t.cuts == 1 ? over_sum(sum, top, head) : 1.f;
+            const float by = t.cuts == 1 ? over_sum(A, sum, top - kUnit, head) : 1.f;
 #pragma unroll
             for (int i = 0; i <= HD / 64; ++i)
                 if (64 * i + lane < dim) dst[64 * i + lane] = acc[i] * by;
-            if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top, sum};
+            if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top - kUnit, sum};
         }
     }
     __device__ __forceinline__ float element(const char* base, int64_t at) const
@@ -996,7 +1071,9 @@ struct Attn {
 #pragma unroll
                         for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b));
                     }
-                    follow_maximum(s, NT);
+                    const bool apart = follow_maximum(s, NT);
+                    if constexpr (TYPE == 1)
+                        if (__builtin_expect(apart, false)) take_apart(s, NT, here + NT * kBlock);
                     float sum = 0.f;
 #pragma unroll
                     for (int b = 0; b < NT; ++b) sum += weigh(s[b], here + (NT + b) * kBlock);
@@ -1017,10 +1094,10 @@ struct Attn {
         float by = 1.f;
         if (t.cuts == 1) {
             dst = A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim;
-            by = over_sum(l, m, head);
+            by = over_sum(A, l, m - kUnit, head);
         } else {
             dst = values_of(row);
-            if (half == 0) *state_of(row) = f2_t{m, l};
+            if (half == 0) *state_of(row) = f2_t{m - kUnit, l};
         }
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
@@ -1063,8 +1140,10 @@ struct Attn {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::false_type(), rows.k, kb);
                 if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
-                follow_maximum(s, 1);
+                const bool apart = follow_maximum(s, 1);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");                 // the values too: the next keys are left
+                if constexpr (TYPE == 1)
+                    if (__builtin_expect(apart, false)) take_apart(s, 1, vb);
                 add_weights(weigh(s[0], vb));
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::true_type(), rows.v, vb);
@@ -1077,7 +1156,7 @@ struct Attn {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (wave < kKeyWaves) {
             if (const bool found = odd_result(col); lane == 0) odd[wave] = found;
-            if (half == 0) states[wave][col] = f2_t{m, l};
+            if (half == 0) states[wave][col] = f2_t{m - kUnit, l};
             const lds_t row = lds + (wave * 32 + col) * HD * 4;
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
@@ -1110,7 +1189,7 @@ struct Attn {
             place(row, &token, &head);
             if (t.cuts == 1) {
                 *reinterpret_cast<f4_t*>(A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim + 4 * piece) =
-                    v * over_sum(sum, top, head);
+                    v * over_sum(A, sum, top, head);
             } else {
                 *reinterpret_cast<f4_t*>(values_of(row) + 4 * piece) = v;
                 if (piece == 0) *state_of(row) = f2_t{top, sum};
@@ -1207,12 +1286,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
         for (int w = 1; w < WAVES; ++w) join(sums[w].x, sums[w].y, values_in[w][lane]);
     }
     if (!mine) return;
-    float by = 0.f;
-    if (sum > 0.f) {
-        if (A.sinks) sum += __builtin_amdgcn_exp2f(A.sinks[head] * kLog2e - top + kBias);
-        by = 1.0f / sum;
-    }
-    *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * by;
+    *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * over_sum(A, sum, top, head);
 }
 
 }  // namespace

@@ -28,7 +28,7 @@ def one_sequence(torch, k, v, page):
     return PagedKVCache(*put, torch.arange(pages - 1, -1, -1, dtype=torch.int32, device="cuda")[None])
 
 
-def attend(hip, torch, q, cache, contexts, scale):
+def attend(hip, torch, q, cache, contexts, scale, sinks=None):
     """a sequence over the same pages for every context"""
     from tensorsharp_amd import PagedKVCache
     out = torch.full_like(q, 7.5)
@@ -36,7 +36,7 @@ def attend(hip, torch, q, cache, contexts, scale):
     starts = np.arange(seqs + 1) * (len(q) // seqs)
     if seqs > 1:
         cache = PagedKVCache(cache.k, cache.v, cache.page_table.expand(seqs, -1).contiguous())
-    hip.PagedAttention(out, q, cache, i32(torch, starts), i32(torch, contexts), scale)
+    hip.PagedAttention(out, q, cache, i32(torch, starts), i32(torch, contexts), scale, sinks=sinks)
     return out
 
 
@@ -57,12 +57,13 @@ def definition(q, k, v, position, sink=None):
     return ref, size
 
 
-@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("gap", [4.0, 8.0, 12.0, 16.0, 20.0, 23.0, 30.0, 40.0])
-@pytest.mark.parametrize("rows,seqs,ctx", [(300, 1, 16384), (4, 4, 16384), (1, 1, 40000), (160, 1, 3000)])
-def test_a_key_that_takes_nearly_all(hip, dtype, gap, rows, seqs, ctx):
-    """the first key (or one in the middle) stands `gap` above the others, which are alike or nearly so, and has the value 0 or 0.05: what is left
-    of the result is the others', to the last bits of each (256 KV heads leave the keys of 300 rows, or 4 sequences, in one piece)"""
+@pytest.mark.parametrize("rows,seqs,ctx", [(300, 1, 16384), (4, 4, 16384), (1, 1, 40000), (160, 1, 3000), (50, 1, 60)])
+@pytest.mark.parametrize("count", [1, 2])
+def test_keys_that_take_nearly_all(hip, dtype, gap, rows, seqs, ctx, count):
+    """the first key (or one in the middle), and one that is nine behind it, stand `gap` above the others, which are alike or nearly so, and have the value
+    0 or 0.05: what is left of the result is the others', to the last bits of each (256 KV heads leave the keys of 300 rows, or 4 sequences, in one piece)"""
     import torch
     rng = np.random.default_rng(int(gap) + rows)
     kv, dim = (256, 16) if ctx == 16384 else (2, 64)
@@ -72,8 +73,8 @@ def test_a_key_that_takes_nearly_all(hip, dtype, gap, rows, seqs, ctx):
     v = torch.randn((ctx, kv, dim), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 0.5 + 1.0
     k[:, heads[1]:, 3] = torch.from_numpy(rng.uniform(-0.5, 0.5, ctx).astype(np.float32)).cuda()[:, None]
     for h, a in zip(heads, at):
-        k[a, h, 3] = gap
-        v[a, h] = 0.0 if h != heads[1] else 0.05
+        k[a:a + 9 * count:9, h, 3] = gap
+        v[a:a + 9 * count:9, h] = 0.0 if h != heads[1] else 0.05
     k, v = (t.to(getattr(torch, dtype)) for t in (k, v))
     q = torch.zeros((rows, kv, dim), device="cuda")
     q[:, :, 3] = torch.from_numpy(rng.choice([1.0, 0.75, 0.5], rows).astype(np.float32)).cuda()[:, None] if rows > 1 else 1.0
@@ -88,3 +89,26 @@ def test_a_key_that_takes_nearly_all(hip, dtype, gap, rows, seqs, ctx):
         most = (np.abs(qh) * np.abs(kh).max())[:, None]
         d = np.abs(out[some, h] - ref)
         assert np.all(d <= (2.0 ** -23 * (2 * most + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size), (h, float((d / size).max()))
+
+
+@pytest.mark.parametrize("sink", [-200.0, -30.0, 0.0, 30.0, 60.0, 200.0])
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("rows,ctx", [(1, 300), (100, 300), (1, 9000)])
+def test_a_sink_far_above_or_below_the_scores(hip, dtype, sink, rows, ctx):
+    import torch
+    rng = np.random.default_rng(7)
+    k = torch.zeros((ctx, 2, 64), device="cuda")
+    k[:, :, 5] = torch.from_numpy(rng.uniform(-2, 2, (ctx, 2)).astype(np.float32)).cuda()
+    k[3, 0, 5] = 25.0
+    v = torch.from_numpy(rng.standard_normal((ctx, 2, 64)).astype(np.float32)).cuda() + 1.0
+    v[3, 0] = 0.0
+    k, v = (t.to(getattr(torch, dtype)) for t in (k, v))
+    q = torch.zeros((rows, 2, 64), device="cuda")
+    q[:, :, 5] = 1.0
+    out = attend(hip, torch, q.view(rows, -1), one_sequence(torch, k, v, 16), [ctx], 1.0, torch.full((2,), sink, device="cuda"))
+    out = out.view(rows, 2, 64).double().cpu().numpy()
+    for h in range(2):
+        kh, vh = k[:, h, 5].double().cpu().numpy(), v[:, h].double().cpu().numpy()
+        ref, size = definition(np.ones(rows), kh, vh, np.arange(ctx - rows, ctx), sink)
+        room = (2.0 ** -23 * (2 * max(abs(sink), 25.0) + 4) + 2.0 ** -20) * size + additions(dtype, ctx, rows > 32) * size + 2.0 ** -126
+        assert np.all(np.abs(out[:, h] - ref) <= room), h
