@@ -226,7 +226,7 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 // than kRise above it, so that the accumulators are rescaled (exactly) a few times a row and not at every step.  In two parts of fp16 a weight's last
 // bit is 2^-24, so below 2^-2 it has not all of its own.  For an fp16 cache m therefore lies kAhead above the largest score that it was set by,
 // whose weight is 2^8 then, grows up to 2^15 and falls down to 2^1 (kFall below m) before m follows - down too: the keys behind one that takes nearly
-// all have the same bits as before it, however little they count.
+// all have the same bits as before it, however little they count.  For other caches, whose values may be as large as fp32 is, weights stay below 1.
 //
 // Sequences with at most 32 rows (answers): all wavefronts have the same rows and walk over different keys, each through LDS of its
 // own, and meet at the end.  Others (prompts): tiles of 128 rows, each wavefront has 32 of them and all share the keys in LDS.
@@ -245,6 +245,7 @@ typedef __attribute__((address_space(3))) uint8_t* lds_t;
 constexpr int kAttnWaves = 4, kAttnThreads = 64 * kAttnWaves;
 constexpr int kKeyRows = 32;         // rows of a sequence up to which its wavefronts share rows and not keys
 constexpr int kTileRows = 32 * kAttnWaves;
+constexpr int kMaxPieces = 1024;      // that a tile's keys are cut into
 constexpr float kLog2e = 1.44269504088896340736f;
 // rows that a lane's page has not (past the end, or no page at all) are read from here
 __device__ __attribute__((aligned(16))) uint8_t g_zero_row[kMaxDim * 4];
@@ -521,7 +522,7 @@ struct Attn {
     static constexpr int kCacheParts = TYPE == 0 ? 3 : 1;
     static constexpr int kSteps = HD / 16, kDims = HD / 32;
     // of the weights, as exponents (see above)
-    static constexpr float kUnit = TYPE == 1 ? 15.f : 7.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 14.f, kMost = 64.f, kApart = 20.f;
+    static constexpr float kUnit = TYPE == 1 ? 15.f : -8.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 14.f, kMost = 64.f, kApart = 20.f;
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
     static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU
     static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD >= 128);
@@ -969,7 +970,7 @@ struct Attn {
     __device__ __forceinline__ float* values_of(int row) const { return A.partial + slot_row(A, t.slot, kvh, row) * A.cache.head_dim; }
     __device__ __forceinline__ f2_t* state_of(int row) const { return states_of(A) + slot_row(A, t.slot, kvh, row); }
     // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
-    // 64) for the values.  Slow, for rows with infinities or NaN in their results.
+    // 64) for the values, whose mean is carried along, so that finite values never add up to infinity.  Slow, for rows with infinities or NaN in their results.
     __device__ __forceinline__ void plainly(int row, int step)
     {
         const int dim = A.cache.head_dim;
@@ -978,7 +979,7 @@ struct Attn {
             place(row, &token, &head);
             const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
             const int last = t.p0 + token, first = first_key(last, A.window);
-            float top = -INFINITY, sum = 0.f, acc[HD / 64 + 1] = {};
+            float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
                 const int j = j0 + lane;
                 int id = -1;
@@ -997,29 +998,34 @@ struct Attn {
                 }
                 float most = score;
                 for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-                const float mn = fmaxf(top, most), base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
-                const float w = seen ? __builtin_amdgcn_exp2f(score - base + kUnit) : 0.f;
+                const float mn = fmaxf(top, __builtin_ceilf(most)), base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
+                const float w = seen ? __builtin_amdgcn_exp2f(score - base) : 0.f;
                 float all = w;
                 for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
-                sum = sum * f + all;
+                const float before = sum * f;
+                sum = before + all;
                 top = mn;
+                const float by = sum == 0.f ? 0.f : 1.0f / sum;      // (weights of 0 alone: nothing; NaN stays)
 #pragma unroll
-                for (int i = 0; i <= HD / 64; ++i) acc[i] *= f;
+                for (int i = 0; i <= HD / 64; ++i) mean[i] *= before * by;
                 for (uint64_t rest = lanes; rest != 0; rest &= rest - 1) {
                     const int at = __ffsll((unsigned long long)rest) - 1;
-                    const float wk = __shfl(w, at);
+                    const float wk = __shfl(w, at) * by;
                     const int64_t vk = (int64_t)__shfl((long long)v_at, at);
 #pragma unroll
                     for (int i = 0; i <= HD / 64; ++i)
-                        if (64 * i + lane < dim) acc[i] += wk * element(A.cache.v, vk + 64 * i + lane);
+                        if (64 * i + lane < dim) mean[i] += wk * element(A.cache.v, vk + 64 * i + lane);
                 }
             }
+            // a piece's state in units in which its sum is at most 1
+            const int e = sum > 0.f ? __builtin_amdgcn_frexp_expf(sum) : 0;
+            const float part = ldexpf(sum, -e);
             float* dst = t.cuts == 1 ? A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * dim : values_of(row);
-            const float by = t.cuts == 1 ? over_sum(A, sum, top - kUnit, head) : 1.f;
+            const float by = t.cuts == 1 ? sum * over_sum(A, sum, top, head) : part;
 #pragma unroll
             for (int i = 0; i <= HD / 64; ++i)
-                if (64 * i + lane < dim) dst[64 * i + lane] = acc[i] * by;
-            if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top - kUnit, sum};
+                if (64 * i + lane < dim) dst[64 * i + lane] = mean[i] * by;
+            if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top + (float)e, part};
         }
     }
     __device__ __forceinline__ float element(const char* base, int64_t at) const
@@ -1176,7 +1182,8 @@ struct Attn {
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kKeyWaves; ++w) top = fmaxf(top, states[w][row].x);
-            const float base = top == -INFINITY ? 0.f : top;
+            // (two powers more, so that what up to four of them have adds up to no infinity)
+            const float unit = top + 2.f, base = top == -INFINITY ? 0.f : unit;
             float sum = 0.f;
             f4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1189,10 +1196,10 @@ struct Attn {
             place(row, &token, &head);
             if (t.cuts == 1) {
                 *reinterpret_cast<f4_t*>(A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim + 4 * piece) =
-                    v * over_sum(A, sum, top, head);
+                    v * over_sum(A, sum, unit, head);
             } else {
                 *reinterpret_cast<f4_t*>(values_of(row) + 4 * piece) = v;
-                if (piece == 0) *state_of(row) = f2_t{top, sum};
+                if (piece == 0) *state_of(row) = f2_t{unit, sum};
             }
         }
         return false;
@@ -1248,11 +1255,14 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
     const float* values = A.partial + first * dim;
     const f2_t* states = states_of(A) + first;
     constexpr int U = WAVES == 1 ? 8 : 4;
+    // (a piece's values may be as large as fp32 is: what is joined counts in units of 2^(top + kSpare), which leave room for kMaxPieces of them)
+    constexpr float kSpare = 10.f;
+    static_assert(kMaxPieces <= 1 << (int)kSpare);
     f4_t acc = {0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.f;
-    auto join = [&](float t, float w, const f4_t& v) {
+    auto join = [&](float t, float w, const f4_t& v, float spare) {
         const float m = fmaxf(top, t), base = m == -INFINITY ? 0.f : m;
-        const float f = __builtin_amdgcn_exp2f(top - base), g = __builtin_amdgcn_exp2f(t - base);
+        const float f = __builtin_amdgcn_exp2f(top - base), g = __builtin_amdgcn_exp2f(t - base - spare);
         sum = sum * f + w * g;
         acc = acc * f + v * g;
         top = m;
@@ -1268,7 +1278,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (s0 + u * step < cuts) join(st[u].x, st[u].y, v[u]);
+            if (s0 + u * step < cuts) join(st[u].x, st[u].y, v[u], kSpare);
     }
     if constexpr (WAVES > 1) {
         for (int o = wide; o < 64; o <<= 1) {
@@ -1276,17 +1286,17 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
             f4_t v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = __shfl_xor(acc[i], o);
-            join(t, w, v);
+            join(t, w, v, 0.f);
         }
         if (lane == 0) sums[wave] = f2_t{top, sum};
         if (lane < wide) values_in[wave][lane] = acc;
         __syncthreads();
         if (wave > 0 || lane >= wide) return;
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) join(sums[w].x, sums[w].y, values_in[w][lane]);
+        for (int w = 1; w < WAVES; ++w) join(sums[w].x, sums[w].y, values_in[w][lane], 0.f);
     }
     if (!mine) return;
-    *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * over_sum(A, sum, top, head);
+    *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * over_sum(A, sum, top + kSpare, head);
 }
 
 }  // namespace
@@ -1344,7 +1354,7 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
     const int64_t tiles = all / kTileRows + std::min<int64_t>(cache.seqs, rows);
     // workgroups that are resident at once
     const int at_once = device_info().num_cus * (dim <= 64 && cache.element_type != kTypeF32 ? 3 : dim <= 128 ? 2 : 1);
-    const int64_t pieces = std::max(1, at_once / cache.kv_heads), keys = (int64_t)cache.max_pages * cache.page.d;
+    const int64_t pieces = std::min(kMaxPieces, std::max(1, at_once / cache.kv_heads)), keys = (int64_t)cache.max_pages * cache.page.d;
     const int64_t most = std::min<int64_t>(keys, window > 0 ? window : keys);
     const int hd = dims_of(dim);
     const Worth least = worth_of(cache.element_type, hd, key_waves_of(cache.element_type, hd));

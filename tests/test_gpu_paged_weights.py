@@ -1,4 +1,4 @@
-"""GPU: what the softmax weights of the attention over pages keep of their bits.
+"""GPU: what the softmax weights of the attention over pages keep of their bits, and sums at the ends of the types' range.
 
 Bounds.  Where one product makes a score it is exact; the exponent's argument rounds twice relative to the score (the scale in powers of two, the
 fused product) and once to its own size, the exponential once: 2^-24 (2 |s| + 4) of each weight, twice that of a result (its sum has the same).  Weights
@@ -112,3 +112,26 @@ def test_a_sink_far_above_or_below_the_scores(hip, dtype, sink, rows, ctx):
         ref, size = definition(np.ones(rows), kh, vh, np.arange(ctx - rows, ctx), sink)
         room = (2.0 ** -23 * (2 * max(abs(sink), 25.0) + 4) + 2.0 ** -20) * size + additions(dtype, ctx, rows > 32) * size + 2.0 ** -126
         assert np.all(np.abs(out[:, h] - ref) <= room), h
+
+
+@pytest.mark.parametrize("dtype,large", [("float16", 65504.0), ("bfloat16", 3.2e38), ("float32", 3.2e38), ("float32", 1e37), ("bfloat16", 1e37)])
+@pytest.mark.parametrize("rows,ctx,seqs", [(1, 1, 1), (1, 700, 1), (100, 700, 1), (1, 9000, 1), (3, 5000, 1), (60, 4000, 1), (2, 600, 2)])
+def test_values_next_to_the_largest(hip, dtype, large, rows, ctx, seqs):
+    """what is averaged is finite, so is the average: keys that count alike (their sum is far beyond the type), and one that takes all"""
+    import torch
+    rng = np.random.default_rng(3)
+    k = torch.zeros((ctx, 4, 64), device="cuda")
+    k[:, 1, 0] = torch.from_numpy(np.linspace(-3, 3, ctx).astype(np.float32)).cuda()
+    k[:, 2, 0] = torch.from_numpy(np.linspace(40, -40, ctx).astype(np.float32)).cuda()
+    v = torch.full((ctx, 4, 64), large, device="cuda")
+    v[:, 3] *= torch.from_numpy(rng.choice([-1.0, 1.0, 0.5], (ctx, 64)).astype(np.float32)).cuda()
+    k, v = (t.to(getattr(torch, dtype)) for t in (k, v))
+    q = torch.zeros((rows, 4, 64), device="cuda")
+    q[..., 0] = 1.0
+    contexts = [ctx - 3 * i for i in range(seqs)]
+    out = attend(hip, torch, q.view(rows, -1), one_sequence(torch, k, v, 16), contexts, 1.0).view(rows, 4, 64).double().cpu().numpy()
+    position = np.concatenate([np.arange(c - rows // seqs, c) for c in contexts])
+    for h in range(4):
+        kh, vh = k[:, h, 0].double().cpu().numpy(), v[:, h].double().cpu().numpy()
+        ref, size = definition(np.ones(rows), kh, vh, position)
+        assert np.all(np.abs(out[:, h] - ref) <= (2.0 ** -23 * (2 * 40 + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size), h
