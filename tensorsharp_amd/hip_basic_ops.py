@@ -321,15 +321,23 @@ class RotaryPositions:
     def __init__(self, dims, mode=2, base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0,
                  original_context=0, freq_factors=None):
         address = None
+        self.device = None                       # of freq_factors; without them any
         if freq_factors is not None:
             torch = _torch()
             if not freq_factors.is_cuda:
                 raise ValueError("freq_factors must be in GPU memory.")
-            address = _vector(freq_factors, torch.float32, int(dims) // 2, "freq_factors", freq_factors.get_device())
+            self.device = freq_factors.get_device()
+            address = _vector(freq_factors, torch.float32, int(dims) // 2, "freq_factors", self.device)
         self._keepalive = freq_factors
         self.native = N.Rope(int(dims), int(mode), float(base), float(freq_scale), float(ext_factor), float(attn_factor), float(beta_fast),
                              float(beta_slow), int(original_context), address)
         self.ref = C.byref(self.native)
+
+    def _reference(self, device):
+        """the descriptor for a call on that device"""
+        if self.device is not None and self.device != device:
+            raise ValueError("freq_factors is not on the device of the other tensors.")
+        return self.ref
 
 
 class PagedKVCache:
@@ -780,9 +788,9 @@ class HipBasicOps:
         device = input.get_device()
         if result.get_device() != device:
             raise ValueError("RoPE requires tensors in GPU memory of one device.")
-        pos = _vector(positions, _torch().int32, iv.dim0, "positions", device)
+        pos, how = _vector(positions, _torch().int32, iv.dim0, "positions", device), rope._reference(device)
         _use_stream_of(device)
-        ok = N.lib().TSHip_RoPEF32Device(rv, iv, pos, rope.ref)
+        ok = N.lib().TSHip_RoPEF32Device(rv, iv, pos, how)
         N.check_result(ok, "rope")
 
     @staticmethod
@@ -796,12 +804,12 @@ class HipBasicOps:
         qv, xv = _device_view(query), _device_view(qkv)
         dim, device = cache.head_dim, cache.device
         starts, lens = cache._sequences(row_starts, context_lens, i32)
-        pos = _vector(positions, i32, xv.dim0, "positions", device)
+        pos, how = _vector(positions, i32, xv.dim0, "positions", device), rope._reference(device)
         qn, kn = _vector(q_norm, f32, dim, "q_norm", device), _vector(k_norm, f32, dim, "k_norm", device)
         if query.get_device() != device or qkv.get_device() != device:
             raise ValueError("query and qkv must be on the device of the cache.")
         _use_stream_of(device)
-        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, qv.dim1 // dim, cache.ref, starts, lens, pos, qn, kn, eps, rope.ref)
+        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, qv.dim1 // dim, cache.ref, starts, lens, pos, qn, kn, eps, how)
         N.check_result(ok, "rope_store_paged")
 
     @staticmethod

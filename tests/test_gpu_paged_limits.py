@@ -55,3 +55,20 @@ def test_windows_behind_the_page_table(hip, n, page):
     some = attend(hip, torch, c, q, [n], [200], 0.125, 120)
     ref, _ = po.attend(q.cpu().numpy().astype(np.float64).reshape(n, 4, 64), k, v, np.arange(200 - n, 200), 0.125, 120)
     assert np.abs(some.cpu().numpy().reshape(n, 4, 64) - ref).max() < 1e-5
+
+
+def test_factors_of_a_rotation_on_another_device_are_refused(hip):
+    """(a device number as a second one would give it: one is enough for this test)"""
+    import torch
+    from tensorsharp_amd import PagedKVCache, RotaryPositions
+    rope = RotaryPositions(64, freq_factors=torch.ones(32, device="cuda"))
+    x, pages = torch.ones((3, 2, 64), device="cuda"), torch.zeros((2, 4, 1, 64), device="cuda")
+    cache = PagedKVCache(pages, pages.clone(), i32(torch, [[0, 1]]))
+    query, qkv = torch.zeros((3, 128), device="cuda"), torch.ones((3, 256), device="cuda")
+    hip.RoPE(torch.empty_like(x), x, i32(torch, [0, 1, 2]), rope)
+    hip.RoPEStorePaged(query, qkv, cache, i32(torch, [0, 3]), i32(torch, [3]), rope)
+    rope.device += 1
+    with pytest.raises(ValueError, match="freq_factors is not on the device"):
+        hip.RoPE(torch.empty_like(x), x, i32(torch, [0, 1, 2]), rope)
+    with pytest.raises(ValueError, match="freq_factors is not on the device"):
+        hip.RoPEStorePaged(query, qkv, cache, i32(torch, [0, 3]), i32(torch, [3]), rope)
