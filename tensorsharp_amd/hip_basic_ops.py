@@ -817,6 +817,8 @@ class HipBasicOps:
         """Attention of the sequences' new tokens (rows as in RoPEStorePaged) over a PagedKVCache that holds their keys and values already:
         each sees the positions up to its own, the last `window` of them (0: all).  query and result [rows, heads head_dim]
         float32 (may be one tensor); sinks [heads] float32: logits that take part in the softmax and carry no value."""
+        if not -2 ** 31 <= window < 2 ** 31:         # (the call takes 32 bits of it)
+            raise ValueError("PagedAttention requires a window below 2^31.")
         torch = _torch()
         rv, qv = _device_view(result), _device_view(query)
         heads, device = qv.dim1 // cache.head_dim, cache.device

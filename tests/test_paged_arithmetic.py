@@ -43,3 +43,11 @@ def test_first_key_of_a_window(compiled):
     pairs = [(p, w) for p in positions for w in edge]
     for (p, w), got in zip(pairs, compiled("first_key", pairs)):
         assert got == (max(0, p - w + 1) if w else 0), (p, w, got)
+
+
+def test_a_window_of_more_than_32_bits_is_refused():
+    """a call from C would take its lower bits: 2^32 + 5 as 5"""
+    from tensorsharp_amd import HipBasicOps
+    for window in (2 ** 31, 2 ** 32, 2 ** 32 + 5, -2 ** 31 - 1, -2 ** 32 + 7):
+        with pytest.raises(ValueError, match="window below 2"):
+            HipBasicOps.PagedAttention(None, None, None, None, None, 1.0, window=window)
