@@ -591,8 +591,18 @@ SampleLayout layout_of(int rows, int vocab)
     L.total = off;
     return L;
 }
-// rows of a launch: their lists take twice the memory of their logits
-int rows_at_once(int rows, int vocab) { return (int)std::max<int64_t>(1, std::min<int64_t>({rows, 65535, ((int64_t)1 << 25) / vocab})); }
+// Rows of a launch.  Their lists take twice the memory of their logits, and a row takes 17 KiB for its histogram and list at least; a stream keeps what a call
+// took.
+int rows_at_once(int rows, int vocab)
+{
+    constexpr size_t kMost = (size_t)5 << 26;
+    int n = std::min(rows, 65535);
+    for (;;) {
+        const size_t bytes = layout_of(n, vocab).total;
+        if (n == 1 || bytes <= kMost) return n;
+        n = std::max(1, std::min(n - 1, (int)((double)n * (double)kMost / (double)bytes)));
+    }
+}
 
 }  // namespace
 
