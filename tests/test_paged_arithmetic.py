@@ -17,6 +17,7 @@ int main(int argc, char** argv)
     long long a, b;
     while (std::scanf("%lld %lld", &a, &b) == 2)
         if (!std::strcmp(argv[1], "first_key")) std::printf("%d\\n", first_key((int)a, (int)b));
+        else if (!std::strcmp(argv[1], "quotient")) std::printf("%u\\n", FastDiv((uint32_t)b).quot((uint32_t)a));
         else return 1;
 }
 """
@@ -43,6 +44,17 @@ def test_first_key_of_a_window(compiled):
     pairs = [(p, w) for p in positions for w in edge]
     for (p, w), got in zip(pairs, compiled("first_key", pairs)):
         assert got == (max(0, p - w + 1) if w else 0), (p, w, got)
+
+
+def test_the_quotient_by_a_page_size_or_group(compiled):
+    """the multiplication and shift that stand for it, for every dividend next to a multiple that it could miss"""
+    rng = np.random.default_rng(0)
+    divisors = [1, 2, 3, 5, 7, 16, 24, 100, 255, 256, 4095, 4096, 65537, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1] + [int(v) for v in rng.integers(1, 2 ** 31, 200)]
+    pairs = []
+    for d in divisors:
+        near = np.arange(0, 2 ** 31, max(d, 2 ** 31 // 100), dtype=np.int64)[:150] // d * d
+        pairs += [(int(n), d) for n in np.concatenate([near, near - 1, near + d - 1, rng.integers(0, 2 ** 31, 100), [0, 2 ** 31 - 1]]) if 0 <= n < 2 ** 31]
+    assert compiled("quotient", pairs) == [n // d for n, d in pairs]
 
 
 def test_a_window_of_more_than_32_bits_is_refused():
