@@ -224,9 +224,11 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 //
 // m need not be the maximum: weights are 2^kUnit times what they are against m, a whole number that follows when a step's largest score is more
 // than kRise above it, so that the accumulators are rescaled (exactly) a few times a row and not at every step.  In two parts of fp16 a weight's last
-// bit is 2^-24, so below 2^-2 it has not all of its own.  For an fp16 cache m therefore lies kAhead above the largest score that it was set by,
-// whose weight is 2^8 then, grows up to 2^15 and falls down to 2^1 (kFall below m) before m follows - down too: the keys behind one that takes nearly
-// all have the same bits as before it, however little they count.  For other caches, whose values may be as large as fp32 is, weights stay below 1.
+// bit is 2^-24, so that one below 2^-2 has less than 22 bits: nothing beside what larger ones have summed up to, unless their values are next to
+// nothing, as those of a first token that takes what no other key asks for are.  So for an fp16 cache m comes down too, where a step's largest score is
+// kFall below it, once in kWait steps at most (peaked scores would have it at every step: prompts took 1.4 to 2 times as long).  It is set kAhead above
+// the largest score, whose weight is 2^8 then, or right at a score that stands kApart above the step's others, which have 2^-39 of its weight left to
+// them.  For other caches, whose values may be as large as fp32 is, weights stay below 1.
 //
 // Sequences with at most 32 rows (answers): all wavefronts have the same rows and walk over different keys, each through LDS of its
 // own, and meet at the end.  Others (prompts): tiles of 128 rows, each wavefront has 32 of them and all share the keys in LDS.
@@ -235,7 +237,6 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef float f16_t __attribute__((ext_vector_type(16)));
@@ -522,7 +523,8 @@ struct Attn {
     static constexpr int kCacheParts = TYPE == 0 ? 3 : 1;
     static constexpr int kSteps = HD / 16, kDims = HD / 32;
     // of the weights, as exponents (see above)
-    static constexpr float kUnit = TYPE == 1 ? 15.f : -8.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 14.f, kMost = 64.f, kApart = 20.f;
+    static constexpr float kUnit = TYPE == 1 ? 15.f : -8.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 20.f, kApart = 20.f, kMost = 64.f;
+    static constexpr int kWait = 16;
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
     static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU
     static constexpr bool kTight = HD == 256 || (TYPE == 0 && HD >= 128);
@@ -554,6 +556,7 @@ struct Attn {
     f16_t o[kDims];
     float c, m, l, l_rest;           // score to exponent, what weights are counted against, this lane's part of their sum and what its roundings left
     float low;                       // fp16: a step's largest score below this takes m with it
+    int wait;                        // steps until it may
     int p, lo;                       // position of this lane's row, first key it sees
 
     __device__ __forceinline__ Attn(const AttnArgs& args, const AttnTile& tile, int kv_head, lds_t smem)
@@ -635,6 +638,7 @@ struct Attn {
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
         m = low = -INFINITY;
         l = l_rest = 0.f;
+        wait = 0;
         stay();
     }
 
@@ -798,30 +802,35 @@ struct Attn {
             if (k > last || k < first || !((bits >> k) & 1)) s[i] = -INFINITY;
         }
     }
-    // Returns whether (fp16) a step's largest score, which m rose for, stands kApart above the row's others.
-    __device__ __forceinline__ bool follow_maximum(const f16_t* s, int blocks)
+    __device__ __forceinline__ void follow_maximum(const f16_t* s, int blocks)
     {
-        bool apart = false;
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < blocks; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
         top = both_halves(top, larger) * c;
-        const bool above = top > m + kRise, below = TYPE == 1 && top < low && top > -INFINITY;
+        const bool above = top > m + kRise, below = TYPE == 1 && wait <= 0 && top < low && top > -INFINITY;
+        --wait;
         if (__any(above || below)) {                                 // (m starts at -infinity)
             float mn = m;
             if (above) mn = __builtin_ceilf(top) + kAhead;
             if constexpr (TYPE == 1) {
+                // (all but one or two of the step's scores are below `others` if that is below them: the lower of the maxima of eight and of eight others)
+                const f16_t& x = s[0];
+                const float some = fmaxf(fmaxf(x[1], x[6]), fmaxf(x[11], x[12])), more = fmaxf(fmaxf(x[3], x[4]), fmaxf(x[9], x[14]));
+                const float others = fminf(both_halves(some, larger), both_halves(more, larger)) * c;
+                if (above && top - others > kApart) mn = __builtin_ceilf(top);
                 if (above) low = mn - kFall;
-                const float others = others_of(s[0]) * c;
-                apart = __any(above && others > -INFINITY && top - others > kApart);
-                // (not so far down that the sum passes 2^kMost: with values up to 2^16 the accumulators stay finite)
-                const float least = m - fmaxf(0.f, kMost - (float)__builtin_amdgcn_frexp_expf(both_halves(l, larger)));
-                if (below) {
-                    mn = __builtin_ceilf(top) + kAhead;
-                    low = mn - kFall;
-                    if (mn < least) mn = least, low = -INFINITY;
+                if (__any(below)) {
+                    // (not so far down that the sum passes 2^kMost: with values up to 2^16 the accumulators stay finite)
+                    const float least = m - fmaxf(0.f, kMost - (float)__builtin_amdgcn_frexp_expf(both_halves(l, larger)));
+                    wait = kWait;
+                    if (below) {
+                        mn = __builtin_ceilf(top) + kAhead;
+                        low = mn < least ? -INFINITY : mn - kFall;
+                        mn = fmaxf(mn, least);
+                    }
                 }
             }
             const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
@@ -834,57 +843,6 @@ struct Attn {
             m = mn;
         }
         stay();
-        return apart;
-    }
-    // a score that all but one or two of a row's in a step are certain to be below if it is far below the largest: the lower of the maxima of eight keys
-    // and eight others
-    __device__ __forceinline__ float others_of(const f16_t& s) const
-    {
-        const float a = fmaxf(fmaxf(s[1], s[6]), fmaxf(s[11], s[12])), b = fmaxf(fmaxf(s[3], s[4]), fmaxf(s[9], s[14]));
-        return fminf(both_halves(a, larger), both_halves(b, larger));
-    }
-    // Where one or two keys of a step stand kApart above its others, these would have few bits of their own in fp16 (and where the large ones' values are 0,
-    // as those of a first token that takes what no other key asks for nearly are, the others are the result).  The large ones, at most two, are weighed in 32
-    // bits by themselves, and m follows what is left.  Looked for where m rises, so that it costs nothing at other steps (32 x 4096 positions of 128
-    // dimensions 103.5 -> 103.4 us, a prompt's chunk of 512 at 4096 79.8 -> 80.7).
-    __device__ __forceinline__ void take_apart(f16_t* s, int blocks, lds_t values)
-    {
-        const float others = others_of(s[0]) * c;
-        for (int n = 0; n < 2; ++n) {
-            float big = -INFINITY;
-            int at = 0;
-#pragma unroll
-            for (int b = 0; b < blocks; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (s[b][i] > big) {
-                        big = s[b][i];
-                        at = 32 * b + 8 * (i / 4) + i % 4;
-                    }
-            const u2_t bigs = __builtin_amdgcn_permlane32_swap(__float_as_uint(big), __float_as_uint(big), false, false);
-            at += 4 * half;
-            const u2_t ats = __builtin_amdgcn_permlane32_swap(at, at, false, false);
-            const int from = __uint_as_float(bigs.x) >= __uint_as_float(bigs.y) ? 0 : 1, key = from ? (int)ats.y : (int)ats.x;
-            big = __uint_as_float(from ? bigs.y : bigs.x) * c;
-            if (!(others > -INFINITY && big - others > kApart)) continue;                   // (a lane whose row is not like this)
-            const float w = __builtin_amdgcn_exp2f(big - (m - kUnit));
-            if (half == 0) add_weights(w);
-#pragma unroll
-            for (int b = 0; b < blocks; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (half == from && 32 * b + 8 * (i / 4) + i % 4 + 4 * half == key) s[b][i] = -INFINITY;
-            const lds_t row = values + key * kRow + half * 8;
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const h4_t v = *reinterpret_cast<const __attribute__((address_space(3))) h4_t*>(row + (((4 * d + i) ^ v_swizzle(key)) << 4));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[d][4 * i + j] = __builtin_fmaf(w, (float)v[j], o[d][4 * i + j]);
-                }
-        }
-        follow_maximum(s, blocks);
     }
     // large heads: the accumulators stay in accumulation registers from one step to the next
     __device__ __forceinline__ void stay()
@@ -1077,9 +1035,7 @@ struct Attn {
 #pragma unroll
                         for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b));
                     }
-                    const bool apart = follow_maximum(s, NT);
-                    if constexpr (TYPE == 1)
-                        if (__builtin_expect(apart, false)) take_apart(s, NT, here + NT * kBlock);
+                    follow_maximum(s, NT);
                     float sum = 0.f;
 #pragma unroll
                     for (int b = 0; b < NT; ++b) sum += weigh(s[b], here + (NT + b) * kBlock);
@@ -1146,10 +1102,8 @@ struct Attn {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::false_type(), rows.k, kb);
                 if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
-                const bool apart = follow_maximum(s, 1);
+                follow_maximum(s, 1);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");                 // the values too: the next keys are left
-                if constexpr (TYPE == 1)
-                    if (__builtin_expect(apart, false)) take_apart(s, 1, vb);
                 add_weights(weigh(s[0], vb));
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::true_type(), rows.v, vb);

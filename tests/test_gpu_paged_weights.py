@@ -4,7 +4,10 @@ Bounds.  Where one product makes a score it is exact; the exponent's argument ro
 fused product) and once to its own size, the exponential once: 2^-24 (2 |s| + 4) of each weight, twice that of a result (its sum has the same).  Weights
 and their sum add the 2^-20 of sum p |v| of test_gpu_paged_attention.py: all of a row's weights keep that, however small they are against its largest.
 The weighted values of a long run of keys are summed in 32 bits, 16 keys and one part of the weights (six products of parts in fp32) at a time: each of these
-additions rounds by at most 2^-24 of what is summed by then, which is no more than the whole (`additions`)."""
+additions rounds by at most 2^-24 of what is summed by then, which is no more than the whole (`additions`).
+Over an fp16 cache a weight's last bit is 2^-24, its rounding 2^-25.  The keys of one step (64 at most) have the weights of its largest score to go by, 2^8 or
+more, above 2^14 where that stands out of the step's others by 2^20: 64 x 2^-33 of its share of the row, or 64 x 2^-39 (`same_step`).  Keys of other
+steps have weights of their own."""
 import numpy as np
 import pytest
 
@@ -45,16 +48,21 @@ def additions(dtype, keys, together):
     return 2.0 ** -24 * (keys if together else keys / 2) / 16 * {"float16": 2, "bfloat16": 3, "float32": 6}[dtype]
 
 
+def same_step(dtype, gap, share, v):
+    """gap: by how much the largest score surely stands out of others"""
+    return (64 * np.where(gap / np.log(2) > 22, 2.0 ** -39, 2.0 ** -33) * share * np.abs(v).max())[:, None] if dtype == "float16" else 0.0
+
+
 def definition(q, k, v, position, sink=None):
-    """one head; q [rows], k [keys]: the one dimension that is not zero; v [keys, dim]"""
-    ref, size = (np.zeros((len(q),) + v.shape[1:]) for _ in range(2))
+    """one head; q [rows], k [keys]: the one dimension that is not zero; v [keys, dim].  The result, sum p |v| and the largest p"""
+    ref, size, share = np.zeros((len(q),) + v.shape[1:]), np.zeros((len(q),) + v.shape[1:]), np.zeros(len(q))
     for r in range(len(q)):
         s = q[r] * k[:position[r] + 1]
         m = s.max() if sink is None else max(s.max(), sink)
         w = np.exp(s - m)
         total = w.sum() + (0.0 if sink is None else np.exp(sink - m))
-        ref[r], size[r] = w @ v[:position[r] + 1] / total, w @ np.abs(v[:position[r] + 1]) / total
-    return ref, size
+        ref[r], size[r], share[r] = w @ v[:position[r] + 1] / total, w @ np.abs(v[:position[r] + 1]) / total, w.max() / total
+    return ref, size, share
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
@@ -85,10 +93,33 @@ def test_keys_that_take_nearly_all(hip, dtype, gap, rows, seqs, ctx, count):
     position = np.concatenate([np.arange(c - rows // seqs, c) for c in contexts])
     for h in heads:
         kh, vh, qh = k[:, h, 3].double().cpu().numpy(), v[:, h].double().cpu().numpy(), q[some, h, 3].double().cpu().numpy()
-        ref, size = definition(qh, kh, vh, position[some])
+        ref, size, share = definition(qh, kh, vh, position[some])
         most = (np.abs(qh) * np.abs(kh).max())[:, None]
         d = np.abs(out[some, h] - ref)
-        assert np.all(d <= (2.0 ** -23 * (2 * most + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size), (h, float((d / size).max()))
+        room = (2.0 ** -23 * (2 * most + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size + same_step(dtype, (gap - 0.5) * qh, share, vh)
+        assert np.all(d <= room), (h, float((d / size).max()))
+
+
+@pytest.mark.parametrize("gap", [16.0, 23.0, 30.0, 36.0])
+@pytest.mark.parametrize("rows,seqs,ctx", [(300, 1, 4000), (4, 4, 4000), (100, 1, 700)])
+def test_the_steps_behind_a_key_that_takes_all(hip, gap, rows, seqs, ctx):
+    """the first key's value and those of its step (64 keys) are 0: all that is left are weights of other steps, which have all their bits (in fp16 as well)"""
+    import torch
+    kv, dim = 256, 16
+    k = torch.zeros((ctx, kv, dim), device="cuda")
+    k[0, :, 3] = gap
+    v = torch.randn((ctx, kv, dim), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)) * 0.5 + 1.0
+    v[:64] = 0.0
+    k, v = k.half(), v.half()
+    q = torch.zeros((rows, kv, dim), device="cuda")
+    q[:, :, 3] = 1.0
+    contexts = [ctx - 5 * i for i in range(seqs)]
+    out = attend(hip, torch, q.view(rows, -1), one_sequence(torch, k, v, 16), contexts, 1.0).view(rows, kv, dim).double().cpu().numpy()
+    position = np.concatenate([np.arange(c - rows // seqs, c) for c in contexts])
+    for h in (0, 100, 255):
+        ref, size, _ = definition(np.ones(rows), k[:, h, 3].double().cpu().numpy(), v[:, h].double().cpu().numpy(), position)
+        room = (2.0 ** -23 * (2 * gap + 4) + 2.0 ** -20 + additions("float16", ctx, rows // seqs > 32)) * size
+        assert np.all(np.abs(out[:, h] - ref) <= room), (h, float((np.abs(out[:, h] - ref) / size).max()))
 
 
 @pytest.mark.parametrize("sink", [-200.0, -30.0, 0.0, 30.0, 60.0, 200.0])
@@ -109,8 +140,9 @@ def test_a_sink_far_above_or_below_the_scores(hip, dtype, sink, rows, ctx):
     out = out.view(rows, 2, 64).double().cpu().numpy()
     for h in range(2):
         kh, vh = k[:, h, 5].double().cpu().numpy(), v[:, h].double().cpu().numpy()
-        ref, size = definition(np.ones(rows), kh, vh, np.arange(ctx - rows, ctx), sink)
+        ref, size, share = definition(np.ones(rows), kh, vh, np.arange(ctx - rows, ctx), sink)
         room = (2.0 ** -23 * (2 * max(abs(sink), 25.0) + 4) + 2.0 ** -20) * size + additions(dtype, ctx, rows > 32) * size + 2.0 ** -126
+        room += same_step(dtype, np.full(rows, 23.0 if h == 0 else 0.0), share, vh)
         assert np.all(np.abs(out[:, h] - ref) <= room), h
 
 
@@ -133,5 +165,5 @@ def test_values_next_to_the_largest(hip, dtype, large, rows, ctx, seqs):
     position = np.concatenate([np.arange(c - rows // seqs, c) for c in contexts])
     for h in range(4):
         kh, vh = k[:, h, 0].double().cpu().numpy(), v[:, h].double().cpu().numpy()
-        ref, size = definition(np.ones(rows), kh, vh, position)
+        ref, size, _ = definition(np.ones(rows), kh, vh, position)
         assert np.all(np.abs(out[:, h] - ref) <= (2.0 ** -23 * (2 * 40 + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size), h
