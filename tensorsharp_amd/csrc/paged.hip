@@ -259,7 +259,7 @@ struct AttnArgs {
     int64_t ld_query, ld_out;
     float c;                     // |scale| log2 e
     float sign;                  // of scale, 0 where it is 0
-    int rows, heads, group, window, capacity;
+    int rows, group, window, capacity;
     int slots, slot_rows;        // of partial
     FastDiv by_group;
     PagedKv cache;
@@ -541,7 +541,6 @@ struct Attn {
         return TYPE == 0 ? key & 7 : kPieces % 8 == 0 ? (key & 3) << 1 : ((key >> 1) & 1) << 1;
     }
 
-    typedef typename std::conditional<TYPE == 1, h8_t, b8_t>::type operand_t;
     __device__ static __forceinline__ f16_t mfma(const u4_t& a, const u4_t& b, const f16_t& c)
     {
         if constexpr (TYPE == 1) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
@@ -1358,7 +1357,6 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     args.c = scale == 0.f ? 1.f : (float)(std::fabs((double)scale) * 1.44269504088896340736);
     args.sign = scale == 0.f ? 0.f : scale < 0.f ? -1.f : 1.f;
     args.rows = rows;
-    args.heads = heads;
     args.group = heads / cache.kv_heads;
     args.window = window;
     args.capacity = cache.max_pages * (int)cache.page.d;
