@@ -505,8 +505,9 @@ TSHIP_EXPORT int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTen
  * position p = context_lens[s] - new tokens + i and sees positions max(0, p - window + 1) .. p (window 0: all from 0),
  *   result[row][h] = sum_j e^(scale q.k_j - m) v_j / (sum_j e^(scale q.k_j - m) + e^(sinks[h] - m)),
  * grouped heads sharing KV head h / (num_heads / num_kv_heads); sinks (device, num_heads logits) may be NULL (no such term).  A row that sees
- * nothing is zero, rows that belong to no sequence are left as they were.  query and result [rows x num_heads head_dim]; result may be
- * query.  Sums are fp32; 16-bit caches are multiplied on the matrix cores with queries and weights in as many 16-bit parts as fp32 needs. */
+ * nothing, or scores of -infinity only, is zero, rows that belong to no sequence are left as they were.  query and result [rows x num_heads
+ * head_dim]; result may be query.  Sums are fp32; products go through the matrix cores, queries and weights cut into 16-bit parts: 24 bits over bf16 and
+ * fp32 caches; over an fp16 cache 22 bits, of weights 2^-33 of the largest that the row met at most 1024 positions before where that is more. */
 TSHIP_EXPORT int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
                                                const int32_t* row_starts, const int32_t* context_lens, float scale, int window,
                                                const float* sinks);

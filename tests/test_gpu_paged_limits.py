@@ -72,3 +72,20 @@ def test_factors_of_a_rotation_on_another_device_are_refused(hip):
         hip.RoPE(torch.empty_like(x), x, i32(torch, [0, 1, 2]), rope)
     with pytest.raises(ValueError, match="freq_factors is not on the device"):
         hip.RoPEStorePaged(query, qkv, cache, i32(torch, [0, 3]), i32(torch, [3]), rope)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("n,ctx", [(1, 1), (1, 70), (1, 5000), (40, 50), (3, 9)])
+def test_scores_of_minus_infinity_alone_give_zero(hip, dtype, n, ctx):
+    """one head's keys are all -infinity in a dimension in which the queries are positive, another's are ordinary"""
+    import torch
+    rng = np.random.default_rng(ctx)
+    c = po.Cache(torch, rng, [ctx], 16, 2, 64, getattr(torch, dtype))
+    c.k[:, :, 0, 5] = -np.inf
+    q = torch.from_numpy(rng.standard_normal((n, 4, 64)).astype(np.float32)).cuda()
+    q[:, :, 5] = torch.tensor([1.0, 1.2345, 0.1, 3.0], device="cuda")
+    out = attend(hip, torch, c, q.view(n, -1), [n], [ctx], 0.125, 0).cpu().numpy().reshape(n, 4, 64)
+    assert np.all(out[:, :2] == 0.0)
+    k, v = c.rows(0)
+    ref, _ = po.attend(q.cpu().numpy().astype(np.float64)[:, 2:], k[:, 1:], v[:, 1:], np.arange(ctx - n, ctx), 0.125)
+    assert np.abs(out[:, 2:] - ref).max() < 1e-5
