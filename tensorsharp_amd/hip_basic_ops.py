@@ -333,11 +333,8 @@ class RotaryPositions:
                              float(beta_slow), int(original_context), address)
         self.ref = C.byref(self.native)
 
-    def _reference(self, device):
-        """the descriptor for a call on that device"""
-        if self.device is not None and self.device != device:
-            raise ValueError("freq_factors is not on the device of the other tensors.")
-        return self.ref
+    def _elsewhere(self):
+        raise ValueError("freq_factors is not on the device of the other tensors.")
 
 
 class PagedKVCache:
@@ -788,9 +785,11 @@ class HipBasicOps:
         device = input.get_device()
         if result.get_device() != device:
             raise ValueError("RoPE requires tensors in GPU memory of one device.")
-        pos, how = _vector(positions, _torch().int32, iv.dim0, "positions", device), rope._reference(device)
+        if rope.device is not None and rope.device != device:
+            rope._elsewhere()
+        pos = _vector(positions, _torch().int32, iv.dim0, "positions", device)
         _use_stream_of(device)
-        ok = N.lib().TSHip_RoPEF32Device(rv, iv, pos, how)
+        ok = N.lib().TSHip_RoPEF32Device(rv, iv, pos, rope.ref)
         N.check_result(ok, "rope")
 
     @staticmethod
@@ -804,12 +803,14 @@ class HipBasicOps:
         qv, xv = _device_view(query), _device_view(qkv)
         dim, device = cache.head_dim, cache.device
         starts, lens = cache._sequences(row_starts, context_lens, i32)
-        pos, how = _vector(positions, i32, xv.dim0, "positions", device), rope._reference(device)
+        if rope.device is not None and rope.device != device:
+            rope._elsewhere()
+        pos = _vector(positions, i32, xv.dim0, "positions", device)
         qn, kn = _vector(q_norm, f32, dim, "q_norm", device), _vector(k_norm, f32, dim, "k_norm", device)
         if query.get_device() != device or qkv.get_device() != device:
             raise ValueError("query and qkv must be on the device of the cache.")
         _use_stream_of(device)
-        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, qv.dim1 // dim, cache.ref, starts, lens, pos, qn, kn, eps, how)
+        ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, qv.dim1 // dim, cache.ref, starts, lens, pos, qn, kn, eps, rope.ref)
         N.check_result(ok, "rope_store_paged")
 
     @staticmethod
