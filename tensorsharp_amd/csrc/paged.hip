@@ -445,7 +445,7 @@ __device__ __forceinline__ float over_sum(const AttnArgs& A, float sum, float un
     if (!(sum > 0.f)) return 0.f;
     if (!A.sinks) return 1.0f / sum;
     const float e = A.sinks[head] * kLog2e - unit, h = fmaxf(e, 0.f), by = __builtin_amdgcn_exp2f(-h);
-    return by / (sum * by + __builtin_amdgcn_exp2f(e - h));
+    return by / (sum * by + (e > 0.f ? 1.f : __builtin_amdgcn_exp2f(e)));
 }
 // the tile of a row and head and its first piece; false: of no sequence
 __device__ __forceinline__ bool find_row(const Lens& H, const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)

@@ -89,3 +89,19 @@ def test_scores_of_minus_infinity_alone_give_zero(hip, dtype, n, ctx):
     k, v = c.rows(0)
     ref, _ = po.attend(q.cpu().numpy().astype(np.float64)[:, 2:], k[:, 1:], v[:, 1:], np.arange(ctx - n, ctx), 0.125)
     assert np.abs(out[:, 2:] - ref).max() < 1e-5
+
+
+@pytest.mark.parametrize("n,ctx", [(1, 300), (100, 300), (1, 9000), (5, 6000)])
+def test_sinks_of_infinity(hip, n, ctx):
+    """-infinity: as without; infinity: it takes all"""
+    import torch
+    from tensorsharp_amd import PagedKVCache
+    rng = np.random.default_rng(n)
+    c = po.Cache(torch, rng, [ctx], 16, 2, 64, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((n, 256)).astype(np.float32)).cuda()
+    want = attend(hip, torch, c, q, [n], [ctx], 0.125, 0)
+    out = torch.full_like(q, 7.5)
+    sinks = torch.tensor([-np.inf, np.inf, -np.inf, np.inf], dtype=torch.float32, device="cuda")
+    hip.PagedAttention(out, q, PagedKVCache(c.k, c.v, c.table_dev), i32(torch, [0, n]), i32(torch, [ctx]), 0.125, sinks=sinks)
+    out, want = out.view(n, 4, 64), want.view(n, 4, 64)
+    assert torch.equal(out[:, 0::2], want[:, 0::2]) and torch.all(out[:, 1::2] == 0)
