@@ -228,7 +228,8 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 // nothing, as those of a first token that takes what no other key asks for are.  So for an fp16 cache m comes down too, where a step's largest score is
 // kFall below it, once in kWait steps at most (peaked scores would have it at every step: prompts took 1.4 to 2 times as long).  It is set kAhead above
 // the largest score, whose weight is 2^8 then, or right at a score that stands kApart above the step's others, which have 2^-39 of its weight left to
-// them.  For other caches, whose values may be as large as fp32 is, weights stay below 1.
+// them.  For other caches weights begin at 2^7, so that the parts of small values and weights stay normal numbers; where large values add up to
+// infinity then, the rows are done again by plainly().
 //
 // Sequences with at most 32 rows (answers): all wavefronts have the same rows and walk over different keys, each through LDS of its
 // own, and meet at the end.  Others (prompts): tiles of 128 rows, each wavefront has 32 of them and all share the keys in LDS.
@@ -523,7 +524,7 @@ struct Attn {
     static constexpr int kCacheParts = TYPE == 0 ? 3 : 1;
     static constexpr int kSteps = HD / 16, kDims = HD / 32;
     // of the weights, as exponents (see above)
-    static constexpr float kUnit = TYPE == 1 ? 15.f : -8.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 20.f, kApart = 20.f, kMost = 64.f;
+    static constexpr float kUnit = TYPE == 1 ? 15.f : 7.f, kRise = TYPE == 1 ? 0.f : 8.f, kAhead = TYPE == 1 ? 7.f : 0.f, kFall = 20.f, kApart = 20.f, kMost = 64.f;
     static constexpr int kWait = 16;
     static constexpr int NT = TYPE == 1 ? 2 : 1;                     // 32-key blocks of a step where wavefronts share the keys
     static constexpr bool kOneWave = HD > 128;     // registers for one workgroup per CU

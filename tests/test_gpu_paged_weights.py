@@ -167,3 +167,22 @@ def test_values_next_to_the_largest(hip, dtype, large, rows, ctx, seqs):
         kh, vh = k[:, h, 0].double().cpu().numpy(), v[:, h].double().cpu().numpy()
         ref, size, _ = definition(np.ones(rows), kh, vh, position)
         assert np.all(np.abs(out[:, h] - ref) <= (2.0 ** -23 * (2 * 40 + 4) + 2.0 ** -20 + additions(dtype, ctx, rows // seqs > 32)) * size), h
+
+
+@pytest.mark.parametrize("dtype,tiny", [("bfloat16", 1e-34), ("bfloat16", 1e-36), ("float32", 1e-30), ("float32", 1e-32)])
+@pytest.mark.parametrize("rows,ctx,seqs", [(1, 1, 1), (1, 700, 1), (100, 700, 1), (1, 9000, 1), (60, 4000, 1)])
+def test_values_next_to_the_smallest(hip, dtype, tiny, rows, ctx, seqs):
+    """weighted by what they have of a row, values and their parts (2^-8 and 2^-16 of them in fp32) stay above the smallest normal number, 1.2e-38"""
+    import torch
+    rng = np.random.default_rng(4)
+    k = torch.zeros((ctx, 2, 64), device="cuda")
+    k[:, :, 0] = torch.from_numpy(rng.uniform(-1, 1, (ctx, 2)).astype(np.float32)).cuda()
+    v = torch.from_numpy((rng.uniform(0.5, 1.5, (ctx, 2, 64)) * tiny).astype(np.float32)).cuda()
+    k, v = (t.to(getattr(torch, dtype)) for t in (k, v))
+    q = torch.zeros((rows, 2, 64), device="cuda")
+    q[..., 0] = 1.0
+    out = attend(hip, torch, q.view(rows, -1), one_sequence(torch, k, v, 16), [ctx], 1.0).view(rows, 2, 64).double().cpu().numpy()
+    for h in range(2):
+        kh, vh = k[:, h, 0].double().cpu().numpy(), v[:, h].double().cpu().numpy()
+        ref, size, _ = definition(np.ones(rows), kh, vh, np.arange(ctx - rows, ctx))
+        assert np.all(np.abs(out[:, h] - ref) <= (2.0 ** -23 * (2 + 4) + 2.0 ** -20 + additions(dtype, ctx, rows > 32)) * size), h
