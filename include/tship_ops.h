@@ -470,11 +470,15 @@ typedef struct TSHipRope {
 /* A cache of pages.  Position p of sequence s has its key of head h at k + page * k_page_stride + (p % page_size) * k_token_stride +
  * h * k_head_stride elements, page = page_table[s * table_stride + p / page_size], and its value likewise.  Rows of head_dim
  * elements (a multiple of 16 up to 256) are contiguous and 16-byte aligned.  A page id outside [0, num_pages) holds nothing: it is
- * neither written nor read. */
+ * neither written nor read.
+ * Type MXFP4 holds values in four bits, in blocks of 32 along a head (head_dim a multiple of 32): an element of k and v is a byte of two codes
+ * (the first dimension's in the lower bits; a row has head_dim / 2 of them), k_scales and v_scales have a byte e per block (rows of head_dim / 32,
+ * strides in bytes, no alignment).  A code is sign, two bits of exponent and one of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6) and stands for
+ * that times 2^(e - 127), for NaN where e is 255.  (The block format of GGUF's MXFP4 with codes and scales apart.)  The fields behind max_pages are read for this type only. */
 typedef struct TSHipPagedCache {
     void* k;
     void* v;
-    int element_type;            /* TSHIP_TYPE_F32, _F16 or _BF16 */
+    int element_type;            /* TSHIP_TYPE_F32, _F16, _BF16 or _MXFP4 */
     int num_kv_heads;
     int head_dim;
     int page_size;
@@ -485,6 +489,10 @@ typedef struct TSHipPagedCache {
     int64_t table_stride;
     int num_seqs;
     int max_pages;               /* entries of a sequence in the table */
+    void* k_scales;
+    void* v_scales;
+    int64_t k_scales_page_stride, k_scales_token_stride, k_scales_head_stride;
+    int64_t v_scales_page_stride, v_scales_token_stride, v_scales_head_stride;
 } TSHipPagedCache;
 
 /* Rotary positions: result[t][h] = input[t][h] turned by positions[t] (device).  Views [tokens x heads x head_dim] with head_dim a multiple of
@@ -496,7 +504,9 @@ TSHIP_EXPORT int TSHip_RoPEF32Device(TSHipTensorView3D result, TSHipTensorView3D
  * tokens counted; row_starts must not fall, and what is outside the rows is cut off).  Rows of keys and values may not overlap.  Per head of q and k: RMSNorm * q_norm / k_norm (skipped when NULL), rotation by the token's position in its
  * sequence (or positions[row], device, when given).  q goes to query [rows x num_heads head_dim] (may be the q columns of qkv), k and
  * v are rounded to the cache's type and stored at the token's position.  A token whose position is negative, beyond the table or on no page is not
- * stored; rows that belong to no sequence are left as they were. */
+ * stored; rows that belong to no sequence are left as they were.
+ * MXFP4: e - 127 is the least whole number of at least -126 for which the block's largest magnitude is at most 7 * 2^(e - 127), a code the nearest value
+ * (between two of them the even code, beyond 6 the last); a block with a value of 2^127 or more, an infinity or a NaN is NaN (e 255). */
 TSHIP_EXPORT int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv, int num_heads, const TSHipPagedCache* cache,
                                                const int32_t* row_starts, const int32_t* context_lens, const int32_t* positions,
                                                const float* q_norm, const float* k_norm, float eps, const TSHipRope* rope);
@@ -511,6 +521,46 @@ TSHIP_EXPORT int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTen
 TSHIP_EXPORT int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
                                                const int32_t* row_starts, const int32_t* context_lens, float scale, int window,
                                                const float* sinks);
+/* Pages that sequences share: table as in TSHipPagedCache (one for the caches of all layers), context_lens the tokens that each sequence has, references
+ * how many sequences have a page (num_pages; 0: free).  A sequence has the pages of its first ceil(context_lens / page_size) entries; what lies behind
+ * them is -1.  All device memory, changed by the calls below as if in one step each; an entry outside [0, num_pages) is no page and counts nowhere.
+ * scratch: device memory for TSHip_PagePoolScratchDevice() int32, which belongs to the pool, so that captured graphs of several pools or streams share none. */
+typedef struct TSHipPagePool {
+    int32_t* page_table;
+    int64_t table_stride;
+    int num_seqs;
+    int max_pages;
+    int page_size;
+    int64_t num_pages;           /* up to 2^28 */
+    int32_t* references;         /* 16-byte aligned */
+    int32_t* context_lens;
+    int32_t* scratch;
+} TSHipPagePool;
+
+/* int32 values of scratch that a pool of these sizes needs; 0: sizes out of range */
+TSHIP_EXPORT int64_t TSHip_PagePoolScratchDevice(int num_seqs, int max_pages, int64_t num_pages);
+
+/* context_lens[s] becomes lengths[s] (device, num_seqs; negative: stays; more than the table has room for: that much).  Pages behind the ends of
+ * shorter sequences (0 tokens: all) are given back first.  Longer ones get the lowest free pages, in the order of sequences; one that goes on in a begun page
+ * which others have too gets a page in its place, and the copy that this asks for is listed: moves[i] = (from, to), num_seqs pairs, -1 behind the last.
+ * Where free pages do not suffice no sequence grows, and missing[0] (device) is how many more it takes, else 0. */
+TSHIP_EXPORT int TSHip_ResizeSequencesDevice(const TSHipPagePool* pool, const int32_t* lengths, int32_t* moves, int32_t* missing);
+
+/* Sequence children[i] becomes what parents[i] was before the call (device, count of each; of pairs with one child the last counts, a pair outside the
+ * sequences does not): its pages are given back, it shares the whole pages of its parent.  Of those that have a parent's begun page afterwards one keeps it (the
+ * parent, else the lowest child), others get copies in free pages (free before the call), in the order of sequences: moves as above, count pairs.
+ * Where free pages do not suffice nothing changes and missing[0] says how many more it takes. */
+TSHIP_EXPORT int TSHip_ForkSequencesDevice(const TSHipPagePool* pool, const int32_t* children, const int32_t* parents, int count, int32_t* moves,
+                                           int32_t* missing);
+
+/* Used pages from the last on go into the free ones among the first as many pages as are used, the lowest first; at most max_moves of them, listed in moves
+ * (max_moves pairs, -1 behind the last).  Tables and references follow. */
+TSHIP_EXPORT int TSHip_CompactPagesDevice(const TSHipPagePool* pool, int32_t* moves, int max_moves);
+
+/* Page moves[i].to of dst becomes page moves[i].from of src, keys and values (moves: device, count pairs; one outside the pages is left out).  The caches
+ * have one page size, number of heads and head_dim; types may differ (rounded as above).  src may be dst; of the pages that are written none may be
+ * read or written by another pair.  The page tables are not used. */
+TSHIP_EXPORT int TSHip_CopyPagesDevice(const TSHipPagedCache* dst, const TSHipPagedCache* src, const int32_t* moves, int count);
 
 /* One token for each row of logits [rows x vocab] (vocab up to 2^20); every other pointer is a device array with one entry per row.
  * Weights e^((l - l_max) / temperature) in 64 bits; candidates ranked by logit, the lowest index first among equals.  Of these stay, in

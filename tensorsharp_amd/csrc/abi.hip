@@ -3033,18 +3033,75 @@ bool validate_rows(const TSHipTensorView2D& d, int64_t columns, bool written, co
     return true;
 }
 
-bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_starts, const int32_t* context_lens, PagedKv* out)
+// keys and values, and the scales of a cache in four bits, as the kernels see them
+bool validate_pages(const TSHipPagedCache* c, PagedKv* out, MxScales* scales)
 {
-    if (c == nullptr || c->k == nullptr || c->v == nullptr || c->page_table == nullptr || row_starts == nullptr || context_lens == nullptr) {
+    if (c == nullptr || c->k == nullptr || c->v == nullptr) {
         set_last_error("paged cache: null pointer.");
         return false;
     }
-    if (c->element_type != kTypeF32 && c->element_type != kTypeF16 && c->element_type != kTypeBF16) {
-        set_last_error("paged cache: the element type must be F32, F16 or BF16.");
+    const bool mx = c->element_type == kTypeMXFP4;
+    if (c->element_type != kTypeF32 && c->element_type != kTypeF16 && c->element_type != kTypeBF16 && !mx) {
+        set_last_error("paged cache: the element type must be F32, F16, BF16 or MXFP4.");
         return false;
     }
-    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16 != 0) {
-        set_last_error("paged cache: head_dim must be a multiple of 16 up to 256.");
+    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % (mx ? 32 : 16) != 0) {
+        set_last_error(mx ? "paged cache: head_dim must be a multiple of 32 up to 256 for MXFP4." : "paged cache: head_dim must be a multiple of 16 up to 256.");
+        return false;
+    }
+    if (c->num_kv_heads <= 0 || c->page_size <= 0 || c->page_size > (1 << 30) || c->num_pages <= 0 || c->num_pages > INT32_MAX) {
+        set_last_error("paged cache: invalid page size or number of heads or pages.");
+        return false;
+    }
+    const int64_t row = mx ? c->head_dim / 2 : c->head_dim, per = mx ? 16 : 16 / block_bytes(c->element_type);           // elements of a row, of 16 bytes
+    const int64_t strides[6] = {c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride, c->v_token_stride, c->v_head_stride};
+    const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
+    int64_t s[6];
+    for (int i = 0; i < 6; ++i) {
+        s[i] = counts[i % 3] > 1 ? strides[i] : 0;
+        if (counts[i % 3] > 1 && (s[i] < row || s[i] % per != 0)) {
+            set_last_error("paged cache: strides must be multiples of 16 bytes and at least head_dim.");
+            return false;
+        }
+    }
+    if (!aligned16(c->k) || !aligned16(c->v)) {
+        set_last_error("paged cache: keys and values must be 16-byte aligned.");
+        return false;
+    }
+    *out = {};
+    *scales = {};
+    if (mx) {
+        if (c->k_scales == nullptr || c->v_scales == nullptr) {
+            set_last_error("paged cache: null pointer (scales of MXFP4).");
+            return false;
+        }
+        const int64_t of[6] = {c->k_scales_page_stride, c->k_scales_token_stride, c->k_scales_head_stride,
+                               c->v_scales_page_stride, c->v_scales_token_stride, c->v_scales_head_stride};
+        int64_t z[6];
+        for (int i = 0; i < 6; ++i) {
+            z[i] = counts[i % 3] > 1 ? of[i] : 0;
+            if (counts[i % 3] > 1 && z[i] < c->head_dim / 32) {
+                set_last_error("paged cache: strides of the scales must be at least head_dim / 32.");
+                return false;
+            }
+        }
+        *scales = {static_cast<uint8_t*>(c->k_scales), static_cast<uint8_t*>(c->v_scales), z[0], z[1], z[2], z[3], z[4], z[5]};
+    }
+    out->k = static_cast<char*>(c->k);
+    out->v = static_cast<char*>(c->v);
+    out->k_page = s[0], out->k_token = s[1], out->k_head = s[2], out->v_page = s[3], out->v_token = s[4], out->v_head = s[5];
+    out->element_type = c->element_type;
+    out->kv_heads = c->num_kv_heads;
+    out->head_dim = c->head_dim;
+    out->num_pages = (int)c->num_pages;
+    out->page = FastDiv((uint32_t)c->page_size);
+    return true;
+}
+
+bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_starts, const int32_t* context_lens, PagedKv* out, MxScales* scales)
+{
+    if (c == nullptr || c->page_table == nullptr || row_starts == nullptr || context_lens == nullptr) {
+        set_last_error("paged cache: null pointer.");
         return false;
     }
     if (c->num_kv_heads <= 0 || num_heads <= 0 || num_heads % c->num_kv_heads != 0) {
@@ -3056,47 +3113,27 @@ bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_
         set_last_error("paged cache: invalid page size, page table or number of pages or sequences.");
         return false;
     }
-    const int64_t per = 16 / block_bytes(c->element_type);           // elements of 16 bytes
-    const int64_t strides[6] = {c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride, c->v_token_stride, c->v_head_stride};
-    const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
-    int64_t s[6];
-    for (int i = 0; i < 6; ++i) {
-        s[i] = counts[i % 3] > 1 ? strides[i] : 0;
-        if (counts[i % 3] > 1 && (s[i] < c->head_dim || s[i] % per != 0)) {
-            set_last_error("paged cache: strides must be multiples of 16 bytes and at least head_dim.");
-            return false;
-        }
-    }
-    if (!aligned16(c->k) || !aligned16(c->v)) {
-        set_last_error("paged cache: keys and values must be 16-byte aligned.");
-        return false;
-    }
-    *out = {};
-    out->k = static_cast<char*>(c->k);
-    out->v = static_cast<char*>(c->v);
-    out->k_page = s[0], out->k_token = s[1], out->k_head = s[2], out->v_page = s[3], out->v_token = s[4], out->v_head = s[5];
+    if (!validate_pages(c, out, scales)) return false;
     out->table = c->page_table;
     out->table_stride = c->table_stride;
     out->row_starts = row_starts;
     out->context_lens = context_lens;
-    out->element_type = c->element_type;
-    out->kv_heads = c->num_kv_heads;
-    out->head_dim = c->head_dim;
-    out->num_pages = (int)c->num_pages;
     out->max_pages = c->max_pages;
     out->seqs = c->num_seqs;
-    out->page = FastDiv((uint32_t)c->page_size);
     return true;
 }
 
 // rows of a cache that share memory, which may not be written
 bool rows_overlap(const TSHipPagedCache* c)
 {
+    const bool mx = c->element_type == kTypeMXFP4;
     const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
-    for (const int64_t* s : {&c->k_page_stride, &c->v_page_stride}) {
+    for (const int64_t* s : {&c->k_page_stride, &c->v_page_stride, &c->k_scales_page_stride, &c->v_scales_page_stride}) {
+        const bool of_scales = s == &c->k_scales_page_stride || s == &c->v_scales_page_stride;
+        if (of_scales && !mx) break;                                 // (not read for other types)
         std::pair<int64_t, int64_t> d[3] = {{s[0], counts[0]}, {s[1], counts[1]}, {s[2], counts[2]}};
         std::sort(d, d + 3);
-        int64_t span = c->head_dim;
+        int64_t span = of_scales ? c->head_dim / 32 : mx ? c->head_dim / 2 : c->head_dim;
         for (const auto& [stride, count] : d) {
             if (count == 1) continue;
             if (stride < span) return true;
@@ -3179,8 +3216,9 @@ int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv
     return guarded(0, "rope_store_paged", [&]() -> int {
         if (!ensure_backend()) return 0;
         PagedKv kv;
+        MxScales scales;
         RopeSpec spec;
-        if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv) || !validate_rope(rope, kv.head_dim, &spec)) return 0;
+        if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv, &scales) || !validate_rope(rope, kv.head_dim, &spec)) return 0;
         if (!validate_rows(query, (int64_t)num_heads * kv.head_dim, true, "query") ||
             !validate_rows(qkv, ((int64_t)num_heads + 2 * (int64_t)kv.kv_heads) * kv.head_dim, false, "qkv"))
             return 0;
@@ -3204,8 +3242,11 @@ int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv
             set_last_error("rope_store_paged: query overlaps qkv without being its first columns.");
             return 0;
         }
-        if (!launch_rope_store(static_cast<const float*>(qkv.data), qkv.stride0, static_cast<float*>(query.data), query.stride0, T, num_heads, kv,
-                               positions, q_norm, k_norm, eps, spec, t_stream))
+        const float* x = static_cast<const float*>(qkv.data);
+        float* q = static_cast<float*>(query.data);
+        if (kv.element_type == kTypeMXFP4
+                ? !launch_rope_store_mx(x, qkv.stride0, q, query.stride0, T, num_heads, kv, scales, positions, q_norm, k_norm, eps, spec, t_stream)
+                : !launch_rope_store(x, qkv.stride0, q, query.stride0, T, num_heads, kv, positions, q_norm, k_norm, eps, spec, t_stream))
             return 0;
         clear_last_error();
         return 1;
@@ -3218,7 +3259,12 @@ int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D qu
     return guarded(0, "paged_attention", [&]() -> int {
         if (!ensure_backend()) return 0;
         PagedKv kv;
-        if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv)) return 0;
+        MxScales scales;
+        if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv, &scales)) return 0;
+        if (kv.element_type == kTypeMXFP4) {
+            set_last_error("paged_attention: not over MXFP4 yet.");
+            return 0;
+        }
         const int64_t columns = (int64_t)num_heads * kv.head_dim;
         if (!validate_rows(result, columns, true, "result") || !validate_rows(query, columns, false, "query")) return 0;
         if (query.dim0 != result.dim0) {
@@ -3266,6 +3312,178 @@ int TSHip_SampleTokensF32Device(TSHipTensorView2D logits, const float* uniforms,
         if (!launch_sample(static_cast<const float*>(logits.data), logits.dim0 > 1 ? logits.stride0 : 0, logits.dim0, logits.dim1, uniforms, temperature,
                            top_k, top_p, min_p, tokens, probabilities, lease.ptr(), t_stream))
             return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+bool validate_pool(const TSHipPagePool* p, PagePoolArgs* out)
+{
+    if (p == nullptr || p->page_table == nullptr || p->references == nullptr || p->context_lens == nullptr || p->scratch == nullptr) {
+        set_last_error("page pool: null pointer.");
+        return false;
+    }
+    if (TSHip_PagePoolScratchDevice(p->num_seqs, p->max_pages, p->num_pages) == 0 || p->page_size <= 0 ||
+        (int64_t)p->max_pages * p->page_size > (1 << 30) || (p->num_seqs > 1 && p->table_stride < p->max_pages)) {
+        set_last_error("page pool: invalid page size, page table or number of pages or sequences.");
+        return false;
+    }
+    if (!aligned16(p->references)) {
+        set_last_error("page pool: the references must be 16-byte aligned.");
+        return false;
+    }
+    *out = {p->page_table, p->table_stride, p->num_seqs, p->max_pages, p->page_size, (int)p->num_pages, p->references, p->context_lens, p->scratch};
+    return true;
+}
+
+// from the first byte to behind the last of keys (values) or of their scales
+struct Span {
+    uintptr_t begin, end;
+};
+Span span_of(const void* at, const int64_t* strides, const TSHipPagedCache* c, int64_t row, int64_t size)
+{
+    const uintptr_t p = reinterpret_cast<uintptr_t>(at);
+    const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
+    int64_t last = row;
+    for (int i = 0; i < 3; ++i) last += counts[i] > 1 ? (counts[i] - 1) * strides[i] : 0;
+    return {p, p + (uintptr_t)(last * size)};
+}
+void spans_of(const TSHipPagedCache* c, Span (&out)[4])
+{
+    const bool mx = c->element_type == kTypeMXFP4;
+    const int64_t row = mx ? c->head_dim / 2 : c->head_dim, size = mx ? 1 : block_bytes(c->element_type);
+    out[0] = span_of(c->k, &c->k_page_stride, c, row, size);
+    out[1] = span_of(c->v, &c->v_page_stride, c, row, size);
+    out[2] = mx ? span_of(c->k_scales, &c->k_scales_page_stride, c, c->head_dim / 32, 1) : Span{0, 0};
+    out[3] = mx ? span_of(c->v_scales, &c->v_scales_page_stride, c, c->head_dim / 32, 1) : Span{0, 0};
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t TSHip_PagePoolScratchDevice(int num_seqs, int max_pages, int64_t num_pages)
+{
+    if (num_seqs <= 0 || num_seqs > 65535 || max_pages <= 0 || num_pages <= 0 || num_pages > (1 << 28)) return 0;
+    return page_pool_scratch(num_seqs, max_pages, num_pages);
+}
+
+int TSHip_ResizeSequencesDevice(const TSHipPagePool* pool, const int32_t* lengths, int32_t* moves, int32_t* missing)
+{
+    return guarded(0, "resize_sequences", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        PagePoolArgs args;
+        if (!validate_pool(pool, &args)) return 0;
+        if (lengths == nullptr || moves == nullptr || missing == nullptr) {
+            set_last_error("resize_sequences: null pointer.");
+            return 0;
+        }
+        if (!launch_resize_sequences(args, lengths, moves, missing, t_stream)) return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+int TSHip_ForkSequencesDevice(const TSHipPagePool* pool, const int32_t* children, const int32_t* parents, int count, int32_t* moves,
+                              int32_t* missing)
+{
+    return guarded(0, "fork_sequences", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        PagePoolArgs args;
+        if (!validate_pool(pool, &args)) return 0;
+        if (children == nullptr || parents == nullptr || moves == nullptr || missing == nullptr) {
+            set_last_error("fork_sequences: null pointer.");
+            return 0;
+        }
+        if (count <= 0) {
+            set_last_error("fork_sequences: the count must be positive.");
+            return 0;
+        }
+        if (!launch_fork_sequences(args, children, parents, count, moves, missing, t_stream)) return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+int TSHip_CompactPagesDevice(const TSHipPagePool* pool, int32_t* moves, int max_moves)
+{
+    return guarded(0, "compact_pages", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        PagePoolArgs args;
+        if (!validate_pool(pool, &args)) return 0;
+        if (moves == nullptr || max_moves <= 0) {
+            set_last_error("compact_pages: there must be room for moves.");
+            return 0;
+        }
+        if (!launch_compact_pages(args, moves, max_moves, t_stream)) return 0;
+        clear_last_error();
+        return 1;
+    });
+}
+
+int TSHip_CopyPagesDevice(const TSHipPagedCache* dst, const TSHipPagedCache* src, const int32_t* moves, int count)
+{
+    return guarded(0, "copy_pages", [&]() -> int {
+        if (!ensure_backend()) return 0;
+        PagedKv d, s;
+        MxScales dx, sx;
+        if (!validate_pages(dst, &d, &dx) || !validate_pages(src, &s, &sx)) return 0;
+        if (moves == nullptr || count <= 0) {
+            set_last_error("copy_pages: null pointer or no moves.");
+            return 0;
+        }
+        if (dst->page_size != src->page_size || d.kv_heads != s.kv_heads || d.head_dim != s.head_dim) {
+            set_last_error("Size mismatch: the caches of copy_pages differ in page size, heads or head_dim.");
+            return 0;
+        }
+        if (rows_overlap(dst)) {
+            set_last_error("copy_pages: rows of keys or values overlap.");
+            return 0;
+        }
+        const int64_t units = (int64_t)dst->page_size * d.kv_heads * (d.head_dim / 8);
+        if (units > (1 << 26)) {
+            set_last_error("copy_pages: pages are too large.");
+            return 0;
+        }
+        const bool mx = d.element_type == kTypeMXFP4;
+        const bool same = d.element_type == s.element_type && d.k == s.k && d.v == s.v && d.num_pages == s.num_pages && d.k_page == s.k_page && d.k_token == s.k_token &&
+            d.k_head == s.k_head && d.v_page == s.v_page && d.v_token == s.v_token && d.v_head == s.v_head &&
+            (!mx || (dx.k == sx.k && dx.v == sx.v && dx.k_page == sx.k_page && dx.k_token == sx.k_token && dx.k_head == sx.k_head && dx.v_page == sx.v_page &&
+                     dx.v_token == sx.v_token && dx.v_head == sx.v_head));
+        Span of[4], to[4];
+        spans_of(src, of);
+        spans_of(dst, to);
+        for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < 4; ++j)
+                if (!same && of[i].begin < to[j].end && to[j].begin < of[i].end) {
+                    set_last_error("copy_pages: the caches overlap without being the same.");
+                    return 0;
+                }
+        PageCopyArgs args{};
+        // (tokens or heads inside, whichever lie closer together where they are written)
+        const bool heads_inside = d.k_token == 0 || (d.k_head != 0 && d.k_head <= d.k_token);
+        auto rows = [&](const PagedKv& c, const MxScales& x, bool v) {
+            const int64_t size = c.element_type == kTypeMXFP4 ? 1 : block_bytes(c.element_type);
+            const int64_t token = (v ? c.v_token : c.k_token) * size, head = (v ? c.v_head : c.k_head) * size;
+            const int64_t x_token = v ? x.v_token : x.k_token, x_head = v ? x.v_head : x.k_head;
+            return PageRows{v ? c.v : c.k, (v ? c.v_page : c.k_page) * size, heads_inside ? token : head, heads_inside ? head : token,
+                            v ? x.v : x.k, v ? x.v_page : x.k_page, heads_inside ? x_token : x_head, heads_inside ? x_head : x_token};
+        };
+        for (int i = 0; i < 2; ++i) {
+            args.src[i] = rows(s, sx, i == 1);
+            args.dst[i] = rows(d, dx, i == 1);
+        }
+        args.src_pages = s.num_pages;
+        args.dst_pages = d.num_pages;
+        args.same = same;
+        args.units = (uint32_t)units;
+        args.by_row = FastDiv((uint32_t)d.head_dim / 8);
+        args.by_inner = FastDiv((uint32_t)(heads_inside ? d.kv_heads : dst->page_size));
+        if (!launch_copy_pages(moves, count, args, s.element_type, d.element_type, t_stream)) return 0;
         clear_last_error();
         return 1;
     });

@@ -3,8 +3,10 @@
 //
 //   rope_kernel              head-wise rotation of a [tokens x heads x head_dim] tensor
 //   rope_store_kernel        norm and rotation of q and k heads of QKV rows, k and v into the cache
+//   rope_store_mx_kernel     the same into a cache in four bits
 //   paged_attention_kernel   softmax(scale q K^T) V of a sequence's new tokens over its pages
 #include "tship_internal.h"
+#include "mx4.h"
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -203,6 +205,75 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_kernel(const float* q
                 store_quad(dst, turned(q, R, u, turns), R, u);
             }
         }
+    }
+}
+
+// The same into a cache in four bits.  What a key or value head becomes goes through LDS, since the lanes that turn pairs do not hold neighbours: then a lane
+// has eight values that follow one another, four lanes a block, whose largest magnitude they find among them.
+template <int LANES>
+__global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int heads,
+                                                                     const int32_t* positions, const float* q_norm, const float* k_norm,
+                                                                     float eps, const PagedKv C, const MxScales X, const RopeSpec R)
+{
+    __shared__ f2_t turns[kMaxDim / 2];
+    constexpr int kHeads = kRopeThreads / LANES;
+    __shared__ __attribute__((aligned(16))) float heads_here[kHeads][4 * LANES];
+    const int t = blockIdx.x;
+    const Place at = place_of_row(C, t, gridDim.x);
+    if (at.seq < 0) return;                                          // uniform
+    const int u = threadIdx.x % LANES, dim = C.head_dim, all = heads + 2 * C.kv_heads, slot = threadIdx.x / LANES;
+    const bool live = 4 * u < dim;
+    const int where = max(C.context_lens[at.seq], -(1 << 30)) - at.count + (t - at.first);
+    const int position = positions ? positions[t] : where;
+    int within = 0;
+    const int page = where >= 0 ? page_of(C, at.seq, where, &within) : -1;
+    if ((int)threadIdx.x < R.dims / 2) turns[threadIdx.x] = turn_of(R, threadIdx.x, position);
+    __syncthreads();
+    for (int h0 = blockIdx.y * kHeads; h0 < all; h0 += gridDim.y * kHeads) {
+        const int h = h0 + slot;
+        const bool here = live && h < all, is_v = h >= heads + C.kv_heads;
+        const float* src = qkv + t * ld_qkv + (int64_t)min(h, all - 1) * dim;
+        Quad q{};
+        if (here) {
+            if (is_v) {
+                const f4_t v = *reinterpret_cast<const f4_t*>(src + 4 * u);
+                q = {f2_t{v.x, v.y}, f2_t{v.z, v.w}};
+            } else {
+                q = load_quad(src, R, u);
+            }
+        }
+        const float* norm = h < heads ? q_norm : k_norm;
+        if (q_norm || k_norm) {                                      // uniform
+            float ss = q.a.x * q.a.x + q.a.y * q.a.y + q.b.x * q.b.x + q.b.y * q.b.y;
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+            if (here && !is_v && norm) {
+                const float by = 1.0f / sqrtf(ss / (float)dim + eps);
+                const Quad w = load_quad(norm, R, u);
+                q = {q.a * by * w.a, q.b * by * w.b};
+            }
+        }
+        if (here) {
+            if (h < heads) store_quad(query + t * ld_query + (int64_t)h * dim, turned(q, R, u, turns), R, u);
+            else if (is_v) put4(&heads_here[slot][4 * u], q.a.x, q.a.y, q.b.x, q.b.y);
+            else store_quad(&heads_here[slot][0], turned(q, R, u, turns), R, u);
+        }
+        if (page < 0 || h0 + kHeads <= heads) continue;              // uniform
+        __syncthreads();
+        const int units = dim / 8, n = threadIdx.x / units, unit = threadIdx.x - n * units, kv = h0 + n - heads;
+        if (n < kHeads && kv >= 0 && kv < 2 * C.kv_heads) {          // (the same for the four lanes of a block)
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = heads_here[n][8 * unit + i];
+            const uint32_t e = mx4_scale(mx4_top(x));
+            const bool v = kv >= C.kv_heads;
+            const int head = v ? kv - C.kv_heads : kv;
+            char* codes = v ? C.v + page * C.v_page + within * C.v_token + head * C.v_head : C.k + page * C.k_page + within * C.k_token + head * C.k_head;
+            uint8_t* scales = v ? X.v + page * X.v_page + within * X.v_token + head * X.v_head : X.k + page * X.k_page + within * X.k_token + head * X.k_head;
+            reinterpret_cast<uint32_t*>(codes)[unit] = mx4_codes(x, e);
+            if (unit % 4 == 0) scales[unit / 4] = (uint8_t)e;
+        }
+        __syncthreads();
     }
 }
 
@@ -1295,6 +1366,26 @@ bool launch_rope_store(const float* qkv, int64_t ld_qkv, float* query, int64_t l
     default: TSHIP_STORE_T(64) break;
     }
 #undef TSHIP_STORE_T
+#undef TSHIP_STORE
+    return hip_ok(hipGetLastError(), "rope store launch");
+}
+
+bool launch_rope_store_mx(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int rows, int heads, const PagedKv& cache,
+                          const MxScales& scales, const int32_t* positions, const float* q_norm, const float* k_norm, float eps,
+                          const RopeSpec& rope, hipStream_t stream)
+{
+    const int lanes = lanes_of(cache.head_dim), at_once = kRopeThreads / lanes, all = heads + 2 * cache.kv_heads;
+    const int chunks = std::max(1, std::min((all + at_once - 1) / at_once, 2048 / rows));
+    const dim3 grid(rows, chunks);
+#define TSHIP_STORE(L)                                                                                                                 \
+    hipLaunchKernelGGL((rope_store_mx_kernel<L>), grid, dim3(kRopeThreads), 0, stream, qkv, ld_qkv, query, ld_query, heads, positions, q_norm, \
+                       k_norm, eps, cache, scales, rope)
+    switch (lanes) {
+    case 8: TSHIP_STORE(8); break;
+    case 16: TSHIP_STORE(16); break;
+    case 32: TSHIP_STORE(32); break;
+    default: TSHIP_STORE(64); break;
+    }
 #undef TSHIP_STORE
     return hip_ok(hipGetLastError(), "rope store launch");
 }

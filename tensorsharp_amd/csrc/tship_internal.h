@@ -338,12 +338,21 @@ struct PagedKv {
     FastDiv page;
 };
 
+// The scales of a cache in four bits; strides in bytes, 0 where there is one page (token, head).
+struct MxScales {
+    uint8_t *k, *v;
+    int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+};
+
 // x [tokens x heads x head_dim] (strides in elements) -> out, which may be x
 bool launch_rope(const float* x, int64_t x_token, int64_t x_head, float* out, int64_t o_token, int64_t o_head, int tokens, int heads,
                  int head_dim, const int32_t* positions, const RopeSpec& rope, hipStream_t stream);
 // rows [q heads | k heads | v heads] -> query rows and the cache; norm weights, positions optional
 bool launch_rope_store(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int rows, int heads, const PagedKv& cache,
                        const int32_t* positions, const float* q_norm, const float* k_norm, float eps, const RopeSpec& rope, hipStream_t stream);
+bool launch_rope_store_mx(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int rows, int heads, const PagedKv& cache,
+                          const MxScales& scales, const int32_t* positions, const float* q_norm, const float* k_norm, float eps,
+                          const RopeSpec& rope, hipStream_t stream);
 
 // How the attention of a call is cut; depends on the shapes alone (where the cuts are, the kernels find out from the lengths).
 struct PagedAttnPlan {
@@ -354,6 +363,37 @@ struct PagedAttnPlan {
 PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window);
 bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64_t ld_query, float* out, int64_t ld_out, int rows, int heads,
                             const PagedKv& cache, float scale, int window, const float* sinks, void* ws, hipStream_t stream);
+
+// Who has which pages (the device memory of a TSHipPagePool).
+struct PagePoolArgs {
+    int32_t* table;
+    int64_t table_stride;
+    int seqs, max_pages, page_size, num_pages;
+    int32_t* references;
+    int32_t* context_lens;
+    int32_t* scratch;
+};
+int64_t page_pool_scratch(int64_t seqs, int64_t max_pages, int64_t num_pages);
+bool launch_resize_sequences(const PagePoolArgs& pool, const int32_t* lengths, int32_t* moves, int32_t* missing, hipStream_t stream);
+bool launch_fork_sequences(const PagePoolArgs& pool, const int32_t* children, const int32_t* parents, int count, int32_t* moves, int32_t* missing,
+                           hipStream_t stream);
+bool launch_compact_pages(const PagePoolArgs& pool, int32_t* moves, int max_moves, hipStream_t stream);
+
+// Keys or values of a cache for copies of its pages: rows of a token and head, of which `inner` is what lies closer together; strides in bytes
+struct PageRows {
+    char* at;
+    int64_t page, outer, inner;
+    uint8_t* scales;               // MXFP4
+    int64_t scale_page, scale_outer, scale_inner;
+};
+struct PageCopyArgs {
+    PageRows src[2], dst[2];       // keys, values
+    int src_pages, dst_pages;
+    bool same;                     // src is dst
+    uint32_t units;                // of eight values, in a page
+    FastDiv by_row, by_inner;      // units of a row, rows of an outer one
+};
+bool launch_copy_pages(const int32_t* moves, int count, const PageCopyArgs& args, int src_type, int dst_type, hipStream_t stream);
 
 constexpr int kMaxSampleVocab = 1 << 20;
 size_t sample_ws_bytes(int rows, int vocab);

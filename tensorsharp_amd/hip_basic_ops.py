@@ -342,31 +342,84 @@ class PagedKVCache:
     bfloat16 (any strides with contiguous rows of head_dim, so that heads may lie before tokens in memory), page_table [sequences,
     pages of a sequence] int32 on the device.  Position p of sequence s is token p % page_size of page page_table[s, p // page_size]; an
     entry outside the pages stands for none.  The contiguous cache [kv heads, max_seq, head_dim] of the whole-layer
-    decode is one page: PagedKVCache(k.transpose(0, 1)[None], v.transpose(0, 1)[None], table of one 0)."""
+    decode is one page: PagedKVCache(k.transpose(0, 1)[None], v.transpose(0, 1)[None], table of one 0).
 
-    def __init__(self, k, v, page_table):
+    In four bits (MXFP4: blocks of 32 along a head): k and v uint8 [pages, tokens, kv heads, head_dim / 2], two codes a byte with the first
+    dimension's in the lower bits, k_scales and v_scales uint8 [pages, tokens, kv heads, head_dim / 32].  A code is sign, two bits of exponent and
+    one of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6) and stands for that times 2^(scale - 127), for NaN where the scale is 255."""
+
+    def __init__(self, k, v, page_table, k_scales=None, v_scales=None):
         torch = _torch()
-        types = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16}
+        types = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16, torch.uint8: N.TYPE_MXFP4}
         if k.dim() != 4 or k.shape != v.shape:
             raise ValueError("PagedKVCache requires 4D tensors of one shape for k and v.")
         if k.dtype not in types or v.dtype != k.dtype:
-            raise ValueError("PagedKVCache requires Float32, Float16 or BFloat16 keys and values of one type.")
+            raise ValueError("PagedKVCache requires Float32, Float16 or BFloat16 keys and values of one type, or UInt8 codes.")
+        four, head_dim, scales = k.dtype is torch.uint8, k.shape[3], ()
+        if four != (k_scales is not None) or four != (v_scales is not None):
+            raise ValueError("PagedKVCache requires k_scales and v_scales with codes of four bits, and only with those.")
+        if four:
+            head_dim *= 2
+            if k_scales.dtype is not torch.uint8 or v_scales.dtype is not torch.uint8 or head_dim % 32 != 0 or \
+                    tuple(k_scales.shape) != (*k.shape[:3], head_dim // 32) or v_scales.shape != k_scales.shape:
+                raise ValueError("PagedKVCache requires UInt8 scales [pages, tokens, kv heads, head_dim / 32], head_dim a multiple of 32.")
+            if k_scales.device != k.device or v_scales.device != k.device:
+                raise ValueError("PagedKVCache requires tensors in GPU memory of one device.")
+            if head_dim > 32 and (k_scales.stride(3) != 1 or v_scales.stride(3) != 1):
+                raise NotImplementedError("PagedKVCache requires contiguous rows of scales.")
+            scales = (k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride()[:3], *v_scales.stride()[:3])
         if page_table.dim() != 2 or page_table.dtype != torch.int32:
             raise ValueError("PagedKVCache requires a 2D Int32 page table.")
         if not k.is_cuda or v.device != k.device or page_table.device != k.device:
             raise ValueError("PagedKVCache requires tensors in GPU memory of one device.")
         if k.stride(3) != 1 or v.stride(3) != 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
             raise NotImplementedError("PagedKVCache requires contiguous rows of head_dim and of the page table.")
-        self.k, self.v, self.page_table = k, v, page_table
-        self.num_kv_heads, self.head_dim, self.num_seqs = k.shape[2], k.shape[3], page_table.shape[0]
-        self.native = N.PagedCache(k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[2], k.shape[3], k.shape[1], k.shape[0], *k.stride()[:3],
-                                   *v.stride()[:3], page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1])
+        self.k, self.v, self.page_table, self.k_scales, self.v_scales = k, v, page_table, k_scales, v_scales
+        self.num_kv_heads, self.head_dim, self.num_seqs = k.shape[2], head_dim, page_table.shape[0]
+        self.native = N.PagedCache(k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[2], head_dim, k.shape[1], k.shape[0], *k.stride()[:3],
+                                   *v.stride()[:3], page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], *scales)
         self.ref = C.byref(self.native)
         self.device = k.get_device()
 
     def _sequences(self, row_starts, context_lens, i32):
         return (_vector(row_starts, i32, self.num_seqs + 1, "row_starts", self.device),
                 _vector(context_lens, i32, self.num_seqs, "context_lens", self.device))
+
+
+class PagePool:
+    """Pages that sequences share, for the caches of all layers: page_table [sequences, pages of a sequence] int32 (the one of the PagedKVCaches),
+    references [pages] int32 (how many sequences have a page, 0: free), context_lens [sequences] int32 (tokens), all on one device and changed in place by
+    ResizeSequences, ForkSequences and CompactPages.  A sequence has the pages of its first ceil(tokens / page_size) entries, behind them is -1: an empty
+    pool is a table of -1 and zeros.  It keeps scratch of its own (an int32 for each entry of the table and for each page)."""
+
+    def __init__(self, page_table, references, context_lens, page_size):
+        torch = _torch()
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_cuda:
+            raise ValueError("PagePool requires a 2D Int32 page table in GPU memory.")
+        if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+            raise NotImplementedError("PagePool requires contiguous rows of the page table.")
+        self.device = page_table.get_device()
+        self.num_seqs, self.num_pages = page_table.shape[0], references.numel()
+        addresses = (_vector(references, torch.int32, self.num_pages, "references", self.device),
+                     _vector(context_lens, torch.int32, self.num_seqs, "context_lens", self.device))
+        count = N.lib().TSHip_PagePoolScratchDevice(self.num_seqs, page_table.shape[1], self.num_pages)
+        if count == 0:
+            raise ValueError("PagePool requires 1 to 65535 sequences and 1 to 2^28 pages.")
+        self.page_table, self.references, self.context_lens, self.page_size = page_table, references, context_lens, int(page_size)
+        self._scratch = torch.empty((count,), dtype=torch.int32, device=page_table.device)
+        self.native = N.PagePool(page_table.data_ptr(), page_table.stride(0), self.num_seqs, page_table.shape[1], self.page_size, self.num_pages, *addresses,
+                                 self._scratch.data_ptr())
+        self.ref = C.byref(self.native)
+
+    def _moves(self, moves, count):
+        """address of a list of pairs, `count` of them (None: as many as there are)"""
+        return _pairs(moves, count, self.device)
+
+
+def _pairs(moves, count, device):
+    if moves.dim() != 2 or moves.shape[1] != 2 or (count is not None and moves.shape[0] != count):
+        raise ValueError(f"moves must be an Int32 tensor [{count if count is not None else 'moves'}, 2].")
+    return _vector(moves, _torch().int32, moves.shape[0] * 2, "moves", device)
 
 
 class HipBasicOps:
@@ -812,6 +865,52 @@ class HipBasicOps:
         _use_stream_of(device)
         ok = N.lib().TSHip_RoPEStorePagedF32Device(qv, xv, qv.dim1 // dim, cache.ref, starts, lens, pos, qn, kn, eps, rope.ref)
         N.check_result(ok, "rope_store_paged")
+
+    @staticmethod
+    def ResizeSequences(pool, lengths, moves, missing):
+        """Sequences of a PagePool become lengths[s] tokens long (int32; negative: stay as they are; 0: have no pages).  Shorter ones give back the pages behind their
+        ends first, longer ones get the lowest free pages; one that goes on in a begun page which others have too gets a page in its place, and moves
+        [sequences, 2] int32 lists the copies (from, to) for CopyPages, -1 behind the last.  Where the free pages do not suffice none grows, and missing [1] int32 says
+        how many more it takes (else 0)."""
+        i32 = _torch().int32
+        to = _vector(lengths, i32, pool.num_seqs, "lengths", pool.device)
+        if to is None or missing is None:
+            raise ValueError("ResizeSequences requires lengths and missing.")
+        m, short = pool._moves(moves, pool.num_seqs), _vector(missing, i32, 1, "missing", pool.device)
+        _use_stream_of(pool.device)
+        N.check_result(N.lib().TSHip_ResizeSequencesDevice(pool.ref, to, m, short), "resize_sequences")
+
+    @staticmethod
+    def ForkSequences(pool, children, parents, moves, missing):
+        """Sequences children[i] of a PagePool become what parents[i] were before the call (int32; of pairs with one child the last counts): they give back their
+        pages and share the whole ones of their parents.  One of those that have a begun page keeps it (the parent, else the lowest child), the others get copies in
+        free pages, listed in moves [pairs, 2] as in ResizeSequences.  Where the free pages do not suffice nothing changes, and missing [1] says how many more it takes."""
+        i32 = _torch().int32
+        if children is None or parents is None or missing is None:
+            raise ValueError("ForkSequences requires children, parents and missing.")
+        count = children.numel()
+        c, p = _vector(children, i32, count, "children", pool.device), _vector(parents, i32, count, "parents", pool.device)
+        m, short = pool._moves(moves, count), _vector(missing, i32, 1, "missing", pool.device)
+        _use_stream_of(pool.device)
+        N.check_result(N.lib().TSHip_ForkSequencesDevice(pool.ref, c, p, count, m, short), "fork_sequences")
+
+    @staticmethod
+    def CompactPages(pool, moves):
+        """Used pages of a PagePool move to the front: the last ones into the lowest free ones, as many as moves [room, 2] int32 has room for; it lists the
+        copies (from, to) for CopyPages, -1 behind the last."""
+        m = pool._moves(moves, None)
+        _use_stream_of(pool.device)
+        N.check_result(N.lib().TSHip_CompactPagesDevice(pool.ref, m, moves.shape[0]), "compact_pages")
+
+    @staticmethod
+    def CopyPages(dst, src, moves):
+        """Pages moves[i, 0] of the PagedKVCache src go into pages moves[i, 1] of dst (int32 [moves, 2]; a pair outside the pages, as -1 is, is left out): one cache
+        or two of one page size, number of heads and head_dim, of one type or two (rounded as RoPEStorePaged does).  No page that is written may be in another pair."""
+        if src.device != dst.device:
+            raise ValueError("CopyPages requires caches on one device.")
+        m = _pairs(moves, None, dst.device)
+        _use_stream_of(dst.device)
+        N.check_result(N.lib().TSHip_CopyPagesDevice(dst.ref, src.ref, m, moves.shape[0]), "copy_pages")
 
     @staticmethod
     def PagedAttention(result, query, cache, row_starts, context_lens, scale, window=0, sinks=None):

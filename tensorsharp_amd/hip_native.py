@@ -43,11 +43,20 @@ class Rope(C.Structure):
 
 
 class PagedCache(C.Structure):
-    """TSHipPagedCache: pages of keys and values and the table that names them; strides in elements."""
+    """TSHipPagedCache: pages of keys and values and the table that names them; strides in elements (of a cache in four bits in bytes)."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("element_type", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int),
                 ("page_size", C.c_int), ("num_pages", C.c_int64), ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64),
                 ("k_head_stride", C.c_int64), ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
-                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("num_seqs", C.c_int), ("max_pages", C.c_int)]
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("num_seqs", C.c_int), ("max_pages", C.c_int), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p), ("k_scales_page_stride", C.c_int64), ("k_scales_token_stride", C.c_int64),
+                ("k_scales_head_stride", C.c_int64), ("v_scales_page_stride", C.c_int64), ("v_scales_token_stride", C.c_int64),
+                ("v_scales_head_stride", C.c_int64)]
+
+
+class PagePool(C.Structure):
+    """TSHipPagePool: which sequence has which pages, and how many have each."""
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("num_seqs", C.c_int), ("max_pages", C.c_int), ("page_size", C.c_int),
+                ("num_pages", C.c_int64), ("references", C.c_void_p), ("context_lens", C.c_void_p), ("scratch", C.c_void_p)]
 
 
 class NativeLibraryMissing(RuntimeError):
@@ -154,6 +163,11 @@ SIGNATURES.update({
                                                 C.c_void_p, C.c_void_p, C.c_float, C.POINTER(Rope)]),
     "TSHip_PagedAttentionF32Device": (C.c_int, [TensorView2D, TensorView2D, C.c_int, C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_float,
                                                 C.c_int, C.c_void_p]),
+    "TSHip_PagePoolScratchDevice": (C.c_int64, [C.c_int, C.c_int, C.c_int64]),
+    "TSHip_ResizeSequencesDevice": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "TSHip_ForkSequencesDevice": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "TSHip_CompactPagesDevice": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_int]),
+    "TSHip_CopyPagesDevice": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedCache), C.c_void_p, C.c_int]),
     "TSHip_SampleTokensF32Device": (C.c_int, [TensorView2D, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
 })
 # the host-pointer forms take the same argument lists
