@@ -521,6 +521,11 @@ TSHIP_EXPORT int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTen
 TSHIP_EXPORT int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
                                                const int32_t* row_starts, const int32_t* context_lens, float scale, int window,
                                                const float* sinks);
+/* The same with the first `first` positions visible behind the window: position p sees j <= p where j > p - window or j < first (window 0: all). */
+TSHIP_EXPORT int TSHip_PagedAttentionFirstF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
+                                                    const int32_t* row_starts, const int32_t* context_lens, float scale, int window, int first,
+                                                    const float* sinks);
+
 /* Pages that sequences share: table as in TSHipPagedCache (one for the caches of all layers), context_lens the tokens that each sequence has, references
  * how many sequences have a page (num_pages; 0: free).  A sequence has the pages of its first ceil(context_lens / page_size) entries; what lies behind
  * them is -1.  All device memory, changed by the calls below as if in one step each; an entry outside [0, num_pages) is no page and counts nowhere.

@@ -3256,15 +3256,18 @@ int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTensorView2D qkv
 int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
                                   const int32_t* row_starts, const int32_t* context_lens, float scale, int window, const float* sinks)
 {
+    return TSHip_PagedAttentionFirstF32Device(result, query, num_heads, cache, row_starts, context_lens, scale, window, 0, sinks);
+}
+
+int TSHip_PagedAttentionFirstF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
+                                       const int32_t* row_starts, const int32_t* context_lens, float scale, int window, int first,
+                                       const float* sinks)
+{
     return guarded(0, "paged_attention", [&]() -> int {
         if (!ensure_backend()) return 0;
         PagedKv kv;
         MxScales scales;
         if (!validate_cache(cache, num_heads, row_starts, context_lens, &kv, &scales)) return 0;
-        if (kv.element_type == kTypeMXFP4) {
-            set_last_error("paged_attention: not over MXFP4 yet.");
-            return 0;
-        }
         const int64_t columns = (int64_t)num_heads * kv.head_dim;
         if (!validate_rows(result, columns, true, "result") || !validate_rows(query, columns, false, "query")) return 0;
         if (query.dim0 != result.dim0) {
@@ -3275,6 +3278,11 @@ int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D qu
             set_last_error("paged_attention: the window must not be negative and the scale finite.");
             return 0;
         }
+        if (first < 0) {
+            set_last_error("paged_attention: the number of first positions must not be negative.");
+            return 0;
+        }
+        if (window == 0) first = 0;                                    // (all positions are visible)
         const int T = query.dim0;
         const TSHipTensorView3D r3{result.data, T, 1, result.dim1, result.stride0, 0, 1, result.raw_bytes};
         const TSHipTensorView3D q3{query.data, T, 1, query.dim1, query.stride0, 0, 1, query.raw_bytes};
@@ -3282,11 +3290,11 @@ int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D qu
             set_last_error("paged_attention: result overlaps query without being the same view.");
             return 0;
         }
-        const PagedAttnPlan plan = plan_paged_attention(T, num_heads, kv, window);
+        const PagedAttnPlan plan = plan_paged_attention(T, num_heads, kv, window, first);
         WsLease lease(t_stream, plan.ws_bytes);
         if (!lease.ok()) return 0;
         if (!launch_paged_attention(plan, static_cast<const float*>(query.data), query.stride0, static_cast<float*>(result.data), result.stride0, T,
-                                    num_heads, kv, scale, window, sinks, lease.ptr(), t_stream))
+                                    num_heads, kv, scales, scale, window, first, sinks, lease.ptr(), t_stream))
             return 0;
         clear_last_error();
         return 1;

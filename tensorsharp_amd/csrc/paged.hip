@@ -7,6 +7,7 @@
 //   paged_attention_kernel   softmax(scale q K^T) V of a sequence's new tokens over its pages
 #include "tship_internal.h"
 #include "mx4.h"
+#include "paged_tiles.h"
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -18,11 +19,6 @@
 
 namespace tship {
 namespace {
-
-constexpr int kMaxDim = 256;
-
-typedef float f2_t __attribute__((ext_vector_type(2)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
 
 // ---- rotary positions ----------------------------------------------------------------------------
 
@@ -306,288 +302,9 @@ int lanes_of(int head_dim) { return head_dim <= 32 ? 8 : head_dim <= 64 ? 16 : h
 // own, and meet at the end.  Others (prompts): tiles of 128 rows, each wavefront has 32 of them and all share the keys in LDS.
 // With few tiles the keys are cut further over workgroups, whose states paged_combine_kernel joins.
 
-typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
-typedef float f16_t __attribute__((ext_vector_type(16)));
-typedef short s4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) uint8_t* lds_t;
-
-constexpr int kAttnWaves = 4, kAttnThreads = 64 * kAttnWaves;
-constexpr int kKeyRows = 32;         // rows of a sequence up to which its wavefronts share rows and not keys
-constexpr int kTileRows = 32 * kAttnWaves;
-constexpr int kMaxPieces = 1024;      // that a tile's keys are cut into
-constexpr float kLog2e = 1.44269504088896340736f;
-// rows that a lane's page has not (past the end, or no page at all) are read from here
-__device__ __attribute__((aligned(16))) uint8_t g_zero_row[kMaxDim * 4];
-
-struct AttnArgs {
-    const float* query;
-    float* out;
-    const float* sinks;
-    float* partial;              // [piece][KV head][row of the tile][head_dim] weighted values, then [piece][KV head][row] (unit, sum)
-    int64_t ld_query, ld_out;
-    float c;                     // |scale| log2 e
-    float sign;                  // of scale, 0 where it is 0
-    int rows, group, window, capacity;
-    int slots, slot_rows;        // of partial
-    FastDiv by_group;
-    PagedKv cache;
-};
-
-// A tile: rows row0 .. row0 + count - 1 of the rows of a sequence, whose new tokens are rows first .. of the batch and begin at
-// position p0; and the keys that it has, or the piece of them that a workgroup takes.
-struct AttnTile {
-    int first, tokens, p0, row0, count;
-    int seq;
-    int lo, hi;
-    int cuts, slot;              // pieces of its keys; where the first one's (this one's) state goes
-};
-__device__ __forceinline__ int tiles_of(int rows) { return rows <= kKeyRows ? (rows > 0 ? 1 : 0) : (rows + kTileRows - 1) / kTileRows; }
-__device__ __forceinline__ int clamped(int v, int hi) { return max(0, min(v, hi)); }
-// inclusive sum over the lanes of a wavefront, in registers
-__device__ __forceinline__ int lane_scan(int v)
-{
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);          // from the lane 1, 2, 4, 8 below, within 16 lanes
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);         // the last lane of 16 to the next 16
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);         // of 32 to the upper 32
-    return v;
-}
-__device__ __forceinline__ int lane_sum(int v) { return __builtin_amdgcn_readlane(lane_scan(v), 63); }
-
-// What the kernels need to find their piece.  It stands in front of the other arguments: the hardware delivers the first 14 dwords in
-// registers at wave launch (a structure is read from the argument block instead), so that the lengths are asked for at once.
-struct Lens {
-    const int32_t* row_starts;
-    const int32_t* context_lens;
-    int seqs, rows, group, window;
-    int pieces;                  // per KV head that the chip takes at once; 0: keys are not cut
-    int capacity;                // positions that the page table has room for
-};
-#define TSHIP_LENS_ARGS const int32_t *row_starts, const int32_t *context_lens, int seqs, int rows, int group, int window, int pieces, int capacity
-#define TSHIP_LENS Lens{row_starts, context_lens, seqs, rows, group, window, pieces, capacity}
-
-// 64 sequences, one per lane
-struct Lanes {
-    int start, n, context;
-    int tiles, steps;            // steps of 128 keys that a tile has at most
-    __device__ __forceinline__ void load(const Lens& H, int s0)
-    {
-        const int s = s0 + (threadIdx.x & 63);
-        start = n = context = 0;
-        if (s < H.seqs) {
-            const int a = H.row_starts[s], b = H.row_starts[s + 1];
-            context = max(H.context_lens[s], -(1 << 30));
-            start = clamped(a, H.rows);
-            n = max(0, clamped(b, H.rows) - start);
-        }
-        tiles = tiles_of(n * H.group);
-        // (a tile's rows are of at most 128 tokens)
-        int span = min(max(0, context), H.capacity);
-        if (H.window > 0) span = (int)min((int64_t)span, (int64_t)H.window + min(n, kTileRows));
-        steps = (span + 127) >> 7;
-    }
-    __device__ __forceinline__ int cuts(int len) const { return max(1, (steps + len - 1) / len); }
-};
-
-// Steps of 128 keys that pieces have to save a tile to be worth it.  Joining them takes 5 us where they are few, 8.5 for many short tiles, 7.5
-// for long ones (3 of it the second launch, which comes wherever the page table has room for as many positions).  A step takes a short tile of
-// 64, 128, 256 dimensions 1.0, 1.4, 2.9 us in fp16 (bf16 0.9, 1.6, 3.5; fp32, by fewer wavefronts, 2.1, 8.4, 19.3) and a long one 2.6, 4.4,
-// 8.7 (bf16 4.1, 5.6, 12.2; fp32 7.4, 12.5, 29.5): by the dimensions, near enough.  One sequence of 512 keys, 256 dimensions and 8 KV heads: cut
-// 37 us, uncut 90 in fp32, 18 and 22 in fp16; 16 of 128 dimensions in fp16: 17 and 13.
-struct Worth {
-    int few, many, tall;
-};
-__host__ __device__ constexpr Worth worth_of(int type, int hd, int key_waves)
-{
-    const int step = hd * (type == kTypeF32 ? 14 : 5) / (10 * key_waves);                  // 0.1 us
-    const int tall = hd * (type == kTypeF32 ? 110 : type == kTypeF16 ? 40 : 55) / 100;
-    return {(50 + step - 1) / step, (85 + step - 1) / step, (75 + tall - 1) / tall};
-}
-__host__ __device__ constexpr int key_waves_of(int type, int hd) { return type != kTypeF32 || hd == 64 ? 4 : hd == 96 || hd == 192 ? 3 : 2; }
-__host__ __device__ constexpr int dims_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
-
-// How many steps of 128 keys a piece has, so that the pieces of all tiles are about as many as the chip takes at once and as long as one
-// another (more would wait for a second round, fewer or unequal ones leave compute units without work).  At least their mean, in
-// a few tries up to what is certain to be enough.  32 sequences of 4096 keys and 8 KV heads: 104 us in 512 pieces, 107 in 1024, 136 in 4096.
-__device__ __forceinline__ int piece_steps(const Lens& H, int kv_heads, Worth least, Lanes& L)
-{
-    constexpr int kUncut = 1 << 24;
-    L.load(H, 0);
-    if (H.pieces == 0) return kUncut;
-    int tiles = 0;
-    float steps = 0.f;
-    for (int s0 = 0;;) {
-        tiles += lane_sum(L.tiles);
-        steps += (float)lane_sum(min(L.tiles * min(L.steps, 1 << 16), 1 << 24));
-        s0 += 64;
-        if (s0 >= H.seqs) break;
-        L.load(H, s0);
-    }
-    if (tiles >= H.pieces) {
-        if (H.seqs > 64) L.load(H, 0);
-        return kUncut;
-    }
-    const float mean = steps / (float)H.pieces, enough = fmaxf(steps / (float)(H.pieces - tiles), mean);
-    int len = 0;
-    bool worth = false;
-    float f = 1.f;
-    for (int i = 0;; ++i, f *= 1.15f) {
-        // (a length that no tile exceeds ends it in any case)
-        len = i < 5 ? max(1, (int)ceilf(fminf(mean * f, enough))) : i == 5 ? max(1, (int)ceilf(enough)) : len + len / 8 + 1;
-        int all = 0;
-        worth = false;
-        for (int s0 = 0; s0 < H.seqs; s0 += 64) {
-            if (H.seqs > 64) L.load(H, s0);
-            all += lane_sum(L.tiles * L.cuts(len));
-            worth |= __any(L.steps - len >= (L.n * H.group > kKeyRows ? least.tall : tiles * kv_heads >= 64 ? least.many : least.few));
-        }
-        if (all <= H.pieces) break;
-    }
-    if (!worth) len = kUncut;
-    if (H.seqs > 64) L.load(H, 0);
-    return len;
-}
-
-// rows and keys of tile number `tile` of the sequence of lane `at`
-__device__ __forceinline__ void set_tile(const AttnArgs& A, const Lanes& L, int s0, int at, int tile, int len, AttnTile& t)
-{
-    t.seq = s0 + at;
-    t.first = __builtin_amdgcn_readlane(L.start, at);
-    t.tokens = __builtin_amdgcn_readlane(L.n, at);
-    t.p0 = __builtin_amdgcn_readlane(L.context, at) - t.tokens;
-    t.cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
-    const int rows = t.tokens * A.group;
-    t.row0 = tile * kTileRows;
-    t.count = min(rows - t.row0, rows <= kKeyRows ? kKeyRows : kTileRows);
-    const int p_first = t.p0 + (int)A.by_group.quot(t.row0), p_last = t.p0 + (int)A.by_group.quot(t.row0 + t.count - 1);
-    t.hi = min(p_last + 1, A.capacity);
-    t.lo = min(first_key(p_first, A.window), max(0, t.hi));          // (a window may lie behind what the table has room for)
-}
-// keys of each piece of a tile, whole steps of 128
-__device__ __forceinline__ int piece_keys(const AttnTile& t) { return ((max(0, t.hi - t.lo) + 127) / 128 + t.cuts - 1) / t.cuts * 128; }
-
-__device__ __forceinline__ int64_t slot_row(const AttnArgs& A, int slot, int kvh, int row) { return ((int64_t)slot * A.cache.kv_heads + kvh) * A.slot_rows + row; }
-__device__ __forceinline__ f2_t* states_of(const AttnArgs& A)
-{
-    return reinterpret_cast<f2_t*>(A.partial + (int64_t)A.slots * A.cache.kv_heads * A.slot_rows * A.cache.head_dim);
-}
-// behind the states: piece_steps, from the attention for the kernel that joins
-__device__ __forceinline__ int* steps_of(const AttnArgs& A) { return reinterpret_cast<int*>(states_of(A) + (int64_t)A.slots * A.cache.kv_heads * A.slot_rows); }
-
-// The idx-th piece from the end (the last tiles of a prompt have the most keys and go first); every wavefront looks for itself.
-__device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int kv_heads, Worth least, int idx, AttnTile& t)
-{
-    Lanes L;
-    const int len = piece_steps(H, kv_heads, least, L);
-    if (H.pieces > 0 && blockIdx.x == 0 && idx == 0 && threadIdx.x == 0) *steps_of(A) = len;
-    int cum = lane_scan(L.tiles * L.cuts(len)), total = __builtin_amdgcn_readlane(cum, 63);
-    for (int s0 = 64; s0 < H.seqs; s0 += 64) {
-        L.load(H, s0);
-        total += lane_sum(L.tiles * L.cuts(len));
-    }
-    int want = total - 1 - idx, s0 = 0;
-    if (want < 0) return false;
-    t.slot = want;
-    if (H.seqs > 64) L.load(H, 0);
-    while (want >= __builtin_amdgcn_readlane(cum, 63)) {             // (fewer than the total)
-        want -= __builtin_amdgcn_readlane(cum, 63);
-        s0 += 64;
-        L.load(H, s0);
-        cum = lane_scan(L.tiles * L.cuts(len));
-    }
-    const int at = __ffsll((unsigned long long)__ballot(want < cum)) - 1;
-    const int cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
-    want -= __builtin_amdgcn_readlane(cum, at) - __builtin_amdgcn_readlane(L.tiles, at) * cuts;
-    set_tile(A, L, s0, at, want / cuts, len, t);
-    const int keys = piece_keys(t), begin = t.lo + want % cuts * keys;
-    t.hi = min(begin + keys, t.hi);
-    t.lo = begin;
-    return true;
-}
-// What a row's weighted values are multiplied by: 1 / (sum + the sink's weight), sum being counted in units of 2^unit; 1 / 0 never.  (The sink may be far
-// above the units that m came down to.)
-__device__ __forceinline__ float over_sum(const AttnArgs& A, float sum, float unit, int head)
-{
-    if (!(sum > 0.f)) return 0.f;
-    if (!A.sinks) return 1.0f / sum;
-    const float e = A.sinks[head] * kLog2e - unit, h = fmaxf(e, 0.f), by = __builtin_amdgcn_exp2f(-h);
-    return by / (sum * by + (e > 0.f ? 1.f : __builtin_amdgcn_exp2f(e)));
-}
-// the tile of a row and head and its first piece; false: of no sequence
-__device__ __forceinline__ bool find_row(const Lens& H, const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)
-{
-    const int len = *steps_of(A);
-    Lanes L;
-    int before = 0;
-    for (int s0 = 0; s0 < H.seqs; s0 += 64) {
-        L.load(H, s0);
-        const int cum = lane_scan(L.tiles * L.cuts(len));
-        const uint64_t has = __ballot(row >= L.start && row < L.start + L.n);
-        if (has) {
-            const int at = __ffsll((unsigned long long)has) - 1;
-            const int cuts = __builtin_amdgcn_readlane(L.cuts(len), at);
-            const int r = (row - __builtin_amdgcn_readlane(L.start, at)) * H.group + head % H.group;
-            const int tile = __builtin_amdgcn_readlane(L.n, at) * H.group <= kKeyRows ? 0 : r / kTileRows;
-            set_tile(A, L, s0, at, tile, len, t);
-            t.slot = before + __builtin_amdgcn_readlane(cum, at) + (tile - __builtin_amdgcn_readlane(L.tiles, at)) * cuts;
-            *in_tile = r - t.row0;
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(cum, 63);
-    }
-    return false;
-}
-__device__ __forceinline__ uint32_t high_halves(float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); }
-__device__ __forceinline__ float below_bf16(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-// eight floats as three times eight bf16 that sum up to them
-__device__ __forceinline__ void cut3(const float (&x)[8], u4_t (&part)[3])
-{
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = below_bf16(x0), y1 = below_bf16(x1);
-        part[0][i] = high_halves(x0, x1);
-        part[1][i] = high_halves(y0, y1);
-        part[2][i] = high_halves(below_bf16(y0), below_bf16(y1));
-    }
-}
-// eight floats in fp16's range as twice eight fp16, both to nearest: what is left is below 2^-24 of each, or 2^-25 where that is more
-__device__ __forceinline__ void cut2(const float (&x)[8], u4_t (&part)[2])
-{
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const h2_t hi = __builtin_convertvector((f2_t{x[2 * i], x[2 * i + 1]}), h2_t);
-        const h2_t lo = __builtin_convertvector((f2_t{x[2 * i] - (float)hi[0], x[2 * i + 1] - (float)hi[1]}), h2_t);
-        part[0][i] = __builtin_bit_cast(uint32_t, hi);
-        part[1][i] = __builtin_bit_cast(uint32_t, lo);
-    }
-}
-__device__ __forceinline__ float both_halves(float x, float (*op)(float, float))
-{
-    const u2_t r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return op(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ float added(float a, float b) { return a + b; }
-
-template <int... I, typename F>
-__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f)
-{
-    (f(std::integral_constant<int, I>()), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each_of(F&& f)
-{
-    each_of(std::make_integer_sequence<int, N>(), f);
-}
-
-// TYPE: 0 fp32, 1 fp16, 2 bf16 cache; HD: head_dim rounded up to what the tiles are made for
-template <int TYPE, int HD>
+// TYPE: 0 fp32, 1 fp16, 2 bf16 cache; HD: head_dim rounded up to what the tiles are made for; FIRST: whether first positions stay visible
+// behind a window
+template <int TYPE, int HD, bool FIRST>
 struct Attn {
     static constexpr int kElem = TYPE == 0 ? 4 : 2;
     static constexpr int kRow = HD * kElem, kPieces = kRow / 16;     // a key (value) in LDS, 16 bytes at a time
@@ -861,12 +578,16 @@ struct Attn {
     {
         if constexpr (TYPE == 0 && HD == 128) __builtin_amdgcn_sched_barrier(0);
     }
+    // position of a key, where keys are not there, and whether it is one of the first
+    __device__ __forceinline__ int position(int key) const { return FIRST ? t.position(key) : key; }
+    __device__ __forceinline__ int end_at(int key) const { return FIRST ? t.end_at(key) : t.hi; }
+    __device__ __forceinline__ bool in_head(int key) const { return FIRST && key < t.head; }
     // Of the 16 scores of a lane number i belongs to key 8 (i / 4) + 4 half + i % 4 of the block.
-    __device__ __forceinline__ void mask(f16_t& s, int key0, uint64_t there) const
+    __device__ __forceinline__ void mask(f16_t& s, int key0, uint64_t there, bool head) const
     {
         const int below = 4 * (lane_here() >> 5);
         const uint32_t bits = (uint32_t)(there >> below);
-        const int last = p - key0 - below, first = lo - key0 - below;
+        const int last = p - key0 - below, first = head ? 0 : lo - key0 - below;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int k = 8 * (i / 4) + i % 4;
@@ -1010,9 +731,9 @@ struct Attn {
             const int last = t.p0 + token, first = first_key(last, A.window);
             float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
-                const int j = j0 + lane;
+                const int j = position(j0) + lane;
                 int id = -1;
-                if (j < t.hi && j >= first && j <= last) id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)j)];
+                if (j < end_at(j0) && (in_head(j0) || j >= first) && j <= last) id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)j)];
                 const bool seen = (uint32_t)id < (uint32_t)A.cache.num_pages;
                 const uint64_t lanes = __ballot(seen);
                 if (lanes == 0) continue;
@@ -1087,24 +808,25 @@ struct Attn {
         int buffer = 0;
         if (begin < end) {
             // copies go a step ahead; those behind the last key bring zeros that nothing reads
-            Rows rows = rows_of<true>(begin, end, wave);
+            Rows rows = rows_of<true>(position(begin), end_at(begin), wave);
             stage(rows, lds);
             load_rows(32 * wave + col);                              // (while the first keys are on their way)
-            for (int key0 = begin; key0 < end; key0 += kKeys) {
+            for (int key = begin; key < end; key += kKeys) {
+                const int key0 = position(key);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 const lds_t here = lds + buffer * (2 * NT * kBlock);
                 const uint64_t there = rows.there;
                 buffer ^= 1;
-                rows = rows_of<true>(key0 + kKeys, end, wave);
+                rows = rows_of<true>(position(key + kKeys), end_at(key + kKeys), wave);
                 stage(rows, lds + buffer * (2 * NT * kBlock));
                 // (a wavefront without rows copies only, as does one whose rows see none of the keys)
                 if (32 * wave < t.count && key0 <= p_last) {
                     f16_t s[NT];
 #pragma unroll
                     for (int b = 0; b < NT; ++b) s[b] = scores(here + b * kBlock);
-                    if (~there != 0 || key0 + kKeys - 1 > p_first || key0 < lo_last) {
+                    if (~there != 0 || key0 + kKeys - 1 > p_first || (!in_head(key) && key0 < lo_last)) {
 #pragma unroll
-                        for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b));
+                        for (int b = 0; b < NT; ++b) mask(s[b], key0 + 32 * b, there >> (32 * b), in_head(key));
                     }
                     follow_maximum(s, NT);
                     float sum = 0.f;
@@ -1153,26 +875,27 @@ struct Attn {
         const int p_last = t.p0 + t.tokens - 1;
         const int lo_last = first_key(p_last, A.window);
         const lds_t kb = lds + wave * 2 * kBlock, vb = kb + kBlock;
-        int key0 = begin + 32 * wave;
+        int key = begin + 32 * wave;
         constexpr int kStride = 32 * kKeyWaves;
-        if (wave < kKeyWaves && key0 < end) {
+        if (wave < kKeyWaves && key < end) {
             auto stage = [&](auto is_v, uint64_t rows, lds_t block) {
                 const int ln = lane_here();
                 each_of<kCopies>([&](auto n) { copy<decltype(is_v)::value, decltype(n)::value>(rows, decltype(n)::value, block, ln); });
             };
-            Rows rows = rows_of<false>(key0, end, wave);
+            Rows rows = rows_of<false>(position(key), end_at(key), wave);
             stage(std::false_type(), rows.k, kb);
             stage(std::true_type(), rows.v, vb);
             load_rows(col);                                          // (while the first keys are on their way)
-            for (; key0 < end; key0 += kStride) {
+            for (; key < end; key += kStride) {
+                const int key0 = position(key);
                 // loads answer in order: with kCopies of them left, the values behind the keys, the keys have arrived
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");
                 f16_t s[1] = {scores(kb)};
                 const uint64_t there = rows.there;
-                rows = rows_of<false>(key0 + kStride, end, wave);
+                rows = rows_of<false>(position(key + kStride), end_at(key + kStride), wave);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 stage(std::false_type(), rows.k, kb);
-                if (~there != 0 || key0 + 31 > t.p0 || key0 < lo_last) mask(s[0], key0, there);
+                if (~there != 0 || key0 + 31 > t.p0 || (!in_head(key) && key0 < lo_last)) mask(s[0], key0, there, in_head(key));
                 follow_maximum(s, 1);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");                 // the values too: the next keys are left
                 add_weights(weigh(s[0], vb));
@@ -1232,17 +955,29 @@ struct Attn {
 };
 
 // grid (KV heads, pieces)
-template <int TYPE, int HD>
-__global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD>::kOneWave ? 1 : 2)) paged_attention_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
+template <int TYPE, int HD, bool FIRST>
+__device__ __forceinline__ void attend(const Lens& H, const AttnArgs& A, lds_t smem)
 {
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
     AttnTile t;
-    if (!find_piece(TSHIP_LENS, A, gridDim.x, worth_of(TYPE, HD, key_waves_of(TYPE, HD)), idx, t)) return;
-    Attn<TYPE, HD> a(A, t, kvh, (lds_t)smem);
+    if (!find_piece(H, A, gridDim.x, worth_of(TYPE, HD, key_waves_of(TYPE, HD)), idx, t)) return;
+    Attn<TYPE, HD, FIRST> a(A, t, kvh, smem);
     const bool own = t.tokens * A.group <= kKeyRows;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (own ? a.own_keys() : a.shared_keys()) a.plainly(own ? wave : 32 * wave, own ? kAttnWaves : 1);
+}
+template <int TYPE, int HD>
+__global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD, false>::kOneWave ? 1 : 2)) paged_attention_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    attend<TYPE, HD, false>(TSHIP_LENS, A, (lds_t)smem);
+}
+// A kernel of its own, so that what has no first positions does without their arithmetic.
+template <int TYPE, int HD>
+__global__ void __launch_bounds__(kAttnThreads, (Attn<TYPE, HD, true>::kOneWave ? 1 : 2)) paged_first_attention_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    attend<TYPE, HD, true>(TSHIP_LENS, A, (lds_t)smem);
 }
 
 __host__ __device__ constexpr int wide_of(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
@@ -1276,9 +1011,9 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
     int in_tile;
     if (!find_row(TSHIP_LENS, A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all heads of a row)
     const int cuts = t.cuts, step = WAVES == 1 ? 1 : WAVES * parts;
-    const int64_t first = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
-    const float* values = A.partial + first * dim;
-    const f2_t* states = states_of(A) + first;
+    const int64_t at0 = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
+    const float* values = A.partial + at0 * dim;
+    const f2_t* states = states_of(A) + at0;
     constexpr int U = WAVES == 1 ? 8 : 4;
     // (a piece's values may be as large as fp32 is: what is joined counts in units of 2^(top + kSpare), which leave room for kMaxPieces of them)
     constexpr float kSpare = 10.f;
@@ -1390,7 +1125,7 @@ bool launch_rope_store_mx(const float* qkv, int64_t ld_qkv, float* query, int64_
     return hip_ok(hipGetLastError(), "rope store launch");
 }
 
-PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window)
+PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window, int first)
 {
     const int group = heads / cache.kv_heads, dim = cache.head_dim;
     const int64_t all = (int64_t)rows * group;
@@ -1400,7 +1135,7 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
     // workgroups that are resident at once
     const int at_once = device_info().num_cus * (dim <= 64 && cache.element_type != kTypeF32 ? 3 : dim <= 128 ? 2 : 1);
     const int64_t pieces = std::min(kMaxPieces, std::max(1, at_once / cache.kv_heads)), keys = (int64_t)cache.max_pages * cache.page.d;
-    const int64_t most = std::min<int64_t>(keys, window > 0 ? window : keys);
+    const int64_t most = std::min<int64_t>(keys, window > 0 ? (int64_t)window + first : keys);
     const int hd = dims_of(dim);
     const Worth least = worth_of(cache.element_type, hd, key_waves_of(cache.element_type, hd));
     const bool cut = (all + kTileRows - 1) / kTileRows < pieces &&
@@ -1418,10 +1153,10 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
 template <int TYPE, int HD>
 static bool launch_attention(const Lens& H, const AttnArgs& args, const dim3& grid, hipStream_t stream)
 {
-    const auto kern = paged_attention_kernel<TYPE, HD>;
-    constexpr size_t lds = Attn<TYPE, HD>::kLds;
+    const auto kern = args.first > 0 ? paged_first_attention_kernel<TYPE, HD> : paged_attention_kernel<TYPE, HD>;
+    constexpr size_t lds = Attn<TYPE, HD, false>::kLds;
     if (!raise_lds_limit(reinterpret_cast<const void*>(kern), lds)) return false;
-    hipLaunchKernelGGL(kern, grid, dim3(kAttnThreads), lds, stream, H.row_starts, H.context_lens, H.seqs, H.rows, H.group, H.window, H.pieces, H.capacity, args);
+    hipLaunchKernelGGL(kern, grid, dim3(kAttnThreads), lds, stream, TSHIP_LENS_OF(H), args);
     return hip_ok(hipGetLastError(), "paged attention launch");
 }
 template <int TYPE>
@@ -1437,7 +1172,8 @@ static bool launch_attention(const Lens& H, const AttnArgs& args, const dim3& gr
 }
 
 bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64_t ld_query, float* out, int64_t ld_out, int rows, int heads,
-                            const PagedKv& cache, float scale, int window, const float* sinks, void* ws, hipStream_t stream)
+                            const PagedKv& cache, const MxScales& scales, float scale, int window, int first, const float* sinks, void* ws,
+                            hipStream_t stream)
 {
     AttnArgs args{};
     args.query = query;
@@ -1451,6 +1187,7 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     args.rows = rows;
     args.group = heads / cache.kv_heads;
     args.window = window;
+    args.first = first;
     args.capacity = cache.max_pages * (int)cache.page.d;
     args.slots = plan.pieces;
     args.slot_rows = plan.slot_rows;
@@ -1460,23 +1197,22 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
         set_last_error("paged_attention: too many rows for one call.");
         return false;
     }
-    const Lens H{cache.row_starts, cache.context_lens, cache.seqs, rows, args.group, window, plan.pieces, args.capacity};
+    const Lens H{cache.row_starts, cache.context_lens, cache.seqs, rows, args.group, window, first, plan.pieces, args.capacity};
     const unsigned layers = (plan.slots + 65534u) / 65535u;
     const dim3 grid(cache.kv_heads, (plan.slots + layers - 1) / layers, layers);
     bool ok;
     switch (cache.element_type) {
     case kTypeF32: ok = launch_attention<0>(H, args, grid, stream); break;
     case kTypeF16: ok = launch_attention<1>(H, args, grid, stream); break;
+    case kTypeMXFP4: ok = launch_mx_attention(H, args, scales, grid, stream); break;
     default: ok = launch_attention<2>(H, args, grid, stream); break;
     }
     if (!ok || plan.pieces == 0) return ok;
     if ((int64_t)rows * heads <= 8 * device_info().num_cus) {
-        hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens, H.seqs, H.rows, H.group, H.window,
-                           H.pieces, H.capacity, args);
+        hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, TSHIP_LENS_OF(H), args);
     } else {
         const int parts = 64 / wide_of(cache.head_dim), waves = rows * ((args.group + parts - 1) / parts);
-        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(cache.kv_heads, (waves + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, H.row_starts, H.context_lens,
-                           H.seqs, H.rows, H.group, H.window, H.pieces, H.capacity, args);
+        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(cache.kv_heads, (waves + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, TSHIP_LENS_OF(H), args);
     }
     return hip_ok(hipGetLastError(), "paged attention combine launch");
 }

@@ -1,0 +1,654 @@
+// Attention over a paged cache in four bits (MXFP4: blocks of 32 along a head).
+//
+// The tiles, pieces and states are those of the attention over caches of 16 and 32 bits (paged_tiles.h), and so are the products' order, S^T = K Q^T and
+// O^T += V^T P^T, and what weights are counted against.  What differs follows from the block format:
+//
+// * K goes into the block-scaled matrix instruction as it is: a lane's operand is one block, 16 bytes of codes and the power as the operand's scale, loaded
+//   from memory into the registers that the instruction reads.  Nothing is unpacked.  A row of Q is cut into kParts terms of fp6 (E2M3, four significant bits) in
+//   blocks of 32 with a power of its own each, the next one from what rounding left, so that five of them hold 22 bits and more of the block's largest.  A
+//   term takes a quarter of the time of one in 16 bits: 5 / 4 of a product in 16 bits, where the exact values in bf16 would take three, and their unpacking.
+// * V's blocks lie along its dimensions, but O^T adds over keys, along which the powers differ: there is no such operand.  A lane turns one block into bf16 (exact:
+//   two significant bits and the power) with the instruction that converts two codes at a time, through LDS, from which the operand is read transposed.
+//   Weights go in as three parts of bf16, 24 bits.
+#include "tship_internal.h"
+#include "mx4.h"
+#include "paged_tiles.h"
+
+namespace tship {
+namespace {
+
+typedef int i8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u6_t __attribute__((ext_vector_type(6)));
+typedef float v32_t __attribute__((ext_vector_type(32)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kParts = 5;
+
+// 32 floats of a row as fp6 terms with a power each (biased; byte i of scale[i / 4])
+struct Terms {
+    u6_t t[kParts];
+    uint32_t scale[2];
+};
+// The least power of which the largest magnitude is at most 7.5, the last fp6 value; at least 2^-126, 255 for infinities and NaN.
+__device__ __forceinline__ uint32_t fp6_power(uint32_t top)
+{
+    if (top >= 0x7f800000u) return 255;
+    const int e = (int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0);
+    return e < 1 ? 1u : (uint32_t)e;
+}
+__device__ __forceinline__ void cut_terms(f16_t a, f16_t b, Terms& out)      // a: the even ones, b: the odd ones
+{
+    out.scale[0] = out.scale[1] = 0;
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+        const uint32_t e = fp6_power(top);
+        const float by = __uint_as_float(e == 255 ? 127u << 23 : e << 23);
+        out.t[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, by);
+        out.scale[n / 4] |= e << (8 * (n % 4));
+        if (n + 1 < kParts) {
+            const v32_t back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(out.t[n], by);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                a[i] -= back[2 * i];
+                b[i] -= back[2 * i + 1];
+            }
+        }
+    }
+}
+__device__ __forceinline__ i8_t operand(const u4_t& x) { return i8_t{(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0}; }
+__device__ __forceinline__ i8_t operand(const u6_t& x) { return i8_t{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)x[4], (int)x[5], 0, 0}; }
+
+// a block of codes with its power as 32 bf16 values, 16 bytes at a time
+__device__ __forceinline__ u4_t as_bf16(uint32_t codes, float scale)
+{
+    u4_t r;
+    r[0] = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+    r[1] = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+    r[2] = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+    r[3] = __builtin_bit_cast(uint32_t, (b2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+    return r;
+}
+
+typedef __attribute__((address_space(3))) u4_t* lds4_t;
+
+// HD: head_dim rounded up to what the tiles are made for
+template <int HD>
+struct AttnMx {
+    static constexpr int kBlocks = HD / 32;                          // of a key (value)
+    static constexpr float kUnit = 7.f, kRise = 8.f;                 // weights begin at 2^7, m follows a score 2^8 above it
+    // A value in LDS has 32 bytes behind it: what a transposed read takes at a time is 32 bytes of each of eight keys, which then lie in different banks.
+    static constexpr int kRow = HD * 2 + 32;
+    static constexpr int kOwnValues = 32 * kRow;                     // of a wavefront that has keys of its own
+    static constexpr int kOwnLds = kAttnWaves * (kOwnValues > 16 * HD * 4 ? kOwnValues : 16 * HD * 4);
+    static constexpr int NB = HD > 192 ? 1 : 2, kKeys = 32 * NB;     // 32-key blocks of a step where wavefronts share the keys: as many as registers hold
+    static constexpr int kSharedLds = 2 * kKeys * kRow;
+    static constexpr int kLds = kOwnLds > kSharedLds ? kOwnLds : kSharedLds;
+
+    const AttnArgs& A;
+    const MxScales& X;
+    const AttnTile t;
+    const int kvh, lane, wave;
+    lds_t lds;
+
+    __device__ __forceinline__ AttnMx(const AttnArgs& args, const MxScales& scales, const AttnTile& tile, int kv_head, lds_t smem)
+        : A(args), X(scales), t(tile), kvh(kv_head), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lds(smem)
+    {
+    }
+
+    __device__ __forceinline__ void place(int row, int* token, int* head) const
+    {
+        const int r = t.row0 + row, i = (int)A.by_group.quot(r);
+        *token = i;
+        *head = kvh * A.group + (r - i * A.group);
+    }
+    __device__ __forceinline__ float* values_of(int row) const { return A.partial + slot_row(A, t.slot, kvh, row) * A.cache.head_dim; }
+    __device__ __forceinline__ f2_t* state_of(int row) const { return states_of(A) + slot_row(A, t.slot, kvh, row); }
+    __device__ __forceinline__ int blocks() const { return A.cache.head_dim / 32; }
+
+    // terms of block `block` of a row of the tile; rows and blocks that are not there are zero
+    __device__ __forceinline__ void load_terms(int row, int block, Terms& out) const
+    {
+        const bool live = row < t.count && block < blocks();
+        int token, head;
+        place(row < t.count ? row : 0, &token, &head);
+        const float* src = live ? A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * A.cache.head_dim + 32 * block : reinterpret_cast<const float*>(g_zero_row);
+        f16_t a, b;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const f4_t v = *reinterpret_cast<const f4_t*>(src + 4 * i);
+            a[2 * i] = v[0] * A.sign, b[2 * i] = v[1] * A.sign, a[2 * i + 1] = v[2] * A.sign, b[2 * i + 1] = v[3] * A.sign;
+        }
+        cut_terms(a, b, out);
+    }
+
+    // ---- where keys lie ----
+    struct Key {
+        const uint8_t *k, *v, *ks, *vs;
+        bool there;
+    };
+    // page of the key at a position; -1 for one that is not there
+    __device__ __forceinline__ int page_at(int p, int end) const
+    {
+        if (p >= end) return -1;
+        const int id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)p)];
+        return (uint32_t)id < (uint32_t)A.cache.num_pages ? id : -1;
+    }
+    __device__ __forceinline__ Key key_at(int p, int id) const
+    {
+        const int within = p - (int)A.cache.page.quot((uint32_t)p) * (int)A.cache.page.d;
+        const uint8_t* zero = g_zero_row;
+        const bool there = id >= 0;
+        return {there ? reinterpret_cast<const uint8_t*>(A.cache.k) + (id * A.cache.k_page + within * A.cache.k_token + kvh * A.cache.k_head) : zero,
+                there ? reinterpret_cast<const uint8_t*>(A.cache.v) + (id * A.cache.v_page + within * A.cache.v_token + kvh * A.cache.v_head) : zero,
+                there ? X.k + (id * X.k_page + within * X.k_token + kvh * X.k_head) : zero,
+                there ? X.v + (id * X.v_page + within * X.v_token + kvh * X.v_head) : zero, there};
+    }
+
+    // ---- infinities and NaN ----
+    __device__ __forceinline__ float element(const uint8_t* codes, const uint8_t* scales, int d) const
+    {
+        const uint32_t c = codes[d >> 1] >> (4 * (d & 1)), m = c & 7;
+        const float size = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1) << 22);
+        return (c & 8 ? -size : size) * mx4_power(scales[d >> 5]);
+    }
+    // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
+    // 64) for the values, whose mean is carried along, so that finite values never add up to infinity.  Slow, for rows with infinities or NaN in their results.
+    __device__ __forceinline__ void plainly(int row, int step)
+    {
+        const int dim = A.cache.head_dim;
+        for (int n = 0; n < 32 && row < t.count; ++n, row += step) {
+            int token, head;
+            place(row, &token, &head);
+            const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
+            const int last = t.p0 + token, first = first_key(last, A.window);
+            float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
+            for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
+                const int j = t.position(j0) + lane;
+                const bool wanted = (j0 < t.head || j >= first) && j <= last;
+                const Key key = key_at(j, wanted ? page_at(j, t.end_at(j0)) : -1);
+                const uint64_t lanes = __ballot(key.there);
+                if (lanes == 0) continue;
+                float score = -INFINITY;
+                if (key.there) {
+                    float dot = 0.f;
+                    for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(key.k, key.ks, d);
+                    score = dot * A.c;
+                }
+                float most = score;
+                for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+                const float mn = fmaxf(top, __builtin_ceilf(most)), base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
+                const float w = key.there ? __builtin_amdgcn_exp2f(score - base) : 0.f;
+                float all = w;
+                for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
+                const float before = sum * f;
+                sum = before + all;
+                top = mn;
+                const float by = sum == 0.f ? 0.f : 1.0f / sum;      // (weights of 0 alone: nothing; NaN stays)
+#pragma unroll
+                for (int i = 0; i <= HD / 64; ++i) mean[i] *= before * by;
+                for (uint64_t rest = lanes; rest != 0; rest &= rest - 1) {
+                    const int at = __ffsll((unsigned long long)rest) - 1;
+                    const float wk = __shfl(w, at) * by;
+                    const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)key.v, at));
+                    const uint8_t* vs = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)key.vs, at));
+#pragma unroll
+                    for (int i = 0; i <= HD / 64; ++i)
+                        if (64 * i + lane < dim) mean[i] += wk * element(v, vs, 64 * i + lane);
+                }
+            }
+            // a piece's state in units in which its sum is at most 1
+            const int e = sum > 0.f ? __builtin_amdgcn_frexp_expf(sum) : 0;
+            const float part = ldexpf(sum, -e);
+            float* dst = t.cuts == 1 ? A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * dim : values_of(row);
+            const float by = t.cuts == 1 ? sum * over_sum(A, sum, top, head) : part;
+#pragma unroll
+            for (int i = 0; i <= HD / 64; ++i)
+                if (64 * i + lane < dim) dst[64 * i + lane] = mean[i] * by;
+            if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top + (float)e, part};
+        }
+    }
+
+    __device__ __forceinline__ static void add_weights(float sum, float& l, float& rest)
+    {
+        const float large = fmaxf(l, sum), small = fminf(l, sum);
+        l = large + small;
+        rest += small - (l - large);
+    }
+    __device__ __forceinline__ static u4_t transposed(lds_t at, lds_t further)
+    {
+        const s4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)at);
+        const s4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)further);
+        const u2_t a0 = __builtin_bit_cast(u2_t, v0), a1 = __builtin_bit_cast(u2_t, v1);
+        return u4_t{a0.x, a0.y, a1.x, a1.y};
+    }
+    // a block's values into LDS
+    __device__ __forceinline__ static void put_values(const u4_t& codes, uint32_t e, lds_t at)
+    {
+        const float scale = mx4_power(e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(lds4_t)(at + 16 * i) = as_bf16(codes[i], scale);
+    }
+
+    // ---- few rows: every wavefront over keys of its own, 16 rows at a time ----
+    static constexpr int kChunks = (HD + 127) / 128, kTiles = HD / 16;
+
+    // a step of 32 keys: key idx of each 16, block 4 c + g of it
+    struct Step {
+        u4_t k[2][kChunks], v[2][kChunks];
+        uint32_t ks[2][kChunks], vs[2][kChunks];
+        uint32_t there;
+    };
+    __device__ __forceinline__ void load_step(int key, int g, int idx, Step& s) const
+    {
+        const int p0 = t.position(key), end = t.end_at(key);
+        int id[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) id[b] = page_at(p0 + 16 * b + idx, key < t.hi ? end : 0);
+        s.there = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const Key at = key_at(p0 + 16 * b + idx, id[b]);
+            s.there |= (uint32_t)(__ballot(at.there) & 0xffff) << (16 * b);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int block = 4 * c + g;
+                const bool has = block < blocks();
+                const uint8_t *k = has ? at.k + 16 * block : g_zero_row, *v = has ? at.v + 16 * block : g_zero_row;
+                const uint8_t *ks = has ? at.ks + block : g_zero_row, *vs = has ? at.vs + block : g_zero_row;
+                s.k[b][c] = *reinterpret_cast<const u4_t*>(k);
+                s.v[b][c] = *reinterpret_cast<const u4_t*>(v);
+                s.ks[b][c] = *ks;
+                s.vs[b][c] = *vs;
+            }
+        }
+    }
+    __device__ __forceinline__ static float of_rows(float x, float (*op)(float, float))
+    {
+        const u2_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return both_halves(op(__uint_as_float(r.x), __uint_as_float(r.y)), op);
+    }
+
+    // rows r0 .. r0 + 15 of the tile; whether these have to be done by plainly()
+    __device__ __forceinline__ bool own_keys(int r0)
+    {
+        __shared__ f2_t states[kAttnWaves][16];
+        __shared__ int odd[kAttnWaves];
+        const int idx = lane & 15, g = lane >> 4, row = r0 + idx;
+        const int rows = min(16, t.count - r0);
+        f4_t o[kTiles];
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f, l_rest = 0.f;
+        const lds_t values = lds + wave * kOwnValues;
+        int key = t.lo + 32 * wave;
+        constexpr int kStride = 32 * kAttnWaves;
+        if (key < t.hi) {
+            Step now, next;
+            load_step(key, g, idx, now);
+            load_step(key + kStride, g, idx, next);
+            Terms q[kChunks];
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) load_terms(row, 4 * c + g, q[c]);
+            int token, head;
+            place(min(row, t.count - 1), &token, &head);
+            const int p = t.p0 + token, lo = first_key(p, A.window);
+            for (; key < t.hi; key += kStride) {
+                f4_t s[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) s[b] = f4_t{0.f, 0.f, 0.f, 0.f};
+                // (small terms first, the two blocks in turn)
+                auto product = [&](auto part) {
+                    constexpr int n = decltype(part)::value;
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+                            s[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(now.k[b][c]), operand(q[c].t[n]), s[b], 4, 2, 0, (int)now.ks[b][c], n % 4,
+                                                                                    (int)q[c].scale[n / 4]);
+                };
+                each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
+                // the values of the step, for the transposed reads below
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+                        if (4 * c + g < kBlocks) put_values(now.v[b][c], now.vs[b][c], values + (16 * b + idx) * kRow + 64 * (4 * c + g));
+                // score i of block b belongs to key 16 b + 4 g + i
+                const bool in_head = key < t.head;
+                const int p0 = t.position(key), last = p - p0 - 4 * g, first = in_head ? 0 : lo - p0 - 4 * g;
+                const uint32_t there = now.there >> (4 * g);
+                float top = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = 16 * b + i;
+                        if (k > last || k < first || !((there >> k) & 1)) s[b][i] = -INFINITY;
+                        top = fmaxf(top, s[b][i]);
+                    }
+                now = next;
+                load_step(key + 2 * kStride, g, idx, next);
+                top = of_rows(top, larger) * A.c;
+                if (__any(top > m + kRise)) {                        // (m starts at -infinity)
+                    float mn = m;
+                    if (top > m + kRise) mn = __builtin_ceilf(top);
+                    const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                    l *= f;
+                    l_rest *= f;
+#pragma unroll
+                    for (int d = 0; d < kTiles; ++d) o[d] *= f;
+                    m = mn;
+                }
+                const float bias = kUnit - (m == -INFINITY ? 0.f : m);
+                float w[8], sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], A.c, bias));
+                    sum += w[i];
+                }
+                add_weights(sum, l, l_rest);
+                u4_t part[3];
+                cut3(w, part);
+                // a lane gives the place of four dimensions of one key and gets one dimension of four keys, within 16 lanes
+                const lds_t at = values + (4 * g + (idx >> 2)) * kRow + 8 * (idx & 3);
+#pragma unroll
+                for (int d = 0; d < kTiles; ++d) {
+                    const u4_t a = transposed(at + 32 * d, at + 32 * d + 16 * kRow);
+#pragma unroll
+                    for (int n = 2; n >= 0; --n)
+                        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
+                }
+            }
+        }
+        l = of_rows(l + l_rest, added);
+        float z = 0.f;
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[d][i], 0.f, z);
+        __syncthreads();                                             // (the states take the place of the values)
+        if (const bool found = __any(idx < rows && z != z); lane == 0) odd[wave] = found;
+        if (g == 0) states[wave][idx] = f2_t{m - kUnit, l};
+        const lds_t mine = lds + (wave * 16 + idx) * HD * 4;
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d)
+            *reinterpret_cast<__attribute__((address_space(3))) f4_t*>(mine + (((4 * d + g) ^ (idx & 7)) << 4)) = o[d];
+        __syncthreads();
+        int any = 0;
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) any |= odd[w];
+        const bool again = __builtin_amdgcn_readfirstlane(any);
+        const int pieces = A.cache.head_dim / 4;
+        for (int i = threadIdx.x; !again && i < rows * pieces; i += kAttnThreads) {
+            const int r = i / pieces, piece = i - r * pieces;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, states[w][r].x);
+            // (two powers more, so that what up to four of them have adds up to no infinity)
+            const float unit = top + 2.f, base = top == -INFINITY ? 0.f : unit;
+            float sum = 0.f;
+            f4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kAttnWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(states[w][r].x - base);
+                sum += states[w][r].y * f;
+                v += *reinterpret_cast<const __attribute__((address_space(3))) f4_t*>(lds + (w * 16 + r) * HD * 4 + ((piece ^ (r & 7)) << 4)) * f;
+            }
+            int token, head;
+            place(r0 + r, &token, &head);
+            if (t.cuts == 1) {
+                *reinterpret_cast<f4_t*>(A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim + 4 * piece) =
+                    v * over_sum(A, sum, unit, head);
+            } else {
+                *reinterpret_cast<f4_t*>(values_of(r0 + r) + 4 * piece) = v;
+                if (piece == 0) *state_of(r0 + r) = f2_t{unit, sum};
+            }
+        }
+        __syncthreads();                                             // (before the next rows)
+        return again;
+    }
+
+    // ---- many rows: all wavefronts over the same keys, 32 rows each ----
+    static constexpr int kHalves = (HD + 63) / 64, kDims = HD / 32, kMine = (kKeys * kBlocks + kAttnThreads - 1) / kAttnThreads;
+
+    // keys of a step: key col of each 32, block 2 c + half of it
+    struct Keys {
+        u4_t k[NB][kHalves];
+        uint32_t ks[NB][kHalves];
+        uint64_t there;              // (bits of keys that a step has not are set)
+    };
+    __device__ __forceinline__ void load_keys(int key, int col, int half, Keys& s) const
+    {
+        const int p0 = t.position(key), end = key < t.hi ? t.end_at(key) : 0;
+        int id[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) id[b] = page_at(p0 + 32 * b + col, end);
+        s.there = NB == 2 ? 0 : ~0xffffffffull;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const Key at = key_at(p0 + 32 * b + col, id[b]);
+            s.there |= (__ballot(at.there) & 0xffffffffull) << (32 * b);
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c) {
+                const int block = 2 * c + half;
+                const bool has = block < blocks();
+                s.k[b][c] = *reinterpret_cast<const u4_t*>(has ? at.k + 16 * block : g_zero_row);
+                s.ks[b][c] = *(has ? at.ks + block : g_zero_row);
+            }
+        }
+    }
+    // and the blocks of values that a thread turns
+    struct Values {
+        u4_t v[kMine];
+        uint32_t vs[kMine];
+    };
+    __device__ __forceinline__ void load_values(int key, Values& s) const
+    {
+        const int p0 = t.position(key), end = key < t.hi ? t.end_at(key) : 0;
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int unit = n * kAttnThreads + threadIdx.x, row = unit / kBlocks, block = unit - row * kBlocks;
+            const int p = p0 + row;
+            const Key at = key_at(p, row < kKeys && block < blocks() ? page_at(p, end) : -1);
+            s.v[n] = *reinterpret_cast<const u4_t*>(at.there ? at.v + 16 * block : g_zero_row);
+            s.vs[n] = *(at.there ? at.vs + block : g_zero_row);
+        }
+    }
+    __device__ __forceinline__ void turn_values(const Values& s, lds_t buffer) const
+    {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int unit = n * kAttnThreads + threadIdx.x, row = unit / kBlocks, block = unit - row * kBlocks;
+            if (kKeys * kBlocks % kAttnThreads == 0 || row < kKeys) put_values(s.v[n], s.vs[n], buffer + row * kRow + 64 * block);
+        }
+    }
+
+    __device__ __forceinline__ bool shared_keys()
+    {
+        const int col = lane & 31, half = lane >> 5, row = 32 * wave + col;
+        const int p_first = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave, t.count - 1));
+        const int p_last = t.p0 + (int)A.by_group.quot(t.row0 + min(32 * wave + 31, t.count - 1));
+        const int lo_last = first_key(p_last, A.window);
+        f16_t o[kDims];
+        auto nothing_yet = [&]() {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+        };
+        float m = -INFINITY, l = 0.f, l_rest = 0.f;
+        if (t.lo >= t.hi) {
+            nothing_yet();
+        } else {
+            Keys keys;
+            Values values;
+            load_keys(t.lo, col, half, keys);
+            load_values(t.lo, values);
+            Terms q[kHalves];
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c) load_terms(row, 2 * c + half, q[c]);
+            asm volatile("" ::: "memory");                           // (the accumulators come after the cutting of rows, which takes registers too)
+            nothing_yet();
+            int token, head;
+            place(min(row, t.count - 1), &token, &head);
+            const int p = t.p0 + token, lo = first_key(p, A.window);
+            int buffer = 0;
+            for (int key = t.lo; key < t.hi; key += kKeys) {
+                const lds_t here = lds + buffer * (kKeys * kRow);
+                buffer ^= 1;
+                turn_values(values, here);
+                __syncthreads();                                     // (what the other buffer held has been read by all)
+                load_values(key + kKeys, values);
+                const int p0 = t.position(key);
+                const bool in_head = key < t.head, mine = 32 * wave < t.count && p0 <= p_last;
+                f16_t s[NB];
+                if (mine) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+                    auto product = [&](auto part) {
+                        constexpr int n = decltype(part)::value;
+#pragma unroll
+                        for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b)
+                                s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(keys.k[b][c]), operand(q[c].t[n]), s[b], 4, 2, 0, (int)keys.ks[b][c], n % 4,
+                                                                                       (int)q[c].scale[n / 4]);
+                    };
+                    each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
+                }
+                const uint64_t there = keys.there;
+                load_keys(key + kKeys, col, half, keys);
+                if (!mine) continue;
+                // score i of block b belongs to key 32 b + 8 (i / 4) + 4 half + i % 4
+                if (~there != 0 || p0 + kKeys - 1 > p_first || (!in_head && p0 < lo_last)) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int below = 32 * b + 4 * half, last = p - p0 - below, first = in_head ? 0 : lo - p0 - below;
+                        const uint32_t bits = (uint32_t)(there >> below);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int k = 8 * (i / 4) + i % 4;
+                            if (k > last || k < first || !((bits >> k) & 1)) s[b][i] = -INFINITY;
+                        }
+                    }
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+                top = both_halves(top, larger) * A.c;
+                if (__any(top > m + kRise)) {
+                    float mn = m;
+                    if (top > m + kRise) mn = __builtin_ceilf(top);
+                    const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                    l *= f;
+                    l_rest *= f;
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] *= f;
+                    m = mn;
+                }
+                const float bias = kUnit - (m == -INFINITY ? 0.f : m);
+                float sum = 0.f;
+                const lds_t at = here + (4 * half + ((lane & 15) >> 2)) * kRow + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+#pragma unroll
+                for (int h = 0; h < 2 * NB; ++h) {                   // 16 keys
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h / 2][8 * (h % 2) + i], A.c, bias));
+                        sum += w[i];
+                    }
+                    u4_t part[3];
+                    cut3(w, part);
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d) {
+                        const u4_t a = transposed(at + 64 * d + 16 * h * kRow, at + 64 * d + (16 * h + 8) * kRow);
+#pragma unroll
+                        for (int n = 2; n >= 0; --n)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
+                    }
+                }
+                add_weights(sum, l, l_rest);
+            }
+        }
+        float z = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z = __builtin_fmaf(o[d][i], 0.f, z);
+        if (__any(row < t.count && z != z)) return true;
+        l = both_halves(l + l_rest, added);
+        if (row >= t.count) return false;
+        int token, head;
+        place(row, &token, &head);
+        float* dst;
+        float by = 1.f;
+        if (t.cuts == 1) {
+            dst = A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * A.cache.head_dim;
+            by = over_sum(A, l, m - kUnit, head);
+        } else {
+            dst = values_of(row);
+            if (half == 0) *state_of(row) = f2_t{m - kUnit, l};
+        }
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = 32 * d + 8 * i + 4 * half;
+                if (at < A.cache.head_dim)
+                    *reinterpret_cast<f4_t*>(dst + at) = f4_t{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * by;
+            }
+        return false;
+    }
+};
+
+// grid (KV heads, pieces)
+template <int HD>
+__global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_attention_kernel(TSHIP_LENS_ARGS, const AttnArgs A, const MxScales X)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
+    AttnTile t;
+    if (!find_piece(TSHIP_LENS, A, gridDim.x, worth_of(kTypeMXFP4, HD, kAttnWaves), idx, t)) return;
+    AttnMx<HD> a(A, X, t, kvh, (lds_t)smem);
+    if (t.tokens * A.group <= kKeyRows) {
+        bool again = false;
+        for (int r0 = 0; r0 < t.count; r0 += 16) again |= a.own_keys(r0);
+        if (again) a.plainly(a.wave, kAttnWaves);
+    } else if (a.shared_keys()) {
+        a.plainly(32 * a.wave, 1);
+    }
+}
+
+template <int HD>
+bool launch_mx(const Lens& H, const AttnArgs& args, const MxScales& scales, const dim3& grid, hipStream_t stream)
+{
+    const auto kern = paged_mx_attention_kernel<HD>;
+    constexpr size_t lds = AttnMx<HD>::kLds;
+    if (!raise_lds_limit(reinterpret_cast<const void*>(kern), lds)) return false;
+    hipLaunchKernelGGL(kern, grid, dim3(kAttnThreads), lds, stream, TSHIP_LENS_OF(H), args, scales);
+    return hip_ok(hipGetLastError(), "paged attention launch");
+}
+
+}  // namespace
+
+bool launch_mx_attention(const Lens& H, const AttnArgs& args, const MxScales& scales, const dim3& grid, hipStream_t stream)
+{
+    switch (dims_of(args.cache.head_dim)) {
+    case 64: return launch_mx<64>(H, args, scales, grid, stream);
+    case 96: return launch_mx<96>(H, args, scales, grid, stream);
+    case 128: return launch_mx<128>(H, args, scales, grid, stream);
+    case 192: return launch_mx<192>(H, args, scales, grid, stream);
+    default: return launch_mx<256>(H, args, scales, grid, stream);
+    }
+}
+
+}  // namespace tship

@@ -360,9 +360,10 @@ struct PagedAttnPlan {
     int slots, slot_rows;      // pieces there can be, rows of each
     size_t ws_bytes;
 };
-PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window);
+PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window, int first);
 bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64_t ld_query, float* out, int64_t ld_out, int rows, int heads,
-                            const PagedKv& cache, float scale, int window, const float* sinks, void* ws, hipStream_t stream);
+                            const PagedKv& cache, const MxScales& scales, float scale, int window, int first, const float* sinks, void* ws,
+                            hipStream_t stream);
 
 // Who has which pages (the device memory of a TSHipPagePool).
 struct PagePoolArgs {

@@ -913,12 +913,14 @@ class HipBasicOps:
         N.check_result(N.lib().TSHip_CopyPagesDevice(dst.ref, src.ref, m, moves.shape[0]), "copy_pages")
 
     @staticmethod
-    def PagedAttention(result, query, cache, row_starts, context_lens, scale, window=0, sinks=None):
+    def PagedAttention(result, query, cache, row_starts, context_lens, scale, window=0, sinks=None, first=0):
         """Attention of the sequences' new tokens (rows as in RoPEStorePaged) over a PagedKVCache that holds their keys and values already:
-        each sees the positions up to its own, the last `window` of them (0: all).  query and result [rows, heads head_dim]
+        each sees the positions up to its own, the last `window` of them (0: all) and, of those before, the first `first` of the sequence.  query and result [rows, heads head_dim]
         float32 (may be one tensor); sinks [heads] float32: logits that take part in the softmax and carry no value."""
         if not -2 ** 31 <= window < 2 ** 31:         # (the call takes 32 bits of it)
             raise ValueError("PagedAttention requires a window below 2^31.")
+        if not 0 <= first < 2 ** 31:
+            raise ValueError("PagedAttention requires a number of first positions from 0 to below 2^31.")
         torch = _torch()
         rv, qv = _device_view(result), _device_view(query)
         heads, device = qv.dim1 // cache.head_dim, cache.device
@@ -927,7 +929,10 @@ class HipBasicOps:
         if query.get_device() != device or result.get_device() != device:
             raise ValueError("query and result must be on the device of the cache.")
         _use_stream_of(device)
-        ok = N.lib().TSHip_PagedAttentionF32Device(rv, qv, heads, cache.ref, starts, lens, scale, window, extra)
+        if first:
+            ok = N.lib().TSHip_PagedAttentionFirstF32Device(rv, qv, heads, cache.ref, starts, lens, scale, window, first, extra)
+        else:
+            ok = N.lib().TSHip_PagedAttentionF32Device(rv, qv, heads, cache.ref, starts, lens, scale, window, extra)
         N.check_result(ok, "paged_attention")
 
     @staticmethod

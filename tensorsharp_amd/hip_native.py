@@ -163,6 +163,8 @@ SIGNATURES.update({
                                                 C.c_void_p, C.c_void_p, C.c_float, C.POINTER(Rope)]),
     "TSHip_PagedAttentionF32Device": (C.c_int, [TensorView2D, TensorView2D, C.c_int, C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_float,
                                                 C.c_int, C.c_void_p]),
+    "TSHip_PagedAttentionFirstF32Device": (C.c_int, [TensorView2D, TensorView2D, C.c_int, C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_float,
+                                                     C.c_int, C.c_int, C.c_void_p]),
     "TSHip_PagePoolScratchDevice": (C.c_int64, [C.c_int, C.c_int, C.c_int64]),
     "TSHip_ResizeSequencesDevice": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_void_p, C.c_void_p]),
     "TSHip_ForkSequencesDevice": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),

@@ -8,13 +8,8 @@ def scales(x):
     """bytes [.., dim / 32] of the blocks of x [.., dim] (float64)"""
     b = np.abs(np.asarray(x, dtype=np.float64).reshape(*x.shape[:-1], -1, 32))
     top = np.where(np.isnan(b).any(-1), np.inf, np.nan_to_num(b, nan=0.0, posinf=np.inf).max(-1))
-    out = np.full(top.shape, 255, dtype=np.uint8)
-    for at in np.argwhere(top < 2.0 ** 127):
-        e = -126
-        while top[tuple(at)] > 7.0 * 2.0 ** e:
-            e += 1
-        out[tuple(at)] = e + 127
-    return out
+    borders = 7.0 * 2.0 ** np.arange(-126, 128)                      # the first that is not below it
+    return np.where(top < 2.0 ** 127, np.searchsorted(borders, top) + 1, 255).astype(np.uint8)
 
 
 def codes(x, e):
