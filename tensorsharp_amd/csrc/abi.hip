@@ -3085,6 +3085,11 @@ bool validate_pages(const TSHipPagedCache* c, PagedKv* out, MxScales* scales)
                 return false;
             }
         }
+        for (int i = 0; i < 6; ++i)
+            if (s[i] > UINT32_MAX || z[i] > UINT32_MAX) {            // (the kernels multiply by 32 bits)
+                set_last_error("paged cache: strides of MXFP4 must be below 2^32 bytes.");
+                return false;
+            }
         *scales = {static_cast<uint8_t*>(c->k_scales), static_cast<uint8_t*>(c->v_scales), z[0], z[1], z[2], z[3], z[4], z[5]};
     }
     out->k = static_cast<char*>(c->k);

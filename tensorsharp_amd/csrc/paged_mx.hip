@@ -125,26 +125,50 @@ struct AttnMx {
     }
 
     // ---- where keys lie ----
-    struct Key {
-        const uint8_t *k, *v, *ks, *vs;
+    // Lane i has the id of page id_base + i of the sequence: read again when a step passes the last of them, so that no step's loads wait for a
+    // table's (loads are waited for in order, with everything before them).
+    int ids, id_base = -64;
+    __device__ __forceinline__ void bring_pages(int p0, int keys)
+    {
+        const int page = (int)A.cache.page.quot((uint32_t)p0);       // uniform
+        if ((int)A.cache.page.quot((uint32_t)(p0 + keys - 1)) - id_base >= 64) {
+            id_base = page;
+            ids = A.cache.table[t.seq * A.cache.table_stride + min(page + lane, A.cache.max_pages - 1)];
+        }
+    }
+    // The row at a position that is among those pages.  One that is not there is a row of page 0: its codes may be any, so what is loaded of it counts
+    // with a power that makes it nothing.
+    struct Row {
+        uint32_t page, within;
         bool there;
     };
-    // page of the key at a position; -1 for one that is not there
-    __device__ __forceinline__ int page_at(int p, int end) const
+    __device__ __forceinline__ Row row_at(int p, int end) const
     {
-        if (p >= end) return -1;
-        const int id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)p)];
-        return (uint32_t)id < (uint32_t)A.cache.num_pages ? id : -1;
+        const int q = (int)A.cache.page.quot((uint32_t)p), id = __shfl(ids, q - id_base);
+        const bool there = p < end && (uint32_t)id < (uint32_t)A.cache.num_pages;
+        return {there ? (uint32_t)id : 0u, (uint32_t)(p - q * (int)A.cache.page.d), there};
     }
-    __device__ __forceinline__ Key key_at(int p, int id) const
+    // where a lane's block of row 0 of page 0 lies, and how far pages and tokens are apart (below 2^32 bytes, so that each is one multiplication)
+    struct Source {
+        uint64_t at;
+        uint32_t page, token;
+        __device__ __forceinline__ const uint8_t* of(const Row& r) const { return reinterpret_cast<const uint8_t*>(at + (uint64_t)r.page * page + (uint64_t)r.within * token); }
+    };
+    __device__ __forceinline__ Source keys_from(int block) const
     {
-        const int within = p - (int)A.cache.page.quot((uint32_t)p) * (int)A.cache.page.d;
-        const uint8_t* zero = g_zero_row;
-        const bool there = id >= 0;
-        return {there ? reinterpret_cast<const uint8_t*>(A.cache.k) + (id * A.cache.k_page + within * A.cache.k_token + kvh * A.cache.k_head) : zero,
-                there ? reinterpret_cast<const uint8_t*>(A.cache.v) + (id * A.cache.v_page + within * A.cache.v_token + kvh * A.cache.v_head) : zero,
-                there ? X.k + (id * X.k_page + within * X.k_token + kvh * X.k_head) : zero,
-                there ? X.v + (id * X.v_page + within * X.v_token + kvh * X.v_head) : zero, there};
+        return {(uint64_t)(uintptr_t)A.cache.k + kvh * A.cache.k_head + 16 * min(block, blocks() - 1), (uint32_t)A.cache.k_page, (uint32_t)A.cache.k_token};
+    }
+    __device__ __forceinline__ Source values_from(int block) const
+    {
+        return {(uint64_t)(uintptr_t)A.cache.v + kvh * A.cache.v_head + 16 * min(block, blocks() - 1), (uint32_t)A.cache.v_page, (uint32_t)A.cache.v_token};
+    }
+    __device__ __forceinline__ Source key_scales_from(int block) const
+    {
+        return {(uint64_t)(uintptr_t)X.k + kvh * X.k_head + min(block, blocks() - 1), (uint32_t)X.k_page, (uint32_t)X.k_token};
+    }
+    __device__ __forceinline__ Source value_scales_from(int block) const
+    {
+        return {(uint64_t)(uintptr_t)X.v + kvh * X.v_head + min(block, blocks() - 1), (uint32_t)X.v_page, (uint32_t)X.v_token};
     }
 
     // ---- infinities and NaN ----
@@ -167,20 +191,24 @@ struct AttnMx {
             float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
                 const int j = t.position(j0) + lane;
-                const bool wanted = (j0 < t.head || j >= first) && j <= last;
-                const Key key = key_at(j, wanted ? page_at(j, t.end_at(j0)) : -1);
-                const uint64_t lanes = __ballot(key.there);
+                int id = -1;
+                if ((j0 < t.head || j >= first) && j <= last && j < t.end_at(j0)) id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)j)];
+                const bool seen = (uint32_t)id < (uint32_t)A.cache.num_pages;
+                const uint64_t lanes = __ballot(seen);
                 if (lanes == 0) continue;
+                const Row at{seen ? (uint32_t)id : 0u, (uint32_t)(j - (int)A.cache.page.quot((uint32_t)j) * (int)A.cache.page.d), seen};
+                const uint8_t *v_at = values_from(0).of(at), *vs_at = value_scales_from(0).of(at);
                 float score = -INFINITY;
-                if (key.there) {
+                if (seen) {
+                    const uint8_t *k = keys_from(0).of(at), *ks = key_scales_from(0).of(at);
                     float dot = 0.f;
-                    for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(key.k, key.ks, d);
+                    for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(k, ks, d);
                     score = dot * A.c;
                 }
                 float most = score;
                 for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
                 const float mn = fmaxf(top, __builtin_ceilf(most)), base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
-                const float w = key.there ? __builtin_amdgcn_exp2f(score - base) : 0.f;
+                const float w = seen ? __builtin_amdgcn_exp2f(score - base) : 0.f;
                 float all = w;
                 for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
                 const float before = sum * f;
@@ -190,10 +218,10 @@ struct AttnMx {
 #pragma unroll
                 for (int i = 0; i <= HD / 64; ++i) mean[i] *= before * by;
                 for (uint64_t rest = lanes; rest != 0; rest &= rest - 1) {
-                    const int at = __ffsll((unsigned long long)rest) - 1;
-                    const float wk = __shfl(w, at) * by;
-                    const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)key.v, at));
-                    const uint8_t* vs = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)key.vs, at));
+                    const int lane_of = __ffsll((unsigned long long)rest) - 1;
+                    const float wk = __shfl(w, lane_of) * by;
+                    const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)v_at, lane_of));
+                    const uint8_t* vs = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)vs_at, lane_of));
 #pragma unroll
                     for (int i = 0; i <= HD / 64; ++i)
                         if (64 * i + lane < dim) mean[i] += wk * element(v, vs, 64 * i + lane);
@@ -227,7 +255,7 @@ struct AttnMx {
     // a block's values into LDS
     __device__ __forceinline__ static void put_values(const u4_t& codes, uint32_t e, lds_t at)
     {
-        const float scale = mx4_power(e);
+        const float scale = __uint_as_float(e << 23);                // (0 is 2^-127 to the instruction and 255 NaN)
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(lds4_t)(at + 16 * i) = as_bf16(codes[i], scale);
     }
@@ -239,29 +267,27 @@ struct AttnMx {
     struct Step {
         u4_t k[2][kChunks], v[2][kChunks];
         uint32_t ks[2][kChunks], vs[2][kChunks];
-        uint32_t there;
+        uint32_t there;                                              // a bit for each key
     };
-    __device__ __forceinline__ void load_step(int key, int g, int idx, Step& s) const
+    struct Sources {
+        Source k[kChunks], v[kChunks], ks[kChunks], vs[kChunks];
+    };
+    __device__ __forceinline__ void load_step(int key, int idx, const Sources& from, Step& s)
     {
+        if (key >= t.hi) return;
         const int p0 = t.position(key), end = t.end_at(key);
-        int id[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) id[b] = page_at(p0 + 16 * b + idx, key < t.hi ? end : 0);
+        bring_pages(p0, 32);
         s.there = 0;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const Key at = key_at(p0 + 16 * b + idx, id[b]);
+            const Row at = row_at(p0 + 16 * b + idx, end);
             s.there |= (uint32_t)(__ballot(at.there) & 0xffff) << (16 * b);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-                const int block = 4 * c + g;
-                const bool has = block < blocks();
-                const uint8_t *k = has ? at.k + 16 * block : g_zero_row, *v = has ? at.v + 16 * block : g_zero_row;
-                const uint8_t *ks = has ? at.ks + block : g_zero_row, *vs = has ? at.vs + block : g_zero_row;
-                s.k[b][c] = *reinterpret_cast<const u4_t*>(k);
-                s.v[b][c] = *reinterpret_cast<const u4_t*>(v);
-                s.ks[b][c] = *ks;
-                s.vs[b][c] = *vs;
+                s.k[b][c] = *reinterpret_cast<const u4_t*>(from.k[c].of(at));
+                s.ks[b][c] = *from.ks[c].of(at);
+                s.v[b][c] = *reinterpret_cast<const u4_t*>(from.v[c].of(at));
+                s.vs[b][c] = *from.vs[c].of(at);
             }
         }
     }
@@ -284,21 +310,41 @@ struct AttnMx {
         float m = -INFINITY, l = 0.f, l_rest = 0.f;
         const lds_t values = lds + wave * kOwnValues;
         int key = t.lo + 32 * wave;
+        id_base = -64;                                               // (the keys of the rows before are begun again)
         constexpr int kStride = 32 * kAttnWaves;
         if (key < t.hi) {
-            Step now, next;
-            load_step(key, g, idx, now);
-            load_step(key + kStride, g, idx, next);
+            Sources from;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+                from.k[c] = keys_from(4 * c + g), from.v[c] = values_from(4 * c + g), from.ks[c] = key_scales_from(4 * c + g), from.vs[c] = value_scales_from(4 * c + g);
+            Step even, odd_one;
+            load_step(key, idx, from, even);
+            load_step(key + kStride, idx, from, odd_one);
             Terms q[kChunks];
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) load_terms(row, 4 * c + g, q[c]);
             int token, head;
             place(min(row, t.count - 1), &token, &head);
-            const int p = t.p0 + token, lo = first_key(p, A.window);
-            for (; key < t.hi; key += kStride) {
+            const int p = t.p0 + token, lo = first_key(p, A.window), lo_last = first_key(t.p0 + t.tokens - 1, A.window);
+            // a step; the one after the next takes its place
+            auto step = [&](Step& now) {
                 f4_t s[2];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) s[b] = f4_t{0.f, 0.f, 0.f, 0.f};
+                const int p0 = t.position(key);
+                const bool whole = now.there == ~0u, in_head = key < t.head;
+                if constexpr (HD != 128) {                           // (lanes without a block have another's, for which rows have zeros: NaN would stay one)
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) now.ks[b][c] = 4 * c + g < blocks() ? now.ks[b][c] : 0;
+                }
+                if (!whole) {                                        // (a value of the least power under a weight of 0)
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) now.vs[b][c] = (now.there >> (16 * b + idx)) & 1 ? now.vs[b][c] : 0;
+                }
                 // (small terms first, the two blocks in turn)
                 auto product = [&](auto part) {
                     constexpr int n = decltype(part)::value;
@@ -317,20 +363,21 @@ struct AttnMx {
                     for (int c = 0; c < kChunks; ++c)
                         if (4 * c + g < kBlocks) put_values(now.v[b][c], now.vs[b][c], values + (16 * b + idx) * kRow + 64 * (4 * c + g));
                 // score i of block b belongs to key 16 b + 4 g + i
-                const bool in_head = key < t.head;
-                const int p0 = t.position(key), last = p - p0 - 4 * g, first = in_head ? 0 : lo - p0 - 4 * g;
-                const uint32_t there = now.there >> (4 * g);
-                float top = -INFINITY;
+                if (!whole || p0 + 31 > t.p0 || (!in_head && p0 < lo_last)) {
+                    const int last = p - p0 - 4 * g, first = in_head ? 0 : lo - p0 - 4 * g;
+                    const uint32_t there = now.there >> (4 * g);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int k = 16 * b + i;
-                        if (k > last || k < first || !((there >> k) & 1)) s[b][i] = -INFINITY;
-                        top = fmaxf(top, s[b][i]);
-                    }
-                now = next;
-                load_step(key + 2 * kStride, g, idx, next);
+                        for (int i = 0; i < 4; ++i) {
+                            const int k = 16 * b + i;
+                            if (k > last || k < first || !((there >> k) & 1)) s[b][i] = -INFINITY;
+                        }
+                }
+                load_step(key + 2 * kStride, idx, from, now);
+                float top = s[0][0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
                 top = of_rows(top, larger) * A.c;
                 if (__any(top > m + kRise)) {                        // (m starts at -infinity)
                     float mn = m;
@@ -361,6 +408,12 @@ struct AttnMx {
                     for (int n = 2; n >= 0; --n)
                         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
                 }
+            };
+            for (;;) {
+                step(even);
+                if ((key += kStride) >= t.hi) break;
+                step(odd_one);
+                if ((key += kStride) >= t.hi) break;
             }
         }
         l = of_rows(l + l_rest, added);
@@ -420,23 +473,23 @@ struct AttnMx {
         uint32_t ks[NB][kHalves];
         uint64_t there;              // (bits of keys that a step has not are set)
     };
-    __device__ __forceinline__ void load_keys(int key, int col, int half, Keys& s) const
+    struct KeySources {
+        Source k[kHalves], ks[kHalves];
+    };
+    __device__ __forceinline__ void load_keys(int key, int col, const KeySources& from, Keys& s)
     {
-        const int p0 = t.position(key), end = key < t.hi ? t.end_at(key) : 0;
-        int id[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) id[b] = page_at(p0 + 32 * b + col, end);
+        if (key >= t.hi) return;
+        const int p0 = t.position(key), end = t.end_at(key);
+        bring_pages(p0, kKeys);
         s.there = NB == 2 ? 0 : ~0xffffffffull;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const Key at = key_at(p0 + 32 * b + col, id[b]);
+            const Row at = row_at(p0 + 32 * b + col, end);
             s.there |= (__ballot(at.there) & 0xffffffffull) << (32 * b);
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) {
-                const int block = 2 * c + half;
-                const bool has = block < blocks();
-                s.k[b][c] = *reinterpret_cast<const u4_t*>(has ? at.k + 16 * block : g_zero_row);
-                s.ks[b][c] = *(has ? at.ks + block : g_zero_row);
+                s.k[b][c] = *reinterpret_cast<const u4_t*>(from.k[c].of(at));
+                s.ks[b][c] = *from.ks[c].of(at);
             }
         }
     }
@@ -444,17 +497,22 @@ struct AttnMx {
     struct Values {
         u4_t v[kMine];
         uint32_t vs[kMine];
+        bool there[kMine];
     };
-    __device__ __forceinline__ void load_values(int key, Values& s) const
+    struct ValueSources {
+        Source v[kMine], vs[kMine];
+    };
+    __device__ __forceinline__ void load_values(int key, const ValueSources& from, Values& s)
     {
-        const int p0 = t.position(key), end = key < t.hi ? t.end_at(key) : 0;
+        if (key >= t.hi) return;
+        const int p0 = t.position(key), end = t.end_at(key);
+        bring_pages(p0, kKeys);
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
-            const int unit = n * kAttnThreads + threadIdx.x, row = unit / kBlocks, block = unit - row * kBlocks;
-            const int p = p0 + row;
-            const Key at = key_at(p, row < kKeys && block < blocks() ? page_at(p, end) : -1);
-            s.v[n] = *reinterpret_cast<const u4_t*>(at.there ? at.v + 16 * block : g_zero_row);
-            s.vs[n] = *(at.there ? at.vs + block : g_zero_row);
+            const Row at = row_at(p0 + min((int)(n * kAttnThreads + threadIdx.x) / kBlocks, kKeys - 1), end);
+            s.there[n] = at.there;
+            s.v[n] = *reinterpret_cast<const u4_t*>(from.v[n].of(at));
+            s.vs[n] = *from.vs[n].of(at);
         }
     }
     __device__ __forceinline__ void turn_values(const Values& s, lds_t buffer) const
@@ -462,7 +520,7 @@ struct AttnMx {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
             const int unit = n * kAttnThreads + threadIdx.x, row = unit / kBlocks, block = unit - row * kBlocks;
-            if (kKeys * kBlocks % kAttnThreads == 0 || row < kKeys) put_values(s.v[n], s.vs[n], buffer + row * kRow + 64 * block);
+            if (kKeys * kBlocks % kAttnThreads == 0 || row < kKeys) put_values(s.v[n], s.there[n] ? s.vs[n] : 0, buffer + row * kRow + 64 * block);
         }
     }
 
@@ -485,8 +543,17 @@ struct AttnMx {
         } else {
             Keys keys;
             Values values;
-            load_keys(t.lo, col, half, keys);
-            load_values(t.lo, values);
+            KeySources keys_at;
+            ValueSources values_at;
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c) keys_at.k[c] = keys_from(2 * c + half), keys_at.ks[c] = key_scales_from(2 * c + half);
+#pragma unroll
+            for (int n = 0; n < kMine; ++n) {
+                const int block = (n * kAttnThreads + threadIdx.x) % kBlocks;
+                values_at.v[n] = values_from(block), values_at.vs[n] = value_scales_from(block);
+            }
+            load_keys(t.lo, col, keys_at, keys);
+            load_values(t.lo, values_at, values);
             Terms q[kHalves];
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) load_terms(row, 2 * c + half, q[c]);
@@ -501,11 +568,17 @@ struct AttnMx {
                 buffer ^= 1;
                 turn_values(values, here);
                 __syncthreads();                                     // (what the other buffer held has been read by all)
-                load_values(key + kKeys, values);
+                load_values(key + kKeys, values_at, values);
                 const int p0 = t.position(key);
                 const bool in_head = key < t.head, mine = 32 * wave < t.count && p0 <= p_last;
                 f16_t s[NB];
                 if (mine) {
+                    if constexpr (HD % 64 != 0 || HD == 64 || HD > 128) {                // (see own_keys)
+#pragma unroll
+                        for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) keys.ks[b][c] = 2 * c + half < blocks() ? keys.ks[b][c] : 0;
+                    }
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -522,7 +595,7 @@ struct AttnMx {
                     each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
                 }
                 const uint64_t there = keys.there;
-                load_keys(key + kKeys, col, half, keys);
+                load_keys(key + kKeys, col, keys_at, keys);
                 if (!mine) continue;
                 // score i of block b belongs to key 32 b + 8 (i / 4) + 4 half + i % 4
                 if (~there != 0 || p0 + kKeys - 1 > p_first || (!in_head && p0 < lo_last)) {
