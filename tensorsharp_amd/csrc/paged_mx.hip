@@ -73,6 +73,8 @@ __device__ __forceinline__ u4_t as_bf16(uint32_t codes, float scale)
 }
 
 typedef __attribute__((address_space(3))) u4_t* lds4_t;
+typedef const __attribute__((address_space(1))) uint8_t* mem_t;      // (a generic pointer's loads would be counted with LDS)
+typedef const __attribute__((address_space(1))) u4_t* mem4_t;
 
 // HD: head_dim rounded up to what the tiles are made for
 template <int HD>
@@ -134,6 +136,7 @@ struct AttnMx {
         if ((int)A.cache.page.quot((uint32_t)(p0 + keys - 1)) - id_base >= 64) {
             id_base = page;
             ids = A.cache.table[t.seq * A.cache.table_stride + min(page + lane, A.cache.max_pages - 1)];
+            asm volatile("" : "+v"(ids));                            // (it is waited for here, and nowhere else)
         }
     }
     // The row at a position that is among those pages.  One that is not there is a row of page 0: its codes may be any, so what is loaded of it counts
@@ -152,7 +155,7 @@ struct AttnMx {
     struct Source {
         uint64_t at;
         uint32_t page, token;
-        __device__ __forceinline__ const uint8_t* of(const Row& r) const { return reinterpret_cast<const uint8_t*>(at + (uint64_t)r.page * page + (uint64_t)r.within * token); }
+        __device__ __forceinline__ mem_t of(const Row& r) const { return (mem_t)(at + (uint64_t)r.page * page + (uint64_t)r.within * token); }
     };
     __device__ __forceinline__ Source keys_from(int block) const
     {
@@ -172,7 +175,7 @@ struct AttnMx {
     }
 
     // ---- infinities and NaN ----
-    __device__ __forceinline__ float element(const uint8_t* codes, const uint8_t* scales, int d) const
+    __device__ __forceinline__ float element(mem_t codes, mem_t scales, int d) const
     {
         const uint32_t c = codes[d >> 1] >> (4 * (d & 1)), m = c & 7;
         const float size = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1) << 22);
@@ -197,10 +200,10 @@ struct AttnMx {
                 const uint64_t lanes = __ballot(seen);
                 if (lanes == 0) continue;
                 const Row at{seen ? (uint32_t)id : 0u, (uint32_t)(j - (int)A.cache.page.quot((uint32_t)j) * (int)A.cache.page.d), seen};
-                const uint8_t *v_at = values_from(0).of(at), *vs_at = value_scales_from(0).of(at);
+                const mem_t v_at = values_from(0).of(at), vs_at = value_scales_from(0).of(at);
                 float score = -INFINITY;
                 if (seen) {
-                    const uint8_t *k = keys_from(0).of(at), *ks = key_scales_from(0).of(at);
+                    const mem_t k = keys_from(0).of(at), ks = key_scales_from(0).of(at);
                     float dot = 0.f;
                     for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(k, ks, d);
                     score = dot * A.c;
@@ -220,8 +223,8 @@ struct AttnMx {
                 for (uint64_t rest = lanes; rest != 0; rest &= rest - 1) {
                     const int lane_of = __ffsll((unsigned long long)rest) - 1;
                     const float wk = __shfl(w, lane_of) * by;
-                    const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)v_at, lane_of));
-                    const uint8_t* vs = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)vs_at, lane_of));
+                    const mem_t v = (mem_t)__shfl((unsigned long long)v_at, lane_of);
+                    const mem_t vs = (mem_t)__shfl((unsigned long long)vs_at, lane_of);
 #pragma unroll
                     for (int i = 0; i <= HD / 64; ++i)
                         if (64 * i + lane < dim) mean[i] += wk * element(v, vs, 64 * i + lane);
@@ -263,10 +266,11 @@ struct AttnMx {
     // ---- few rows: every wavefront over keys of its own, 16 rows at a time ----
     static constexpr int kChunks = (HD + 127) / 128, kTiles = HD / 16;
 
-    // a step of 32 keys: key idx of each 16, block 4 c + g of it
+    // A step of 32 keys: key idx of each 16, block 4 c + g of it.  Steps behind the last are loaded like others (of page 0): what is waited for is counted, and a
+    // load that might not be there would have all of them waited for.
     struct Step {
         u4_t k[2][kChunks], v[2][kChunks];
-        uint32_t ks[2][kChunks], vs[2][kChunks];
+        uint8_t ks[2][kChunks], vs[2][kChunks];                      // (as loaded: widened ahead of their use they would be waited for)
         uint32_t there;                                              // a bit for each key
     };
     struct Sources {
@@ -274,7 +278,6 @@ struct AttnMx {
     };
     __device__ __forceinline__ void load_step(int key, int idx, const Sources& from, Step& s)
     {
-        if (key >= t.hi) return;
         const int p0 = t.position(key), end = t.end_at(key);
         bring_pages(p0, 32);
         s.there = 0;
@@ -284,9 +287,9 @@ struct AttnMx {
             s.there |= (uint32_t)(__ballot(at.there) & 0xffff) << (16 * b);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-                s.k[b][c] = *reinterpret_cast<const u4_t*>(from.k[c].of(at));
+                s.k[b][c] = *(mem4_t)(from.k[c].of(at));
                 s.ks[b][c] = *from.ks[c].of(at);
-                s.v[b][c] = *reinterpret_cast<const u4_t*>(from.v[c].of(at));
+                s.v[b][c] = *(mem4_t)(from.v[c].of(at));
                 s.vs[b][c] = *from.vs[c].of(at);
             }
         }
@@ -318,8 +321,18 @@ struct AttnMx {
             for (int c = 0; c < kChunks; ++c)
                 from.k[c] = keys_from(4 * c + g), from.v[c] = values_from(4 * c + g), from.ks[c] = key_scales_from(4 * c + g), from.vs[c] = value_scales_from(4 * c + g);
             Step even, odd_one;
-            load_step(key, idx, from, even);
-            load_step(key + kStride, idx, from, odd_one);
+            // (a loop of pairs of steps has no other way out, so that each waits for its own loads alone; the first of an odd number goes before it)
+            const bool single = ((t.hi - key + kStride - 1) / kStride) & 1;
+            if (single) {
+                load_step(key, idx, from, odd_one);
+                asm volatile("" ::: "memory");
+                load_step(key + kStride, idx, from, even);
+            } else {
+                load_step(key, idx, from, even);
+                asm volatile("" ::: "memory");
+                load_step(key + kStride, idx, from, odd_one);
+            }
+            asm volatile("" ::: "memory");
             Terms q[kChunks];
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) load_terms(row, 4 * c + g, q[c]);
@@ -409,11 +422,15 @@ struct AttnMx {
                         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
                 }
             };
-            for (;;) {
-                step(even);
-                if ((key += kStride) >= t.hi) break;
+            if (single) {
                 step(odd_one);
-                if ((key += kStride) >= t.hi) break;
+                key += kStride;
+            }
+            while (key < t.hi) {
+                step(even);
+                key += kStride;
+                step(odd_one);
+                key += kStride;
             }
         }
         l = of_rows(l + l_rest, added);
@@ -470,7 +487,7 @@ struct AttnMx {
     // keys of a step: key col of each 32, block 2 c + half of it
     struct Keys {
         u4_t k[NB][kHalves];
-        uint32_t ks[NB][kHalves];
+        uint8_t ks[NB][kHalves];
         uint64_t there;              // (bits of keys that a step has not are set)
     };
     struct KeySources {
@@ -478,7 +495,6 @@ struct AttnMx {
     };
     __device__ __forceinline__ void load_keys(int key, int col, const KeySources& from, Keys& s)
     {
-        if (key >= t.hi) return;
         const int p0 = t.position(key), end = t.end_at(key);
         bring_pages(p0, kKeys);
         s.there = NB == 2 ? 0 : ~0xffffffffull;
@@ -488,7 +504,7 @@ struct AttnMx {
             s.there |= (__ballot(at.there) & 0xffffffffull) << (32 * b);
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) {
-                s.k[b][c] = *reinterpret_cast<const u4_t*>(from.k[c].of(at));
+                s.k[b][c] = *(mem4_t)(from.k[c].of(at));
                 s.ks[b][c] = *from.ks[c].of(at);
             }
         }
@@ -496,7 +512,7 @@ struct AttnMx {
     // and the blocks of values that a thread turns
     struct Values {
         u4_t v[kMine];
-        uint32_t vs[kMine];
+        uint8_t vs[kMine];
         bool there[kMine];
     };
     struct ValueSources {
@@ -504,14 +520,13 @@ struct AttnMx {
     };
     __device__ __forceinline__ void load_values(int key, const ValueSources& from, Values& s)
     {
-        if (key >= t.hi) return;
         const int p0 = t.position(key), end = t.end_at(key);
         bring_pages(p0, kKeys);
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
             const Row at = row_at(p0 + min((int)(n * kAttnThreads + threadIdx.x) / kBlocks, kKeys - 1), end);
             s.there[n] = at.there;
-            s.v[n] = *reinterpret_cast<const u4_t*>(from.v[n].of(at));
+            s.v[n] = *(mem4_t)(from.v[n].of(at));
             s.vs[n] = *from.vs[n].of(at);
         }
     }
