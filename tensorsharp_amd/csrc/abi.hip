@@ -3090,7 +3090,8 @@ bool validate_pages(const TSHipPagedCache* c, PagedKv* out, MxScales* scales)
                 set_last_error("paged cache: strides of MXFP4 must be below 2^32 bytes.");
                 return false;
             }
-        *scales = {static_cast<uint8_t*>(c->k_scales), static_cast<uint8_t*>(c->v_scales), z[0], z[1], z[2], z[3], z[4], z[5]};
+        *scales = {static_cast<uint8_t*>(c->k_scales), static_cast<uint8_t*>(c->v_scales), z[0], z[1], z[2], z[3], z[4], z[5],
+                   s[0] == s[3] && s[1] == s[4] && s[0] == 16 * z[0] && s[1] == 16 * z[1] && s[0] == 16 * z[3] && s[1] == 16 * z[4]};
     }
     out->k = static_cast<char*>(c->k);
     out->v = static_cast<char*>(c->v);

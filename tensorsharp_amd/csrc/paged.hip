@@ -987,8 +987,9 @@ __host__ __device__ constexpr int wide_of(int dim) { return dim <= 64 ? 16 : dim
 // grids: with 8 of them a piece is read on the die whose cache it was written through.)  WAVES 4: grid (rows, heads), the lanes side by side and the
 // wavefronts have different pieces.  Bound: the way from the lengths to the states, then memory (512 rows of 32 heads of 128 in 4 pieces, 34 MB: 9.7
 // us; 11.0 with rows leading).
-template <int WAVES>
-__global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
+// DEALT: whether the work was dealt out by deal_out
+template <int WAVES, bool DEALT>
+__device__ __forceinline__ void join_parts(const Lens& H, const AttnArgs& A)
 {
     __shared__ f2_t sums[kAttnWaves];
     __shared__ f4_t values_in[kAttnWaves][kMaxDim / 4];
@@ -1009,7 +1010,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
     }
     AttnTile t;
     int in_tile;
-    if (!find_row(TSHIP_LENS, A, row, head, t, &in_tile) || t.cuts == 1) return;      // (the same for all heads of a row)
+    if (!(DEALT ? find_dealt_row(H, A, row, head, t, &in_tile) : find_row(H, A, row, head, t, &in_tile)) || t.cuts == 1) return;      // (the same for all heads of a row)
     const int cuts = t.cuts, step = WAVES == 1 ? 1 : WAVES * parts;
     const int64_t at0 = slot_row(A, t.slot, head / A.group, in_tile), next = (int64_t)A.cache.kv_heads * A.slot_rows;
     const float* values = A.partial + at0 * dim;
@@ -1057,6 +1058,16 @@ __global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_
     }
     if (!mine) return;
     *reinterpret_cast<f4_t*>(A.out + (int64_t)row * A.ld_out + (int64_t)head * dim + d) = acc * over_sum(A, sum, top + kSpare, head);
+}
+template <int WAVES>
+__global__ void __launch_bounds__(kAttnThreads) paged_combine_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
+{
+    join_parts<WAVES, false>(TSHIP_LENS, A);
+}
+template <int WAVES>
+__global__ void __launch_bounds__(kAttnThreads) paged_combine_dealt_kernel(TSHIP_LENS_ARGS, const AttnArgs A)
+{
+    join_parts<WAVES, true>(TSHIP_LENS, A);
 }
 
 }  // namespace
@@ -1145,8 +1156,10 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
     plan.pieces = cut ? (int)pieces : 0;
     plan.slots = (int)std::min<int64_t>(INT32_MAX, cut ? std::max(tiles, pieces) : tiles);
     plan.slot_rows = all <= kKeyRows ? kKeyRows : kTileRows;
-    // (a tile that is cut is one of at most `pieces` pieces)
-    if (cut) plan.ws_bytes = (size_t)pieces * cache.kv_heads * plan.slot_rows * (dim + 2) * sizeof(float) + sizeof(int);
+    // (a tile that is cut is one of at most `pieces` pieces; dealt out in runs, where a part's slot is the number of its workgroup and its tile, there are fewer
+    // tiles than pieces)
+    plan.parts = (int)(cut ? pieces * (cache.element_type == kTypeMXFP4 ? 2 : 1) : 0);
+    if (cut) plan.ws_bytes = (size_t)plan.parts * cache.kv_heads * plan.slot_rows * (dim + 2) * sizeof(float) + sizeof(Deal);
     return plan;
 }
 
@@ -1189,7 +1202,7 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     args.window = window;
     args.first = first;
     args.capacity = cache.max_pages * (int)cache.page.d;
-    args.slots = plan.pieces;
+    args.slots = plan.parts;
     args.slot_rows = plan.slot_rows;
     args.by_group = FastDiv((uint32_t)args.group);
     args.cache = cache;
@@ -1208,11 +1221,13 @@ bool launch_paged_attention(const PagedAttnPlan& plan, const float* query, int64
     default: ok = launch_attention<2>(H, args, grid, stream); break;
     }
     if (!ok || plan.pieces == 0) return ok;
+    const bool mx = cache.element_type == kTypeMXFP4;
     if ((int64_t)rows * heads <= 8 * device_info().num_cus) {
-        hipLaunchKernelGGL(paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, TSHIP_LENS_OF(H), args);
+        hipLaunchKernelGGL(mx ? paged_combine_dealt_kernel<kAttnWaves> : paged_combine_kernel<kAttnWaves>, dim3(rows, heads), dim3(kAttnThreads), 0, stream, TSHIP_LENS_OF(H), args);
     } else {
         const int parts = 64 / wide_of(cache.head_dim), waves = rows * ((args.group + parts - 1) / parts);
-        hipLaunchKernelGGL(paged_combine_kernel<1>, dim3(cache.kv_heads, (waves + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0, stream, TSHIP_LENS_OF(H), args);
+        hipLaunchKernelGGL(mx ? paged_combine_dealt_kernel<1> : paged_combine_kernel<1>, dim3(cache.kv_heads, (waves + kAttnWaves - 1) / kAttnWaves), dim3(kAttnThreads), 0,
+                           stream, TSHIP_LENS_OF(H), args);
     }
     return hip_ok(hipGetLastError(), "paged attention combine launch");
 }

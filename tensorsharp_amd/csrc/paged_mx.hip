@@ -83,8 +83,8 @@ struct AttnMx {
     static constexpr float kUnit = 7.f, kRise = 8.f;                 // weights begin at 2^7, m follows a score 2^8 above it
     // A value in LDS has 32 bytes behind it: what a transposed read takes at a time is 32 bytes of each of eight keys, which then lie in different banks.
     static constexpr int kRow = HD * 2 + 32;
-    static constexpr int kOwnValues = 32 * kRow;                     // of a wavefront that has keys of its own
-    static constexpr int kOwnLds = kAttnWaves * (kOwnValues > 16 * HD * 4 ? kOwnValues : 16 * HD * 4);
+    static constexpr int kOwnLds = kAttnWaves * 32 * kRow;           // of wavefronts that have keys of their own
+    static_assert(32 * kRow >= 16 * HD * 4, "the states take the place of the values");
     static constexpr int NB = HD > 192 ? 1 : 2, kKeys = 32 * NB;     // 32-key blocks of a step where wavefronts share the keys: as many as registers hold
     static constexpr int kSharedLds = 2 * kKeys * kRow;
     static constexpr int kLds = kOwnLds > kSharedLds ? kOwnLds : kSharedLds;
@@ -92,11 +92,11 @@ struct AttnMx {
     const AttnArgs& A;
     const MxScales& X;
     const AttnTile t;
-    const int kvh, lane, wave;
+    const int kvh, thread, lane, wave;
     lds_t lds;
 
-    __device__ __forceinline__ AttnMx(const AttnArgs& args, const MxScales& scales, const AttnTile& tile, int kv_head, lds_t smem)
-        : A(args), X(scales), t(tile), kvh(kv_head), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lds(smem)
+    __device__ __forceinline__ AttnMx(const AttnArgs& args, const MxScales& scales, const AttnTile& tile, int kv_head, int thread_id, lds_t smem)
+        : A(args), X(scales), t(tile), kvh(kv_head), thread(thread_id), lane(thread_id & 63), wave(__builtin_amdgcn_readfirstlane(thread_id >> 6)), lds(smem)
     {
     }
 
@@ -110,21 +110,24 @@ struct AttnMx {
     __device__ __forceinline__ f2_t* state_of(int row) const { return states_of(A) + slot_row(A, t.slot, kvh, row); }
     __device__ __forceinline__ int blocks() const { return A.cache.head_dim / 32; }
 
-    // terms of block `block` of a row of the tile; rows and blocks that are not there are zero
-    __device__ __forceinline__ void load_terms(int row, int block, Terms& out) const
+    // Block `block` of a row of the tile, even and odd dimensions apart as the conversion takes them; rows and blocks that are not there are zero.  (Loaded ahead of
+    // keys and values and cut behind them, while they are on their way: loads answer in order.)
+    struct RowBlock {
+        f16_t a, b;
+    };
+    __device__ __forceinline__ void load_row(int row, int block, RowBlock& x) const
     {
         const bool live = row < t.count && block < blocks();
         int token, head;
         place(row < t.count ? row : 0, &token, &head);
         const float* src = live ? A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * A.cache.head_dim + 32 * block : reinterpret_cast<const float*>(g_zero_row);
-        f16_t a, b;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const f4_t v = *reinterpret_cast<const f4_t*>(src + 4 * i);
-            a[2 * i] = v[0] * A.sign, b[2 * i] = v[1] * A.sign, a[2 * i + 1] = v[2] * A.sign, b[2 * i + 1] = v[3] * A.sign;
+            const f4_t v = *(const __attribute__((address_space(1))) f4_t*)(uint64_t)(uintptr_t)(src + 4 * i);
+            x.a[2 * i] = v[0], x.b[2 * i] = v[1], x.a[2 * i + 1] = v[2], x.b[2 * i + 1] = v[3];
         }
-        cut_terms(a, b, out);
     }
+    __device__ __forceinline__ void cut_row(const RowBlock& x, Terms& out) const { cut_terms(x.a * A.sign, x.b * A.sign, out); }
 
     // ---- where keys lie ----
     // Lane i has the id of page id_base + i of the sequence: read again when a step passes the last of them, so that no step's loads wait for a
@@ -151,28 +154,24 @@ struct AttnMx {
         const bool there = p < end && (uint32_t)id < (uint32_t)A.cache.num_pages;
         return {there ? (uint32_t)id : 0u, (uint32_t)(p - q * (int)A.cache.page.d), there};
     }
-    // where a lane's block of row 0 of page 0 lies, and how far pages and tokens are apart (below 2^32 bytes, so that each is one multiplication)
-    struct Source {
-        uint64_t at;
-        uint32_t page, token;
-        __device__ __forceinline__ mem_t of(const Row& r) const { return (mem_t)(at + (uint64_t)r.page * page + (uint64_t)r.within * token); }
+    // Where rows lie: pages and tokens are below 2^32 bytes apart, so that each is one multiplication, and mostly one serves codes and scales of keys and values
+    // (X.alike: a row has 16 bytes of codes for one of scales, so their strides are 16 times those of scales where both are dense).
+    struct Place {
+        uint64_t k, v, ks, vs;                                       // bytes from a head's first row
     };
-    __device__ __forceinline__ Source keys_from(int block) const
+    template <bool ALIKE>
+    __device__ __forceinline__ Place place_of(const Row& r) const
     {
-        return {(uint64_t)(uintptr_t)A.cache.k + kvh * A.cache.k_head + 16 * min(block, blocks() - 1), (uint32_t)A.cache.k_page, (uint32_t)A.cache.k_token};
+        auto at = [&](int64_t page, int64_t token) { return (uint64_t)r.page * (uint32_t)page + (uint64_t)r.within * (uint32_t)token; };
+        const uint64_t k = at(A.cache.k_page, A.cache.k_token);
+        if constexpr (ALIKE) return {k, k, k >> 4, k >> 4};
+        return {k, at(A.cache.v_page, A.cache.v_token), at(X.k_page, X.k_token), at(X.v_page, X.v_token)};
     }
-    __device__ __forceinline__ Source values_from(int block) const
-    {
-        return {(uint64_t)(uintptr_t)A.cache.v + kvh * A.cache.v_head + 16 * min(block, blocks() - 1), (uint32_t)A.cache.v_page, (uint32_t)A.cache.v_token};
-    }
-    __device__ __forceinline__ Source key_scales_from(int block) const
-    {
-        return {(uint64_t)(uintptr_t)X.k + kvh * X.k_head + min(block, blocks() - 1), (uint32_t)X.k_page, (uint32_t)X.k_token};
-    }
-    __device__ __forceinline__ Source value_scales_from(int block) const
-    {
-        return {(uint64_t)(uintptr_t)X.v + kvh * X.v_head + min(block, blocks() - 1), (uint32_t)X.v_page, (uint32_t)X.v_token};
-    }
+    __device__ __forceinline__ uint32_t block_of(int block) const { return min(block, blocks() - 1); }
+    __device__ __forceinline__ uint64_t keys() const { return (uint64_t)(uintptr_t)A.cache.k + kvh * A.cache.k_head; }
+    __device__ __forceinline__ uint64_t values() const { return (uint64_t)(uintptr_t)A.cache.v + kvh * A.cache.v_head; }
+    __device__ __forceinline__ uint64_t key_scales() const { return (uint64_t)(uintptr_t)X.k + kvh * X.k_head; }
+    __device__ __forceinline__ uint64_t value_scales() const { return (uint64_t)(uintptr_t)X.v + kvh * X.v_head; }
 
     // ---- infinities and NaN ----
     __device__ __forceinline__ float element(mem_t codes, mem_t scales, int d) const
@@ -200,10 +199,11 @@ struct AttnMx {
                 const uint64_t lanes = __ballot(seen);
                 if (lanes == 0) continue;
                 const Row at{seen ? (uint32_t)id : 0u, (uint32_t)(j - (int)A.cache.page.quot((uint32_t)j) * (int)A.cache.page.d), seen};
-                const mem_t v_at = values_from(0).of(at), vs_at = value_scales_from(0).of(at);
+                const Place place_here = place_of<false>(at);
+                const mem_t v_at = (mem_t)(values() + place_here.v), vs_at = (mem_t)(value_scales() + place_here.vs);
                 float score = -INFINITY;
                 if (seen) {
-                    const mem_t k = keys_from(0).of(at), ks = key_scales_from(0).of(at);
+                    const mem_t k = (mem_t)(keys() + place_here.k), ks = (mem_t)(key_scales() + place_here.ks);
                     float dot = 0.f;
                     for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(k, ks, d);
                     score = dot * A.c;
@@ -266,31 +266,40 @@ struct AttnMx {
     // ---- few rows: every wavefront over keys of its own, 16 rows at a time ----
     static constexpr int kChunks = (HD + 127) / 128, kTiles = HD / 16;
 
-    // A step of 32 keys: key idx of each 16, block 4 c + g of it.  Steps behind the last are loaded like others (of page 0): what is waited for is counted, and a
-    // load that might not be there would have all of them waited for.
+    // A step of 16 KB keys: key idx of each 16, block 4 c + g of it
+    template <int KB>
     struct Step {
-        u4_t k[2][kChunks], v[2][kChunks];
-        uint8_t ks[2][kChunks], vs[2][kChunks];                      // (as loaded: widened ahead of their use they would be waited for)
-        uint32_t there;                                              // a bit for each key
+        u4_t k[KB][kChunks], v[KB][kChunks];
+        uint8_t ks[KB][kChunks], vs[KB][kChunks];                    // (as loaded: widened ahead of their use they would be waited for)
+        uint64_t there;                                              // a bit for each key
     };
-    struct Sources {
-        Source k[kChunks], v[kChunks], ks[kChunks], vs[kChunks];
+    // blocks of a lane in a head's first row
+    struct Blocks {
+        uint64_t k[kChunks], v[kChunks], ks[kChunks], vs[kChunks];
     };
-    __device__ __forceinline__ void load_step(int key, int idx, const Sources& from, Step& s)
+    template <int KB>
+    __device__ __forceinline__ void load_step(int key, int idx, const Blocks& of, Step<KB>& s)
     {
-        const int p0 = t.position(key), end = t.end_at(key);
-        bring_pages(p0, 32);
+        const int p0 = t.position(key);
+        bring_pages(p0, 16 * KB);
+        if (X.alike) load_rows<KB, true>(p0, t.end_at(key), idx, of, s);
+        else load_rows<KB, false>(p0, t.end_at(key), idx, of, s);
+    }
+    template <int KB, bool ALIKE>
+    __device__ __forceinline__ void load_rows(int p0, int end, int idx, const Blocks& of, Step<KB>& s) const
+    {
         s.there = 0;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < KB; ++b) {
             const Row at = row_at(p0 + 16 * b + idx, end);
-            s.there |= (uint32_t)(__ballot(at.there) & 0xffff) << (16 * b);
+            s.there |= (uint64_t)(__ballot(at.there) & 0xffff) << (16 * b);
+            const Place here = place_of<ALIKE>(at);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-                s.k[b][c] = *(mem4_t)(from.k[c].of(at));
-                s.ks[b][c] = *from.ks[c].of(at);
-                s.v[b][c] = *(mem4_t)(from.v[c].of(at));
-                s.vs[b][c] = *from.vs[c].of(at);
+                s.k[b][c] = *(mem4_t)(of.k[c] + here.k);
+                s.ks[b][c] = *(mem_t)(of.ks[c] + here.ks);
+                s.v[b][c] = *(mem4_t)(of.v[c] + here.v);
+                s.vs[b][c] = *(mem_t)(of.vs[c] + here.vs);
             }
         }
     }
@@ -301,6 +310,7 @@ struct AttnMx {
     }
 
     // rows r0 .. r0 + 15 of the tile; whether these have to be done by plainly()
+    template <int KB>
     __device__ __forceinline__ bool own_keys(int r0)
     {
         __shared__ f2_t states[kAttnWaves][16];
@@ -311,86 +321,83 @@ struct AttnMx {
 #pragma unroll
         for (int d = 0; d < kTiles; ++d) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f, l_rest = 0.f;
-        const lds_t values = lds + wave * kOwnValues;
-        int key = t.lo + 32 * wave;
+        const lds_t mine_values = lds + wave * (16 * KB * kRow);
+        int key = t.lo + 16 * KB * wave;
         id_base = -64;                                               // (the keys of the rows before are begun again)
-        constexpr int kStride = 32 * kAttnWaves;
+        constexpr int kStride = 16 * KB * kAttnWaves;
+        constexpr uint64_t kWhole = KB == 4 ? ~0ull : (1ull << (16 * KB)) - 1;
         if (key < t.hi) {
-            Sources from;
+            Blocks of;
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-                from.k[c] = keys_from(4 * c + g), from.v[c] = values_from(4 * c + g), from.ks[c] = key_scales_from(4 * c + g), from.vs[c] = value_scales_from(4 * c + g);
-            Step even, odd_one;
-            // (a loop of pairs of steps has no other way out, so that each waits for its own loads alone; the first of an odd number goes before it)
-            const bool single = ((t.hi - key + kStride - 1) / kStride) & 1;
-            if (single) {
-                load_step(key, idx, from, odd_one);
-                asm volatile("" ::: "memory");
-                load_step(key + kStride, idx, from, even);
-            } else {
-                load_step(key, idx, from, even);
-                asm volatile("" ::: "memory");
-                load_step(key + kStride, idx, from, odd_one);
+            for (int c = 0; c < kChunks; ++c) {
+                const uint32_t block = block_of(4 * c + g);
+                of.k[c] = keys() + 16 * block, of.v[c] = values() + 16 * block, of.ks[c] = key_scales() + block, of.vs[c] = value_scales() + block;
             }
+            RowBlock x[kChunks];
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) load_row(row, 4 * c + g, x[c]);
+            asm volatile("" ::: "memory");
+            Step<KB> even, odd_one;
+            load_step(key, idx, of, even);
+            asm volatile("" ::: "memory");
+            load_step(key + kStride, idx, of, odd_one);
             asm volatile("" ::: "memory");
             Terms q[kChunks];
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) load_terms(row, 4 * c + g, q[c]);
+            for (int c = 0; c < kChunks; ++c) cut_row(x[c], q[c]);
             int token, head;
             place(min(row, t.count - 1), &token, &head);
             const int p = t.p0 + token, lo = first_key(p, A.window), lo_last = first_key(t.p0 + t.tokens - 1, A.window);
-            // a step; the one after the next takes its place
-            auto step = [&](Step& now) {
-                f4_t s[2];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) s[b] = f4_t{0.f, 0.f, 0.f, 0.f};
+            auto step = [&](Step<KB>& now) {
                 const int p0 = t.position(key);
-                const bool whole = now.there == ~0u, in_head = key < t.head;
+                const bool whole = now.there == kWhole, in_head = key < t.head;
                 if constexpr (HD != 128) {                           // (lanes without a block have another's, for which rows have zeros: NaN would stay one)
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) now.ks[b][c] = 4 * c + g < blocks() ? now.ks[b][c] : 0;
+                        for (int b = 0; b < KB; ++b) now.ks[b][c] = 4 * c + g < blocks() ? now.ks[b][c] : 0;
                 }
                 if (!whole) {                                        // (a value of the least power under a weight of 0)
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) now.vs[b][c] = (now.there >> (16 * b + idx)) & 1 ? now.vs[b][c] : 0;
+                        for (int b = 0; b < KB; ++b) now.vs[b][c] = (now.there >> (16 * b + idx)) & 1 ? now.vs[b][c] : 0;
                 }
-                // (small terms first, the two blocks in turn)
+                f4_t s[KB];
+#pragma unroll
+                for (int b = 0; b < KB; ++b) s[b] = f4_t{0.f, 0.f, 0.f, 0.f};
+                // (small terms first, the blocks in turn)
                 auto product = [&](auto part) {
                     constexpr int n = decltype(part)::value;
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
+                        for (int b = 0; b < KB; ++b)
                             s[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(now.k[b][c]), operand(q[c].t[n]), s[b], 4, 2, 0, (int)now.ks[b][c], n % 4,
                                                                                     (int)q[c].scale[n / 4]);
                 };
                 each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
                 // the values of the step, for the transposed reads below
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < KB; ++b)
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c)
-                        if (4 * c + g < kBlocks) put_values(now.v[b][c], now.vs[b][c], values + (16 * b + idx) * kRow + 64 * (4 * c + g));
+                        if (4 * c + g < kBlocks) put_values(now.v[b][c], now.vs[b][c], mine_values + (16 * b + idx) * kRow + 64 * (4 * c + g));
                 // score i of block b belongs to key 16 b + 4 g + i
-                if (!whole || p0 + 31 > t.p0 || (!in_head && p0 < lo_last)) {
+                if (!whole || p0 + 16 * KB - 1 > t.p0 || (!in_head && p0 < lo_last)) {
                     const int last = p - p0 - 4 * g, first = in_head ? 0 : lo - p0 - 4 * g;
-                    const uint32_t there = now.there >> (4 * g);
+                    const uint64_t there = now.there >> (4 * g);
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < KB; ++b)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int k = 16 * b + i;
                             if (k > last || k < first || !((there >> k) & 1)) s[b][i] = -INFINITY;
                         }
                 }
-                load_step(key + 2 * kStride, idx, from, now);
                 float top = s[0][0];
 #pragma unroll
-                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+                for (int i = 1; i < 4 * KB; ++i) top = fmaxf(top, s[i / 4][i % 4]);
                 top = of_rows(top, larger) * A.c;
                 if (__any(top > m + kRise)) {                        // (m starts at -infinity)
                     float mn = m;
@@ -403,34 +410,39 @@ struct AttnMx {
                     m = mn;
                 }
                 const float bias = kUnit - (m == -INFINITY ? 0.f : m);
-                float w[8], sum = 0.f;
+                float sum = 0.f;
+                // a lane gives the place of four dimensions of one key and gets one dimension of four keys, within 16 lanes
+                const lds_t at = mine_values + (4 * g + (idx >> 2)) * kRow + 8 * (idx & 3);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], A.c, bias));
-                    sum += w[i];
+                for (int h = 0; h < KB / 2; ++h) {                   // 32 keys
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + i / 4][i % 4], A.c, bias));
+                        sum += w[i];
+                    }
+                    u4_t part[3];
+                    cut3(w, part);
+#pragma unroll
+                    for (int d = 0; d < kTiles; ++d) {
+                        const u4_t a = transposed(at + 32 * d + 32 * h * kRow, at + 32 * d + (32 * h + 16) * kRow);
+#pragma unroll
+                        for (int n = 2; n >= 0; --n)
+                            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
+                    }
                 }
                 add_weights(sum, l, l_rest);
-                u4_t part[3];
-                cut3(w, part);
-                // a lane gives the place of four dimensions of one key and gets one dimension of four keys, within 16 lanes
-                const lds_t at = values + (4 * g + (idx >> 2)) * kRow + 8 * (idx & 3);
-#pragma unroll
-                for (int d = 0; d < kTiles; ++d) {
-                    const u4_t a = transposed(at + 32 * d, at + 32 * d + 16 * kRow);
-#pragma unroll
-                    for (int n = 2; n >= 0; --n)
-                        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
-                }
             };
-            if (single) {
-                step(odd_one);
-                key += kStride;
-            }
-            while (key < t.hi) {
+            // Two steps are under way: what a step has is loaded anew behind it, in this order and whether there is one or not, so that each waits for its own
+            // loads alone (they are counted).
+            for (; key < t.hi; key += kStride) {
                 step(even);
+                load_step(key + 2 * kStride, idx, of, even);
+                asm volatile("" ::: "memory");
                 key += kStride;
-                step(odd_one);
-                key += kStride;
+                if (key < t.hi) step(odd_one);
+                load_step(key + 2 * kStride, idx, of, odd_one);
+                asm volatile("" ::: "memory");
             }
         }
         l = of_rows(l + l_rest, added);
@@ -452,7 +464,7 @@ struct AttnMx {
         for (int w = 0; w < kAttnWaves; ++w) any |= odd[w];
         const bool again = __builtin_amdgcn_readfirstlane(any);
         const int pieces = A.cache.head_dim / 4;
-        for (int i = threadIdx.x; !again && i < rows * pieces; i += kAttnThreads) {
+        for (int i = thread; !again && i < rows * pieces; i += kAttnThreads) {
             const int r = i / pieces, piece = i - r * pieces;
             float top = -INFINITY;
 #pragma unroll
@@ -490,22 +502,29 @@ struct AttnMx {
         uint8_t ks[NB][kHalves];
         uint64_t there;              // (bits of keys that a step has not are set)
     };
-    struct KeySources {
-        Source k[kHalves], ks[kHalves];
+    struct KeyBlocks {
+        uint64_t k[kHalves], ks[kHalves];
     };
-    __device__ __forceinline__ void load_keys(int key, int col, const KeySources& from, Keys& s)
+    __device__ __forceinline__ void load_keys(int key, int col, const KeyBlocks& of, Keys& s)
     {
-        const int p0 = t.position(key), end = t.end_at(key);
+        const int p0 = t.position(key);
         bring_pages(p0, kKeys);
+        if (X.alike) load_keys<true>(p0, t.end_at(key), col, of, s);
+        else load_keys<false>(p0, t.end_at(key), col, of, s);
+    }
+    template <bool ALIKE>
+    __device__ __forceinline__ void load_keys(int p0, int end, int col, const KeyBlocks& of, Keys& s) const
+    {
         s.there = NB == 2 ? 0 : ~0xffffffffull;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const Row at = row_at(p0 + 32 * b + col, end);
             s.there |= (__ballot(at.there) & 0xffffffffull) << (32 * b);
+            const Place here = place_of<ALIKE>(at);
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) {
-                s.k[b][c] = *(mem4_t)(from.k[c].of(at));
-                s.ks[b][c] = *from.ks[c].of(at);
+                s.k[b][c] = *(mem4_t)(of.k[c] + here.k);
+                s.ks[b][c] = *(mem_t)(of.ks[c] + here.ks);
             }
         }
     }
@@ -515,26 +534,33 @@ struct AttnMx {
         uint8_t vs[kMine];
         bool there[kMine];
     };
-    struct ValueSources {
-        Source v[kMine], vs[kMine];
+    struct ValueBlocks {
+        uint64_t v[kMine], vs[kMine];
     };
-    __device__ __forceinline__ void load_values(int key, const ValueSources& from, Values& s)
+    __device__ __forceinline__ void load_values(int key, const ValueBlocks& of, Values& s)
     {
-        const int p0 = t.position(key), end = t.end_at(key);
+        const int p0 = t.position(key);
         bring_pages(p0, kKeys);
+        if (X.alike) load_values<true>(p0, t.end_at(key), of, s);
+        else load_values<false>(p0, t.end_at(key), of, s);
+    }
+    template <bool ALIKE>
+    __device__ __forceinline__ void load_values(int p0, int end, const ValueBlocks& of, Values& s) const
+    {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
-            const Row at = row_at(p0 + min((int)(n * kAttnThreads + threadIdx.x) / kBlocks, kKeys - 1), end);
+            const Row at = row_at(p0 + min((n * kAttnThreads + thread) / kBlocks, kKeys - 1), end);
+            const Place here = place_of<ALIKE>(at);
             s.there[n] = at.there;
-            s.v[n] = *(mem4_t)(from.v[n].of(at));
-            s.vs[n] = *from.vs[n].of(at);
+            s.v[n] = *(mem4_t)(of.v[n] + here.v);
+            s.vs[n] = *(mem_t)(of.vs[n] + here.vs);
         }
     }
     __device__ __forceinline__ void turn_values(const Values& s, lds_t buffer) const
     {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
-            const int unit = n * kAttnThreads + threadIdx.x, row = unit / kBlocks, block = unit - row * kBlocks;
+            const int unit = n * kAttnThreads + thread, row = unit / kBlocks, block = unit - row * kBlocks;
             if (kKeys * kBlocks % kAttnThreads == 0 || row < kKeys) put_values(s.v[n], s.there[n] ? s.vs[n] : 0, buffer + row * kRow + 64 * block);
         }
     }
@@ -556,22 +582,28 @@ struct AttnMx {
         if (t.lo >= t.hi) {
             nothing_yet();
         } else {
-            Keys keys;
-            Values values;
-            KeySources keys_at;
-            ValueSources values_at;
+            Keys step;
+            Values turned;
+            KeyBlocks keys_at;
+            ValueBlocks values_at;
 #pragma unroll
-            for (int c = 0; c < kHalves; ++c) keys_at.k[c] = keys_from(2 * c + half), keys_at.ks[c] = key_scales_from(2 * c + half);
+            for (int c = 0; c < kHalves; ++c) keys_at.k[c] = keys() + 16 * block_of(2 * c + half), keys_at.ks[c] = key_scales() + block_of(2 * c + half);
 #pragma unroll
             for (int n = 0; n < kMine; ++n) {
-                const int block = (n * kAttnThreads + threadIdx.x) % kBlocks;
-                values_at.v[n] = values_from(block), values_at.vs[n] = value_scales_from(block);
+                const uint32_t block = block_of((n * kAttnThreads + thread) % kBlocks);
+                values_at.v[n] = values() + 16 * block, values_at.vs[n] = value_scales() + block;
             }
-            load_keys(t.lo, col, keys_at, keys);
-            load_values(t.lo, values_at, values);
+            load_keys(t.lo, col, keys_at, step);
+            load_values(t.lo, values_at, turned);
+            asm volatile("" ::: "memory");
+            // (rows behind them here: held ahead of their cutting they would take registers that are not there)
             Terms q[kHalves];
 #pragma unroll
-            for (int c = 0; c < kHalves; ++c) load_terms(row, 2 * c + half, q[c]);
+            for (int c = 0; c < kHalves; ++c) {
+                RowBlock x;
+                load_row(row, 2 * c + half, x);
+                cut_row(x, q[c]);
+            }
             asm volatile("" ::: "memory");                           // (the accumulators come after the cutting of rows, which takes registers too)
             nothing_yet();
             int token, head;
@@ -581,9 +613,9 @@ struct AttnMx {
             for (int key = t.lo; key < t.hi; key += kKeys) {
                 const lds_t here = lds + buffer * (kKeys * kRow);
                 buffer ^= 1;
-                turn_values(values, here);
+                turn_values(turned, here);
                 __syncthreads();                                     // (what the other buffer held has been read by all)
-                load_values(key + kKeys, values_at, values);
+                load_values(key + kKeys, values_at, turned);
                 const int p0 = t.position(key);
                 const bool in_head = key < t.head, mine = 32 * wave < t.count && p0 <= p_last;
                 f16_t s[NB];
@@ -592,7 +624,7 @@ struct AttnMx {
 #pragma unroll
                         for (int c = 0; c < kHalves; ++c)
 #pragma unroll
-                            for (int b = 0; b < NB; ++b) keys.ks[b][c] = 2 * c + half < blocks() ? keys.ks[b][c] : 0;
+                            for (int b = 0; b < NB; ++b) step.ks[b][c] = 2 * c + half < blocks() ? step.ks[b][c] : 0;
                     }
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
@@ -604,13 +636,13 @@ struct AttnMx {
                         for (int c = 0; c < kHalves; ++c)
 #pragma unroll
                             for (int b = 0; b < NB; ++b)
-                                s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(keys.k[b][c]), operand(q[c].t[n]), s[b], 4, 2, 0, (int)keys.ks[b][c], n % 4,
+                                s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(step.k[b][c]), operand(q[c].t[n]), s[b], 4, 2, 0, (int)step.ks[b][c], n % 4,
                                                                                        (int)q[c].scale[n / 4]);
                     };
                     each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
                 }
-                const uint64_t there = keys.there;
-                load_keys(key + kKeys, col, keys_at, keys);
+                const uint64_t there = step.there;
+                load_keys(key + kKeys, col, keys_at, step);
                 if (!mine) continue;
                 // score i of block b belongs to key 32 b + 8 (i / 4) + 4 half + i % 4
                 if (~there != 0 || p0 + kKeys - 1 > p_first || (!in_head && p0 < lo_last)) {
@@ -698,21 +730,42 @@ struct AttnMx {
     }
 };
 
-// grid (KV heads, pieces)
+constexpr float kTall = 3.f;                                         // what a step of a long tile takes, a short one's being 1
+
+// grid (KV heads, workgroups)
 template <int HD>
 __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_attention_kernel(TSHIP_LENS_ARGS, const AttnArgs A, const MxScales X)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
+    const Lens H = TSHIP_LENS;
+    // (every line of the arguments is asked for at once: read where they are needed they cost one trip to memory after the other, 3 us)
+    asm volatile("" ::"s"(A.query), "s"(A.ld_out), "s"(A.by_group.m), "s"(A.cache.k), "s"(A.cache.v_head), "s"(A.cache.table_stride), "s"(A.cache.max_pages), "s"(X.k), "s"(X.v_head));
+    const Deal deal = deal_out(H, gridDim.x, worth_of(kTypeMXFP4, HD, kAttnWaves), kTall);
+    if (H.pieces > 0 && blockIdx.x == 0 && idx == 0 && threadIdx.x == 0) *deal_of(A) = deal;
     AttnTile t;
-    if (!find_piece(TSHIP_LENS, A, gridDim.x, worth_of(kTypeMXFP4, HD, kAttnWaves), idx, t)) return;
-    AttnMx<HD> a(A, X, t, kvh, (lds_t)smem);
-    if (t.tokens * A.group <= kKeyRows) {
+    const bool whole = deal.tall < 0;
+    if (whole || idx < deal.tall) {
+        if (!(whole ? find_whole(H, A, idx, t) : find_tall(H, A, deal, idx, t))) return;
+        if (t.tokens * A.group > kKeyRows) {
+            AttnMx<HD> a(A, X, t, kvh, threadIdx.x, (lds_t)smem);
+            if (a.shared_keys()) a.plainly(32 * a.wave, 1);
+            return;
+        }
+    } else if (idx >= H.pieces) {
+        return;
+    }
+    const int run = idx - deal.tall;
+    for (int at = whole ? 0 : run * deal.run_steps, end = whole ? 1 : at + deal.run_steps; at < end;) {
+        const int steps = whole ? 1 : find_run(H, A, deal, run, at, t);
+        if (steps == 0) return;
+        at += steps;
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));                             // (what follows from it is worked out for each tile: kept from one to the next it would be spilled)
+        AttnMx<HD> a(A, X, t, kvh, thread, (lds_t)smem);
         bool again = false;
-        for (int r0 = 0; r0 < t.count; r0 += 16) again |= a.own_keys(r0);
+        for (int r0 = 0; r0 < t.count; r0 += 16) again |= a.template own_keys<2>(r0);
         if (again) a.plainly(a.wave, kAttnWaves);
-    } else if (a.shared_keys()) {
-        a.plainly(32 * a.wave, 1);
     }
 }
 

@@ -233,6 +233,166 @@ __device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int
     t.lo = begin;
     return true;
 }
+// ---- another way to deal out the same work ----
+// Pieces of sequences whose lengths have nothing to do with each other are between half as long and as long as the longest.  Here the steps of all short tiles (of
+// sequences with at most 32 rows), one after the other, are cut into runs of equal length: a run may have the end of one tile, whole ones and the beginning of another, to
+// which its workgroup turns one after the other.  Long tiles are cut into pieces by themselves, with their share of the workgroups, one piece each.  Parts of tiles
+// have slots as pieces have: a long tile's piece its number, a run's part the number of its workgroup plus that of its tile.
+struct Deal {
+    int tall;                    // workgroups for pieces of long tiles; -1: every tile is one workgroup's
+    int tall_steps, run_steps;   // 128 keys each: of a piece, of a run
+};
+__device__ __forceinline__ bool is_tall(const Lens& H, const Lanes& L) { return L.n * H.group > kKeyRows; }
+__device__ __forceinline__ int tall_tiles(const Lens& H, const Lanes& L) { return is_tall(H, L) ? L.tiles : 0; }
+__device__ __forceinline__ int short_steps(const Lens& H, const Lanes& L) { return L.tiles > 0 && !is_tall(H, L) ? max(1, min(L.steps, 1 << 16)) : 0; }
+// tall: what a step of a long tile takes, a short one's being 1
+__device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth least, float tall)
+{
+    constexpr Deal kWhole{-1, 0, 0};
+    if (H.pieces == 0) return kWhole;
+    Lanes L;
+    int tiles = 0, long_tiles = 0, most = 0, long_most = 0;
+    float steps = 0.f, long_steps = 0.f;
+    for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
+        const int n = short_steps(H, L), m = tall_tiles(H, L);
+        tiles += lane_sum(L.tiles);
+        long_tiles += lane_sum(m);
+        steps += (float)lane_sum(n);
+        long_steps += (float)lane_sum(min(m * min(L.steps, 1 << 16), 1 << 24));
+        int high = n, long_high = m > 0 ? L.steps : 0;
+        for (int o = 32; o > 0; o >>= 1) high = max(high, __shfl_xor(high, o)), long_high = max(long_high, __shfl_xor(long_high, o));
+        most = max(most, __builtin_amdgcn_readfirstlane(high)), long_most = max(long_most, __builtin_amdgcn_readfirstlane(long_high));
+    }
+    if (tiles >= H.pieces) return kWhole;
+    const bool runs = tiles > long_tiles;
+    Deal d{0, 1, 1};
+    if (long_tiles > 0) {
+        const float share = tall * long_steps / (tall * long_steps + steps);
+        d.tall = runs ? min(max((int)(share * H.pieces + 0.5f), long_tiles), H.pieces - 1) : H.pieces;
+        // (a length that no tile exceeds ends it in any case: there are no more tiles than pieces)
+        for (d.tall_steps = max(1, (int)ceilf(long_steps / (float)d.tall));; d.tall_steps += 1 + d.tall_steps / 16) {
+            int all = 0;
+            for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+                L.load(H, s0);
+                all += lane_sum(min(tall_tiles(H, L) * L.cuts(d.tall_steps), 1 << 24));
+            }
+            if (all <= d.tall) break;
+        }
+    }
+    if (runs) d.run_steps = max(1, (int)ceilf(steps / (float)(H.pieces - d.tall)));
+    const bool worth = (long_tiles > 0 && long_most - d.tall_steps >= least.tall) || (runs && most - d.run_steps >= (tiles * kv_heads >= 64 ? least.many : least.few));
+    return worth ? d : kWhole;
+}
+// behind the states: the deal, from the attention for the kernel that joins
+__device__ __forceinline__ Deal* deal_of(const AttnArgs& A) { return reinterpret_cast<Deal*>(steps_of(A)); }
+
+// the idx-th tile from the end (the last tiles of a prompt have the most keys and go first), whole; false: there is none
+__device__ __forceinline__ bool find_whole(const Lens& H, const AttnArgs& A, int idx, AttnTile& t)
+{
+    Lanes L;
+    int tiles = 0, s0 = 0;
+    for (; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
+        tiles += lane_sum(L.tiles);
+    }
+    int want = tiles - 1 - idx, cum;
+    if (want < 0) return false;
+    for (s0 = 0;; s0 += 64) {                                        // (fewer than the total)
+        L.load(H, s0);
+        cum = lane_scan(L.tiles);
+        if (want < __builtin_amdgcn_readlane(cum, 63)) break;
+        want -= __builtin_amdgcn_readlane(cum, 63);
+    }
+    const int at = __ffsll((unsigned long long)__ballot(want < cum)) - 1;
+    set_tile(A, L, s0, at, want - __builtin_amdgcn_readlane(cum - L.tiles, at), 1 << 24, t);
+    t.cuts = 1;
+    return true;
+}
+// piece number idx of the long tiles; false: there is none
+__device__ __forceinline__ bool find_tall(const Lens& H, const AttnArgs& A, const Deal& d, int idx, AttnTile& t)
+{
+    Lanes L;
+    int want = idx;
+    for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
+        const int all = tall_tiles(H, L) * L.cuts(d.tall_steps), cum = lane_scan(all);
+        if (want >= __builtin_amdgcn_readlane(cum, 63)) {
+            want -= __builtin_amdgcn_readlane(cum, 63);
+            continue;
+        }
+        const int at = __ffsll((unsigned long long)__ballot(want < cum)) - 1, cuts = __builtin_amdgcn_readlane(L.cuts(d.tall_steps), at);
+        want -= __builtin_amdgcn_readlane(cum - all, at);
+        set_tile(A, L, s0, at, want / cuts, d.tall_steps, t);
+        t.slot = idx;
+        const int keys = piece_keys(t), begin = t.lo + want % cuts * keys;
+        t.hi = min(begin + keys, t.hi);
+        t.lo = begin;
+        return true;
+    }
+    return false;
+}
+// step `at` of the short tiles' and what follows of its tile up to the end of run number `run`; how many steps these are, 0: there are no more
+__device__ __forceinline__ int find_run(const Lens& H, const AttnArgs& A, const Deal& d, int run, int at, AttnTile& t)
+{
+    Lanes L;
+    int want = at, number = 0;
+    for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
+        const int all = short_steps(H, L), cum = lane_scan(all);
+        const uint64_t tiles = __ballot(all > 0);
+        if (want >= __builtin_amdgcn_readlane(cum, 63)) {
+            want -= __builtin_amdgcn_readlane(cum, 63);
+            number += __popcll(tiles);
+            continue;
+        }
+        const int lane = __ffsll((unsigned long long)__ballot(want < cum)) - 1, steps = __builtin_amdgcn_readlane(all, lane);
+        const int x0 = want - __builtin_amdgcn_readlane(cum - all, lane), x1 = min(steps, x0 + (run + 1) * d.run_steps - at), start = at - x0;
+        set_tile(A, L, s0, lane, 0, 1 << 24, t);
+        t.cuts = (start + steps - 1) / d.run_steps - start / d.run_steps + 1;
+        t.slot = d.tall + run + number + __popcll(tiles & ((1ull << lane) - 1));
+        const int begin = t.lo + 128 * x0;
+        t.hi = x1 == steps ? t.hi : min(t.hi, t.lo + 128 * x1);
+        t.lo = begin;
+        return x1 - x0;
+    }
+    return 0;
+}
+// the tile of a row and head as it was dealt out and its first part; false: of no sequence
+__device__ __forceinline__ bool find_dealt_row(const Lens& H, const AttnArgs& A, int row, int head, AttnTile& t, int* in_tile)
+{
+    const Deal d = *deal_of(A);
+    t.cuts = 1;
+    if (d.tall < 0) return true;
+    Lanes L;
+    int pieces = 0, before = 0, numbers = 0;
+    for (int s0 = 0; s0 < H.seqs; s0 += 64) {
+        L.load(H, s0);
+        const int all = tall_tiles(H, L) * L.cuts(d.tall_steps), n = short_steps(H, L), cum = lane_scan(all), steps_cum = lane_scan(n);
+        const uint64_t has = __ballot(row >= L.start && row < L.start + L.n), tiles = __ballot(n > 0);
+        if (has) {
+            const int at = __ffsll((unsigned long long)has) - 1;
+            const int r = (row - __builtin_amdgcn_readlane(L.start, at)) * H.group + head % H.group, steps = __builtin_amdgcn_readlane(n, at);
+            if (steps == 0) {
+                const int tile = r / kTileRows;
+                t.cuts = __builtin_amdgcn_readlane(L.cuts(d.tall_steps), at);
+                t.slot = pieces + __builtin_amdgcn_readlane(cum - all, at) + tile * t.cuts;
+                *in_tile = r - tile * kTileRows;
+            } else {
+                const int start = before + __builtin_amdgcn_readlane(steps_cum - n, at);
+                t.cuts = (start + steps - 1) / d.run_steps - start / d.run_steps + 1;
+                t.slot = d.tall + start / d.run_steps + numbers + __popcll(tiles & ((1ull << at) - 1));
+                *in_tile = r;
+            }
+            return true;
+        }
+        pieces += __builtin_amdgcn_readlane(cum, 63);
+        before += __builtin_amdgcn_readlane(steps_cum, 63);
+        numbers += __popcll(tiles);
+    }
+    return false;
+}
+
 // What a row's weighted values are multiplied by: 1 / (sum + the sink's weight), sum being counted in units of 2^unit; 1 / 0 never.  (The sink may be far
 // above the units that m came down to.)
 __device__ __forceinline__ float over_sum(const AttnArgs& A, float sum, float unit, int head)

@@ -342,6 +342,7 @@ struct PagedKv {
 struct MxScales {
     uint8_t *k, *v;
     int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+    bool alike;                // keys and values have the same strides, 16 times those of their scales
 };
 
 // x [tokens x heads x head_dim] (strides in elements) -> out, which may be x
@@ -358,6 +359,7 @@ bool launch_rope_store_mx(const float* qkv, int64_t ld_qkv, float* query, int64_
 struct PagedAttnPlan {
     int pieces;                // per KV head that the keys are cut into, 0: not cut
     int slots, slot_rows;      // pieces there can be, rows of each
+    int parts;                 // whose states have room
     size_t ws_bytes;
 };
 PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, int window, int first);
