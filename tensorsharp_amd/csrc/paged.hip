@@ -462,7 +462,8 @@ struct Attn {
     {
         constexpr int kKeys = SHARED ? 32 * NT : 32;
         const int first = (int)A.cache.page.quot((uint32_t)key0);   // uniform
-        if ((int)A.cache.page.quot((uint32_t)(key0 + kKeys - 1)) - id_base >= 64) {
+        // (what follows the first positions may begin before the end of their last step)
+        if ((FIRST && first < id_base) || (int)A.cache.page.quot((uint32_t)(key0 + kKeys - 1)) - id_base >= 64) {
             id_base = first;
             ids = A.cache.table[t.seq * A.cache.table_stride + min(first + lane, A.cache.max_pages - 1)];
         }

@@ -105,3 +105,22 @@ def test_infinities_and_nan_between_the_first_and_the_window(hip, dtype, news):
     assert np.all(out[:, 2:, 5] == np.inf)
     out[:, 2:, 5] = ref[:, 2:, 5]
     assert np.all(np.abs(out - ref) <= 1e-5 * size)
+
+
+@pytest.mark.parametrize("page", [1, 3, 5, 7, 11])
+@pytest.mark.parametrize("kind", ["float16", "bfloat16", "float32", "four bits"])
+def test_pages_where_the_first_positions_end(hip, kind, page):
+    """what follows the first positions lies before the end of their last step, on a page before the last one that was looked up"""
+    import torch
+    from attention_oracle import FourBits
+    from test_gpu_attention_four_bits import run as run_four_bits
+    rng = np.random.default_rng(page)
+    heads, kv, dim = 8, 1, 64
+    news, contexts = [40, 70], [1990, 2600]
+    four = kind == "four bits"
+    c = FourBits(torch, rng, contexts, page, kv, dim) if four else po.Cache(torch, rng, contexts, page, kv, dim, getattr(torch, kind))
+    q = torch.from_numpy((2.0 * rng.standard_normal((sum(news), heads * dim))).astype(np.float32)).cuda()
+    for first in (1729, 1793, 1857, 1921, 1900, 900):
+        for window in (90, 700):
+            out = (run_four_bits if four else run)(hip, torch, c, q, news, contexts, 0.125, window, first)
+            check(out, c, q, news, contexts, heads, dim, 0.125, window, first, terms=four)
