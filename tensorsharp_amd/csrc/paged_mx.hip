@@ -85,7 +85,7 @@ struct AttnMx {
     static constexpr int kRow = HD * 2 + 32;
     static constexpr int kOwnLds = kAttnWaves * 32 * kRow;           // of wavefronts that have keys of their own
     static_assert(32 * kRow >= 16 * HD * 4, "the states take the place of the values");
-    static constexpr int kKeys = 32;                                 // of a step where wavefronts share the keys
+    static constexpr int NB = HD > 192 ? 1 : 2, kKeys = 32 * NB;     // 32-key blocks of a step where wavefronts share the keys: as many as registers hold
     static constexpr int kSharedLds = 2 * kKeys * kRow;
     static constexpr int kLds = kOwnLds > kSharedLds ? kOwnLds : kSharedLds;
 
@@ -497,11 +497,11 @@ struct AttnMx {
     // ---- many rows: all wavefronts over the same keys, 32 rows each ----
     static constexpr int kHalves = (HD + 63) / 64, kDims = HD / 32, kMine = (kKeys * kBlocks + kAttnThreads - 1) / kAttnThreads;
 
-    // a step's keys: key col, block 2 c + half of it
+    // keys of a step: key col of each 32, block 2 c + half of it
     struct Keys {
-        u4_t k[kHalves];
-        uint8_t ks[kHalves];
-        uint32_t there;
+        u4_t k[NB][kHalves];
+        uint8_t ks[NB][kHalves];
+        uint64_t there;              // (bits of keys that a step has not are set)
     };
     struct KeyBlocks {
         uint64_t k[kHalves], ks[kHalves];
@@ -516,13 +516,17 @@ struct AttnMx {
     template <bool ALIKE>
     __device__ __forceinline__ void load_keys(int p0, int end, int col, const KeyBlocks& of, Keys& s) const
     {
-        const Row at = row_at(p0 + col, end);
-        s.there = (uint32_t)__ballot(at.there);
-        const Place here = place_of<ALIKE>(at);
+        s.there = NB == 2 ? 0 : ~0xffffffffull;
 #pragma unroll
-        for (int c = 0; c < kHalves; ++c) {
-            s.k[c] = *(mem4_t)(of.k[c] + here.k);
-            s.ks[c] = *(mem_t)(of.ks[c] + here.ks);
+        for (int b = 0; b < NB; ++b) {
+            const Row at = row_at(p0 + 32 * b + col, end);
+            s.there |= (__ballot(at.there) & 0xffffffffull) << (32 * b);
+            const Place here = place_of<ALIKE>(at);
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c) {
+                s.k[b][c] = *(mem4_t)(of.k[c] + here.k);
+                s.ks[b][c] = *(mem_t)(of.ks[c] + here.ks);
+            }
         }
     }
     // and the blocks of values that a thread turns
@@ -562,28 +566,6 @@ struct AttnMx {
         }
     }
 
-    // S^T of a step (small terms first)
-    __device__ __forceinline__ f16_t scores(const Keys& step, const Terms (&q)[kHalves], int half) const
-    {
-        f16_t s;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.f;
-        auto product = [&](auto part) {
-            constexpr int n = decltype(part)::value;
-#pragma unroll
-            for (int c = 0; c < kHalves; ++c) {
-                // (see own_keys)
-                const int e = HD % 64 != 0 || HD == 64 || HD > 128 ? (2 * c + half < blocks() ? step.ks[c] : 0) : step.ks[c];
-                s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(step.k[c]), operand(q[c].t[n]), s, 4, 2, 0, e, n % 4, (int)q[c].scale[n / 4]);
-            }
-        };
-        each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
-        return s;
-    }
-
-    // While a step's weights are formed and multiplied with its values, the next one's scores are: the matrix instructions (34 of 32 cycles for 32 keys of 128
-    // dimensions) and the vector instructions (some 260 of 4) of one wavefront take about the same time, and only beside each other within a
-    // wavefront do they overlap reliably.
     __device__ __forceinline__ bool shared_keys()
     {
         const int col = lane & 31, half = lane >> 5, row = 32 * wave + col;
@@ -628,24 +610,59 @@ struct AttnMx {
             int token, head;
             place(min(row, t.count - 1), &token, &head);
             const int p = t.p0 + token, lo = first_key(p, A.window);
-            f16_t s;
-            // the scores of the step at `key` are there: what its rows do not see of it, and what its weights are counted against
-            auto look = [&](int key, uint32_t there) {
+            int buffer = 0;
+            for (int key = t.lo; key < t.hi; key += kKeys) {
+                const lds_t here = lds + buffer * (kKeys * kRow);
+                buffer ^= 1;
+                turn_values(turned, here);
+                __syncthreads();                                     // (what the other buffer held has been read by all)
+                load_values(key + kKeys, values_at, turned);
                 const int p0 = t.position(key);
-                const bool in_head = key < t.head;
-                // score i belongs to key 8 (i / 4) + 4 half + i % 4
-                if (~there != 0 || p0 + 31 > p_first || (!in_head && p0 < lo_last)) {
-                    const int last = p - p0 - 4 * half, first = in_head ? 0 : lo - p0 - 4 * half;
-                    const uint32_t bits = there >> (4 * half);
+                const bool in_head = key < t.head, mine = 32 * wave < t.count && p0 <= p_last;
+                f16_t s[NB];
+                if (mine) {
+                    if constexpr (HD % 64 != 0 || HD == 64 || HD > 128) {                // (see own_keys)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int k = 8 * (i / 4) + i % 4;
-                        if (k > last || k < first || !((bits >> k) & 1)) s[i] = -INFINITY;
+                        for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) step.ks[b][c] = 2 * c + half < blocks() ? step.ks[b][c] : 0;
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+                    auto product = [&](auto part) {
+                        constexpr int n = decltype(part)::value;
+#pragma unroll
+                        for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b)
+                                s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(step.k[b][c]), operand(q[c].t[n]), s[b], 4, 2, 0, (int)step.ks[b][c], n % 4,
+                                                                                       (int)q[c].scale[n / 4]);
+                    };
+                    each_of<kParts>([&](auto i) { product(std::integral_constant<int, kParts - 1 - decltype(i)::value>()); });
+                }
+                const uint64_t there = step.there;
+                load_keys(key + kKeys, col, keys_at, step);
+                if (!mine) continue;
+                // score i of block b belongs to key 32 b + 8 (i / 4) + 4 half + i % 4
+                if (~there != 0 || p0 + kKeys - 1 > p_first || (!in_head && p0 < lo_last)) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int below = 32 * b + 4 * half, last = p - p0 - below, first = in_head ? 0 : lo - p0 - below;
+                        const uint32_t bits = (uint32_t)(there >> below);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int k = 8 * (i / 4) + i % 4;
+                            if (k > last || k < first || !((bits >> k) & 1)) s[b][i] = -INFINITY;
+                        }
                     }
                 }
-                float top = s[0];
+                float top = s[0][0];
 #pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
                 top = both_halves(top, larger) * A.c;
                 if (__any(top > m + kRise)) {
                     float mn = m;
@@ -659,58 +676,28 @@ struct AttnMx {
                         for (int i = 0; i < 16; ++i) o[d][i] *= f;
                     m = mn;
                 }
-            };
-            // (once a wavefront's rows see no more keys, they see none that follow; of the first positions they may see some)
-            auto mine = [&](int key) { return 32 * wave < t.count && key < t.hi && (key < t.head || t.position(key) <= p_last); };
-            turn_values(turned, lds);
-            load_values(t.lo + kKeys, values_at, turned);
-            if (mine(t.lo)) s = scores(step, q, half);
-            uint32_t there = step.there;
-            load_keys(t.lo + kKeys, col, keys_at, step);
-            if (mine(t.lo)) look(t.lo, there);
-            __syncthreads();
-            int buffer = 0;
-            for (int key = t.lo; key < t.hi; key += kKeys) {
-                const lds_t here = lds + buffer * (kKeys * kRow);
-                buffer ^= 1;
-                const bool now = mine(key);
-                there = step.there;
-                if (now) {
-                    const float bias = kUnit - (m == -INFINITY ? 0.f : m);
-                    const lds_t at = here + (4 * half + ((lane & 15) >> 2)) * kRow + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-                    u4_t part[2][3];
-                    float sum = 0.f;
-                    auto weigh = [&](int h) {                        // 16 keys
-                        float w[8];
+                const float bias = kUnit - (m == -INFINITY ? 0.f : m);
+                float sum = 0.f;
+                const lds_t at = here + (4 * half + ((lane & 15) >> 2)) * kRow + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * h + i], A.c, bias));
-                            sum += w[i];
-                        }
-                        cut3(w, part[h]);
-                    };
-                    auto multiply = [&](int h) {
+                for (int h = 0; h < 2 * NB; ++h) {                   // 16 keys
+                    float w[8];
 #pragma unroll
-                        for (int d = 0; d < kDims; ++d) {
-                            const u4_t a = transposed(at + 64 * d + 16 * h * kRow, at + 64 * d + (16 * h + 8) * kRow);
+                    for (int i = 0; i < 8; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h / 2][8 * (h % 2) + i], A.c, bias));
+                        sum += w[i];
+                    }
+                    u4_t part[3];
+                    cut3(w, part);
 #pragma unroll
-                            for (int n = 2; n >= 0; --n)
-                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[h][n]), o[d], 0, 0, 0);
-                        }
-                    };
-                    const f16_t next = scores(step, q, half);        // (of no keys behind the last step, and not looked at)
-                    weigh(0);
-                    weigh(1);
-                    multiply(0);
-                    multiply(1);
-                    add_weights(sum, l, l_rest);
-                    s = next;
+                    for (int d = 0; d < kDims; ++d) {
+                        const u4_t a = transposed(at + 64 * d + 16 * h * kRow, at + 64 * d + (16 * h + 8) * kRow);
+#pragma unroll
+                        for (int n = 2; n >= 0; --n)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, part[n]), o[d], 0, 0, 0);
+                    }
                 }
-                load_keys(key + 2 * kKeys, col, keys_at, step);
-                turn_values(turned, lds + buffer * (kKeys * kRow));
-                load_values(key + 2 * kKeys, values_at, turned);
-                if (now && mine(key + kKeys)) look(key + kKeys, there);
-                __syncthreads();
+                add_weights(sum, l, l_rest);
             }
         }
         float z = 0.f;
@@ -774,6 +761,7 @@ __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_atten
         const int steps = whole ? 1 : find_run(H, A, deal, run, at, t);
         if (steps == 0) return;
         at += steps;
+        if (!whole && !t.mine) continue;
         int thread = threadIdx.x;
         asm volatile("" : "+v"(thread));                             // (what follows from it is worked out for each tile: kept from one to the next it would be spilled)
         AttnMx<HD> a(A, X, t, kvh, thread, (lds_t)smem);

@@ -50,6 +50,7 @@ struct AttnTile {
     int seq;
     int lo, hi;
     int cuts, slot;              // pieces of its keys; where the first one's (this one's) state goes
+    bool mine;                   // of a run: it has a part of the tile's keys, not only of what the tile costs besides
     // With first positions that stay visible the keys are numbered on: positions 0 .. head_end - 1 as 0 .. head - 1 (whole steps of 64, so that no step of the
     // kernels has keys of both), then the window's, `jump` further on.  All rows see of the former what lies before them, of the latter what is in their window.
     int head, head_end, jump;
@@ -238,13 +239,16 @@ __device__ __forceinline__ bool find_piece(const Lens& H, const AttnArgs& A, int
 // sequences with at most 32 rows), one after the other, are cut into runs of equal length: a run may have the end of one tile, whole ones and the beginning of another, to
 // which its workgroup turns one after the other.  Long tiles are cut into pieces by themselves, with their share of the workgroups, one piece each.  Parts of tiles
 // have slots as pieces have: a long tile's piece its number, a run's part the number of its workgroup plus that of its tile.
+// A tile costs its workgroup more than its steps: its rows, page ids and first keys come one trip to memory after the other, and the states of the wavefronts meet at its end (9 us, a step
+// 1.6), so in a run it counts as so many steps more.
+constexpr int kTurn = 5;
 struct Deal {
     int tall;                    // workgroups for pieces of long tiles; -1: every tile is one workgroup's
     int tall_steps, run_steps;   // 128 keys each: of a piece, of a run
 };
 __device__ __forceinline__ bool is_tall(const Lens& H, const Lanes& L) { return L.n * H.group > kKeyRows; }
 __device__ __forceinline__ int tall_tiles(const Lens& H, const Lanes& L) { return is_tall(H, L) ? L.tiles : 0; }
-__device__ __forceinline__ int short_steps(const Lens& H, const Lanes& L) { return L.tiles > 0 && !is_tall(H, L) ? max(1, min(L.steps, 1 << 16)) : 0; }
+__device__ __forceinline__ int short_steps(const Lens& H, const Lanes& L) { return L.tiles > 0 && !is_tall(H, L) ? kTurn + max(1, min(L.steps, 1 << 16)) : 0; }
 // tall: what a step of a long tile takes, a short one's being 1
 __device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth least, float tall)
 {
@@ -281,7 +285,7 @@ __device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth leas
         }
     }
     if (runs) d.run_steps = max(1, (int)ceilf(steps / (float)(H.pieces - d.tall)));
-    const bool worth = (long_tiles > 0 && long_most - d.tall_steps >= least.tall) || (runs && most - d.run_steps >= (tiles * kv_heads >= 64 ? least.many : least.few));
+    const bool worth = (long_tiles > 0 && long_most - d.tall_steps >= least.tall) || (runs && most - kTurn - d.run_steps >= (tiles * kv_heads >= 64 ? least.many : least.few));
     return worth ? d : kWhole;
 }
 // behind the states: the deal, from the attention for the kernel that joins
@@ -332,7 +336,8 @@ __device__ __forceinline__ bool find_tall(const Lens& H, const AttnArgs& A, cons
     }
     return false;
 }
-// step `at` of the short tiles' and what follows of its tile up to the end of run number `run`; how many steps these are, 0: there are no more
+// Step `at` of the short tiles' and what follows of its tile up to the end of run number `run` (its first kTurn are no keys'); how many steps these are, 0: there
+// are no more.
 __device__ __forceinline__ int find_run(const Lens& H, const AttnArgs& A, const Deal& d, int run, int at, AttnTile& t)
 {
     Lanes L;
@@ -349,10 +354,11 @@ __device__ __forceinline__ int find_run(const Lens& H, const AttnArgs& A, const 
         const int lane = __ffsll((unsigned long long)__ballot(want < cum)) - 1, steps = __builtin_amdgcn_readlane(all, lane);
         const int x0 = want - __builtin_amdgcn_readlane(cum - all, lane), x1 = min(steps, x0 + (run + 1) * d.run_steps - at), start = at - x0;
         set_tile(A, L, s0, lane, 0, 1 << 24, t);
-        t.cuts = (start + steps - 1) / d.run_steps - start / d.run_steps + 1;
+        t.cuts = (start + steps - 1) / d.run_steps - (start + kTurn) / d.run_steps + 1;
         t.slot = d.tall + run + number + __popcll(tiles & ((1ull << lane) - 1));
-        const int begin = t.lo + 128 * x0;
-        t.hi = x1 == steps ? t.hi : min(t.hi, t.lo + 128 * x1);
+        t.mine = x1 > kTurn;
+        const int begin = t.lo + 128 * max(0, x0 - kTurn);
+        t.hi = x1 == steps ? t.hi : min(t.hi, t.lo + 128 * max(0, x1 - kTurn));
         t.lo = begin;
         return x1 - x0;
     }
@@ -380,8 +386,8 @@ __device__ __forceinline__ bool find_dealt_row(const Lens& H, const AttnArgs& A,
                 *in_tile = r - tile * kTileRows;
             } else {
                 const int start = before + __builtin_amdgcn_readlane(steps_cum - n, at);
-                t.cuts = (start + steps - 1) / d.run_steps - start / d.run_steps + 1;
-                t.slot = d.tall + start / d.run_steps + numbers + __popcll(tiles & ((1ull << at) - 1));
+                t.cuts = (start + steps - 1) / d.run_steps - (start + kTurn) / d.run_steps + 1;
+                t.slot = d.tall + (start + kTurn) / d.run_steps + numbers + __popcll(tiles & ((1ull << at) - 1));
                 *in_tile = r;
             }
             return true;
@@ -428,16 +434,19 @@ __device__ __forceinline__ bool find_row(const Lens& H, const AttnArgs& A, int r
 }
 __device__ __forceinline__ uint32_t high_halves(float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); }
 __device__ __forceinline__ float below_bf16(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-// eight floats as three times eight bf16 that sum up to them
+// two floats as three times two bf16 that sum up to them
+__device__ __forceinline__ void cut3_pair(float x0, float x1, u4_t (&part)[3], int i)
+{
+    const float y0 = below_bf16(x0), y1 = below_bf16(x1);
+    part[0][i] = high_halves(x0, x1);
+    part[1][i] = high_halves(y0, y1);
+    part[2][i] = high_halves(below_bf16(y0), below_bf16(y1));
+}
+// and eight
 __device__ __forceinline__ void cut3(const float (&x)[8], u4_t (&part)[3])
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = below_bf16(x0), y1 = below_bf16(x1);
-        part[0][i] = high_halves(x0, x1);
-        part[1][i] = high_halves(y0, y1);
-        part[2][i] = high_halves(below_bf16(y0), below_bf16(y1));
-    }
+    for (int i = 0; i < 4; ++i) cut3_pair(x[2 * i], x[2 * i + 1], part, i);
 }
 // eight floats in fp16's range as twice eight fp16, both to nearest: what is left is below 2^-24 of each, or 2^-25 where that is more
 __device__ __forceinline__ void cut2(const float (&x)[8], u4_t (&part)[2])
