@@ -1,12 +1,12 @@
 // The life of a cache's pages: who has which (tables, reference counts, lengths, all on the device), and copies of pages between caches.
 //
 //   page_drop_kernel, page_plan_kernel, page_fill_kernel     sequences get other lengths
-//   fork_plan_kernel, fork_rows_kernel, fork_store_kernel    sequences go on from what others have
+//   fork_plan_kernel, fork_tables_kernel (fork_rows_kernel, fork_store_kernel)      sequences go on from what others have
 //   compact_plan_kernel, compact_tables_kernel               used pages move to the front
 //   copy_pages_kernel                                        pages of one cache or two, of one type or two
 //
 // The lists are short next to the caches (a reference count for each page, an entry for each page of a sequence), so what counts is the number of dependent steps.  What
-// has to know all sequences or all pages in order - sums up to a sequence, the lowest free pages - is one workgroup that takes 16384 pages in a step; what
+// has to know all sequences or all pages in order - sums up to a sequence, the lowest free pages - is one workgroup that takes thousands of pages in a step; what
 // walks over the tables has a workgroup for 1024 entries.  Two or three launches a call, nothing that one workgroup waits for another for.  Counts change by
 // atomic additions of whole numbers, whose order changes nothing.
 #include "tship_internal.h"
@@ -69,39 +69,120 @@ __device__ __forceinline__ int64_t before_me(int64_t v, int64_t* all)
     return first + sum - v;
 }
 
-// 16 pages of a thread: which of them are as wanted, as bits
+// The lowest free pages.  A thread takes 16 pages that follow one another: only those that are free are gone through, which counts where a call wants many of them.
 constexpr int kScan = 16 * kPlanThreads;
-template <bool FREE>
-__device__ __forceinline__ uint32_t pages_here(const int32_t* references, int64_t p0, int64_t end)
+__device__ __forceinline__ uint32_t free_here(const int32_t* references, int p, int end)
 {
     uint32_t bits = 0;
-    if (p0 + 16 <= end) {
+    if (p < end - 15) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int4 r = *reinterpret_cast<const int4*>(references + p0 + 4 * i);
-            bits |= ((r.x <= 0) == FREE ? 1u : 0u) << (4 * i) | ((r.y <= 0) == FREE ? 2u : 0u) << (4 * i) | ((r.z <= 0) == FREE ? 4u : 0u) << (4 * i) |
-                ((r.w <= 0) == FREE ? 8u : 0u) << (4 * i);
+            const int4 r = *reinterpret_cast<const int4*>(references + p + 4 * i);
+            bits |= (uint32_t)((r.x <= 0) | (r.y <= 0) << 1 | (r.z <= 0) << 2 | (r.w <= 0) << 3) << (4 * i);
         }
     } else {
-        for (int i = 0; i < 16 && p0 + i < end; ++i) bits |= ((references[p0 + i] <= 0) == FREE ? 1u : 0u) << i;
+        for (int i = 0; i < 16 && p < end - i; ++i) bits |= (uint32_t)(references[p + i] <= 0) << i;
     }
     return bits;
 }
-// Calls each(number, page) for every page of [begin, end) (begin a multiple of 16) that is free (used), numbered from below, until `want` are found; returns how
-// many there are up to where it stopped.
-template <bool FREE, typename F>
-__device__ __forceinline__ int64_t find_pages(const int32_t* references, int64_t begin, int64_t end, int64_t want, F&& each)
+// Calls each(number, page) for the lowest `want` free pages or as many as there are; returns how many it found (perhaps some more).
+template <typename F>
+__device__ __forceinline__ int find_free(const int32_t* references, int pages, int want, F&& each)
 {
-    int64_t found = 0;
-    for (int64_t p = begin; p < end && found < want; p += kScan) {
-        const int64_t mine = p + 16 * (int64_t)threadIdx.x;
-        uint32_t bits = pages_here<FREE>(references, mine, end);
+    int found = 0;
+    for (int64_t p = 0; p < pages && found < want; p += kScan) {
+        const int64_t mine = p + 16 * (int)threadIdx.x;
+        uint32_t free = mine < pages ? free_here(references, (int)mine, pages) : 0;
         int64_t all;
-        int64_t number = found + before_me(__popc(bits), &all);
-        for (; bits != 0; bits &= bits - 1) each(number++, mine + __ffs(bits) - 1);
-        found += all;
+        int number = found + (int)before_me(__popc(free), &all);
+        for (; free != 0 && number < want; free &= free - 1) each(number++, (int)mine + __ffs(free) - 1);
+        found += (int)all;
     }
     return found;
+}
+
+// Pages in steps of up to 32768: wavefront w has 256 L of them that follow one another, lane i four of each 256, so that L loads of 16 bytes a lane are under way at once and lie
+// side by side.
+constexpr int kLoads = 8;
+struct Step {
+    int4 r[kLoads];              // references; -1 where there is no page
+    int loads;                   // L
+    int first;                   // this wavefront's
+};
+__device__ __forceinline__ int pages_in(int loads) { return loads * 256 * kPlanWaves; }
+__device__ __forceinline__ Step step_at(const int32_t* references, int begin, int end)
+{
+    Step t;
+    t.loads = max(0, min(kLoads, (end - begin + pages_in(1) - 1) / pages_in(1)));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    t.first = begin + wave * 256 * t.loads;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int p = t.first + 256 * i + 4 * lane;
+        t.r[i] = int4{-1, -1, -1, -1};
+        if (i < t.loads && p < end) {
+            if (p + 4 <= end) t.r[i] = *reinterpret_cast<const int4*>(references + p);
+            else {
+                t.r[i].x = references[p];
+                if (p + 1 < end) t.r[i].y = references[p + 1];
+                if (p + 2 < end) t.r[i].z = references[p + 2];
+            }
+        }
+    }
+    return t;
+}
+// four bits of each load: which pages are in use
+__device__ __forceinline__ uint32_t used_of(const Step& t)
+{
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) bits |= (uint32_t)((t.r[i].x > 0) | (t.r[i].y > 0) << 1 | (t.r[i].z > 0) << 2 | (t.r[i].w > 0) << 3) << (4 * i);
+    return bits;
+}
+__device__ __forceinline__ int wave_sum(int v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// of one number a wavefront: the sum of those before this one's, and of all
+__device__ __forceinline__ int waves_before(int mine, int* all)
+{
+    __shared__ int sums[kPlanWaves];
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    int first = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        if (w < (int)(threadIdx.x >> 6)) first += sums[w];
+        total += sums[w];
+    }
+    __syncthreads();
+    *all = total;
+    return first;
+}
+// Calls each(page, used, number of used pages before it) for every page of the step that exists; before: of the wavefronts before
+template <typename F>
+__device__ __forceinline__ void pages_of_step(const Step& t, uint32_t used, int before, int end, F&& each)
+{
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        if (i >= t.loads) break;
+        const uint32_t mine = (used >> (4 * i)) & 15;
+        int n = before;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t b = __ballot((mine >> j) & 1);
+            n = __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, n));
+            before += __popcll(b);
+        }
+        const int p = t.first + 256 * i + 4 * (threadIdx.x & 63);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (p + j < end) each(p + j, (mine >> j) & 1, n);
+            n += (mine >> j) & 1;
+        }
+    }
 }
 
 // ---- other lengths -------------------------------------------------------------------------------
@@ -156,9 +237,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PagePoolA
         need += all;
         copies += copies_here;
     }
-    const int64_t found = need == 0 ? 0 : find_pages<true>(P.references, 0, P.num_pages, need, [&](int64_t i, int64_t page) {
-        if (i < need) W.pages[i] = (int)page;
-    });
+    const int found = need == 0 ? 0 : find_free(P.references, P.num_pages, (int)min(need, (int64_t)INT32_MAX), [&](int i, int page) { W.pages[i] = page; });
     const bool fits = found >= need;
     for (int i = threadIdx.x; i < P.seqs; i += kPlanThreads)
         if (!fits || i >= copies) moves[2 * i] = moves[2 * i + 1] = -1;
@@ -199,76 +278,119 @@ __global__ void __launch_bounds__(kRowThreads) page_fill_kernel(const PagePoolAr
 
 // ---- forks ---------------------------------------------------------------------------------------
 
-// Maxima and minima are formed in the second-level cache: what they leave is read there too, once every wavefront's have arrived.
-__device__ __forceinline__ int seen(const int* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// Maxima and minima in memory are formed in the second-level cache: what they leave is read there too, once every wavefront's have arrived.
+template <bool LOCAL>
+__device__ __forceinline__ int seen(const int* at)
+{
+    return LOCAL ? *at : __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool LOCAL>
+__device__ __forceinline__ void put(int* at, int v)
+{
+    if constexpr (LOCAL) *at = v;
+    else __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 __device__ __forceinline__ void settled()
 {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
 }
 
-// One workgroup.  a: the sequence that each becomes; b: the lowest that becomes it; c: the fresh page in place of the begun one, -1: none; d: tokens before
+// One workgroup; LOCAL: what it works out of sequences fits LDS (4096 of them; through memory each of its steps is a trip there and back, 9.4 us for 32 sequences).  For the kernels behind
+// it a: the sequence that each becomes, c: the fresh page in place of the begun one, -1: none, d: tokens before
+constexpr int kLocal = 4096;
+template <bool LOCAL>
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolArgs P, const int32_t* children, const int32_t* parents, int count,
                                                                  int32_t* moves, int32_t* missing)
 {
+    extern __shared__ int local[];
     const Scratch W = scratch_of(P);
+    // of: that each becomes; low: the lowest that becomes it; tokens and begun page before
+    int *of_all = LOCAL ? local : W.a, *low = LOCAL ? local + kLocal : W.b, *tokens = LOCAL ? local + 2 * kLocal : W.d, *begun = LOCAL ? local + 3 * kLocal : W.c;
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        __hip_atomic_store(W.a + s, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(W.b + s, P.seqs, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        W.d[s] = P.context_lens[s];
+        put<LOCAL>(of_all + s, -1);
+        put<LOCAL>(low + s, P.seqs);
+        const int n = P.context_lens[s], held = pages_of(P, n);
+        int page = -1;
+        if (held > 0 && n % P.page_size != 0 && n <= (int64_t)P.max_pages * P.page_size) page = P.table[s * P.table_stride + held - 1];
+        tokens[s] = n;
+        begun[s] = is_page(P, page) ? page : -1;
     }
     settled();
     for (int i = threadIdx.x; i < count; i += kPlanThreads)
-        if ((uint32_t)children[i] < (uint32_t)P.seqs && (uint32_t)parents[i] < (uint32_t)P.seqs) atomicMax(W.a + children[i], i);
+        if ((uint32_t)children[i] < (uint32_t)P.seqs && (uint32_t)parents[i] < (uint32_t)P.seqs) atomicMax(of_all + children[i], i);
     settled();
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        const int pair = seen(W.a + s), of = pair >= 0 ? parents[pair] : s;
-        __hip_atomic_store(W.a + s, of, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        atomicMin(W.b + of, s);
+        const int pair = seen<LOCAL>(of_all + s), of = pair >= 0 ? parents[pair] : s;
+        put<LOCAL>(of_all + s, of);
+        atomicMin(low + of, s);
     }
     settled();
     // (a parent that stays what it is keeps its begun page)
-    auto begun_page = [&](int of) -> int {
-        const int tokens = W.d[of], held = pages_of(P, tokens);
-        if (held == 0 || tokens % P.page_size == 0 || tokens > (int64_t)P.max_pages * P.page_size) return -1;
-        const int e = P.table[of * P.table_stride + held - 1];
-        return is_page(P, e) ? e : -1;
-    };
     int64_t need = 0;
     for (int s0 = 0; s0 < P.seqs; s0 += kPlanThreads) {
         const int s = s0 + threadIdx.x;
-        int copied = 0;
+        int copied = 0, of = 0;
         if (s < P.seqs) {
-            const int of = seen(W.a + s), keeper = seen(W.a + of) == of ? of : seen(W.b + of);
-            copied = keeper != s && begun_page(of) >= 0;
+            of = seen<LOCAL>(of_all + s);
+            const int keeper = seen<LOCAL>(of_all + of) == of ? of : seen<LOCAL>(low + of);
+            copied = keeper != s && begun[of] >= 0;
         }
         int64_t all;
         const int64_t number = need + before_me(copied, &all);
-        if (s < P.seqs) W.c[s] = copied ? (int)number : -1;
+        if (copied) moves[2 * number] = begun[of];                   // (as many as there are children at most)
+        if (s < P.seqs) W.rows[s] = copied ? (int)number : -1;       // (rows of the table come there later)
         need += all;
     }
-    const int64_t found = need == 0 ? 0 : find_pages<true>(P.references, 0, P.num_pages, need, [&](int64_t i, int64_t page) {
-        if (i < need) W.pages[i] = (int)page;
-    });
+    const int found = need == 0 ? 0 : find_free(P.references, P.num_pages, (int)need, [&](int i, int page) { moves[2 * i + 1] = page; });
     const bool fits = found >= need;
     if (threadIdx.x == 0) {
         W.head[0] = fits;
         missing[0] = fits ? 0 : (int)(need - found);
     }
+    settled();
     for (int i = threadIdx.x; i < count; i += kPlanThreads)
         if (!fits || i >= need) moves[2 * i] = moves[2 * i + 1] = -1;
-    __syncthreads();                                                 // (the list)
-    if (!fits) return;
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        const int number = W.c[s];
-        if (number < 0) continue;
-        const int page = W.pages[number];
-        W.c[s] = page;
-        moves[2 * number] = begun_page(seen(W.a + s));
-        moves[2 * number + 1] = page;
+        const int number = W.rows[s];
+        if constexpr (LOCAL) W.a[s] = of_all[s], W.d[s] = tokens[s];
+        W.c[s] = fits && number >= 0 ? moves[2 * number + 1] : -1;
     }
 }
 
+// Rows of up to 1024 sequences, a workgroup for 16 entries of all of them: what they become is read before any of it is written.
+constexpr int kForkEntries = 16, kForkRows = kPlanThreads / kForkEntries, kForkMost = 1024;
+__global__ void __launch_bounds__(kPlanThreads) fork_tables_kernel(const PagePoolArgs P)
+{
+    const Scratch W = scratch_of(P);
+    if (W.head[0] == 0) return;
+    const int j = blockIdx.x * kForkEntries + threadIdx.x % kForkEntries, s0 = threadIdx.x / kForkEntries;
+    int entry[kForkMost / kForkRows];
+    uint32_t changes = 0;
+#pragma unroll
+    for (int n = 0; n < kForkMost / kForkRows; ++n) {
+        const int s = s0 + n * kForkRows;
+        entry[n] = -1;
+        if (s >= P.seqs || j >= P.max_pages) continue;
+        const int of = W.a[s];
+        if (of == s) continue;
+        changes |= 1u << n;
+        const int before = pages_of(P, W.d[s]), held = pages_of(P, W.d[of]), fresh = W.c[s];
+        if (j < held) entry[n] = fresh >= 0 && j == held - 1 ? fresh : P.table[of * P.table_stride + j];
+        const int old = j < before ? P.table[s * P.table_stride + j] : -1;
+        if (entry[n] == old) continue;
+        if (is_page(P, entry[n])) atomicAdd(P.references + entry[n], 1);
+        if (is_page(P, old)) atomicAdd(P.references + old, -1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < kForkMost / kForkRows; ++n) {
+        const int s = s0 + n * kForkRows;
+        if (!((changes >> n) & 1)) continue;
+        P.table[s * P.table_stride + j] = entry[n];
+        if (j == 0) P.context_lens[s] = W.d[W.a[s]];
+    }
+}
 // grid (chunks of entries, sequences): the rows of those that change, and the counts; the table stays as it is until all rows are read
 __global__ void __launch_bounds__(kRowThreads) fork_rows_kernel(const PagePoolArgs P)
 {
@@ -300,40 +422,48 @@ __global__ void __launch_bounds__(kRowThreads) fork_store_kernel(const PagePoolA
 
 // ---- compaction ----------------------------------------------------------------------------------
 
-// One workgroup: the holes below the number of used pages, then the used pages from there on, of which the last goes into the first hole.  pages[p]: where page p
-// is afterwards (from that number on)
+// One workgroup.  With U pages in use and n of them before page p, a free page p < U is hole number p - n, and a page p >= U in use goes into hole number U - 1 - n (the last
+// one into the first hole), so that each finds its place in the list by itself.  pages[p]: where page p is afterwards (from U on)
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePoolArgs P, int32_t* moves, int max_moves)
 {
     const Scratch W = scratch_of(P);
-    for (int i = threadIdx.x; i < max_moves; i += kPlanThreads) moves[2 * i] = moves[2 * i + 1] = -1;
-    int64_t mine = 0, used;
-    for (int64_t p = 16 * (int64_t)threadIdx.x; p < P.num_pages; p += kScan) mine += __popc(pages_here<false>(P.references, p, P.num_pages));
-    before_me(mine, &used);                                          // (and the list is cleared)
-    if (threadIdx.x == 0) W.head[1] = (int)used;
-    const int64_t holes = find_pages<true>(P.references, 0, used, INT64_MAX, [&](int64_t i, int64_t page) {
-        if (i < max_moves) moves[2 * i + 1] = (int)page;
-    });
-    __syncthreads();
-    // (the scan begins at a multiple of 16: pages below the number that are used are passed over)
-    const int64_t begin = used & ~(int64_t)15;
-    int64_t skipped;
-    before_me(threadIdx.x < 16 && begin + threadIdx.x < used ? P.references[begin + threadIdx.x] > 0 : 0, &skipped);
-    for (int64_t p = begin; p < P.num_pages; p += kScan) {           // (all pages keep their place but for those that follow)
-        const int64_t at = p + 16 * (int64_t)threadIdx.x;
-        for (int i = 0; i < 16; ++i)
-            if (at + i < P.num_pages) W.pages[at + i] = (int)(at + i);
+    const Step first = step_at(P.references, 0, P.num_pages);
+    int used = 0, all;
+    waves_before(wave_sum(__popc(used_of(first))), &used);
+    for (int p = pages_in(first.loads); p < P.num_pages;) {
+        const Step t = step_at(P.references, p, P.num_pages);
+        waves_before(wave_sum(__popc(used_of(t))), &all);
+        used += all;
+        p += pages_in(t.loads);
     }
-    __syncthreads();
-    find_pages<false>(P.references, begin, P.num_pages, INT64_MAX, [&](int64_t i, int64_t page) {
-        const int64_t k = holes - 1 - (i - skipped);
-        if (page < used || k < 0 || k >= max_moves) return;
-        const int to = moves[2 * k + 1];
-        moves[2 * k] = (int)page;
-        W.pages[page] = to;
-        P.references[to] = P.references[page];
-        P.references[page] = 0;
-    });
-    // (pages that stay, as there is no room in the list: their holes are taken out of it already, by number)
+    int n = 0, above = 0;                                            // above: of this lane's pages, those in use from U on
+    for (int p = 0; p < P.num_pages;) {
+        const Step t = p == 0 ? first : step_at(P.references, p, P.num_pages);
+        const uint32_t bits = used_of(t);
+        const int before = waves_before(wave_sum(__popc(bits)), &all);
+        pages_of_step(t, bits, n + before, P.num_pages, [&](int page, bool is_used, int k) {
+            if (page < used && !is_used && page - k < max_moves) moves[2 * (page - k) + 1] = page;
+            if (page >= used && is_used && used - 1 - k < max_moves) moves[2 * (used - 1 - k)] = page;
+            if (page >= used) W.pages[page] = page;
+            above += page >= used && is_used;
+        });
+        n += all;
+        p += pages_in(t.loads);
+    }
+    int count;
+    waves_before(wave_sum(above), &count);                           // (and what has been written is there)
+    settled();
+    for (int i = threadIdx.x; i < max_moves; i += kPlanThreads) {
+        if (i >= count) {
+            moves[2 * i] = moves[2 * i + 1] = -1;
+            continue;
+        }
+        const int from = moves[2 * i], to = moves[2 * i + 1];
+        W.pages[from] = to;
+        P.references[to] = P.references[from];
+        P.references[from] = 0;
+    }
+    if (threadIdx.x == 0) W.head[1] = used;
 }
 
 // grid (chunks of entries, sequences)
@@ -391,20 +521,20 @@ __device__ __forceinline__ void store8(char* at, const float (&x)[8])
 
 constexpr int kCopyThreads = 256, kCopyUnits = 4;
 
-// grid (pairs, chunks of a page, keys and values): a lane takes eight values of a row, 16 bytes of a 16-bit cache, so that lanes side by side take what lies side by
-// side; four lanes have a block of a cache in four bits.  Four of them at once, so that their loads are under way together.  Bound: memory.
+// A lane takes eight values of a row, 16 bytes of a 16-bit cache, so that lanes side by side take what lies side by side; four lanes have a block of a cache in four bits.
+// Four of them at once, so that their loads are under way together.  Workgroups go through the items (pair, chunk of a page, keys or values) in turn: lists have room for more
+// pairs than there mostly are, and a workgroup for each of those that are not there took 7 of 25 us (350 of 1543 pairs).  Bound: memory (400 pages of 64 x 8 x 128 from bf16 into
+// four bits or back, 133 MB: 21 us, 6.2 TB/s).
 template <typename S, typename D>
-__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const int32_t* moves, const PageCopyArgs A)
+__device__ __forceinline__ void copy_chunk(const PageCopyArgs& A, int from, int to, uint32_t chunk, bool values)
 {
-    const int from = moves[2 * (int64_t)blockIdx.x], to = moves[2 * (int64_t)blockIdx.x + 1];
-    if ((uint32_t)from >= (uint32_t)A.src_pages || (uint32_t)to >= (uint32_t)A.dst_pages || (A.same && from == to)) return;
-    const PageRows &s = A.src[blockIdx.z], &d = A.dst[blockIdx.z];
+    const PageRows &s = A.src[values], &d = A.dst[values];
     constexpr bool from4 = std::is_same<S, MX4>::value, to4 = std::is_same<D, MX4>::value;
     const char* src = s.at + from * s.page;
     char* dst = d.at + to * d.page;
 #pragma unroll
     for (int n = 0; n < kCopyUnits; ++n) {
-        const uint32_t unit = (blockIdx.y * kCopyUnits + n) * kCopyThreads + threadIdx.x;
+        const uint32_t unit = (chunk * kCopyUnits + n) * kCopyThreads + threadIdx.x;
         if (unit >= A.units) break;
         const uint32_t row = A.by_row.quot(unit), u = unit - row * A.by_row.d;
         const uint32_t outer = A.by_inner.quot(row), inner = row - outer * A.by_inner.d;
@@ -438,6 +568,17 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const int32_t*
     }
 }
 
+template <typename S, typename D>
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const int32_t* moves, const PageCopyArgs A)
+{
+    for (uint32_t item = blockIdx.x; item < A.items; item += gridDim.x) {
+        const uint32_t pair = A.by_chunks.quot(item), rest = item - pair * A.by_chunks.d;
+        const int from = moves[2 * (int64_t)pair], to = moves[2 * (int64_t)pair + 1];
+        if ((uint32_t)from >= (uint32_t)A.src_pages || (uint32_t)to >= (uint32_t)A.dst_pages || (A.same && from == to)) continue;
+        copy_chunk<S, D>(A, from, to, rest >> 1, rest & 1);
+    }
+}
+
 dim3 row_grid(const PagePoolArgs& P) { return dim3((P.max_pages + kRowEntries - 1) / kRowEntries, P.seqs); }
 
 }  // namespace
@@ -457,8 +598,18 @@ bool launch_resize_sequences(const PagePoolArgs& P, const int32_t* lengths, int3
 bool launch_fork_sequences(const PagePoolArgs& P, const int32_t* children, const int32_t* parents, int count, int32_t* moves, int32_t* missing,
                            hipStream_t stream)
 {
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, P, children, parents, count, moves, missing);
+    if (P.seqs <= kLocal) {
+        constexpr size_t lds = 4 * kLocal * sizeof(int);
+        if (!raise_lds_limit(reinterpret_cast<const void*>(fork_plan_kernel<true>), lds)) return false;
+        hipLaunchKernelGGL(fork_plan_kernel<true>, dim3(1), dim3(kPlanThreads), lds, stream, P, children, parents, count, moves, missing);
+    } else {
+        hipLaunchKernelGGL(fork_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, stream, P, children, parents, count, moves, missing);
+    }
     if (!hip_ok(hipGetLastError(), "fork_sequences launch")) return false;
+    if (P.seqs <= kForkMost) {
+        hipLaunchKernelGGL(fork_tables_kernel, dim3((P.max_pages + kForkEntries - 1) / kForkEntries), dim3(kPlanThreads), 0, stream, P);
+        return hip_ok(hipGetLastError(), "fork_sequences launch");
+    }
     hipLaunchKernelGGL(fork_rows_kernel, row_grid(P), dim3(kRowThreads), 0, stream, P);
     if (!hip_ok(hipGetLastError(), "fork_sequences launch")) return false;
     hipLaunchKernelGGL(fork_store_kernel, row_grid(P), dim3(kRowThreads), 0, stream, P);
@@ -484,13 +635,16 @@ static auto copy_kernel_to(int type)
     }
 }
 
-bool launch_copy_pages(const int32_t* moves, int count, const PageCopyArgs& args, int src_type, int dst_type, hipStream_t stream)
+bool launch_copy_pages(const int32_t* moves, int count, PageCopyArgs args, int src_type, int dst_type, hipStream_t stream)
 {
-    const dim3 grid(count, (args.units + kCopyThreads * kCopyUnits - 1) / (kCopyThreads * kCopyUnits), 2);
-    if (grid.y > 65535) {
-        set_last_error("copy_pages: pages are too large.");
+    const int64_t chunks = 2 * (((int64_t)args.units + kCopyThreads * kCopyUnits - 1) / (kCopyThreads * kCopyUnits)), items = chunks * count;
+    if (items > INT32_MAX) {
+        set_last_error("copy_pages: too many pages for one call.");
         return false;
     }
+    args.items = (uint32_t)items;
+    args.by_chunks = FastDiv((uint32_t)chunks);
+    const dim3 grid((unsigned)std::min<int64_t>(items, 16 * device_info().num_cus));
     const auto kern = src_type == kTypeF32 ? copy_kernel_to<F32>(dst_type)
         : src_type == kTypeF16             ? copy_kernel_to<F16>(dst_type)
         : src_type == kTypeBF16            ? copy_kernel_to<BF16>(dst_type)

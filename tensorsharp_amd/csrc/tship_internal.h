@@ -395,8 +395,10 @@ struct PageCopyArgs {
     bool same;                     // src is dst
     uint32_t units;                // of eight values, in a page
     FastDiv by_row, by_inner;      // units of a row, rows of an outer one
+    uint32_t items;                // pairs x chunks of a page x keys and values, set by the launch
+    FastDiv by_chunks;
 };
-bool launch_copy_pages(const int32_t* moves, int count, const PageCopyArgs& args, int src_type, int dst_type, hipStream_t stream);
+bool launch_copy_pages(const int32_t* moves, int count, PageCopyArgs args, int src_type, int dst_type, hipStream_t stream);
 
 constexpr int kMaxSampleVocab = 1 << 20;
 size_t sample_ws_bytes(int rows, int vocab);

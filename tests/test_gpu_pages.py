@@ -66,8 +66,9 @@ class Pool:
 
 
 # sequences, entries of a table, tokens of a page, pages: one of each; a few; more sequences than a workgroup has threads; more pages than a step of the
-# scan; rows of a table longer than a workgroup's part
-SIZES = [(1, 1, 1, 1), (1, 7, 16, 9), (3, 5, 4, 16), (17, 9, 1, 60), (40, 30, 16, 900), (1500, 4, 8, 4001), (70, 300, 2, 17001), (3, 2500, 2, 40000)]
+# scan; rows of a table longer than a workgroup's part; more sequences than fit a workgroup's memory; pages up to the end of a step
+SIZES = [(1, 1, 1, 1), (1, 7, 16, 9), (3, 5, 4, 16), (17, 9, 1, 60), (40, 30, 16, 900), (1500, 4, 8, 4001), (70, 300, 2, 17001), (3, 2500, 2, 40000),
+         (5000, 3, 4, 9999), (1024, 5, 16, 4096), (30, 2200, 1, 70002), (9, 900, 3, 32768)]
 
 
 @pytest.mark.parametrize("seqs,room,page,pages", SIZES)
