@@ -3008,7 +3008,7 @@ bool validate_rope(const TSHipRope* r, int head_dim, RopeSpec* out)
         out->range = std::max(0.001, std::min(r->dims - 1.0, std::ceil(pair(r->beta_slow))) - out->low);
         size *= 1.0 + 0.1 * std::log(1.0 / r->freq_scale);
     }
-    out->size = (float)size;
+    out->size = size;
     return true;
 }
 

@@ -24,17 +24,20 @@ namespace {
 
 // cosine and sine of pair i at a position.  The angle is formed in 64 bits and brought to revolutions in -1/2 .. 1/2 there: at position
 // 10^6 an angle of 32 bits is 0.03 radians off.  What is left loses nothing in 32 bits.
-__device__ __forceinline__ f2_t turn_of(const RopeSpec& R, int pair, int position)
+__device__ __forceinline__ double turns_of(const RopeSpec& R, int pair, int position)
 {
     double f = exp2(R.step * pair);
     if (R.factors) f /= (double)R.factors[pair];
     const double kept = R.ext == 0.0 ? 0.0 : R.ext * (1.0 - fmin(1.0, fmax(0.0, (pair - R.low) / R.range)));
     f *= R.freq_scale * (1.0 - kept) + kept;
-    double turns = (double)position * (f * 0.15915494309189533577);
-    turns -= rint(turns);
+    const double turns = (double)position * (f * 0.15915494309189533577);
+    return turns - rint(turns);
+}
+__device__ __forceinline__ f2_t turn_of(const RopeSpec& R, int pair, int position)
+{
     float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
-    return f2_t{c * R.size, s * R.size};
+    sincospif(2.0f * (float)turns_of(R, pair, position), &s, &c);
+    return f2_t{c * (float)R.size, s * (float)R.size};
 }
 
 // Four dimensions of a head that one lane holds: lane u < dims / 4 the pairs 2u and 2u + 1, the lanes behind them four dimensions
@@ -206,12 +209,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_kernel(const float* q
 
 // The same into a cache in four bits.  What a key or value head becomes goes through LDS, since the lanes that turn pairs do not hold neighbours: then a lane
 // has eight values that follow one another, four lanes a block, whose largest magnitude they find among them.
+// Keys are normed and turned in 64 bits: a code is a step of a quarter to a half of a value, so that an error of 2^-22 on one side of a border is one of 1e-4 over all
+// keys of a store (three prompts of 2048 tokens, 3.6 million values: one or two of them); in 64 bits the code is that of the exact value but where that is within 2^-25 of
+// a border.  Queries, which are not rounded further, stay in 32 bits.
 template <int LANES>
 __global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int heads,
                                                                      const int32_t* positions, const float* q_norm, const float* k_norm,
                                                                      float eps, const PagedKv C, const MxScales X, const RopeSpec R)
 {
     __shared__ f2_t turns[kMaxDim / 2];
+    __shared__ double2 exact_turns[kMaxDim / 2];
     constexpr int kHeads = kRopeThreads / LANES;
     __shared__ __attribute__((aligned(16))) float heads_here[kHeads][4 * LANES];
     const int t = blockIdx.x;
@@ -223,7 +230,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float
     const int position = positions ? positions[t] : where;
     int within = 0;
     const int page = where >= 0 ? page_of(C, at.seq, where, &within) : -1;
-    if ((int)threadIdx.x < R.dims / 2) turns[threadIdx.x] = turn_of(R, threadIdx.x, position);
+    if ((int)threadIdx.x < R.dims / 2) {
+        double s, c;
+        sincospi(2.0 * turns_of(R, threadIdx.x, position), &s, &c);
+        exact_turns[threadIdx.x] = {c * R.size, s * R.size};
+        turns[threadIdx.x] = f2_t{(float)(c * R.size), (float)(s * R.size)};
+    }
     __syncthreads();
     for (int h0 = blockIdx.y * kHeads; h0 < all; h0 += gridDim.y * kHeads) {
         const int h = h0 + slot;
@@ -238,21 +250,42 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float
                 q = load_quad(src, R, u);
             }
         }
-        const float* norm = h < heads ? q_norm : k_norm;
-        if (q_norm || k_norm) {                                      // uniform
-            float ss = q.a.x * q.a.x + q.a.y * q.a.y + q.b.x * q.b.x + q.b.y * q.b.y;
+        if (h0 < heads) {                                            // uniform, as all that leads to sums over lanes
+            if (q_norm) {
+                float ss = q.a.x * q.a.x + q.a.y * q.a.y + q.b.x * q.b.x + q.b.y * q.b.y;
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-            if (here && !is_v && norm) {
-                const float by = 1.0f / sqrtf(ss / (float)dim + eps);
-                const Quad w = load_quad(norm, R, u);
-                q = {q.a * by * w.a, q.b * by * w.b};
+                for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+                if (here && h < heads) {
+                    const float by = 1.0f / sqrtf(ss / (float)dim + eps);
+                    const Quad w = load_quad(q_norm, R, u);
+                    q = {q.a * by * w.a, q.b * by * w.b};
+                }
             }
+            if (here && h < heads) store_quad(query + t * ld_query + (int64_t)h * dim, turned(q, R, u, turns), R, u);
         }
-        if (here) {
-            if (h < heads) store_quad(query + t * ld_query + (int64_t)h * dim, turned(q, R, u, turns), R, u);
-            else if (is_v) put4(&heads_here[slot][4 * u], q.a.x, q.a.y, q.b.x, q.b.y);
-            else store_quad(&heads_here[slot][0], turned(q, R, u, turns), R, u);
+        if (h0 + kHeads > heads) {
+            double x[4] = {q.a.x, q.b.x, q.a.y, q.b.y};              // pairs (0, 1) and (2, 3)
+            if (k_norm) {
+                double ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+                if (here && h >= heads && !is_v) {
+                    const double by = 1.0 / sqrt(ss / dim + (double)eps);
+                    const Quad w = load_quad(k_norm, R, u);
+                    x[0] *= by * w.a.x, x[1] *= by * w.b.x, x[2] *= by * w.a.y, x[3] *= by * w.b.y;
+                }
+            }
+            if (here && is_v) {
+                put4(&heads_here[slot][4 * u], q.a.x, q.a.y, q.b.x, q.b.y);
+            } else if (here && h >= heads) {
+                if (4 * u < R.dims) {
+                    const double2 t0 = exact_turns[2 * u], t1 = exact_turns[2 * u + 1];
+                    const double y0 = x[0] * t0.x - x[1] * t0.y, y2 = x[2] * t1.x - x[3] * t1.y;
+                    x[1] = x[0] * t0.y + x[1] * t0.x, x[3] = x[2] * t1.y + x[3] * t1.x;
+                    x[0] = y0, x[2] = y2;
+                }
+                store_quad(&heads_here[slot][0], Quad{f2_t{(float)x[0], (float)x[2]}, f2_t{(float)x[1], (float)x[3]}}, R, u);
+            }
         }
         if (page < 0 || h0 + kHeads <= heads) continue;              // uniform
         __syncthreads();

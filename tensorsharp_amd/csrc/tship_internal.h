@@ -319,8 +319,7 @@ __host__ __device__ constexpr int first_key(int p, int window) { return window >
 struct RopeSpec {
     int dims;                  // leading dimensions of a head that are turned, a multiple of 4
     int mode;                  // 0: adjacent pairs, 2: pairs half of dims apart
-    double step, freq_scale, ext, low, range;
-    float size;
+    double step, freq_scale, ext, low, range, size;
     const float* factors;      // device, dims / 2 of them, optional
 };
 

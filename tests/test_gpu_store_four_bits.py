@@ -1,7 +1,8 @@
 """New keys and values into a cache in four bits, against 64 bits.
 
-Values are stored as they come: codes and scales are equal.  A turned pair is 6e-7 of its length off, 7e-7 of it and of each value more with a norm
-(test_gpu_rope.py), so that a key's code or scale may be that of a value so far away where a border lies between them."""
+Values are stored as they come: codes and scales are equal.  Keys are normed and turned in 64 bits and rounded to 32 once, so that a key's code or scale
+may be that of a value 2^-24 of its own away (of a turned pair's length; 1 % more for what 64 bits leave) where a border lies between them.  A query is 6e-7
+of its pair's length off, 7e-7 of it and of each value more with a norm (test_gpu_rope.py)."""
 import numpy as np
 import pytest
 
@@ -57,6 +58,7 @@ def test_store(hip, heads, kv, dim, dims, mode, scaling, normed, page, order, ga
         if stored is None:
             assert np.all(np.abs(got - ref) <= room)
         else:
+            room = 1.01 * 2.0 ** -24 * np.maximum(size * lengths(y, dims, mode), np.abs(y))
             assert mx.holds(*stored, ref, room.reshape(*room.shape[:-1], -1, 32).max(-1))
     check(query.cpu().numpy()[:rows].reshape(rows, heads, dim), parts[:, :heads], qn)
     assert torch.all(query[rows:] == 7.5)
