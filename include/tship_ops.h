@@ -564,7 +564,8 @@ TSHIP_EXPORT int TSHip_CompactPagesDevice(const TSHipPagePool* pool, int32_t* mo
 
 /* Page moves[i].to of dst becomes page moves[i].from of src, keys and values (moves: device, count pairs; one outside the pages is left out).  The caches
  * have one page size, number of heads and head_dim; types may differ (rounded as above).  src may be dst; of the pages that are written none may be
- * read or written by another pair.  The page tables are not used. */
+ * read or written by another pair.  Caches that are not the same may not overlap, from their first to their last page.  A page has at most 2^29 values of
+ * keys; count times those, in pieces of 8192, is below 2^30.  The page tables are not used. */
 TSHIP_EXPORT int TSHip_CopyPagesDevice(const TSHipPagedCache* dst, const TSHipPagedCache* src, const int32_t* moves, int count);
 
 /* One token for each row of logits [rows x vocab] (vocab up to 2^20); every other pointer is a device array with one entry per row.
