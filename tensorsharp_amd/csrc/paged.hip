@@ -1177,8 +1177,10 @@ PagedAttnPlan plan_paged_attention(int rows, int heads, const PagedKv& cache, in
     PagedAttnPlan plan{};
     // (a sequence of at most 32 rows has one tile, others a tile per 128 rows begun: no more than this, whatever the lengths)
     const int64_t tiles = all / kTileRows + std::min<int64_t>(cache.seqs, rows);
-    // workgroups that are resident at once
-    const int at_once = device_info().num_cus * (dim <= 64 && cache.element_type != kTypeF32 ? 3 : dim <= 128 ? 2 : 1);
+    // workgroups that are resident at once (three would need 170 registers, four bits take 231: 16 answers of 64 dimensions over up to 4096 positions in pieces for
+    // three 36 us, for two 29)
+    const bool three = dim <= 64 && (cache.element_type == kTypeF16 || cache.element_type == kTypeBF16);
+    const int at_once = device_info().num_cus * (three ? 3 : dim <= 128 ? 2 : 1);
     const int64_t pieces = std::min(kMaxPieces, std::max(1, at_once / cache.kv_heads)), keys = (int64_t)cache.max_pages * cache.page.d;
     const int64_t most = std::min<int64_t>(keys, window > 0 ? (int64_t)window + first : keys);
     const int hd = dims_of(dim);

@@ -731,7 +731,9 @@ struct AttnMx {
     }
 };
 
-constexpr float kTall = 3.f;                                         // what a step of a long tile takes, a short one's being 1
+// What a step of a long tile takes, a short one's being 1.  (A prompt's chunk beside two dozen answers: 1.5 to 4.5 are within 3 % of each other but for 256
+// dimensions, 257 us at 1.5 and 147 from 2.2 on.)
+constexpr float kTall = 3.f;
 
 // grid (KV heads, workgroups)
 template <int HD>

@@ -111,7 +111,7 @@ struct Lanes {
 // Steps of 128 keys that pieces have to save a tile to be worth it.  Joining them takes 5 us where they are few, 8.5 for many short tiles, 7.5
 // for long ones (3 of it the second launch, which comes wherever the page table has room for as many positions).  A step takes a short tile of
 // 64, 128, 256 dimensions 1.0, 1.4, 2.9 us in fp16 (bf16 0.9, 1.6, 3.5; fp32, by fewer wavefronts, 2.1, 8.4, 19.3) and a long one 2.6, 4.4,
-// 8.7 (bf16 4.1, 5.6, 12.2; fp32 7.4, 12.5, 29.5): by the dimensions, near enough.  One sequence of 512 keys, 256 dimensions and 8 KV heads: cut
+// 8.7 (bf16 4.1, 5.6, 12.2; fp32 7.4, 12.5, 29.5; four bits nearly as fp16): by the dimensions, near enough.  One sequence of 512 keys, 256 dimensions and 8 KV heads: cut
 // 37 us, uncut 90 in fp32, 18 and 22 in fp16; 16 of 128 dimensions in fp16: 17 and 13.
 struct Worth {
     int few, many, tall;
