@@ -267,8 +267,8 @@ struct AttnMx {
     // ---- few rows: every wavefront over keys of its own, 16 rows at a time ----
     static constexpr int kChunks = (HD + 127) / 128, kTiles = HD / 16;
 
-    // A step of 16 KB keys: key idx of each 16, block 4 c + g of it
-    template <int KB>
+    // A step of 16 KB keys (64 in place of 32: 86 us for 80 of 32 answers, fewer of them under way): key idx of each 16, block 4 c + g of it
+    static constexpr int KB = 2;
     struct Step {
         u4_t k[KB][kChunks], v[KB][kChunks];
         uint8_t ks[KB][kChunks], vs[KB][kChunks];                    // (as loaded: widened ahead of their use they would be waited for)
@@ -278,16 +278,15 @@ struct AttnMx {
     struct Blocks {
         uint64_t k[kChunks], v[kChunks], ks[kChunks], vs[kChunks];
     };
-    template <int KB>
-    __device__ __forceinline__ void load_step(int key, int idx, const Blocks& of, Step<KB>& s)
+    __device__ __forceinline__ void load_step(int key, int idx, const Blocks& of, Step& s)
     {
         const int p0 = t.position(key);
         bring_pages(p0, 16 * KB);
-        if (X.alike) load_rows<KB, true>(p0, t.end_at(key), idx, of, s);
-        else load_rows<KB, false>(p0, t.end_at(key), idx, of, s);
+        if (X.alike) load_rows<true>(p0, t.end_at(key), idx, of, s);
+        else load_rows<false>(p0, t.end_at(key), idx, of, s);
     }
-    template <int KB, bool ALIKE>
-    __device__ __forceinline__ void load_rows(int p0, int end, int idx, const Blocks& of, Step<KB>& s) const
+    template <bool ALIKE>
+    __device__ __forceinline__ void load_rows(int p0, int end, int idx, const Blocks& of, Step& s) const
     {
         s.there = 0;
 #pragma unroll
@@ -311,7 +310,6 @@ struct AttnMx {
     }
 
     // rows r0 .. r0 + 15 of the tile; whether these have to be done by plainly()
-    template <int KB>
     __device__ __forceinline__ bool own_keys(int r0)
     {
         __shared__ f2_t states[kAttnWaves][16];
@@ -326,7 +324,7 @@ struct AttnMx {
         int key = t.lo + 16 * KB * wave;
         id_base = -64;                                               // (the keys of the rows before are begun again)
         constexpr int kStride = 16 * KB * kAttnWaves;
-        constexpr uint64_t kWhole = KB == 4 ? ~0ull : (1ull << (16 * KB)) - 1;
+        constexpr uint64_t kWhole = (1ull << (16 * KB)) - 1;
         if (key < t.hi) {
             Blocks of;
 #pragma unroll
@@ -338,7 +336,7 @@ struct AttnMx {
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) load_row(row, 4 * c + g, x[c]);
             asm volatile("" ::: "memory");
-            Step<KB> even, odd_one;
+            Step even, odd_one;
             load_step(key, idx, of, even);
             asm volatile("" ::: "memory");
             load_step(key + kStride, idx, of, odd_one);
@@ -349,7 +347,7 @@ struct AttnMx {
             int token, head;
             place(min(row, t.count - 1), &token, &head);
             const int p = t.p0 + token, lo = first_key(p, A.window), lo_last = first_key(t.p0 + t.tokens - 1, A.window);
-            auto step = [&](Step<KB>& now) {
+            auto step = [&](Step& now) {
                 const int p0 = t.position(key);
                 const bool whole = now.there == kWhole, in_head = key < t.head;
                 if constexpr (HD != 128) {                           // (lanes without a block have another's, for which rows have zeros: NaN would stay one)
@@ -768,7 +766,7 @@ __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_atten
         asm volatile("" : "+v"(thread));                             // (what follows from it is worked out for each tile: kept from one to the next it would be spilled)
         AttnMx<HD> a(A, X, t, kvh, thread, (lds_t)smem);
         bool again = false;
-        for (int r0 = 0; r0 < t.count; r0 += 16) again |= a.template own_keys<2>(r0);
+        for (int r0 = 0; r0 < t.count; r0 += 16) again |= a.own_keys(r0);
         if (again) a.plainly(a.wave, kAttnWaves);
     }
 }
