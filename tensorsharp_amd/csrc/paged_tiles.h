@@ -256,13 +256,14 @@ __device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth leas
     if (H.pieces == 0) return kWhole;
     Lanes L;
     int tiles = 0, long_tiles = 0, most = 0, long_most = 0;
-    float steps = 0.f, long_steps = 0.f;
+    uint32_t steps = 0;                                              // (exactly: the runs have to have all of them; up to 1024 tiles of 65541, more are not dealt out)
+    float long_steps = 0.f;
     for (int s0 = 0; s0 < H.seqs; s0 += 64) {
         L.load(H, s0);
         const int n = short_steps(H, L), m = tall_tiles(H, L);
         tiles += lane_sum(L.tiles);
         long_tiles += lane_sum(m);
-        steps += (float)lane_sum(n);
+        steps += (uint32_t)lane_sum(n);
         long_steps += (float)lane_sum(min(m * min(L.steps, 1 << 16), 1 << 24));
         int high = n, long_high = m > 0 ? L.steps : 0;
         for (int o = 32; o > 0; o >>= 1) high = max(high, __shfl_xor(high, o)), long_high = max(long_high, __shfl_xor(long_high, o));
@@ -272,7 +273,7 @@ __device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth leas
     const bool runs = tiles > long_tiles;
     Deal d{0, 1, 1};
     if (long_tiles > 0) {
-        const float share = tall * long_steps / (tall * long_steps + steps);
+        const float share = tall * long_steps / (tall * long_steps + (float)steps);
         d.tall = runs ? min(max((int)(share * H.pieces + 0.5f), long_tiles), H.pieces - 1) : H.pieces;
         // (a length that no tile exceeds ends it in any case: there are no more tiles than pieces)
         for (d.tall_steps = max(1, (int)ceilf(long_steps / (float)d.tall));; d.tall_steps += 1 + d.tall_steps / 16) {
@@ -284,7 +285,7 @@ __device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth leas
             if (all <= d.tall) break;
         }
     }
-    if (runs) d.run_steps = max(1, (int)ceilf(steps / (float)(H.pieces - d.tall)));
+    if (runs) d.run_steps = max(1, (int)((steps + (H.pieces - d.tall) - 1) / (uint32_t)(H.pieces - d.tall)));
     const bool worth = (long_tiles > 0 && long_most - d.tall_steps >= least.tall) || (runs && most - kTurn - d.run_steps >= (tiles * kv_heads >= 64 ? least.many : least.few));
     return worth ? d : kWhole;
 }

@@ -390,7 +390,8 @@ class PagePool:
     """Pages that sequences share, for the caches of all layers: page_table [sequences, pages of a sequence] int32 (the one of the PagedKVCaches),
     references [pages] int32 (how many sequences have a page, 0: free), context_lens [sequences] int32 (tokens), all on one device and changed in place by
     ResizeSequences, ForkSequences and CompactPages.  A sequence has the pages of its first ceil(tokens / page_size) entries, behind them is -1: an empty
-    pool is a table of -1 and zeros.  It keeps scratch of its own (an int32 for each entry of the table and for each page)."""
+    pool is a table of -1 and zeros.  It keeps scratch of its own (an int32 for each entry of the table and for each page): keep the pool until the work of its calls,
+    and graphs that have captured them, are done with."""
 
     def __init__(self, page_table, references, context_lens, page_size):
         torch = _torch()
@@ -417,7 +418,7 @@ class PagePool:
 
 
 def _pairs(moves, count, device):
-    if moves.dim() != 2 or moves.shape[1] != 2 or (count is not None and moves.shape[0] != count):
+    if moves is None or moves.dim() != 2 or moves.shape[1] != 2 or (count is not None and moves.shape[0] != count):
         raise ValueError(f"moves must be an Int32 tensor [{count if count is not None else 'moves'}, 2].")
     return _vector(moves, _torch().int32, moves.shape[0] * 2, "moves", device)
 
