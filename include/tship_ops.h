@@ -517,7 +517,8 @@ TSHIP_EXPORT int TSHip_RoPEStorePagedF32Device(TSHipTensorView2D query, TSHipTen
  * grouped heads sharing KV head h / (num_heads / num_kv_heads); sinks (device, num_heads logits) may be NULL (no such term).  A row that sees
  * nothing, or scores of -infinity only, is zero, rows that belong to no sequence are left as they were.  query and result [rows x num_heads
  * head_dim]; result may be query.  Sums are fp32; products go through the matrix cores, queries and weights cut into 16-bit parts: 24 bits over bf16 and
- * fp32 caches; over an fp16 cache 22 bits, of weights 2^-33 of the largest that the row met at most 1024 positions before where that is more. */
+ * fp32 caches; over an fp16 cache 22 bits, of weights 2^-33 of the largest that the row met at most 1024 positions before where that is more; over MXFP4
+ * queries to 15^-5 of the largest of 32 dimensions, weights to 24 bits. */
 TSHIP_EXPORT int TSHip_PagedAttentionF32Device(TSHipTensorView2D result, TSHipTensorView2D query, int num_heads, const TSHipPagedCache* cache,
                                                const int32_t* row_starts, const int32_t* context_lens, float scale, int window,
                                                const float* sinks);

@@ -71,6 +71,17 @@ __device__ __forceinline__ int lane_scan(int v)
     return v;
 }
 __device__ __forceinline__ int lane_sum(int v) { return __builtin_amdgcn_readlane(lane_scan(v), 63); }
+// the largest of numbers that are not negative (lanes that have none below them get 0)
+__device__ __forceinline__ int lane_max(int v)
+{
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
 
 // What the kernels need to find their piece.  It stands in front of the other arguments: the hardware delivers the first 14 dwords in
 // registers at wave launch (a structure is read from the argument block instead), so that the lengths are asked for at once.
@@ -265,9 +276,8 @@ __device__ __forceinline__ Deal deal_out(const Lens& H, int kv_heads, Worth leas
         long_tiles += lane_sum(m);
         steps += (uint32_t)lane_sum(n);
         long_steps += (float)lane_sum(min(m * min(L.steps, 1 << 16), 1 << 24));
-        int high = n, long_high = m > 0 ? L.steps : 0;
-        for (int o = 32; o > 0; o >>= 1) high = max(high, __shfl_xor(high, o)), long_high = max(long_high, __shfl_xor(long_high, o));
-        most = max(most, __builtin_amdgcn_readfirstlane(high)), long_most = max(long_most, __builtin_amdgcn_readfirstlane(long_high));
+        most = max(most, lane_max(n));
+        long_most = max(long_most, lane_max(m > 0 ? L.steps : 0));
     }
     if (tiles >= H.pieces) return kWhole;
     const bool runs = tiles > long_tiles;
