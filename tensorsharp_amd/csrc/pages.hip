@@ -1,14 +1,14 @@
 // The life of a cache's pages: who has which (tables, reference counts, lengths, all on the device), and copies of pages between caches.
 //
-//   page_drop_kernel, page_plan_kernel, page_fill_kernel     sequences get other lengths
+//   page_drop_kernel, page_plan_kernel, page_fill_kernel (page_few_kernel)          sequences get other lengths
 //   fork_plan_kernel, fork_tables_kernel (fork_rows_kernel, fork_store_kernel)      sequences go on from what others have
-//   compact_plan_kernel, compact_tables_kernel               used pages move to the front
+//   compact_plan_kernel (compact_tables_kernel)              used pages move to the front
 //   copy_pages_kernel                                        pages of one cache or two, of one type or two
 //
 // The lists are short next to the caches (a reference count for each page, an entry for each page of a sequence), so what counts is the number of dependent steps.  What
 // has to know all sequences in order - sums up to a sequence - is one workgroup, and so are the pages of a fork's few copies and of a compaction, thousands in a
 // step; where many pages are given out every wavefront has 64 of them, and their sums come between two launches.  What walks over the tables has a workgroup for
-// 1024 entries.  Two or three launches a call, nothing that one workgroup waits for another for.  Counts change by atomic additions of whole numbers, whose
+// 1024 entries.  One to three launches a call, nothing that one workgroup waits for another for.  Counts change by atomic additions of whole numbers, whose
 // order changes nothing.
 #include "tship_internal.h"
 #include "mx4.h"
@@ -73,6 +73,24 @@ __device__ __forceinline__ int64_t before_me(int64_t v, int64_t* all)
     return first + sum - v;
 }
 
+// the same of numbers whose sum has 32 bits, in registers
+__device__ __forceinline__ int before_me(int v, int* all)
+{
+    __shared__ int waves[kPlanWaves];
+    const int scan = lane_scan(v), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((threadIdx.x & 63) == 63) waves[wave] = scan;
+    __syncthreads();
+    int first = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        if (w < wave) first += waves[w];
+        total += waves[w];
+    }
+    __syncthreads();
+    *all = total;
+    return first + scan - v;
+}
+
 // The lowest free pages.  A thread takes 16 pages that follow one another.
 constexpr int kScan = 16 * kPlanThreads;
 __device__ __forceinline__ uint32_t free_here(const int32_t* references, int p, int end)
@@ -97,10 +115,10 @@ __device__ __forceinline__ int find_free(const int32_t* references, int pages, i
     for (int64_t p = 0; p < pages && found < want; p += kScan) {
         const int64_t mine = p + 16 * (int)threadIdx.x;
         uint32_t free = mine < pages ? free_here(references, (int)mine, pages) : 0;
-        int64_t all;
-        int number = found + (int)before_me(__popc(free), &all);
+        int all;
+        int number = found + before_me((int)__popc(free), &all);
         for (; free != 0 && number < want; free &= free - 1) each(number++, (int)mine + __ffs(free) - 1);
-        found += (int)all;
+        found += all;
     }
     return found;
 }
@@ -143,12 +161,6 @@ __device__ __forceinline__ uint32_t used_of(const Step& t)
     for (int i = 0; i < kLoads; ++i) bits |= (uint32_t)((t.r[i].x > 0) | (t.r[i].y > 0) << 1 | (t.r[i].z > 0) << 2 | (t.r[i].w > 0) << 3) << (4 * i);
     return bits;
 }
-__device__ __forceinline__ int wave_sum(int v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 // of one number a wavefront: the sum of those before this one's, and of all
 __device__ __forceinline__ int waves_before(int mine, int* all)
 {
@@ -187,6 +199,24 @@ __device__ __forceinline__ void pages_of_step(const Step& t, uint32_t used, int 
             n += (mine >> j) & 1;
         }
     }
+}
+
+// Atomic operations on memory are done in the second-level cache: what they leave is read there too, once every wavefront's have arrived.
+template <bool LOCAL>
+__device__ __forceinline__ int seen(const int* at)
+{
+    return LOCAL ? *at : __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool LOCAL>
+__device__ __forceinline__ void put(int* at, int v)
+{
+    if constexpr (LOCAL) *at = v;
+    else __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void settled()
+{
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
 }
 
 // ---- other lengths -------------------------------------------------------------------------------
@@ -284,6 +314,35 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PagePoolA
     }
 }
 
+// the last of the numbers (which do not fall) that is at most i; of(s): the s-th, the first is at most i
+template <typename F>
+__device__ __forceinline__ int last_at_most(int count, int i, F&& of)
+{
+    int s = 0;
+    for (int above = count; above - s > 1;) {
+        const int half = (s + above) >> 1;
+        if (of(half) <= i) s = half;
+        else above = half;
+    }
+    return s;
+}
+// Page number i of those that are given out goes to sequence s, whose first is number `at`: behind the `held` that it has, or, first of all, in the place of the begun page that
+// others have (copy: its number among the copies, -1: none).
+__device__ __forceinline__ void give_page(const PagePoolArgs& P, int i, int page, int s, int at, int held, int copy, int32_t* moves)
+{
+    int32_t* row = P.table + s * P.table_stride;
+    P.references[page] = 1;
+    if (copy < 0 || i > at) {
+        row[held + i - at - (copy >= 0)] = page;
+    } else {
+        const int begun = row[held - 1];
+        row[held - 1] = page;
+        atomicAdd(P.references + begun, -1);
+        moves[2 * copy] = begun;
+        moves[2 * copy + 1] = page;
+    }
+}
+
 // Each free page among the lowest finds the entry that it goes into, if there are enough; the last workgroup: lengths, and what else is to be said.  LOCAL: what is
 // known of the sequences fits LDS, where the page's sequence is looked for by halves.
 template <bool LOCAL>
@@ -337,47 +396,103 @@ __global__ void __launch_bounds__(kPlanThreads) page_fill_kernel(const PagePoolA
         const int i = number + __popcll(bits & ((1ull << lane) - 1)), page = (int)p0 + lane;
         number += __popcll(bits);
         if (!((bits >> lane) & 1) || i >= need) continue;
-        // the last sequence that begins at or before it (one that wants none begins where the next does)
-        int s = 0;
-        for (int above = P.seqs; above - s > 1;) {
-            const int half = (s + above) >> 1;
-            if ((LOCAL ? local[half] : W.b[half]) <= i) s = half;
-            else above = half;
-        }
-        const int at = i - (LOCAL ? local[s] : W.b[s]), held = LOCAL ? local[kLocal + s] : W.a[s], copy = LOCAL ? local[2 * kLocal + s] : W.c[s];
-        int32_t* row = P.table + s * P.table_stride;
-        P.references[page] = 1;
-        if (copy < 0 || at > 0) {
-            row[held + at - (copy >= 0)] = page;
-        } else {                                                     // in the place of the begun page that others have
-            const int begun = row[held - 1];
-            row[held - 1] = page;
-            atomicAdd(P.references + begun, -1);
-            moves[2 * copy] = begun;
-            moves[2 * copy + 1] = page;
-        }
+        // (a sequence that wants none begins where the next does)
+        const int s = last_at_most(P.seqs, i, [&](int k) { return LOCAL ? local[k] : W.b[k]; });
+        give_page(P, i, page, s, LOCAL ? local[s] : W.b[s], LOCAL ? local[kLocal + s] : W.a[s], LOCAL ? local[2 * kLocal + s] : W.c[s], moves);
     }
 }
 
-// ---- forks ---------------------------------------------------------------------------------------
-
-// Maxima and minima in memory are formed in the second-level cache: what they leave is read there too, once every wavefront's have arrived.
-template <bool LOCAL>
-__device__ __forceinline__ int seen(const int* at)
+// All of it in one launch, where one workgroup is enough: a thread for each sequence, 16 pages for each thread, 32 entries at most (48 sequences of 2400 tokens, 32 a page: 7 us for
+// 11 in three launches, 6 for 10 on the host).
+constexpr int kFewEntries = 32 * kPlanThreads;
+__host__ __device__ __forceinline__ bool one_workgroup(const PagePoolArgs& P)
 {
-    return LOCAL ? *at : __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return P.seqs <= kPlanThreads && P.num_pages <= kScan && (int64_t)P.seqs * P.max_pages <= kFewEntries;
 }
-template <bool LOCAL>
-__device__ __forceinline__ void put(int* at, int v)
+// two sums over the threads before this one and over all of them, one barrier (sums: of this call alone)
+struct Two {
+    int a, b;
+};
+__device__ __forceinline__ Two before_me(Two v, Two* all, Two (&sums)[kPlanWaves])
 {
-    if constexpr (LOCAL) *at = v;
-    else __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void settled()
-{
-    __builtin_amdgcn_s_waitcnt(0);
+    const Two scan{lane_scan(v.a), lane_scan(v.b)};
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((threadIdx.x & 63) == 63) sums[wave] = scan;
     __syncthreads();
+    Two first{0, 0}, total{0, 0};
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        const Two x = sums[w];
+        if (w < wave) first.a += x.a, first.b += x.b;
+        total.a += x.a, total.b += x.b;
+    }
+    *all = total;
+    return {first.a + scan.a - v.a, first.b + scan.b - v.b};
 }
+__global__ void __launch_bounds__(kPlanThreads) page_few_kernel(const PagePoolArgs P, const int32_t* lengths, int32_t* moves, int32_t* missing)
+{
+    __shared__ int begins[kPlanThreads], held_of[kPlanThreads], copy_of[kPlanThreads];
+    __shared__ Two sums[3][kPlanWaves];
+    __shared__ uint16_t list[kScan];                                 // the lowest free pages
+    const int s = threadIdx.x;
+    const bool mine = s < P.seqs;
+    const int64_t tokens = mine ? P.context_lens[s] : 0, goal = mine ? goal_of(P, lengths, s) : 0;
+    const int held = pages_of(P, tokens), to = pages_of(P, goal);
+    const bool grows = goal > tokens;
+    const bool into_begun = grows && held > 0 && tokens % P.page_size != 0;
+    const int last = into_begun ? P.table[s * P.table_stride + held - 1] : -1;
+    auto begin_of = [&](int k) { return begins[k]; };
+    // entries behind the ends of shorter sequences, one after the other
+    Two drops;
+    begins[s] = before_me(Two{max(0, held - to), 0}, &drops, sums[0]).a;
+    held_of[s] = to;
+    __syncthreads();
+    constexpr int kAtOnce = 4;
+    for (int i0 = s; i0 < drops.a; i0 += kAtOnce * kPlanThreads) {
+        int32_t* entry[kAtOnce];
+        int e[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int i = i0 + k * kPlanThreads;
+            e[k] = -1;
+            entry[k] = nullptr;
+            if (i >= drops.a) continue;
+            const int of = last_at_most(P.seqs, i, begin_of);
+            entry[k] = P.table + of * P.table_stride + held_of[of] + (i - begins[of]);
+            e[k] = *entry[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (is_page(P, e[k])) atomicAdd(P.references + e[k], -1);
+            if (entry[k]) *entry[k] = -1;
+        }
+    }
+    settled();
+    // what longer ones need, and free pages
+    uint32_t free = 16 * s < P.num_pages ? free_here(P.references, 16 * s, P.num_pages) : 0;
+    // (the last page is begun, and not this sequence's alone)
+    const int copied = is_page(P, last) && seen<false>(P.references + last) > 1;
+    Two need, found;
+    const Two at = before_me(Two{(grows ? to - held : 0) + copied, copied}, &need, sums[1]);
+    int i = before_me(Two{(int)__popc(free), 0}, &found, sums[2]).a;
+    const bool fits = found.a >= need.a;
+    begins[s] = at.a;
+    held_of[s] = held;
+    copy_of[s] = copied ? at.b : -1;
+    for (; fits && free != 0 && i < need.a; free &= free - 1) list[i++] = (uint16_t)(16 * s + __ffs(free) - 1);
+    __syncthreads();
+    for (int n = s; fits && n < need.a; n += kPlanThreads) {
+        const int of = last_at_most(P.seqs, n, begin_of);
+        give_page(P, n, list[n], of, begins[of], held_of[of], copy_of[of], moves);
+    }
+    if (mine) {
+        if (!fits || s >= need.b) moves[2 * s] = moves[2 * s + 1] = -1;
+        if (goal < tokens || (fits && grows)) P.context_lens[s] = (int)goal;
+    }
+    if (s == 0) missing[0] = fits ? 0 : need.a - found.a;
+}
+
+// ---- forks ---------------------------------------------------------------------------------------
 
 // One workgroup; LOCAL: what it works out of sequences fits LDS (4096 of them; through memory each of its steps is a trip there and back, 9.4 us for 32 sequences).  For the kernels behind
 // it a: the sequence that each becomes, c: the fresh page in place of the begun one, -1: none, d: tokens before
@@ -409,7 +524,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
     }
     settled();
     // (a parent that stays what it is keeps its begun page)
-    int64_t need = 0;
+    int need = 0;
     for (int s0 = 0; s0 < P.seqs; s0 += kPlanThreads) {
         const int s = s0 + threadIdx.x;
         int copied = 0, of = 0;
@@ -418,17 +533,17 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
             const int keeper = seen<LOCAL>(of_all + of) == of ? of : seen<LOCAL>(low + of);
             copied = keeper != s && begun[of] >= 0;
         }
-        int64_t all;
-        const int64_t number = need + before_me(copied, &all);
+        int all;
+        const int number = need + before_me(copied, &all);
         if (copied) moves[2 * number] = begun[of];                   // (as many as there are children at most)
-        if (s < P.seqs) W.rows[s] = copied ? (int)number : -1;       // (rows of the table come there later)
+        if (s < P.seqs) W.rows[s] = copied ? number : -1;       // (rows of the table come there later)
         need += all;
     }
-    const int found = need == 0 ? 0 : find_free(P.references, P.num_pages, (int)need, [&](int i, int page) { moves[2 * i + 1] = page; });
+    const int found = need == 0 ? 0 : find_free(P.references, P.num_pages, need, [&](int i, int page) { moves[2 * i + 1] = page; });
     const bool fits = found >= need;
     if (threadIdx.x == 0) {
         W.head[0] = fits;
-        missing[0] = fits ? 0 : (int)(need - found);
+        missing[0] = fits ? 0 : need - found;
     }
     settled();
     for (int i = threadIdx.x; i < count; i += kPlanThreads)
@@ -515,15 +630,17 @@ __global__ void __launch_bounds__(kRowThreads) fork_store_kernel(const PagePoolA
 
 // One workgroup.  With U pages in use and n of them before page p, a free page p < U is hole number p - n, and a page p >= U in use goes into hole number U - 1 - n (the last
 // one into the first hole), so that each finds its place in the list by itself.  pages[p]: where page p is afterwards (from U on)
+// TABLES: with the tables, where one workgroup is enough for these too
+template <bool TABLES>
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePoolArgs P, int32_t* moves, int max_moves)
 {
     const Scratch W = scratch_of(P);
     const Step first = step_at(P.references, 0, P.num_pages);
     int used = 0, all;
-    waves_before(wave_sum(__popc(used_of(first))), &used);
+    waves_before(lane_sum(__popc(used_of(first))), &used);
     for (int p = pages_in(first.loads); p < P.num_pages;) {
         const Step t = step_at(P.references, p, P.num_pages);
-        waves_before(wave_sum(__popc(used_of(t))), &all);
+        waves_before(lane_sum(__popc(used_of(t))), &all);
         used += all;
         p += pages_in(t.loads);
     }
@@ -531,7 +648,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePo
     for (int p = 0; p < P.num_pages;) {
         const Step t = p == 0 ? first : step_at(P.references, p, P.num_pages);
         const uint32_t bits = used_of(t);
-        const int before = waves_before(wave_sum(__popc(bits)), &all);
+        const int before = waves_before(lane_sum(__popc(bits)), &all);
         pages_of_step(t, bits, n + before, P.num_pages, [&](int page, bool is_used, int k) {
             if (page < used && !is_used && page - k < max_moves) moves[2 * (page - k) + 1] = page;
             if (page >= used && is_used && used - 1 - k < max_moves) moves[2 * (used - 1 - k)] = page;
@@ -542,7 +659,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePo
         p += pages_in(t.loads);
     }
     int count;
-    waves_before(wave_sum(above), &count);                           // (and what has been written is there)
+    waves_before(lane_sum(above), &count);                           // (and what has been written is there)
     settled();
     for (int i = threadIdx.x; i < max_moves; i += kPlanThreads) {
         if (i >= count) {
@@ -554,7 +671,28 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePo
         P.references[to] = P.references[from];
         P.references[from] = 0;
     }
-    if (threadIdx.x == 0) W.head[1] = used;
+    if constexpr (!TABLES) {
+        if (threadIdx.x == 0) W.head[1] = used;
+        return;
+    }
+    settled();
+    constexpr int kAtOnce = 4;
+    const uint32_t entries = P.seqs * P.max_pages, room = P.max_pages;
+    for (uint32_t i0 = threadIdx.x; i0 < entries; i0 += kAtOnce * kPlanThreads) {
+        int32_t* entry[kAtOnce];
+        int e[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const uint32_t i = i0 + k * kPlanThreads, s = i / room, j = i - s * room;
+            e[k] = -1;
+            if (i >= entries || (int)j >= pages_of(P, P.context_lens[s])) continue;
+            entry[k] = P.table + s * P.table_stride + j;
+            e[k] = *entry[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+            if (is_page(P, e[k]) && e[k] >= used) *entry[k] = seen<false>(W.pages + e[k]);
+    }
 }
 
 // grid (chunks of entries, sequences)
@@ -679,6 +817,10 @@ int64_t page_pool_scratch(int64_t seqs, int64_t max_pages, int64_t num_pages) { 
 
 bool launch_resize_sequences(const PagePoolArgs& P, const int32_t* lengths, int32_t* moves, int32_t* missing, hipStream_t stream)
 {
+    if (one_workgroup(P)) {
+        hipLaunchKernelGGL(page_few_kernel, dim3(1), dim3(kPlanThreads), 0, stream, P, lengths, moves, missing);
+        return hip_ok(hipGetLastError(), "resize_sequences launch");
+    }
     hipLaunchKernelGGL(page_drop_kernel, row_grid(P), dim3(kRowThreads), 0, stream, P, lengths);
     if (!hip_ok(hipGetLastError(), "resize_sequences launch")) return false;
     const int part = kPart * (int)((P.num_pages + (int64_t)kPart * kMostParts - 1) / ((int64_t)kPart * kMostParts));
@@ -713,7 +855,9 @@ bool launch_fork_sequences(const PagePoolArgs& P, const int32_t* children, const
 
 bool launch_compact_pages(const PagePoolArgs& P, int32_t* moves, int max_moves, hipStream_t stream)
 {
-    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, P, moves, max_moves);
+    const bool one = one_workgroup(P);
+    hipLaunchKernelGGL(one ? compact_plan_kernel<true> : compact_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, stream, P, moves, max_moves);
+    if (one) return hip_ok(hipGetLastError(), "compact_pages launch");
     if (!hip_ok(hipGetLastError(), "compact_pages launch")) return false;
     hipLaunchKernelGGL(compact_tables_kernel, row_grid(P), dim3(kRowThreads), 0, stream, P);
     return hip_ok(hipGetLastError(), "compact_pages launch");

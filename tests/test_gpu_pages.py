@@ -66,9 +66,10 @@ class Pool:
 
 
 # sequences, entries of a table, tokens of a page, pages: one of each; a few; more sequences than a workgroup has threads; more pages than a step of the
-# scan; rows of a table longer than a workgroup's part; more sequences than fit a workgroup's memory; pages up to the end of a step
+# scan; rows of a table longer than a workgroup's part; more sequences than fit a workgroup's memory; pages up to the end of a step; around what one workgroup does alone
 SIZES = [(1, 1, 1, 1), (1, 7, 16, 9), (3, 5, 4, 16), (17, 9, 1, 60), (40, 30, 16, 900), (1500, 4, 8, 4001), (70, 300, 2, 17001), (3, 2500, 2, 40000),
-         (5000, 3, 4, 9999), (1024, 5, 16, 4096), (30, 2200, 1, 70002), (9, 900, 3, 32768)]
+         (5000, 3, 4, 9999), (1024, 5, 16, 4096), (30, 2200, 1, 70002), (9, 900, 3, 32768),
+         (1024, 32, 4, 16384), (1000, 32, 2, 16385), (100, 327, 3, 16384), (1025, 16, 4, 8000)]
 
 
 @pytest.mark.parametrize("seqs,room,page,pages", SIZES)

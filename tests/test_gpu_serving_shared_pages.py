@@ -82,9 +82,9 @@ def buffers(torch, rows, seed):
     return x, [torch.zeros((rows, HEADS * DIM), device="cuda") for _ in range(3)], [torch.zeros((rows, HEADS * DIM), device="cuda") for _ in range(3)]
 
 
-@pytest.mark.parametrize("pages", [40, 14])
+@pytest.mark.parametrize("pages", [40, 14, 17000])
 def test_many_steps(hip, pages):
-    """with pages enough, and with so few that steps and forks are refused until a sequence ends"""
+    """with pages enough, with so few that steps and forks are refused until a sequence ends, and with more than one workgroup looks after"""
     import torch
     seqs = 6
     shared, alone = Server(hip, torch, seqs, pages), Server(hip, torch, seqs, pages, own=True)
@@ -131,7 +131,7 @@ def test_many_steps(hip, pages):
             shared.compact(int(rng.integers(1, 40)))
         held = shared.table[shared.table >= 0]
         assert torch.equal(torch.bincount(held.long(), minlength=pages), shared.pool.references.long()), turn
-    assert refused > 0 or pages == 40
+    assert refused > 0 or pages != 14
 
 
 def test_a_captured_step_and_two_streams(hip):
