@@ -1,7 +1,7 @@
 // The life of a cache's pages: who has which (tables, reference counts, lengths, all on the device), and copies of pages between caches.
 //
 //   page_drop_kernel, page_plan_kernel, page_fill_kernel (page_few_kernel)          sequences get other lengths
-//   fork_plan_kernel, fork_tables_kernel (fork_rows_kernel, fork_store_kernel)      sequences go on from what others have
+//   fork_plan_kernel (fork_tables_kernel or fork_rows_kernel, fork_store_kernel)    sequences go on from what others have
 //   compact_plan_kernel (compact_tables_kernel)              used pages move to the front
 //   copy_pages_kernel                                        pages of one cache or two, of one type or two
 //
@@ -496,7 +496,9 @@ __global__ void __launch_bounds__(kPlanThreads) page_few_kernel(const PagePoolAr
 
 // One workgroup; LOCAL: what it works out of sequences fits LDS (4096 of them; through memory each of its steps is a trip there and back, 9.4 us for 32 sequences).  For the kernels behind
 // it a: the sequence that each becomes, c: the fresh page in place of the begun one, -1: none, d: tokens before
-template <bool LOCAL>
+// TABLES: and the tables, where their entries are 16 a thread at most (32 beams of 2000 tokens: 2 us less than in two launches)
+constexpr int kForkEach = 16;
+template <bool LOCAL, bool TABLES>
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolArgs P, const int32_t* children, const int32_t* parents, int count,
                                                                  int32_t* moves, int32_t* missing)
 {
@@ -549,9 +551,43 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
     for (int i = threadIdx.x; i < count; i += kPlanThreads)
         if (!fits || i >= need) moves[2 * i] = moves[2 * i + 1] = -1;
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        const int number = W.rows[s];
-        if constexpr (LOCAL) W.a[s] = of_all[s], W.d[s] = tokens[s];
-        W.c[s] = fits && number >= 0 ? moves[2 * number + 1] : -1;
+        const int number = W.rows[s], fresh = fits && number >= 0 ? moves[2 * number + 1] : -1;
+        if constexpr (TABLES) {
+            low[s] = fresh;
+            if (fits && of_all[s] != s) P.context_lens[s] = tokens[of_all[s]];
+        } else {
+            if constexpr (LOCAL) W.a[s] = of_all[s], W.d[s] = tokens[s];
+            W.c[s] = fresh;
+        }
+    }
+    if constexpr (TABLES) {
+        if (!fits) return;
+        __syncthreads();
+        const uint32_t entries = P.seqs * P.max_pages, room = P.max_pages;
+        int entry[kForkEach], was[kForkEach];
+        int32_t* at[kForkEach];
+#pragma unroll
+        for (int n = 0; n < kForkEach; ++n) {
+            const uint32_t i = threadIdx.x + n * kPlanThreads, row = i / room, j = i - row * room;
+            entry[n] = was[n] = -1;
+            at[n] = nullptr;
+            if (i >= entries) continue;
+            const int s = row, of = of_all[s];
+            if (of == s) continue;
+            const int held = pages_of(P, tokens[of]);
+            at[n] = P.table + s * P.table_stride + j;
+            if ((int)j < pages_of(P, tokens[s])) was[n] = *at[n];
+            if ((int)j < held) entry[n] = (int)j == held - 1 && low[s] >= 0 ? low[s] : P.table[of * P.table_stride + j];
+        }
+        __syncthreads();                                             // (what rows become has been read)
+#pragma unroll
+        for (int n = 0; n < kForkEach; ++n) {
+            if (!at[n]) continue;
+            *at[n] = entry[n];
+            if (entry[n] == was[n]) continue;
+            if (is_page(P, entry[n])) atomicAdd(P.references + entry[n], 1);
+            if (is_page(P, was[n])) atomicAdd(P.references + was[n], -1);
+        }
     }
 }
 
@@ -835,13 +871,12 @@ bool launch_resize_sequences(const PagePoolArgs& P, const int32_t* lengths, int3
 bool launch_fork_sequences(const PagePoolArgs& P, const int32_t* children, const int32_t* parents, int count, int32_t* moves, int32_t* missing,
                            hipStream_t stream)
 {
-    if (P.seqs <= kLocal) {
-        constexpr size_t lds = 4 * kLocal * sizeof(int);
-        if (!raise_lds_limit(reinterpret_cast<const void*>(fork_plan_kernel<true>), lds)) return false;
-        hipLaunchKernelGGL(fork_plan_kernel<true>, dim3(1), dim3(kPlanThreads), lds, stream, P, children, parents, count, moves, missing);
-    } else {
-        hipLaunchKernelGGL(fork_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, stream, P, children, parents, count, moves, missing);
-    }
+    constexpr size_t lds = 4 * kLocal * sizeof(int);
+    const bool local = P.seqs <= kLocal, tables = local && (int64_t)P.seqs * P.max_pages <= kForkEach * kPlanThreads;
+    const auto plan = tables ? fork_plan_kernel<true, true> : local ? fork_plan_kernel<true, false> : fork_plan_kernel<false, false>;
+    if (local && !raise_lds_limit(reinterpret_cast<const void*>(plan), lds)) return false;
+    hipLaunchKernelGGL(plan, dim3(1), dim3(kPlanThreads), local ? lds : 0, stream, P, children, parents, count, moves, missing);
+    if (tables) return hip_ok(hipGetLastError(), "fork_sequences launch");
     if (!hip_ok(hipGetLastError(), "fork_sequences launch")) return false;
     if (P.seqs <= kForkMost) {
         hipLaunchKernelGGL(fork_tables_kernel, dim3((P.max_pages + kForkEntries - 1) / kForkEntries), dim3(kPlanThreads), 0, stream, P);

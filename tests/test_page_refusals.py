@@ -84,7 +84,7 @@ def test_calls_that_are_refused(stub):  # noqa: F811
         assert ok == 0 and words in error and not launches(log, ""), (call, error)
 
 
-@pytest.mark.parametrize("call,kernels", [("do_store(c=mx())", 1), ("do_attend(c=mx())", 1), ("do_attend(c=mx(max_pages=4096, table_stride=4096))", 2), ("do_first()", 1), ("do_resize()", 1), ("do_resize(pool(num_pages=20000))", 3), ("do_resize(pool(num_seqs=1025))", 3), ("do_resize(pool(max_pages=20000, table_stride=20000))", 3), ("do_fork()", 2), ("do_fork(pool(num_seqs=5000))", 3),
+@pytest.mark.parametrize("call,kernels", [("do_store(c=mx())", 1), ("do_attend(c=mx())", 1), ("do_attend(c=mx(max_pages=4096, table_stride=4096))", 2), ("do_first()", 1), ("do_resize()", 1), ("do_resize(pool(num_pages=20000))", 3), ("do_resize(pool(num_seqs=1025))", 3), ("do_resize(pool(max_pages=20000, table_stride=20000))", 3), ("do_fork()", 1), ("do_fork(pool(max_pages=9000, table_stride=9000))", 2), ("do_fork(pool(num_seqs=5000))", 3),
                                           ("do_compact()", 1), ("do_compact(pool(num_pages=20000))", 2), ("do_copy()", 1)])
 def test_a_launch_that_fails_is_reported(stub, call, kernels):  # noqa: F811
     """whichever of a call's launches it is"""
