@@ -765,9 +765,9 @@ struct Attn {
             const int last = t.p0 + token, first = first_key(last, A.window);
             float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
-                const int j = position(j0) + lane;
+                const int j = position(j0 + lane);                   // (first positions and the window's may meet within 64)
                 int id = -1;
-                if (j < end_at(j0) && (in_head(j0) || j >= first) && j <= last) id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)j)];
+                if (j < end_at(j0 + lane) && (in_head(j0 + lane) || j >= first) && j <= last) id = A.cache.table[t.seq * A.cache.table_stride + (int)A.cache.page.quot((uint32_t)j)];
                 const bool seen = (uint32_t)id < (uint32_t)A.cache.num_pages;
                 const uint64_t lanes = __ballot(seen);
                 if (lanes == 0) continue;

@@ -51,8 +51,8 @@ struct AttnTile {
     int lo, hi;
     int cuts, slot;              // pieces of its keys; where the first one's (this one's) state goes
     bool mine;                   // of a run: it has a part of the tile's keys, not only of what the tile costs besides
-    // With first positions that stay visible the keys are numbered on: positions 0 .. head_end - 1 as 0 .. head - 1 (whole steps of 64, so that no step of the
-    // kernels has keys of both), then the window's, `jump` further on.  All rows see of the former what lies before them, of the latter what is in their window.
+    // With first positions that stay visible the keys are numbered on: positions 0 .. head_end - 1 as 0 .. head - 1 (whole steps of the kernel's, so that none
+    // has keys of both), then the window's, `jump` further on.  All rows see of the former what lies before them, of the latter what is in their window.
     int head, head_end, jump;
     __device__ __forceinline__ int position(int key) const { return key < head ? key : key + jump; }
     __device__ __forceinline__ int end_at(int key) const { return key < head ? min(head_end, hi) : hi + jump; }      // of the positions from that key's on
@@ -197,7 +197,9 @@ __device__ __forceinline__ void set_tile(const AttnArgs& A, const Lanes& L, int 
         const int hi = max(0, t.hi), begin = max(t.lo, A.first);
         t.lo = 0;
         t.head_end = min(hi, A.first);
-        t.head = (t.head_end + 63) & ~63;
+        // (steps of 64 for fp16 and four bits, else of 32: of five first positions and a window of 128 over bf16 a tile has 6 steps in place of 7)
+        const int step = A.cache.element_type == kTypeF16 || A.cache.element_type == kTypeMXFP4 ? 64 : 32;
+        t.head = (t.head_end + step - 1) & ~(step - 1);
         if (hi > A.first) {
             t.jump = begin - t.head;
             t.hi = hi - t.jump;
