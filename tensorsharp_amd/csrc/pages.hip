@@ -502,12 +502,20 @@ template <bool LOCAL, bool TABLES>
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolArgs P, const int32_t* children, const int32_t* parents, int count,
                                                                  int32_t* moves, int32_t* missing)
 {
-    extern __shared__ int local[];
+    extern __shared__ __attribute__((aligned(16))) int local[];
     const Scratch W = scratch_of(P);
-    // of: that each becomes; low: the lowest that becomes it; tokens and begun page before
+    // of: that each becomes; low: the lowest that becomes it; tokens and begun page before; in LDS also the number of each one's copy and their pages, and before
+    // these the last pair of each, with its number above
     int *of_all = LOCAL ? local : W.a, *low = LOCAL ? local + kLocal : W.b, *tokens = LOCAL ? local + 2 * kLocal : W.d, *begun = LOCAL ? local + 3 * kLocal : W.c;
+    int *number_of = LOCAL ? local + 4 * kLocal : W.rows, *fresh_of = local + 5 * kLocal;           // (rows of the table come there later)
+    unsigned long long* pairs = reinterpret_cast<unsigned long long*>(local + 4 * kLocal);
+    auto there = [] {
+        if constexpr (LOCAL) __syncthreads();
+        else settled();
+    };
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        put<LOCAL>(of_all + s, -1);
+        if constexpr (LOCAL) pairs[s] = 0;
+        else put<LOCAL>(of_all + s, -1);
         put<LOCAL>(low + s, P.seqs);
         const int n = P.context_lens[s], held = pages_of(P, n);
         int page = -1;
@@ -515,16 +523,25 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
         tokens[s] = n;
         begun[s] = is_page(P, page) ? page : -1;
     }
-    settled();
-    for (int i = threadIdx.x; i < count; i += kPlanThreads)
-        if ((uint32_t)children[i] < (uint32_t)P.seqs && (uint32_t)parents[i] < (uint32_t)P.seqs) atomicMax(of_all + children[i], i);
-    settled();
+    there();
+    for (int i = threadIdx.x; i < count; i += kPlanThreads) {
+        const int child = children[i], parent = parents[i];
+        if ((uint32_t)child >= (uint32_t)P.seqs || (uint32_t)parent >= (uint32_t)P.seqs) continue;
+        if constexpr (LOCAL) atomicMax(pairs + child, (unsigned long long)(i + 1u) << 32 | (uint32_t)parent);
+        else atomicMax(of_all + child, i);
+    }
+    there();
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        const int pair = seen<LOCAL>(of_all + s), of = pair >= 0 ? parents[pair] : s;
+        int of = s;
+        if constexpr (LOCAL) {
+            if (const unsigned long long pair = pairs[s]) of = (int)(uint32_t)pair;
+        } else {
+            if (const int pair = seen<LOCAL>(of_all + s); pair >= 0) of = parents[pair];
+        }
         put<LOCAL>(of_all + s, of);
         atomicMin(low + of, s);
     }
-    settled();
+    there();
     // (a parent that stays what it is keeps its begun page)
     int need = 0;
     for (int s0 = 0; s0 < P.seqs; s0 += kPlanThreads) {
@@ -538,20 +555,23 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
         int all;
         const int number = need + before_me(copied, &all);
         if (copied) moves[2 * number] = begun[of];                   // (as many as there are children at most)
-        if (s < P.seqs) W.rows[s] = copied ? number : -1;       // (rows of the table come there later)
+        if (s < P.seqs) number_of[s] = copied ? number : -1;
         need += all;
     }
-    const int found = need == 0 ? 0 : find_free(P.references, P.num_pages, need, [&](int i, int page) { moves[2 * i + 1] = page; });
+    const int found = need == 0 ? 0 : find_free(P.references, P.num_pages, need, [&](int i, int page) {
+        moves[2 * i + 1] = page;
+        if constexpr (LOCAL) fresh_of[i] = page;
+    });
     const bool fits = found >= need;
     if (threadIdx.x == 0) {
         W.head[0] = fits;
         missing[0] = fits ? 0 : need - found;
     }
-    settled();
+    there();
     for (int i = threadIdx.x; i < count; i += kPlanThreads)
         if (!fits || i >= need) moves[2 * i] = moves[2 * i + 1] = -1;
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
-        const int number = W.rows[s], fresh = fits && number >= 0 ? moves[2 * number + 1] : -1;
+        const int number = number_of[s], fresh = fits && number >= 0 ? LOCAL ? fresh_of[number] : moves[2 * number + 1] : -1;
         if constexpr (TABLES) {
             low[s] = fresh;
             if (fits && of_all[s] != s) P.context_lens[s] = tokens[of_all[s]];
@@ -871,7 +891,7 @@ bool launch_resize_sequences(const PagePoolArgs& P, const int32_t* lengths, int3
 bool launch_fork_sequences(const PagePoolArgs& P, const int32_t* children, const int32_t* parents, int count, int32_t* moves, int32_t* missing,
                            hipStream_t stream)
 {
-    constexpr size_t lds = 4 * kLocal * sizeof(int);
+    constexpr size_t lds = 6 * kLocal * sizeof(int);
     const bool local = P.seqs <= kLocal, tables = local && (int64_t)P.seqs * P.max_pages <= kForkEach * kPlanThreads;
     const auto plan = tables ? fork_plan_kernel<true, true> : local ? fork_plan_kernel<true, false> : fork_plan_kernel<false, false>;
     if (local && !raise_lds_limit(reinterpret_cast<const void*>(plan), lds)) return false;
