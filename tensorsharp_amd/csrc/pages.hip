@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kRowThreads) fork_store_kernel(const PagePoolA
 
 // One workgroup.  With U pages in use and n of them before page p, a free page p < U is hole number p - n, and a page p >= U in use goes into hole number U - 1 - n (the last
 // one into the first hole), so that each finds its place in the list by itself.  pages[p]: where page p is afterwards (from U on)
-// TABLES: with the tables, where one workgroup is enough for these too
+// TABLES: with the tables, where one workgroup is enough for these too (48 sequences, 5000 pages: 8 us, in two launches 6 and 3)
 template <bool TABLES>
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePoolArgs P, int32_t* moves, int max_moves)
 {
