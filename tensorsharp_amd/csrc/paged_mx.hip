@@ -186,11 +186,12 @@ struct AttnMx {
         return (c & 8 ? -size : size) * mx4_power(scales[d >> 5]);
     }
     // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
-    // 64) for the values, whose mean is carried along, so that finite values never add up to infinity.  Slow, for rows with infinities or NaN in their results.
-    __device__ __forceinline__ void plainly(int row, int step)
+    // 64) for the values, whose mean is carried along, so that finite values never add up to infinity.  Slow, for rows with infinities or NaN in their results; only
+    // for rows that have not been written yet, whose places may be those of the query.
+    __device__ __forceinline__ void plainly(int row, int step, int end)
     {
         const int dim = A.cache.head_dim;
-        for (int n = 0; n < 32 && row < t.count; ++n, row += step) {
+        for (end = min(end, t.count); row < end; row += step) {
             int token, head;
             place(row, &token, &head);
             const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
@@ -754,7 +755,7 @@ __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_atten
         if (!(whole ? find_whole(H, A, idx, t) : find_tall(H, A, deal, idx, t))) return;
         if (t.tokens * A.group > kKeyRows) {
             AttnMx<HD> a(A, X, t, kvh, threadIdx.x, (lds_t)smem);
-            if (a.shared_keys()) a.plainly(32 * a.wave, 1);
+            if (a.shared_keys()) a.plainly(32 * a.wave, 1, 32 * a.wave + 32);
             return;
         }
     } else if (idx >= H.pieces) {
@@ -769,9 +770,8 @@ __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_atten
         int thread = threadIdx.x;
         asm volatile("" : "+v"(thread));                             // (what follows from it is worked out for each tile: kept from one to the next it would be spilled)
         AttnMx<HD> a(A, X, t, kvh, thread, (lds_t)smem);
-        bool again = false;
-        for (int r0 = 0; r0 < t.count; r0 += 16) again |= a.own_keys(r0);
-        if (again) a.plainly(a.wave, kAttnWaves);
+        for (int r0 = 0; r0 < t.count; r0 += 16)
+            if (a.own_keys(r0)) a.plainly(r0 + a.wave, kAttnWaves, r0 + 16);
     }
 }
 
