@@ -524,11 +524,12 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
         begun[s] = is_page(P, page) ? page : -1;
     }
     there();
-    for (int i = threadIdx.x; i < count; i += kPlanThreads) {
+    // (lists may have as many pairs as 32 bits count: what walks over them counts in 64)
+    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads) {
         const int child = children[i], parent = parents[i];
         if ((uint32_t)child >= (uint32_t)P.seqs || (uint32_t)parent >= (uint32_t)P.seqs) continue;
-        if constexpr (LOCAL) atomicMax(pairs + child, (unsigned long long)(i + 1u) << 32 | (uint32_t)parent);
-        else atomicMax(of_all + child, i);
+        if constexpr (LOCAL) atomicMax(pairs + child, (unsigned long long)(i + 1) << 32 | (uint32_t)parent);
+        else atomicMax(of_all + child, (int)i);
     }
     there();
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagePoolA
         missing[0] = fits ? 0 : need - found;
     }
     there();
-    for (int i = threadIdx.x; i < count; i += kPlanThreads)
+    for (int64_t i = threadIdx.x; i < count; i += kPlanThreads)
         if (!fits || i >= need) moves[2 * i] = moves[2 * i + 1] = -1;
     for (int s = threadIdx.x; s < P.seqs; s += kPlanThreads) {
         const int number = number_of[s], fresh = fits && number >= 0 ? LOCAL ? fresh_of[number] : moves[2 * number + 1] : -1;
@@ -717,7 +718,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagePo
     int count;
     waves_before(lane_sum(above), &count);                           // (and what has been written is there)
     settled();
-    for (int i = threadIdx.x; i < max_moves; i += kPlanThreads) {
+    for (int64_t i = threadIdx.x; i < max_moves; i += kPlanThreads) {        // (of a list of 2^31 - 1 moves 32 bits would pass the end)
         if (i >= count) {
             moves[2 * i] = moves[2 * i + 1] = -1;
             continue;
