@@ -899,8 +899,10 @@ bool launch_fork_sequences(const PagePoolArgs& P, const int32_t* children, const
     hipLaunchKernelGGL(plan, dim3(1), dim3(kPlanThreads), local ? lds : 0, stream, P, children, parents, count, moves, missing);
     if (tables) return hip_ok(hipGetLastError(), "fork_sequences launch");
     if (!hip_ok(hipGetLastError(), "fork_sequences launch")) return false;
-    if (P.seqs <= kForkMost) {
-        hipLaunchKernelGGL(fork_tables_kernel, dim3((P.max_pages + kForkEntries - 1) / kForkEntries), dim3(kPlanThreads), 0, stream, P);
+    // (a launch has fewer than 2^32 threads: of rows of more entries each takes two kernels, as those of many sequences)
+    const int64_t columns = ((int64_t)P.max_pages + kForkEntries - 1) / kForkEntries;
+    if (P.seqs <= kForkMost && columns * kPlanThreads <= UINT32_MAX) {
+        hipLaunchKernelGGL(fork_tables_kernel, dim3((unsigned)columns), dim3(kPlanThreads), 0, stream, P);
         return hip_ok(hipGetLastError(), "fork_sequences launch");
     }
     hipLaunchKernelGGL(fork_rows_kernel, row_grid(P), dim3(kRowThreads), 0, stream, P);
