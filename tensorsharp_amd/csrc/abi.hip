@@ -3129,6 +3129,13 @@ bool validate_cache(const TSHipPagedCache* c, int num_heads, const int32_t* row_
     return true;
 }
 
+// from + (count - 1) stride, which for strides that no memory has may pass 64 bits: the largest of these then
+int64_t reach(int64_t from, int64_t count, int64_t stride)
+{
+    const __int128 to = (__int128)from + (__int128)(count - 1) * stride;
+    return to > INT64_MAX ? INT64_MAX : (int64_t)to;
+}
+
 // rows of a cache that share memory, which may not be written
 bool rows_overlap(const TSHipPagedCache* c)
 {
@@ -3143,7 +3150,7 @@ bool rows_overlap(const TSHipPagedCache* c)
         for (const auto& [stride, count] : d) {
             if (count == 1) continue;
             if (stride < span) return true;
-            span += stride * (count - 1);
+            span = reach(span, count, stride);
         }
     }
     return false;
@@ -3363,8 +3370,8 @@ Span span_of(const void* at, const int64_t* strides, const TSHipPagedCache* c, i
     const uintptr_t p = reinterpret_cast<uintptr_t>(at);
     const int64_t counts[3] = {c->num_pages, c->page_size, c->num_kv_heads};
     int64_t last = row;
-    for (int i = 0; i < 3; ++i) last += counts[i] > 1 ? (counts[i] - 1) * strides[i] : 0;
-    return {p, p + (uintptr_t)(last * size)};
+    for (int i = 0; i < 3; ++i) last = counts[i] > 1 ? reach(last, counts[i], strides[i]) : last;
+    return {p, p + (uintptr_t)std::min((unsigned __int128)last * size, (unsigned __int128)(UINTPTR_MAX - p))};
 }
 void spans_of(const TSHipPagedCache* c, Span (&out)[4])
 {
@@ -3458,8 +3465,8 @@ int TSHip_CopyPagesDevice(const TSHipPagedCache* dst, const TSHipPagedCache* src
             set_last_error("copy_pages: rows of keys or values overlap.");
             return 0;
         }
-        const int64_t units = (int64_t)dst->page_size * d.kv_heads * (d.head_dim / 8);
-        if (units > (1 << 26)) {
+        const int64_t of_head = (int64_t)dst->page_size * (d.head_dim / 8), units = of_head * d.kv_heads;
+        if (of_head > (1 << 26) / d.kv_heads) {                        // (their product may pass 64 bits)
             set_last_error("copy_pages: pages are too large.");
             return 0;
         }
