@@ -370,6 +370,8 @@ class PagedKVCache:
             scales = (k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride()[:3], *v_scales.stride()[:3])
         if page_table.dim() != 2 or page_table.dtype != torch.int32:
             raise ValueError("PagedKVCache requires a 2D Int32 page table.")
+        if max(*k.shape[1:3], *page_table.shape) >= 2 ** 31:          # (the call takes 32 bits of them)
+            raise ValueError("PagedKVCache requires fewer than 2^31 tokens of a page, heads, sequences and pages of a sequence.")
         if not k.is_cuda or v.device != k.device or page_table.device != k.device:
             raise ValueError("PagedKVCache requires tensors in GPU memory of one device.")
         if k.stride(3) != 1 or v.stride(3) != 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
@@ -395,6 +397,8 @@ class PagePool:
 
     def __init__(self, page_table, references, context_lens, page_size):
         torch = _torch()
+        if not 0 < page_size < 2 ** 31 or any(n >= 2 ** 31 for n in page_table.shape):          # (the calls take 32 bits of them)
+            raise ValueError("PagePool requires a page size of 1 to 2^31 - 1 tokens, and fewer than 2^31 sequences and pages of a sequence.")
         if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_cuda:
             raise ValueError("PagePool requires a 2D Int32 page table in GPU memory.")
         if page_table.shape[1] > 1 and page_table.stride(1) != 1:
@@ -420,6 +424,8 @@ class PagePool:
 def _pairs(moves, count, device):
     if moves is None or moves.dim() != 2 or moves.shape[1] != 2 or (count is not None and moves.shape[0] != count):
         raise ValueError(f"moves must be an Int32 tensor [{count if count is not None else 'moves'}, 2].")
+    if moves.shape[0] >= 2 ** 31:                    # (the calls take 32 bits of it)
+        raise ValueError("moves must be fewer than 2^31 pairs.")
     return _vector(moves, _torch().int32, moves.shape[0] * 2, "moves", device)
 
 
