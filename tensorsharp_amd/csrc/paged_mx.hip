@@ -179,15 +179,17 @@ struct AttnMx {
     __device__ __forceinline__ uint64_t value_scales() const { return (uint64_t)(uintptr_t)X.v + kvh * X.v_head; }
 
     // ---- infinities and NaN ----
-    __device__ __forceinline__ float element(mem_t codes, mem_t scales, int d) const
+    // (powers go up to 2^127, with which fp32 holds the sizes below 2 alone)
+    __device__ __forceinline__ double element(mem_t codes, mem_t scales, int d) const
     {
-        const uint32_t c = codes[d >> 1] >> (4 * (d & 1)), m = c & 7;
+        const uint32_t c = codes[d >> 1] >> (4 * (d & 1)), m = c & 7, e = scales[d >> 5];
         const float size = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1) << 22);
-        return (c & 8 ? -size : size) * mx4_power(scales[d >> 5]);
+        const double power = e == 255 ? __longlong_as_double(0x7ff8000000000000ll) : __longlong_as_double((long long)(e + 896) << 52);
+        return (c & 8 ? -size : size) * power;
     }
     // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
-    // 64) for the values, whose mean is carried along, so that finite values never add up to infinity.  Slow, for rows with infinities or NaN in their results; only
-    // for rows that have not been written yet, whose places may be those of the query.
+    // 64) for the values, whose mean is carried along in 64 bits, so that finite values never add up to infinity, those that a code of a great power has beyond fp32
+    // neither.  Slow, for rows with infinities or NaN in their results; only for rows that have not been written yet, whose places may be those of the query.
     __device__ __forceinline__ void plainly(int row, int step, int end)
     {
         const int dim = A.cache.head_dim;
@@ -196,7 +198,8 @@ struct AttnMx {
             place(row, &token, &head);
             const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
             const int last = t.p0 + token, first = first_key(last, A.window);
-            float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
+            float top = -INFINITY, sum = 0.f;
+            double mean[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
                 const int j = t.position(j0) + lane;
                 int id = -1;
@@ -210,9 +213,9 @@ struct AttnMx {
                 float score = -INFINITY;
                 if (seen) {
                     const mem_t k = (mem_t)(keys() + place_here.k), ks = (mem_t)(key_scales() + place_here.ks);
-                    float dot = 0.f;
-                    for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * element(k, ks, d);
-                    score = dot * A.c;
+                    double dot = 0.0;
+                    for (int d = 0; d < dim; ++d) dot += (double)(src[d] * A.sign) * element(k, ks, d);
+                    score = (float)(dot * A.c);
                 }
                 float most = score;
                 for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
@@ -236,14 +239,14 @@ struct AttnMx {
                         if (64 * i + lane < dim) mean[i] += wk * element(v, vs, 64 * i + lane);
                 }
             }
-            // a piece's state in units in which its sum is at most 1
-            const int e = sum > 0.f ? __builtin_amdgcn_frexp_expf(sum) : 0;
+            // a piece's state in units in which its sum is at most an eighth, so that fp32 holds its weighted values
+            const int e = (sum > 0.f ? __builtin_amdgcn_frexp_expf(sum) : 0) + 3;
             const float part = ldexpf(sum, -e);
             float* dst = t.cuts == 1 ? A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * dim : values_of(row);
             const float by = t.cuts == 1 ? sum * over_sum(A, sum, top, head) : part;
 #pragma unroll
             for (int i = 0; i <= HD / 64; ++i)
-                if (64 * i + lane < dim) dst[64 * i + lane] = mean[i] * by;
+                if (64 * i + lane < dim) dst[64 * i + lane] = (float)(mean[i] * by);
             if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top + (float)e, part};
         }
     }

@@ -65,6 +65,23 @@ def test_means_of_values(hip, e, keys, heads):
 
 @pytest.mark.parametrize("heads", [1, 40])
 @pytest.mark.parametrize("e", POWERS)
+def test_means_over_pieces_of_keys(hip, e, heads):
+    """4096 keys of one weight, cut into pieces.  A block of 64 keys rounds what was summed before it and its own weights, 4 x 2^-24 of sum p |v|, the join 16 x 2^-24."""
+    import torch
+    keys = 4096
+    v = np.zeros((3, keys, 32), dtype=np.int64)
+    v[0, 77] = np.arange(32) % 16                                    # one value, the others 0
+    v[1] = 3 if e < 254 else 1                                       # alike
+    v[2, 0::2], v[2, 1::2] = 7, 15                                   # the largest and its opposite
+    cache = cache_of(torch, np.zeros_like(v), np.full((3, keys), 127), v, np.full((3, keys), e))
+    values = mx.values(v, np.full((3, keys, 1), e, dtype=np.uint8))
+    got = attend(hip, torch, cache, torch.ones((3, 32 * heads), device="cuda"), keys, 1.0).reshape(3, heads, 32)
+    bound = (4 * keys / 64 + 16) * 2.0 ** -24 * np.abs(values).mean(1) + 2.0 ** -140
+    assert np.all(np.abs(got - values.mean(1)[:, None]) <= bound[:, None])
+
+
+@pytest.mark.parametrize("heads", [1, 40])
+@pytest.mark.parametrize("e", POWERS)
 def test_keys(hip, e, heads):
     """the first key is zero and has the value 1, the second a code in one dimension and the value -1"""
     import torch
