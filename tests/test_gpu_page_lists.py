@@ -45,6 +45,8 @@ def test_a_compaction_with_room_for_every_move(hip, seqs, pages):
     moves = expected.compact(MOST)
     listed(torch, whole[:MOST], moves)
     assert same() and bool((whole[MOST:] == 7).all())
+    del whole
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("seqs", [3, 4200])
@@ -64,3 +66,5 @@ def test_a_fork_of_every_pair(hip, seqs):
     moves, short = expected.fork([c for _, c, _ in pairs], [p for _, _, p in pairs])
     listed(torch, whole[:MOST], moves)
     assert missing.item() == short == 0 and same() and bool((whole[MOST:] == 7).all())
+    del whole, children, parents
+    torch.cuda.empty_cache()
