@@ -207,11 +207,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_kernel(const float* q
     }
 }
 
+// 64 bits in 32 for a further rounding to fewer: what lies between two values becomes the odd one, so that it stays on its side of every border (which is even).
+__device__ __forceinline__ float towards_odd(double x)
+{
+    const float f = (float)x;
+    if ((double)f == x) return f;                                    // (infinities too; a NaN stays one)
+    return __uint_as_float((__float_as_uint(f) - (fabs((double)f) > fabs(x) ? 1u : 0u)) | 1u);
+}
+
 // The same into a cache in four bits.  What a key or value head becomes goes through LDS, since the lanes that turn pairs do not hold neighbours: then a lane
 // has eight values that follow one another, four lanes a block, whose largest magnitude they find among them.
 // Keys are normed and turned in 64 bits: a code is a step of a quarter to a half of a value, so that an error of 2^-22 on one side of a border is one of 1e-4 over all
-// keys of a store (three prompts of 2048 tokens, 3.6 million values: one or two of them); in 64 bits the code is that of the exact value but where that is within 2^-25 of
-// a border.  Queries, which are not rounded further, stay in 32 bits.  Bound: memory, most of it the queries (3515 rows of 32 + 2 x 8 heads of 128: 26 us, 148 MB at 5.7 TB/s),
+// keys of a store (three prompts of 2048 tokens, 3.6 million values: one or two of them); in 64 bits, brought to 32 towards the odd value, the code is that of the exact
+// one (rounded to nearest, one store in ten or so had a key within 2^-25 of a border on its other side).  Queries, which are not rounded further, stay in 32 bits.  Bound: memory, most of it the queries (3515 rows of 32 + 2 x 8 heads of 128: 26 us, 148 MB at 5.7 TB/s),
 // and for few rows the way from lengths to page to address (24 rows: 4.6 us).
 template <int LANES>
 __global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int heads,
@@ -285,7 +293,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float
                     x[1] = x[0] * t0.y + x[1] * t0.x, x[3] = x[2] * t1.y + x[3] * t1.x;
                     x[0] = y0, x[2] = y2;
                 }
-                store_quad(&heads_here[slot][0], Quad{f2_t{(float)x[0], (float)x[2]}, f2_t{(float)x[1], (float)x[3]}}, R, u);
+                store_quad(&heads_here[slot][0], Quad{f2_t{towards_odd(x[0]), towards_odd(x[2])}, f2_t{towards_odd(x[1]), towards_odd(x[3])}}, R, u);
             }
         }
         if (page < 0 || h0 + kHeads <= heads) continue;              // uniform
