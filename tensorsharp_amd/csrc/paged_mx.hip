@@ -179,17 +179,16 @@ struct AttnMx {
     __device__ __forceinline__ uint64_t value_scales() const { return (uint64_t)(uintptr_t)X.v + kvh * X.v_head; }
 
     // ---- infinities and NaN ----
-    // (powers go up to 2^127, with which fp32 holds the sizes below 2 alone)
-    __device__ __forceinline__ double element(mem_t codes, mem_t scales, int d) const
+    // an eighth of an element: fp32 holds that of all, whose powers go up to 2^127 (and down to 2^-127: means below 2^-123 lose up to three bits)
+    __device__ __forceinline__ float eighth(mem_t codes, mem_t scales, int d) const
     {
-        const uint32_t c = codes[d >> 1] >> (4 * (d & 1)), m = c & 7, e = scales[d >> 5];
-        const float size = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1) << 22);
-        const double power = e == 255 ? __longlong_as_double(0x7ff8000000000000ll) : __longlong_as_double((long long)(e + 896) << 52);
-        return (c & 8 ? -size : size) * power;
+        const uint32_t c = codes[d >> 1] >> (4 * (d & 1)), m = c & 7;
+        const float size = m < 2 ? 0.0625f * m : __uint_as_float(((m >> 1) + 123u) << 23 | (m & 1) << 22);
+        return (c & 8 ? -size : size) * mx4_power(scales[d >> 5]);
     }
     // Rows of the tile (piece) again, each over the keys that it sees and no others: a lane per key for the scores, a lane per dimension (of
-    // 64) for the values, whose mean is carried along in 64 bits, so that finite values never add up to infinity, those that a code of a great power has beyond fp32
-    // neither.  Slow, for rows with infinities or NaN in their results; only for rows that have not been written yet, whose places may be those of the query.
+    // 64) for the values, of eighths of which the mean is carried along, so that finite values never add up to infinity, nor do those that codes of the greatest powers have
+    // beyond fp32.  Slow, for rows with infinities or NaN in their results; only for rows that have not been written yet, whose places may be those of the query.
     __device__ __forceinline__ void plainly(int row, int step, int end)
     {
         const int dim = A.cache.head_dim;
@@ -198,8 +197,7 @@ struct AttnMx {
             place(row, &token, &head);
             const float* src = A.query + (int64_t)(t.first + token) * A.ld_query + (int64_t)head * dim;
             const int last = t.p0 + token, first = first_key(last, A.window);
-            float top = -INFINITY, sum = 0.f;
-            double mean[HD / 64 + 1] = {};
+            float top = -INFINITY, sum = 0.f, mean[HD / 64 + 1] = {};
             for (int j0 = t.lo; j0 < t.hi; j0 += 64) {
                 const int j = t.position(j0) + lane;
                 int id = -1;
@@ -213,9 +211,9 @@ struct AttnMx {
                 float score = -INFINITY;
                 if (seen) {
                     const mem_t k = (mem_t)(keys() + place_here.k), ks = (mem_t)(key_scales() + place_here.ks);
-                    double dot = 0.0;
-                    for (int d = 0; d < dim; ++d) dot += (double)(src[d] * A.sign) * element(k, ks, d);
-                    score = (float)(dot * A.c);
+                    float dot = 0.f;
+                    for (int d = 0; d < dim; ++d) dot += src[d] * A.sign * eighth(k, ks, d);
+                    score = dot * A.c * 8.f;
                 }
                 float most = score;
                 for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
@@ -236,17 +234,17 @@ struct AttnMx {
                     const mem_t vs = (mem_t)__shfl((unsigned long long)vs_at, lane_of);
 #pragma unroll
                     for (int i = 0; i <= HD / 64; ++i)
-                        if (64 * i + lane < dim) mean[i] += wk * element(v, vs, 64 * i + lane);
+                        if (64 * i + lane < dim) mean[i] += wk * eighth(v, vs, 64 * i + lane);
                 }
             }
-            // a piece's state in units in which its sum is at most an eighth, so that fp32 holds its weighted values
+            // a piece's state in units in which its sum is at most an eighth
             const int e = (sum > 0.f ? __builtin_amdgcn_frexp_expf(sum) : 0) + 3;
             const float part = ldexpf(sum, -e);
             float* dst = t.cuts == 1 ? A.out + (int64_t)(t.first + token) * A.ld_out + (int64_t)head * dim : values_of(row);
-            const float by = t.cuts == 1 ? sum * over_sum(A, sum, top, head) : part;
+            const float by = 8.f * (t.cuts == 1 ? sum * over_sum(A, sum, top, head) : part);
 #pragma unroll
             for (int i = 0; i <= HD / 64; ++i)
-                if (64 * i + lane < dim) dst[64 * i + lane] = (float)(mean[i] * by);
+                if (64 * i + lane < dim) dst[64 * i + lane] = mean[i] * by;
             if (t.cuts > 1 && lane == 0) *state_of(row) = f2_t{top + (float)e, part};
         }
     }
@@ -758,7 +756,7 @@ __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_atten
         if (!(whole ? find_whole(H, A, idx, t) : find_tall(H, A, deal, idx, t))) return;
         if (t.tokens * A.group > kKeyRows) {
             AttnMx<HD> a(A, X, t, kvh, threadIdx.x, (lds_t)smem);
-            if (a.shared_keys()) a.plainly(32 * a.wave, 1, 32 * a.wave + 32);
+            if (__builtin_expect(a.shared_keys(), 0)) a.plainly(32 * a.wave, 1, 32 * a.wave + 32);
             return;
         }
     } else if (idx >= H.pieces) {
@@ -773,8 +771,9 @@ __global__ void __launch_bounds__(kAttnThreads, HD > 128 ? 1 : 2) paged_mx_atten
         int thread = threadIdx.x;
         asm volatile("" : "+v"(thread));                             // (what follows from it is worked out for each tile: kept from one to the next it would be spilled)
         AttnMx<HD> a(A, X, t, kvh, thread, (lds_t)smem);
-        for (int r0 = 0; r0 < t.count; r0 += 16)
-            if (a.own_keys(r0)) a.plainly(r0 + a.wave, kAttnWaves, r0 + 16);
+        int again = 0;                                               // a bit for every 16 rows, which have not been written then
+        for (int r0 = 0; r0 < t.count; r0 += 16) again |= (int)a.own_keys(r0) << (r0 / 16);
+        if (__builtin_expect(again, 0)) a.plainly((again & 1 ? 0 : 16) + a.wave, kAttnWaves, again & 2 ? 32 : 16);
     }
 }
 
