@@ -51,9 +51,13 @@ __device__ __forceinline__ void cut_terms(f16_t a, f16_t b, Terms& out)      // 
         const uint32_t e = fp6_power(top);
         const float by = __uint_as_float(e == 255 ? 127u << 23 : e << 23);
         out.t[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, by);
+        // (The conversion writes its first results before it has read its last values, so that these may not share registers, which the compiler would have them do where
+        // a and b are of no further use: now and then the last term of 96 dimensions came out another.)
+        asm volatile("" ::"v"(out.t[n]), "v"(a), "v"(b), "v"(by));
         out.scale[n / 4] |= e << (8 * (n % 4));
         if (n + 1 < kParts) {
             const v32_t back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(out.t[n], by);
+            asm volatile("" ::"v"(back), "v"(out.t[n]), "v"(by));
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 a[i] -= back[2 * i];
