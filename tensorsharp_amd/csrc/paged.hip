@@ -219,7 +219,7 @@ __device__ __forceinline__ float towards_odd(double x)
 // has eight values that follow one another, four lanes a block, whose largest magnitude they find among them.
 // Keys are normed and turned in 64 bits: a code is a step of a quarter to a half of a value, so that an error of 2^-22 on one side of a border is one of 1e-4 over all
 // keys of a store (three prompts of 2048 tokens, 3.6 million values: one or two of them); in 64 bits, brought to 32 towards the odd value, the code is that of the exact
-// one (rounded to nearest, one store in ten or so had a key within 2^-25 of a border on its other side).  Queries, which are not rounded further, stay in 32 bits.  Bound: memory, most of it the queries (3515 rows of 32 + 2 x 8 heads of 128: 26 us, 148 MB at 5.7 TB/s),
+// one (none of 100 such stores had another; rounded to nearest 28 of them had a key or two within 2^-25 of a border on its other side).  Queries, which are not rounded further, stay in 32 bits.  Bound: memory, most of it the queries (3515 rows of 32 + 2 x 8 heads of 128: 26 us, 148 MB at 5.7 TB/s),
 // and for few rows the way from lengths to page to address (24 rows: 4.6 us).
 template <int LANES>
 __global__ void __launch_bounds__(kRopeThreads) rope_store_mx_kernel(const float* qkv, int64_t ld_qkv, float* query, int64_t ld_query, int heads,
